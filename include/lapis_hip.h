@@ -428,6 +428,126 @@ int lapis_hip_mht_f64_i32(lapis_hip_csr_plan *plan, int64_t n, int64_t nnz, cons
 int lapis_hip_normalize_mom2_f64(int64_t n, const double *mom1, const double *mom2, double *out,
                                  lapis_hip_stream_t stream);
 
+/* ---- block-sparse attention ---------------------------------------------------
+ *
+ * Attention whose scores exist only where a CSR structure has entries, at the granularity of blocks.  The
+ * reference multiplies with such a structure (the batched CSRV product of examples/bspmm.py:22-50, whose values
+ * are finished attention weights); it has no counterpart of what follows.
+ *
+ * Types: 16-bit elements (bf16, f16); a cache may hold e4m3 codes with one fp32 scale per row of `dim`.  Sums,
+ * softmax statistics and scales are fp32.  `dim` is a multiple of 8; 16-bit operands lie on 16-byte boundaries,
+ * codes on 8-byte ones, strides (in elements) are multiples of 8.  Outputs must not overlap inputs.
+ * Structures: positions and coordinates int32.  A coordinate outside [0, columns) (of pages: outside [0, pages))
+ * and positions outside [0, nnz] are never followed: such an entry counts as absent.  Coordinates need not ascend.
+ * Rows without an entry give zeros, and -infinity as the logarithm of their sum.
+ * No entry point below allocates or synchronises: where scratch memory is needed the caller passes `work` of at least
+ * the bytes the matching _work call says. */
+
+enum lapis_hip_dtype { LAPIS_HIP_BF16 = 0, LAPIS_HIP_F16 = 1, LAPIS_HIP_F8E4M3 = 2 };
+
+/* Rows of `dim` neighbouring elements: row (b, token, head) starts at data + b*stride[0] + token*stride[1] +
+ * head*stride[2].  A stride may be 0 (a broadcast input). */
+typedef struct lapis_hip_rows {
+  void *data;
+  int64_t stride[3];
+} lapis_hip_rows;
+
+/* A cache of keys and values in pages: row (page, head, slot) of both starts at page*stride[0] + head*stride[1] +
+ * slot*stride[2]; its scale (dtype LAPIS_HIP_F8E4M3 only) at page*scale_stride[0] + head*scale_stride[1] + slot*scale_stride[2]. */
+typedef struct lapis_hip_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t stride[3], scale_stride[3];
+  int64_t pages;
+  int32_t heads, page, dim; /* page = slots of a page, a power of two up to 1024; dim up to 256 */
+  int32_t dtype;            /* LAPIS_HIP_BF16, LAPIS_HIP_F16 or LAPIS_HIP_F8E4M3 */
+} lapis_hip_kv_cache;
+
+/* Row t of k and v (stride[0] unused) goes to slot slots[t] (page * cache->page + place in the page) of every head;
+ * a slot outside [0, pages * page) writes nothing.  Slots are distinct (of two tokens for one slot either may win).
+ * With LAPIS_HIP_F8E4M3: scale = max|x| / 448 over the row, codes = x / scale rounded to nearest even; a row of zeros has
+ * scale 0; a NaN stays NaN, a row with an infinity reads back as NaN.  `dtype` is the rows' own. */
+int lapis_hip_kv_store(const lapis_hip_kv_cache *cache, int64_t tokens, const lapis_hip_rows *k, const lapis_hip_rows *v,
+                       int dtype, const int32_t *slots, lapis_hip_stream_t stream);
+/* The way back: row t of k and v is what slot slots[t] holds (scale * code, rounded to `dtype`); zeros for a slot
+ * outside [0, pages * page). */
+int lapis_hip_kv_load(const lapis_hip_kv_cache *cache, int64_t tokens, const int32_t *slots, const lapis_hip_rows *k,
+                      const lapis_hip_rows *v, int dtype, lapis_hip_stream_t stream);
+
+/* One new token of each of `seqs` sequences: out(s, h) = sum_t softmax_t(scale * q(s, h) . k_t) v_t over the tokens of
+ * the pages that a CSR row lists, in list order; of the last page only as many slots count as tokens[row] leaves.
+ * `lists` = seqs: one row per sequence, shared by its heads; = seqs * cache->heads: row s * cache->heads + h' per
+ * key-value head.  heads is a multiple of cache->heads; consecutive heads share a key-value head.  Tokens beyond the
+ * listed pages do not exist.  q and out: row (s, head) at s*stride[0] + head*stride[2].  lse (seqs x heads, may be
+ * NULL) gets the logarithms of the softmax sums.  What lies in the unused slots of a page is never used, whatever it is. */
+typedef struct lapis_hip_paged_args {
+  int64_t seqs, lists, heads, nnz;
+  lapis_hip_rows q, out;
+  int dtype;
+  const int32_t *pos, *crd, *tokens;
+  float *lse;
+  float scale;
+  void *work;
+} lapis_hip_paged_args;
+int lapis_hip_paged_attention_work(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, int64_t *bytes);
+int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, lapis_hip_stream_t stream);
+
+/* 8-bit means: codes(b, h, j, :) * scales(b, h, j) is the mean of x over the `block` tokens from j * block on (fewer at the
+ * end) and the heads of group h (heads / groups consecutive ones).  scale = max|mean| / 127, codes = mean / scale rounded
+ * to nearest even; a mean that is not finite gives codes 0 and scale NaN.  codes: batch x groups x ceil(tokens / block) x
+ * dim, contiguous, on an 8-byte boundary. */
+int lapis_hip_block_pool(int64_t batch, int64_t tokens, int64_t heads, int64_t groups, int64_t dim, int64_t block,
+                         const lapis_hip_rows *x, int dtype, int8_t *codes, float *scales, lapis_hip_stream_t stream);
+
+/* For each row (b, head, block of block_m queries) the `count` best blocks of keys as a CSR structure, ascending:
+ * score = float(q_codes . k_codes) * k_scales, a product of whole numbers that has no rounding (dim <= 1024), so a
+ * selection does not depend on an order of summation; equal scores go to the lowest block, NaN behind all others.  The
+ * first `sink` and the last `local` blocks a row may see are always taken (sink + local <= count).
+ * Row r sees the blocks that hold a key at or before its last query (causal: query i stands at i + keys - queries), or
+ * all of them.  Over a cache: table (batch x table_width page numbers, NULL = none) maps block j of sequence b to a page:
+ * codes and scales are those of page table[b][j] and that number becomes the coordinate; sequence b has blocks[b] blocks
+ * (NULL: all); causal must then be 0.  A table entry outside [0, pages) scores NaN.
+ * k row of block j: k_codes + b*k_stride[0] + head*k_stride[1] + j*k_stride[2] (with a table: page*k_stride[2], stride[0]
+ * unused); scales likewise with scale_stride.  q_codes: batch x heads x ceil(queries / block_m) x dim, contiguous.
+ * pos: rows + 1 and crd: as many as lapis_hip_block_select_entries says (with `blocks` an upper bound). */
+typedef struct lapis_hip_select_args {
+  int64_t batch, heads, queries, keys, dim, block_m, block_n, count, sink, local;
+  int causal;
+  const int8_t *q_codes, *k_codes;
+  const float *k_scales;
+  int64_t k_stride[3], scale_stride[3];
+  const int32_t *table, *blocks;
+  int64_t table_width, pages;
+  int32_t *pos, *crd;
+  void *work;
+} lapis_hip_select_args;
+int lapis_hip_block_select_entries(const lapis_hip_select_args *args, int64_t *entries);
+int lapis_hip_block_select_work(const lapis_hip_select_args *args, int64_t *bytes);
+int lapis_hip_block_select(const lapis_hip_select_args *args, lapis_hip_stream_t stream);
+
+/* out = softmax(scale * q k^T, over the listed blocks only) v, and lse(b, head, query) = log sum exp of its scores.
+ * Row (b * kv_heads + h) * ceil(queries / block_m) + r of the structure lists the blocks of block_n keys (16, 32, 64, 128 or
+ * 256) that the queries r*block_m .. of the heads of group h attend to; causal: only keys at or before
+ * i + keys - queries for query i.  heads is a multiple of kv_heads, dim <= 128.  An entry listed twice counts twice.
+ * lse may be NULL in the forward call. */
+typedef struct lapis_hip_block_args {
+  int64_t batch, queries, keys, heads, kv_heads, dim, block_m, block_n, nnz;
+  int causal, dtype;
+  float scale;
+  const int32_t *pos, *crd;
+  lapis_hip_rows q, k, v, out;
+  float *lse;
+  lapis_hip_rows dout, dq, dk, dv; /* backward only */
+  void *work;                      /* backward only */
+} lapis_hip_block_args;
+int lapis_hip_block_attention(const lapis_hip_block_args *args, lapis_hip_stream_t stream);
+/* Gradients of the forward call whose out and lse these are: dv = P^T dout, dS = P * (dout v^T - rowsum(dout * out)),
+ * dq = scale dS k, dk = scale dS^T q, with P = exp(scale q k^T - lse) on the listed blocks.  Every element of dq, dk and
+ * dv is written; a group's heads add up into their key-value head's gradient.  Sums are taken in a fixed order: the same
+ * inputs give the same bits. */
+int lapis_hip_block_attention_backward_work(const lapis_hip_block_args *args, int64_t *bytes);
+int lapis_hip_block_attention_backward(const lapis_hip_block_args *args, lapis_hip_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,7 +25,8 @@ OBJDIR = os.path.join(CSRC, "build")
 INCLUDE = os.path.join(ROOT, "include")
 
 KERNEL_SOURCES = ["runtime.hip", "spmv.hip", "rowchunk.hip", "colblock.hip", "colgroup.hip", "spmm.hip", "blas1.hip",
-                  "cg.hip", "staging.hip", "calibrate.hip"]
+                  "cg.hip", "staging.hip", "calibrate.hip", "kvcache.hip", "paged.hip", "blockselect.hip", "blockattn.hip",
+                  "blockattn_bwd.hip"]
 SHIM_SOURCES = ["module_shim.hip"]
 
 KERNEL_LIB = os.path.join(LIBDIR, "liblapis_hip.so")

@@ -8,9 +8,12 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/from_blob.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <memory>
 #include <vector>
@@ -612,6 +615,426 @@ LAPIS_PY(py_pcg) {
   });
 }
 
+
+// ---- block-sparse attention: operands are tensors, with strides ----
+
+// A tensor of `dims` dimensions.
+const at::Tensor &tensor(const char *what, const char *name, PyObject *o, int dims) {
+  if (!THPVariable_Check(o)) raise(PyExc_TypeError, "%s: %s is a tensor, got %s", what, name, Py_TYPE(o)->tp_name);
+  const at::Tensor &t = THPVariable_Unpack(o);
+  if (t.dim() != dims) raise(PyExc_ValueError, "%s: %s has %d dimensions, %d expected", what, name, (int)t.dim(), dims);
+  return t;
+}
+
+void of_type(const char *what, const char *name, const at::Tensor &t, at::ScalarType type) {
+  if (t.scalar_type() != type) raise(PyExc_TypeError, "%s: %s of %s, %s expected", what, name, type_name(t.scalar_type()), type_name(type));
+}
+
+void of_shape(const char *what, const char *name, const at::Tensor &t, std::initializer_list<int64_t> sizes) {
+  int64_t i = 0;
+  for (const int64_t s : sizes) {
+    if (t.size(i) != s)
+      raise(PyExc_ValueError, "%s: dimension %d of %s is %lld, %lld expected", what, (int)i, name, (long long)t.size(i), (long long)s);
+    ++i;
+  }
+}
+
+int type_code(const char *what, const char *name, const at::Tensor &t, bool codes = false) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return LAPIS_HIP_BF16;
+    case at::kHalf: return LAPIS_HIP_F16;
+    case at::kFloat8_e4m3fn:
+      if (codes) return LAPIS_HIP_F8E4M3;
+      [[fallthrough]];
+    default: raise(PyExc_TypeError, "%s: %s is bfloat16 or float16%s, got %s", what, name, codes ? " or float8_e4m3fn" : "", type_name(t.scalar_type()));
+  }
+}
+
+// A dimension of one element has no stride to speak of.
+int64_t stride_of(const at::Tensor &t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
+
+void dense_rows(const char *what, const char *name, const at::Tensor &t) {
+  const int64_t last = t.dim() - 1;
+  if (t.size(last) > 1 && t.stride(last) != 1) raise(PyExc_ValueError, "%s: the elements of a row of %s are not neighbours", what, name);
+}
+
+// An output whose elements share memory would depend on who writes last.
+void no_overlap(const char *what, const char *name, const at::Tensor &t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = 1;
+  for (const auto &d : dims) {
+    if (d.first < extent) raise(PyExc_ValueError, "%s: elements of %s share memory", what, name);
+    extent = d.first * (d.second - 1) + extent;
+  }
+}
+
+void contiguous(const char *what, const char *name, const at::Tensor &t) {
+  if (!t.is_contiguous()) raise(PyExc_ValueError, "%s: %s is not contiguous", what, name);
+}
+
+// The kernels read and write device memory only, of one device.
+void on_device(const char *what, PyObject *const *a, Py_ssize_t n) {
+  int device = -1;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!THPVariable_Check(a[i])) continue;
+    const at::Tensor &t = THPVariable_Unpack(a[i]);
+    if (!t.is_cuda()) raise(PyExc_ValueError, "%s: operand %d is not in device memory", what, (int)i);
+    if (device >= 0 && t.device().index() != device) raise(PyExc_ValueError, "%s: operands on different devices", what);
+    device = t.device().index();
+  }
+}
+
+// Rows of a tensor (batch, tokens, heads, dim); with three dimensions (tokens, heads, dim).
+lapis_hip_rows rows_of(const char *what, const char *name, const at::Tensor &t, bool output) {
+  dense_rows(what, name, t);
+  if (output) no_overlap(what, name, t);
+  lapis_hip_rows r = {t.data_ptr(), {0, 0, 0}};
+  const int64_t skip = t.dim() == 4 ? 0 : 1;
+  for (int64_t i = skip; i < 3; ++i) r.stride[i] = stride_of(t, i - skip);
+  return r;
+}
+
+// Device memory for the length of a call on `stream`: torch's allocator hands it on once that stream is done with it.
+struct Scratch {
+  at::Tensor held;
+  Scratch(int64_t bytes, lapis_hip_stream_t stream) {
+    if (bytes <= 0) return;
+    const auto current = c10::hip::getCurrentHIPStream();
+    held = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, current.device_index())));
+    if (stream != (lapis_hip_stream_t)current.stream())
+      c10::hip::HIPCachingAllocator::recordStream(held.storage().data_ptr(),
+                                                  c10::hip::getStreamFromExternal((hipStream_t)stream, current.device_index()));
+  }
+  void *data() const { return held.defined() ? held.data_ptr() : nullptr; }
+};
+
+// k_cache, v_cache (pages, heads, slots of a page, dim) and their scales (pages, heads, slots) or None
+lapis_hip_kv_cache cache_of(const char *what, PyObject *k, PyObject *v, PyObject *ks, PyObject *vs, bool output) {
+  const at::Tensor &kt = tensor(what, "k_cache", k, 4), &vt = tensor(what, "v_cache", v, 4);
+  lapis_hip_kv_cache c = {};
+  c.dtype = type_code(what, "k_cache", kt, true);
+  of_type(what, "v_cache", vt, kt.scalar_type());
+  of_shape(what, "v_cache", vt, {kt.size(0), kt.size(1), kt.size(2), kt.size(3)});
+  for (const at::Tensor *t : {&kt, &vt}) {
+    dense_rows(what, t == &kt ? "k_cache" : "v_cache", *t);
+    if (output) no_overlap(what, t == &kt ? "k_cache" : "v_cache", *t);
+  }
+  for (int i = 0; i < 3; ++i) {
+    c.stride[i] = stride_of(kt, i);
+    if (stride_of(vt, i) != c.stride[i]) raise(PyExc_ValueError, "%s: k_cache and v_cache have different strides", what);
+  }
+  if (kt.size(1) > INT32_MAX || kt.size(2) > INT32_MAX || kt.size(3) > INT32_MAX) raise(PyExc_ValueError, "%s: a cache too large", what);
+  c.k = kt.data_ptr();
+  c.v = vt.data_ptr();
+  c.pages = kt.size(0);
+  c.heads = (int32_t)kt.size(1);
+  c.page = (int32_t)kt.size(2);
+  c.dim = (int32_t)kt.size(3);
+  const bool f8 = c.dtype == LAPIS_HIP_F8E4M3;
+  if (!f8) {
+    if (ks != Py_None || vs != Py_None) raise(PyExc_ValueError, "%s: scales with a cache of %s", what, type_name(kt.scalar_type()));
+    return c;
+  }
+  for (int i = 0; i < 2; ++i) {
+    const char *name = i ? "v_scale" : "k_scale";
+    const at::Tensor &t = tensor(what, name, i ? vs : ks, 3);
+    of_type(what, name, t, at::kFloat);
+    of_shape(what, name, t, {kt.size(0), kt.size(1), kt.size(2)});
+    if (output) no_overlap(what, name, t);
+    (i ? c.v_scale : c.k_scale) = static_cast<float *>(t.data_ptr());
+    for (int j = 0; j < 3; ++j) {
+      if (i && c.scale_stride[j] != stride_of(t, j)) raise(PyExc_ValueError, "%s: k_scale and v_scale have different strides", what);
+      c.scale_stride[j] = stride_of(t, j);
+    }
+  }
+  return c;
+}
+
+// store (k, v, slots, k_cache, v_cache, k_scale, v_scale, stream), load (k_cache, v_cache, slots, k, v, k_scale, v_scale, stream)
+PyObject *kv_move(const char *what, bool store, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] {
+    arguments(what, n, 8);
+    PyObject *const *rows = store ? a : a + 3, *const *cache = store ? a + 3 : a;
+    const lapis_hip_kv_cache c = cache_of(what, cache[0], cache[1], a[5], a[6], store);
+    const at::Tensor &k = tensor(what, "k", rows[0], 3), &v = tensor(what, "v", rows[1], 3), &slots = tensor(what, "slots", a[2], 1);
+    const int dtype = type_code(what, "k", k);
+    of_type(what, "v", v, k.scalar_type());
+    if (c.dtype != LAPIS_HIP_F8E4M3 && c.dtype != dtype) raise(PyExc_TypeError, "%s: rows of %s and a cache of another 16-bit type", what, type_name(k.scalar_type()));
+    of_shape(what, "k", k, {k.size(0), c.heads, c.dim});
+    of_shape(what, "v", v, {k.size(0), c.heads, c.dim});
+    of_type(what, "slots", slots, at::kInt);
+    of_shape(what, "slots", slots, {k.size(0)});
+    contiguous(what, "slots", slots);
+    const lapis_hip_rows kr = rows_of(what, "k", k, !store), vr = rows_of(what, "v", v, !store);
+    const auto s = static_cast<const int32_t *>(slots.data_ptr());
+    on_device(what, a, n);
+    const lapis_hip_stream_t st = stream_of(a[7]);
+    check(store ? lapis_hip_kv_store(&c, k.size(0), &kr, &vr, dtype, s, st) : lapis_hip_kv_load(&c, k.size(0), s, &kr, &vr, dtype, st));
+    PyObject *result = PyTuple_Pack(2, a[3], a[4]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+LAPIS_PY(py_kv_store) { return kv_move("kv_store", true, a, n); }
+LAPIS_PY(py_kv_load) { return kv_move("kv_load", false, a, n); }
+
+// (q, k_cache, v_cache, pos, crd, tokens, out, lse, scale, k_scale, v_scale, stream)
+LAPIS_PY(py_paged_attention) {
+  return guarded([&] {
+    const char *what = "paged_attention";
+    arguments(what, n, 12);
+    const lapis_hip_kv_cache c = cache_of(what, a[1], a[2], a[9], a[10], false);
+    const at::Tensor &q = tensor(what, "q", a[0], 3), &pos = tensor(what, "pos", a[3], 1), &crd = tensor(what, "crd", a[4], 1),
+                     &tokens = tensor(what, "tokens", a[5], 1), &out = tensor(what, "out", a[6], 3);
+    lapis_hip_paged_args p = {};
+    p.dtype = type_code(what, "q", q);
+    if (c.dtype != LAPIS_HIP_F8E4M3 && c.dtype != p.dtype) raise(PyExc_TypeError, "%s: queries of %s and a cache of another 16-bit type", what, type_name(q.scalar_type()));
+    of_shape(what, "q", q, {q.size(0), q.size(1), c.dim});
+    of_type(what, "out", out, q.scalar_type());
+    of_shape(what, "out", out, {q.size(0), q.size(1), c.dim});
+    for (const at::Tensor *t : {&pos, &crd, &tokens}) {
+      of_type(what, "a structure", *t, at::kInt);
+      contiguous(what, "a structure", *t);
+    }
+    p.seqs = q.size(0);
+    p.heads = q.size(1);
+    p.lists = tokens.size(0);
+    of_shape(what, "pos", pos, {p.lists + 1});
+    if (p.lists != p.seqs && p.lists != p.seqs * c.heads)
+      raise(PyExc_ValueError, "%s: %lld lists of pages for %lld sequences and %d key-value heads", what, (long long)p.lists, (long long)p.seqs, (int)c.heads);
+    p.nnz = crd.size(0);
+    p.q = rows_of(what, "q", q, false);
+    p.out = rows_of(what, "out", out, true);
+    for (lapis_hip_rows *r : {&p.q, &p.out}) r->stride[0] = r->stride[1];  // (sequence, head)
+    p.pos = static_cast<const int32_t *>(pos.data_ptr());
+    p.crd = static_cast<const int32_t *>(crd.data_ptr());
+    p.tokens = static_cast<const int32_t *>(tokens.data_ptr());
+    if (a[7] != Py_None) {
+      const at::Tensor &lse = tensor(what, "lse", a[7], 2);
+      of_type(what, "lse", lse, at::kFloat);
+      of_shape(what, "lse", lse, {p.seqs, p.heads});
+      contiguous(what, "lse", lse);
+      p.lse = static_cast<float *>(lse.data_ptr());
+    }
+    p.scale = a[8] == Py_None ? 1.0f / std::sqrt((float)c.dim) : (float)number(a[8]);
+    on_device(what, a, n);
+    const lapis_hip_stream_t st = stream_of(a[11]);
+    int64_t bytes = 0;
+    check(lapis_hip_paged_attention_work(&c, &p, &bytes));
+    const Scratch work(bytes, st);
+    p.work = work.data();
+    check(lapis_hip_paged_attention(&c, &p, st));
+    return give(a[6]);
+  });
+}
+
+// (x, block, codes, scales, stream)
+LAPIS_PY(py_block_pool) {
+  return guarded([&] {
+    const char *what = "block_pool";
+    arguments(what, n, 5);
+    const at::Tensor &x = tensor(what, "x", a[0], 4), &codes = tensor(what, "codes", a[2], 4), &scales = tensor(what, "scales", a[3], 3);
+    const int64_t block = integer(a[1]);
+    const int dtype = type_code(what, "x", x);
+    if (block < 1) raise(PyExc_ValueError, "%s: blocks of %lld tokens", what, (long long)block);
+    of_type(what, "codes", codes, at::kChar);
+    of_type(what, "scales", scales, at::kFloat);
+    const int64_t groups = codes.size(1), blocks = (x.size(1) + block - 1) / block;
+    if (groups < 1 || x.size(2) % groups != 0) raise(PyExc_ValueError, "%s: %lld heads in %lld groups", what, (long long)x.size(2), (long long)groups);
+    of_shape(what, "codes", codes, {x.size(0), groups, blocks, x.size(3)});
+    of_shape(what, "scales", scales, {x.size(0), groups, blocks});
+    contiguous(what, "codes", codes);
+    contiguous(what, "scales", scales);
+    const lapis_hip_rows r = rows_of(what, "x", x, false);
+    on_device(what, a, n);
+    check(lapis_hip_block_pool(x.size(0), x.size(1), x.size(2), groups, x.size(3), block, &r, dtype, static_cast<int8_t *>(codes.data_ptr()),
+                               static_cast<float *>(scales.data_ptr()), stream_of(a[4])));
+    PyObject *result = PyTuple_Pack(2, a[2], a[3]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+
+// (q_codes, k_codes, k_scales, count, pos, crd, queries, keys, block_m, block_n, causal, sink, local, table, blocks, stream)
+struct SelectCall {
+  lapis_hip_select_args p = {};
+  SelectCall(const char *what, PyObject *const *a) {
+    const at::Tensor &q = tensor(what, "q_codes", a[0], 4), &k = tensor(what, "k_codes", a[1], a[13] == Py_None ? 4 : 3),
+                     &s = tensor(what, "k_scales", a[2], (int)k.dim() - 1);
+    of_type(what, "q_codes", q, at::kChar);
+    of_type(what, "k_codes", k, at::kChar);
+    of_type(what, "k_scales", s, at::kFloat);
+    contiguous(what, "q_codes", q);
+    dense_rows(what, "k_codes", k);
+    p.count = integer(a[3]);
+    p.queries = integer(a[6]);
+    p.keys = integer(a[7]);
+    p.block_m = integer(a[8]);
+    p.block_n = integer(a[9]);
+    p.causal = PyObject_IsTrue(a[10]);
+    p.sink = integer(a[11]);
+    p.local = integer(a[12]);
+    if (p.block_m < 1 || p.block_n < 1 || p.queries < 0 || p.keys < 0) raise(PyExc_ValueError, "%s: sizes of blocks and of queries and keys", what);
+    p.batch = q.size(0);
+    p.heads = q.size(1);
+    p.dim = q.size(3);
+    of_shape(what, "q_codes", q, {p.batch, p.heads, (p.queries + p.block_m - 1) / p.block_m, p.dim});
+    if (a[13] == Py_None) {
+      const int64_t columns = (p.keys + p.block_n - 1) / p.block_n;
+      of_shape(what, "k_codes", k, {p.batch, p.heads, columns, p.dim});
+      of_shape(what, "k_scales", s, {p.batch, p.heads, columns});
+      for (int i = 0; i < 3; ++i) p.k_stride[i] = stride_of(k, i), p.scale_stride[i] = stride_of(s, i);
+    } else {
+      const at::Tensor &table = tensor(what, "table", a[13], 2);
+      of_type(what, "table", table, at::kInt);
+      contiguous(what, "table", table);
+      of_shape(what, "table", table, {p.batch, table.size(1)});
+      of_shape(what, "k_codes", k, {k.size(0), p.heads, p.dim});
+      of_shape(what, "k_scales", s, {k.size(0), p.heads});
+      p.table = static_cast<const int32_t *>(table.data_ptr());
+      p.table_width = table.size(1);
+      p.pages = k.size(0);
+      p.k_stride[1] = stride_of(k, 1), p.k_stride[2] = stride_of(k, 0);
+      p.scale_stride[1] = stride_of(s, 1), p.scale_stride[2] = stride_of(s, 0);
+    }
+    if (a[14] != Py_None) {
+      const at::Tensor &blocks = tensor(what, "blocks", a[14], 1);
+      of_type(what, "blocks", blocks, at::kInt);
+      contiguous(what, "blocks", blocks);
+      of_shape(what, "blocks", blocks, {p.batch});
+      p.blocks = static_cast<const int32_t *>(blocks.data_ptr());
+    }
+    p.q_codes = static_cast<const int8_t *>(q.data_ptr());
+    p.k_codes = static_cast<const int8_t *>(k.data_ptr());
+    p.k_scales = static_cast<const float *>(s.data_ptr());
+  }
+};
+LAPIS_PY(py_block_select) {
+  return guarded([&] {
+    const char *what = "block_select";
+    arguments(what, n, 16);
+    SelectCall c(what, a);
+    const at::Tensor &pos = tensor(what, "pos", a[4], 1), &crd = tensor(what, "crd", a[5], 1);
+    of_type(what, "pos", pos, at::kInt);
+    of_type(what, "crd", crd, at::kInt);
+    contiguous(what, "pos", pos);
+    contiguous(what, "crd", crd);
+    on_device(what, a, n);
+    const lapis_hip_stream_t st = stream_of(a[15]);
+    int64_t entries = 0, bytes = 0;
+    check(lapis_hip_block_select_entries(&c.p, &entries));
+    check(lapis_hip_block_select_work(&c.p, &bytes));
+    const int64_t rows = c.p.batch * c.p.heads * ((c.p.queries + c.p.block_m - 1) / c.p.block_m);
+    of_shape(what, "pos", pos, {rows + 1});
+    if (crd.size(0) < entries) raise(PyExc_ValueError, "%s: crd of %lld elements where %lld may be needed", what, (long long)crd.size(0), (long long)entries);
+    c.p.pos = static_cast<int32_t *>(pos.data_ptr());
+    c.p.crd = static_cast<int32_t *>(crd.data_ptr());
+    const Scratch work(bytes, st);
+    c.p.work = work.data();
+    check(lapis_hip_block_select(&c.p, st));
+    PyObject *result = PyTuple_Pack(2, a[4], a[5]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+
+// q, k, v, out, lse (None allowed with `maybe`), pos, crd and the sizes
+lapis_hip_block_args block_of(const char *what, PyObject *q_, PyObject *k_, PyObject *v_, PyObject *pos_, PyObject *crd_, PyObject *out_,
+                              PyObject *lse_, bool forward, PyObject *const *sizes) {
+  const at::Tensor &q = tensor(what, "q", q_, 4), &k = tensor(what, "k", k_, 4), &v = tensor(what, "v", v_, 4),
+                   &pos = tensor(what, "pos", pos_, 1), &crd = tensor(what, "crd", crd_, 1), &out = tensor(what, "out", out_, 4);
+  lapis_hip_block_args p = {};
+  p.dtype = type_code(what, "q", q);
+  p.batch = q.size(0);
+  p.queries = q.size(1);
+  p.heads = q.size(2);
+  p.dim = q.size(3);
+  p.keys = k.size(1);
+  p.kv_heads = k.size(2);
+  p.nnz = crd.size(0);
+  of_type(what, "k", k, q.scalar_type());
+  of_type(what, "v", v, q.scalar_type());
+  of_type(what, "out", out, q.scalar_type());
+  of_shape(what, "k", k, {p.batch, p.keys, p.kv_heads, p.dim});
+  of_shape(what, "v", v, {p.batch, p.keys, p.kv_heads, p.dim});
+  of_shape(what, "out", out, {p.batch, p.queries, p.heads, p.dim});
+  p.block_m = integer(sizes[0]);
+  p.block_n = integer(sizes[1]);
+  p.causal = PyObject_IsTrue(sizes[2]);
+  if (p.block_m < 1 || p.block_n < 1) raise(PyExc_ValueError, "%s: blocks of %lld queries and %lld keys", what, (long long)p.block_m, (long long)p.block_n);
+  if (p.kv_heads < 1 || p.heads % p.kv_heads != 0) raise(PyExc_ValueError, "%s: %lld heads over %lld key-value heads", what, (long long)p.heads, (long long)p.kv_heads);
+  for (const at::Tensor *t : {&pos, &crd}) {
+    of_type(what, "a structure", *t, at::kInt);
+    contiguous(what, "a structure", *t);
+  }
+  of_shape(what, "pos", pos, {p.batch * p.kv_heads * ((p.queries + p.block_m - 1) / p.block_m) + 1});
+  if (lse_ != Py_None || !forward) {
+    const at::Tensor &lse = tensor(what, "lse", lse_, 3);
+    of_type(what, "lse", lse, at::kFloat);
+    of_shape(what, "lse", lse, {p.batch, p.heads, p.queries});
+    contiguous(what, "lse", lse);
+    p.lse = static_cast<float *>(lse.data_ptr());
+  }
+  p.q = rows_of(what, "q", q, false);
+  p.k = rows_of(what, "k", k, false);
+  p.v = rows_of(what, "v", v, false);
+  p.out = rows_of(what, "out", out, forward);
+  p.pos = static_cast<const int32_t *>(pos.data_ptr());
+  p.crd = static_cast<const int32_t *>(crd.data_ptr());
+  p.scale = sizes[3] == Py_None ? 1.0f / std::sqrt((float)p.dim) : (float)number(sizes[3]);
+  return p;
+}
+
+// (q, k, v, pos, crd, out, lse, block_m, block_n, causal, scale, stream)
+LAPIS_PY(py_block_attention) {
+  return guarded([&] {
+    const char *what = "block_attention";
+    arguments(what, n, 12);
+    const lapis_hip_block_args p = block_of(what, a[0], a[1], a[2], a[3], a[4], a[5], a[6], true, a + 7);
+    on_device(what, a, n);
+    check(lapis_hip_block_attention(&p, stream_of(a[11])));
+    PyObject *result = PyTuple_Pack(2, a[5], a[6]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+
+// (dout, q, k, v, out, lse, pos, crd, dq, dk, dv, block_m, block_n, causal, scale, stream)
+LAPIS_PY(py_block_attention_backward) {
+  return guarded([&] {
+    const char *what = "block_attention_backward";
+    arguments(what, n, 16);
+    lapis_hip_block_args p = block_of(what, a[1], a[2], a[3], a[6], a[7], a[4], a[5], false, a + 11);
+    const at::ScalarType type = THPVariable_Unpack(a[1]).scalar_type();
+    const struct {
+      const char *name;
+      PyObject *o;
+      lapis_hip_rows *to;
+      bool queries, output;
+    } more[] = {{"dout", a[0], &p.dout, true, false}, {"dq", a[8], &p.dq, true, true}, {"dk", a[9], &p.dk, false, true}, {"dv", a[10], &p.dv, false, true}};
+    for (const auto &m : more) {
+      const at::Tensor &t = tensor(what, m.name, m.o, 4);
+      of_type(what, m.name, t, type);
+      if (m.queries) of_shape(what, m.name, t, {p.batch, p.queries, p.heads, p.dim});
+      else of_shape(what, m.name, t, {p.batch, p.keys, p.kv_heads, p.dim});
+      *m.to = rows_of(what, m.name, t, m.output);
+    }
+    on_device(what, a, n);
+    const lapis_hip_stream_t st = stream_of(a[15]);
+    int64_t bytes = 0;
+    check(lapis_hip_block_attention_backward_work(&p, &bytes));
+    const Scratch work(bytes, st);
+    p.work = work.data();
+    check(lapis_hip_block_attention_backward(&p, st));
+    PyObject *result = PyTuple_Pack(3, a[8], a[9], a[10]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+
 // setup(check, init)
 PyObject *py_setup(PyObject *, PyObject *args) {
   PyObject *check_fn, *init_fn;
@@ -629,6 +1052,8 @@ PyMethodDef g_methods[] = {LAPIS_METHOD(spmv), LAPIS_METHOD(spmm), LAPIS_METHOD(
                            LAPIS_METHOD(fill), LAPIS_METHOD(copy), LAPIS_METHOD(pcg), LAPIS_METHOD(spmv_overwrite),
                            LAPIS_METHOD(spmv_dot_start), LAPIS_METHOD(dot_start), LAPIS_METHOD(axpby_dot_start),
                            LAPIS_METHOD(dot_finish), LAPIS_METHOD(stage), LAPIS_METHOD(staged_plan), LAPIS_METHOD(fetch),
+                           LAPIS_METHOD(kv_store), LAPIS_METHOD(kv_load), LAPIS_METHOD(paged_attention), LAPIS_METHOD(block_pool),
+                           LAPIS_METHOD(block_select), LAPIS_METHOD(block_attention), LAPIS_METHOD(block_attention_backward),
                            {"setup", py_setup, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_lapis_calls", "Device-resident calls of the gfx950 kernel library.", -1,
                         g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -105,6 +105,10 @@ __device__ __forceinline__ int dpp_mov(int v) {
   return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
 }
 template <int CTRL>
+__device__ __forceinline__ int dpp_get(int v) {
+  return dpp_mov<CTRL>(v);
+}
+template <int CTRL>
 __device__ __forceinline__ float dpp_get(float v) {
   return __builtin_bit_cast(float, dpp_mov<CTRL>(__builtin_bit_cast(int, v)));
 }

@@ -105,6 +105,17 @@ _SIGNATURES = {
                                      ctypes.POINTER(_u64), ctypes.POINTER(_dbl), _vp, _vp],
     "lapis_hip_mht_f64_i32": [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _dbl, _dbl, _u64, _vp, _vp, _vp],
     "lapis_hip_normalize_mom2_f64": [_i64, _vp, _vp, _vp, _vp],
+    "lapis_hip_kv_store": [_vp, _i64, _vp, _vp, _int, _vp, _vp],
+    "lapis_hip_kv_load": [_vp, _i64, _vp, _vp, _vp, _int, _vp],
+    "lapis_hip_paged_attention_work": [_vp, _vp, ctypes.POINTER(_i64)],
+    "lapis_hip_paged_attention": [_vp, _vp, _vp],
+    "lapis_hip_block_pool": [_i64, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp, _vp, _vp],
+    "lapis_hip_block_select_entries": [_vp, ctypes.POINTER(_i64)],
+    "lapis_hip_block_select_work": [_vp, ctypes.POINTER(_i64)],
+    "lapis_hip_block_select": [_vp, _vp],
+    "lapis_hip_block_attention": [_vp, _vp],
+    "lapis_hip_block_attention_backward_work": [_vp, ctypes.POINTER(_i64)],
+    "lapis_hip_block_attention_backward": [_vp, _vp],
     "lapis_hip_pcg_f64_i32": [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _dbl, _u64, _vp,
                               ctypes.POINTER(_u64), ctypes.POINTER(_dbl), _vp, _vp],
 }
@@ -513,3 +524,57 @@ def normalize_mom2(mom1, mom2, out, stream=None):
 def bspmm_csrv(n1, n2, pos, crd, val, V, out, stream=None):
     """out(n1,dh,nh) += A(n1,n2,nh) * V(n2,dh,nh) with CSRV A (examples/bspmm.py)."""
     return _calls.bspmm_csrv(n1, n2, pos, crd, val, V, out, stream)
+
+
+# ---- block-sparse attention ----------------------------------------------------------------------------------
+# Tensors of bfloat16 or float16, with any strides between rows; structures are int32.  Outputs are written in place
+# and returned.
+
+def kv_store(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None, stream=None):
+    """New tokens' keys and values (tokens x heads x dim) into slots (page * page size + place) of a cache in pages
+    (pages x heads x page size x dim).  A float8_e4m3fn cache comes with scales (pages x heads x page size, float32):
+    each row is divided by its largest element / 448 and rounded.  Tokens whose slot is outside the cache are left out."""
+    return _calls.kv_store(k, v, slots, k_cache, v_cache, k_scale, v_scale, stream)
+
+
+def kv_load(k_cache, v_cache, slots, k, v, k_scale=None, v_scale=None, stream=None):
+    """The keys and values that slots of a cache hold, into ``k`` and ``v``; zeros where a slot is outside the cache."""
+    return _calls.kv_load(k_cache, v_cache, slots, k, v, k_scale, v_scale, stream)
+
+
+def paged_attention(q, k_cache, v_cache, pos, crd, tokens, out, lse=None, scale=None, k_scale=None, v_scale=None, stream=None):
+    """One new token of each sequence (q: sequences x heads x dim) against the pages its CSR row (pos, crd) lists:
+    ``tokens`` of them count.  One row per sequence, or one per sequence and key-value head.  ``scale`` defaults to
+    dim ** -0.5; ``lse`` (sequences x heads, float32) gets the logarithms of the softmax sums."""
+    return _calls.paged_attention(q, k_cache, v_cache, pos, crd, tokens, out, lse, scale, k_scale, v_scale, stream)
+
+
+def block_pool(x, block, codes, scales, stream=None):
+    """8-bit means of x (batch x tokens x heads x dim) over blocks of tokens and groups of heads: ``codes`` (batch x
+    groups x blocks x dim, int8) * ``scales`` (batch x groups x blocks, float32)."""
+    return _calls.block_pool(x, block, codes, scales, stream)
+
+
+def block_select(q_codes, k_codes, k_scales, count, pos, crd, queries, keys, block_m, block_n, causal=True, sink=0, local=1,
+                 table=None, blocks=None, stream=None):
+    """The ``count`` best blocks of keys of each block of queries, as a CSR structure written into ``pos`` and ``crd``
+    (ascending; ties to the lowest block).  q_codes: batch x heads x blocks of queries x dim, k_codes and k_scales
+    the same over blocks of keys, as ``block_pool`` leaves them.  The first ``sink`` and last ``local`` blocks that a row
+    may see are always among them.  Over a cache: k_codes are pages x heads x dim, ``table`` (batch x width, int32)
+    gives the page of each block of a sequence, which becomes the coordinate, and ``blocks`` (batch) how many it has."""
+    return _calls.block_select(q_codes, k_codes, k_scales, count, pos, crd, queries, keys, block_m, block_n, causal, sink, local,
+                               table, blocks, stream)
+
+
+def block_attention(q, k, v, pos, crd, out, lse=None, block_m=64, block_n=64, causal=True, scale=None, stream=None):
+    """softmax(scale q k^T) v over the blocks that a CSR structure lists, into ``out``; ``lse`` (batch x heads x queries,
+    float32) gets what the backward pass needs.  q: batch x queries x heads x dim; k, v: batch x keys x kv_heads x dim.
+    Row (batch, key-value head, block of ``block_m`` queries) lists blocks of ``block_n`` keys.  Causal: query i sees keys
+    up to i + keys - queries."""
+    return _calls.block_attention(q, k, v, pos, crd, out, lse, block_m, block_n, causal, scale, stream)
+
+
+def block_attention_backward(dout, q, k, v, out, lse, pos, crd, dq, dk, dv, block_m=64, block_n=64, causal=True, scale=None,
+                             stream=None):
+    """Gradients of ``block_attention`` from its inputs, its results and the gradient of ``out``."""
+    return _calls.block_attention_backward(dout, q, k, v, out, lse, pos, crd, dq, dk, dv, block_m, block_n, causal, scale, stream)

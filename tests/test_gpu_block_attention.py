@@ -1,0 +1,320 @@
+"""Block-sparse attention, forward and backward, against its formulas in 64 bits: sizes around the tiles, lists that are
+empty, unordered or point outside, masks that leave rows empty, strides, non-finite values where nothing is listed."""
+import math
+
+import pytest
+import torch
+
+import attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def make(batch, queries, keys, heads, kv_heads, dim, dtype, seed, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: (torch.randn(s, generator=g) * spread).to(dtype).cuda()  # noqa: E731
+    return r(batch, queries, heads, dim), r(batch, keys, kv_heads, dim), r(batch, keys, kv_heads, dim), r(batch, queries, heads, dim)
+
+
+def random_lists(lists, rows, columns, most, seed, empty=0.1, ordered=True):
+    g = torch.Generator().manual_seed(seed)
+    pos, crd = [0], []
+    for _ in range(lists * rows):
+        n = 0 if torch.rand(1, generator=g) < empty or columns == 0 else int(torch.randint(1, min(most, columns) + 1, (1,), generator=g))
+        c = torch.randperm(columns, generator=g)[:n]
+        crd += (c.sort().values if ordered else c).tolist()
+        pos.append(len(crd))
+    return torch.tensor(pos, dtype=torch.int32).cuda(), torch.tensor(crd, dtype=torch.int32).cuda()
+
+
+def run_forward(gpu, q, k, v, pos, crd, **sizes):
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((q.shape[0], q.shape[2], q.shape[1]), 7.0, device="cuda")
+    gpu.block_attention(q, k, v, pos, crd, out, lse, **sizes)
+    return out, lse
+
+
+def run_backward(gpu, dout, q, k, v, out, lse, pos, crd, **sizes):
+    grads = [torch.full(x.shape, 7.0, dtype=x.dtype, device="cuda") for x in (q, k, v)]
+    gpu.block_attention_backward(dout, q, k, v, out, lse, pos, crd, *grads, **sizes)
+    return grads
+
+
+def check(gpu, what, tensors, pos, crd, block_m, block_n, causal, scale=None, gradient=True):
+    q, k, v, dout = tensors
+    print("case", what, flush=True)
+    sizes = dict(block_m=block_m, block_n=block_n, causal=causal, scale=scale)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    w = ref.pair_weights(pos, crd, q.shape[0], k.shape[2], q.shape[1], k.shape[1], block_m, block_n, causal)
+    want, want_lse, bound, lse_bound = ref.forward(q, k, v, w, scale)
+    ref.assert_within(out, want, bound, what + ": out")
+    ref.assert_within(lse, want_lse, lse_bound, what + ": lse")
+    if gradient:
+        grads = run_backward(gpu, dout, q, k, v, out, lse, pos, crd, **sizes)
+        torch.cuda.synchronize()
+        wants, bounds = ref.backward(dout, q, k, v, out, lse, w, scale)
+        for name, g, x, y in zip(("dq", "dk", "dv"), grads, wants, bounds):
+            ref.assert_within(g, x, y, what + ": " + name)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("queries,keys,block_m,block_n,causal", [
+    (1, 1, 1, 16, True), (1, 300, 1, 32, True), (2, 65, 64, 64, False), (17, 17, 16, 16, True), (63, 64, 64, 64, True),
+    (65, 65, 64, 64, True), (127, 129, 128, 128, True), (200, 200, 37, 16, True), (130, 515, 50, 128, True),
+    (96, 500, 128, 256, False), (257, 100, 64, 32, False), (100, 60, 16, 16, True), (33, 1, 8, 16, False)])
+def test_sizes_around_the_tiles(gpu, dtype, queries, keys, block_m, block_n, causal):
+    # 100 queries and 60 keys, causal: the first 40 queries see no key
+    rows, columns = -(-queries // block_m), -(-keys // block_n)
+    t = make(2, queries, keys, 4, 2, 64, TYPES[dtype], queries + keys)
+    pos, crd = random_lists(4, rows, columns, 6, queries, empty=0.1)
+    check(gpu, "%s %d x %d, blocks %d x %d" % (dtype, queries, keys, block_m, block_n), t, pos, crd, block_m, block_n, causal)
+
+
+@pytest.mark.parametrize("dim", [8, 16, 24, 40, 64, 72, 80, 96, 104, 120, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_row_lengths(gpu, dim, dtype):
+    t = make(1, 70, 150, 2, 1, dim, TYPES[dtype], dim)
+    pos, crd = random_lists(1, 3, 5, 5, dim)
+    check(gpu, "dim %d %s" % (dim, dtype), t, pos, crd, 32, 32, True)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 3), (5, 1), (6, 2), (7, 1), (16, 1), (17, 1), (40, 2), (64, 1)])
+@pytest.mark.parametrize("block_m", [1, 5, 64])
+def test_groups_of_heads(gpu, heads, kv_heads, block_m):
+    t = make(1, 45, 90, heads, kv_heads, 32, torch.bfloat16, heads)
+    pos, crd = random_lists(kv_heads, -(-45 // block_m), 6, 4, heads + block_m)
+    check(gpu, "%d heads over %d, %d queries a row" % (heads, kv_heads, block_m), t, pos, crd, block_m, 16, True)
+
+
+@pytest.mark.parametrize("block_n", [16, 64, 256])
+def test_full_lists_equal_dense_attention(gpu, block_n):
+    t = make(1, 300, 300, 2, 2, 64, torch.bfloat16, 5)
+    rows, columns = 5, -(-300 // block_n)
+    pos = torch.arange(2 * rows + 1, dtype=torch.int32).cuda() * columns
+    crd = torch.arange(columns, dtype=torch.int32).repeat(2 * rows).cuda()
+    check(gpu, "all blocks of %d" % block_n, t, pos, crd, 64, block_n, True)
+
+
+def test_nothing_listed_at_all(gpu):
+    q, k, v, dout = make(1, 100, 100, 2, 1, 64, torch.bfloat16, 1)
+    pos, crd = torch.zeros(3, dtype=torch.int32).cuda(), torch.zeros(0, dtype=torch.int32).cuda()
+    check(gpu, "empty structure", (q, k, v, dout), pos, crd, 64, 64, True)
+
+
+def test_no_queries_and_no_keys(gpu):
+    for queries, keys in ((0, 50), (50, 0), (0, 0)):
+        q, k, v, dout = make(1, queries, keys, 2, 1, 64, torch.bfloat16, 1)
+        pos = torch.zeros(-(-queries // 16) + 1, dtype=torch.int32).cuda()
+        crd = torch.zeros(0, dtype=torch.int32).cuda()
+        out, lse = run_forward(gpu, q, k, v, pos, crd, block_m=16, block_n=16, causal=False)
+        grads = run_backward(gpu, dout, q, k, v, out, lse, pos, crd, block_m=16, block_n=16, causal=False)
+        torch.cuda.synchronize()
+        assert all(bool((x == 0).all()) for x in (out, *grads)) and bool((lse == -math.inf).all())
+
+
+def test_lists_out_of_order_twice_over_and_outside(gpu):
+    t = make(1, 96, 200, 2, 1, 64, torch.float16, 3)
+    # columns 0..6; the last one is cut at 200 keys
+    pos = torch.tensor([0, 5, 5, 11], dtype=torch.int32).cuda()
+    crd = torch.tensor([6, 0, 3, 0, -1, 2, 7, 1 << 30, -2147483648, 6, 2], dtype=torch.int32).cuda()
+    check(gpu, "disorder", t, pos, crd, 32, 32, False)
+
+
+def test_positions_that_make_no_sense_are_not_followed(gpu):
+    t = make(1, 96, 200, 2, 1, 64, torch.float16, 3)
+    pos = torch.tensor([-5, 2, 1, 1000], dtype=torch.int32).cuda()  # rows [0, 2), nothing, [1, 4)
+    crd = torch.tensor([0, 3, 5, 6], dtype=torch.int32).cuda()
+    check(gpu, "positions", t, pos, crd, 32, 32, False)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
+@pytest.mark.parametrize("block_n", [16, 64, 128])
+def test_what_no_query_attends_to_may_be_anything(gpu, bad, block_n):
+    """Keys and values of unlisted blocks, and of listed blocks past every query's position."""
+    queries = keys = 160
+    q, k, v, dout = make(1, queries, keys, 2, 1, 64, torch.bfloat16, 9)
+    rows, columns = 5, -(-keys // block_n)
+    rows_listed = [[c for c in range(columns) if c * block_n <= 32 * r + 31] for r in range(rows)]
+    pos = torch.tensor([0] + [sum(len(x) for x in rows_listed[:r + 1]) for r in range(rows)], dtype=torch.int32).cuda()
+    crd = torch.tensor(sum(rows_listed, []), dtype=torch.int32).cuda()
+    for at in (150, 159, 33):
+        bk, bv = k.clone(), v.clone()
+        bk[:, at:], bv[:, at:] = bad, bad
+        # queries from `at` on do see those keys: only the rows before are compared
+        out, _ = run_forward(gpu, q, bk, bv, pos, crd, block_m=32, block_n=block_n, causal=True)
+        clean, _ = run_forward(gpu, q, k, v, pos, crd, block_m=32, block_n=block_n, causal=True)
+        torch.cuda.synchronize()
+        w = ref.pair_weights(pos, crd, 1, 1, queries, keys, 32, block_n, True)
+        want, _, bound, _ = ref.forward(q, k, v, w, 64 ** -0.5)
+        ref.assert_within(out[:, :at], want[:, :at], bound[:, :at], "rows before %d, %r" % (at, bad))
+        ref.assert_within(clean, want, bound, "clean rows")
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_gradients_beside_values_that_nothing_attends_to(gpu, bad):
+    """Keys past the last query's position and queries in front of the first key hold anything; their rows take no part."""
+    q, k, v, dout = make(1, 90, 90, 2, 1, 64, torch.bfloat16, 4)
+    pos, crd = torch.tensor([0, 1, 3, 6], dtype=torch.int32).cuda(), torch.tensor([0, 0, 1, 0, 1, 2], dtype=torch.int32).cuda()
+    sizes = dict(block_m=32, block_n=32, causal=True)
+    # keys 70.. are seen by queries 70.. only; their dout is zero and they are left out of the comparison
+    w = ref.pair_weights(pos, crd, 1, 1, 90, 90, 32, 32, True)
+    w[:, :, 70:] = 0
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    bk, bv, bq, bd = k.clone(), v.clone(), q.clone(), dout.clone()
+    for x in (bk, bv, bq, bd):
+        x[:, 70:] = bad
+    bo, bl = out.clone(), lse.clone()
+    bo[:, 70:], bl[:, :, 70:] = bad, bad
+    dq, dk, dv = run_backward(gpu, bd, bq, bk, bv, bo, bl, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    lse2, out2, dout2 = lse.clone(), out.clone(), dout.clone()
+    wants, bounds = ref.backward(dout2, q, k, v, out2, lse2, w, 64 ** -0.5)
+    ref.assert_within(dq[:, :70], wants[0][:, :70], bounds[0][:, :70], "dq before the bad keys")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_large_scores_and_scales(gpu, dtype):
+    t = make(1, 64, 256, 2, 2, 64, TYPES[dtype], 8, spread=4.0)
+    pos, crd = random_lists(2, 2, 4, 4, 2, empty=0.0)
+    check(gpu, "scores of hundreds", t, pos, crd, 32, 64, False, scale=1.0)
+    check(gpu, "negative scale", t, pos, crd, 32, 64, False, scale=-0.25)
+    check(gpu, "scale 0", t, pos, crd, 32, 64, False, scale=0.0)
+
+
+def test_scores_of_minus_infinity(gpu):
+    q, k, v, _ = make(1, 32, 64, 1, 1, 64, torch.float16, 2)
+    q[:, :, :, 0], k[:, :32, :, 0] = 60000.0, -math.inf
+    pos, crd = torch.tensor([0, 2], dtype=torch.int32).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda()
+    k[:, 32:, :, 0] = 0.0
+    out, _ = run_forward(gpu, q, k, v, pos, crd, block_m=32, block_n=32, causal=False)
+    only, _ = run_forward(gpu, q, k[:, 32:], v[:, 32:], torch.tensor([0, 1], dtype=torch.int32).cuda(),
+                          torch.zeros(1, dtype=torch.int32).cuda(), block_m=32, block_n=32, causal=False)
+    torch.cuda.synchronize()
+    assert torch.equal(out, only)
+
+
+def test_strides_of_slices_permuted_and_broadcast_operands(gpu):
+    g = torch.Generator().manual_seed(6)
+    packed = torch.randn((2, 130, 4 + 2 + 2, 64), generator=g).to(torch.bfloat16).cuda()
+    q, k, v = packed[:, :, :4], packed[:, :, 4:6], packed[:, :, 6:]
+    dout = torch.randn((2, 4, 130, 64), generator=g).to(torch.bfloat16).cuda().transpose(1, 2)
+    pos, crd = random_lists(4, 3, 5, 5, 3)
+    check(gpu, "slices", (q, k, v, dout), pos, crd, 64, 32, True)
+    k1 = torch.randn((1, 130, 1, 64), generator=g).to(torch.bfloat16).cuda().expand(2, 130, 2, 64)
+    check(gpu, "broadcast keys and values", (q, k1, k1, dout), pos, crd, 64, 32, True)
+    # outputs as slices of a larger tensor leave the rest of it alone
+    big = torch.full((2, 130, 9, 72), 3.0, dtype=torch.bfloat16, device="cuda")
+    out = big[:, :, 2:6, :64]
+    lse = torch.empty((2, 4, 130), device="cuda")
+    gpu.block_attention(q, k, v, pos, crd, out, lse, block_m=64, block_n=32)
+    plain, _ = run_forward(gpu, q, k, v, pos, crd, block_m=64, block_n=32, causal=True)
+    torch.cuda.synchronize()
+    assert torch.equal(out, plain)
+    out.fill_(3.0)
+    assert bool((big == 3.0).all())
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """Keys and values 2^31 elements apart: views into one large buffer."""
+    stride = 1 << 24
+    big = torch.empty(160 << 24, dtype=torch.bfloat16, device="cuda")
+    q, k, v, dout = make(1, 40, 160, 2, 1, 64, torch.bfloat16, 12)
+    far_k = torch.as_strided(big, (1, 160, 1, 64), (0, stride, 0, 1), 0)
+    far_v = torch.as_strided(big, (1, 160, 1, 64), (0, stride, 0, 1), 64)
+    far_k.copy_(k)
+    far_v.copy_(v)
+    assert stride * 159 > 1 << 31
+    pos, crd = torch.tensor([0, 5, 10], dtype=torch.int32).cuda(), torch.tensor([0, 1, 2, 3, 4] * 2, dtype=torch.int32).cuda()
+    check(gpu, "far apart", (q, far_k, far_v, dout), pos, crd, 32, 32, True)
+
+
+def test_the_same_bits_again_and_on_another_stream(gpu):
+    q, k, v, dout = make(2, 500, 500, 8, 2, 128, torch.bfloat16, 21)
+    pos, crd = random_lists(4, 8, 8, 8, 7)
+    sizes = dict(block_m=64, block_n=64, causal=True)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    grads = run_backward(gpu, dout, q, k, v, out, lse, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for stream in (None, side, side.cuda_stream):
+        for _ in range(3):
+            again = [torch.empty_like(x) for x in (out, lse, *grads)]
+            gpu.block_attention(q, k, v, pos, crd, *again[:2], stream=stream, **sizes)
+            gpu.block_attention_backward(dout, q, k, v, *again[:2], pos, crd, *again[2:], stream=stream, **sizes)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(again, (out, lse, *grads)))
+
+
+def test_a_captured_graph_repeats(gpu):
+    q, k, v, dout = make(1, 300, 300, 4, 2, 64, torch.float16, 31)
+    pos, crd = random_lists(2, 5, 5, 4, 8)
+    sizes = dict(block_m=64, block_n=64, causal=True)
+    want = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    want += tuple(run_backward(gpu, dout, q, k, v, *want, pos, crd, **sizes))
+    got = [torch.empty_like(x) for x in want]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.block_attention(q, k, v, pos, crd, *got[:2], **sizes)
+        gpu.block_attention_backward(dout, q, k, v, *got[:2], pos, crd, *got[2:], **sizes)
+    for _ in range(4):
+        for x in got:
+            x.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_gradients_against_differences(gpu, which):
+    """The formula's gradient in 64 bits, to which the kernels are held above, against central differences of the forward
+    formula: both sides on the CPU."""
+    g = torch.Generator().manual_seed(which)
+    q, k, v, dout = (torch.randn(s, generator=g).double() for s in ((1, 9, 4, 8), (1, 12, 2, 8), (1, 12, 2, 8), (1, 9, 4, 8)))
+    w = (torch.rand((1, 2, 9, 12), generator=g) < 0.5).double()
+    w[:, :, 3] = 0
+
+    def loss(*x):
+        s = ref._heads_first(x[0]) @ ref._expand(ref._heads_first(x[1]), 2).transpose(2, 3) * 0.3
+        p = ref._expand(w, 2) * torch.exp(s)
+        total = p.sum(-1, keepdim=True)
+        o = (p / torch.where(total == 0, 1.0, total)) @ ref._expand(ref._heads_first(x[2]), 2)
+        return (o.transpose(1, 2) * dout).sum(), o.transpose(1, 2), torch.where(total == 0, -math.inf, torch.log(total))[..., 0]
+
+    _, out, lse = loss(q, k, v)
+    ref.HALF_ULP[torch.float64], ref.TINY[torch.float64] = 0.0, 0.0
+    grads, _ = ref.backward(dout, q, k, v, out, lse, w, 0.3)
+    x = [q, k, v]
+    h = 1e-5
+    for index in range(0, x[which].numel(), 7):
+        sides = []
+        for sign in (1, -1):
+            moved = [t.clone() for t in x]
+            moved[which].view(-1)[index] += sign * h
+            sides.append(loss(*moved)[0])
+        slope = float((sides[0] - sides[1]) / (2 * h))
+        assert abs(slope - float(grads[which].reshape(-1)[index])) <= 1e-7 * (1 + abs(slope))
+
+
+def test_the_c_entries_refuse(gpu):
+    q, k, v, dout = make(1, 32, 32, 2, 1, 64, torch.bfloat16, 1)
+    pos, crd = torch.tensor([0, 1], dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    out, lse = torch.empty_like(q), torch.empty((1, 2, 32), device="cuda")
+    for bn in (8, 24, 512):
+        with pytest.raises(gpu.LapisHipError, match="INVALID_ARGUMENT"):
+            gpu.block_attention(q, k, v, torch.tensor([0, 1], dtype=torch.int32).cuda(), crd, out, lse, block_m=32, block_n=bn)
+    q4, k4 = q[..., :60], k[..., :60]
+    with pytest.raises(gpu.LapisHipError, match="multiple of 8"):
+        gpu.block_attention(q4, k4, k4, pos, crd, torch.empty((1, 32, 2, 60), dtype=q.dtype, device="cuda"), lse, block_m=32, block_n=32)
+    big = torch.empty((1, 32, 2, 136), dtype=q.dtype, device="cuda")
+    with pytest.raises(gpu.LapisHipError, match="up to 128"):
+        gpu.block_attention(big, big[:, :, :1], big[:, :, :1], pos, crd, torch.empty_like(big), lse, block_m=32, block_n=32)
+    flat = torch.empty(1 * 32 * 2 * 64 + 1, dtype=q.dtype, device="cuda")[1:].view(1, 32, 2, 64)
+    with pytest.raises(gpu.LapisHipError, match="16-byte"):
+        gpu.block_attention(flat, k, v, pos, crd, out, lse, block_m=32, block_n=32)
+    odd = torch.empty((1, 32, 2, 65), dtype=q.dtype, device="cuda")[..., :64]
+    with pytest.raises(gpu.LapisHipError, match="multiples of 8"):
+        gpu.block_attention(odd, k, v, pos, crd, out, lse, block_m=32, block_n=32)

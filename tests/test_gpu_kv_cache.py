@@ -1,0 +1,292 @@
+"""The paged cache: storing with and without 8-bit codes, loading, and attention of one token over its pages."""
+import math
+
+import pytest
+import torch
+
+import attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f8": torch.float8_e4m3fn}
+
+
+def empty_cache(pages, heads, page, dim, dtype, token_major=False):
+    shape = (pages, page, heads, dim) if token_major else (pages, heads, page, dim)
+    make = lambda: torch.full(shape, math.nan, device="cuda").to(dtype)  # noqa: E731
+    k, v = make(), make()
+    ks = vs = None
+    if dtype == TYPES["f8"]:
+        ks, vs = (torch.full(shape[:3], math.nan, device="cuda") for _ in range(2))
+    if token_major:
+        k, v = k.transpose(1, 2), v.transpose(1, 2)
+        ks, vs = (None if s is None else s.transpose(1, 2) for s in (ks, vs))
+    return k, v, ks, vs
+
+
+def read(cache, scale):
+    x = cache.cpu().double()
+    return x if scale is None else x * scale.cpu().double()[..., None]
+
+
+@pytest.mark.parametrize("token_major", [False, True], ids=["heads first", "slots first"])
+@pytest.mark.parametrize("cache", ["f8", "same"])
+@pytest.mark.parametrize("tokens,heads,dim,page,dtype", [
+    (1, 1, 8, 1, "bf16"), (1, 8, 128, 64, "bf16"), (7, 3, 72, 16, "f16"), (130, 2, 64, 32, "bf16"), (33, 5, 256, 8, "f16"),
+    (300, 4, 200, 128, "bf16"), (65, 1, 136, 1024, "f16")])
+def test_store_and_load(gpu, tokens, heads, dim, page, dtype, cache, token_major):
+    g = torch.Generator().manual_seed(tokens)
+    dt = TYPES[dtype]
+    pages = -(-tokens // page) + 2
+    k, v = ((torch.randn((tokens, heads, dim), generator=g) * 5).to(dt) for _ in range(2))
+    k[0, 0] = 0.0
+    v[-1, -1, 0] = 1000.0
+    slots = torch.randperm(pages * page, generator=g)[:tokens].to(torch.int32)
+    if tokens > 4:
+        slots[2], slots[3] = -1, pages * page
+    print("case", tokens, heads, dim, page, dtype, cache, flush=True)
+    kc, vc, ks, vs = empty_cache(pages, heads, page, dim, TYPES["f8"] if cache == "f8" else dt, token_major)
+    gpu.kv_store(k.cuda(), v.cuda(), slots.cuda(), kc, vc, ks, vs)
+    torch.cuda.synchronize()
+    live = (slots >= 0) & (slots < pages * page)
+    where = slots[live].long()
+    untouched = torch.ones(pages * page, dtype=torch.bool)
+    untouched[where] = False
+    flat = lambda t: t.cpu().transpose(1, 2).reshape(pages * page, *t.shape[1:2], *t.shape[3:])  # noqa: E731
+    for x, c, s in ((k, kc, ks), (v, vc, vs)):
+        got = flat(c.float())
+        assert bool(torch.isnan(got[untouched]).all())
+        if cache == "same":
+            assert torch.equal(got[where], x[live].float())
+            continue
+        scale = x[live].float().abs().amax(-1) / 448.0
+        assert torch.equal(flat(s)[where], scale)
+        assert bool(torch.isnan(flat(s)[untouched]).all())
+        codes = torch.where(scale[..., None] > 0, x[live].float() / scale[..., None], torch.zeros(())).to(TYPES["f8"])
+        assert torch.equal(got[where], codes.float())
+        # and against the value itself: half a step of three stored bits, or of the smallest step 2^-9
+        err = (got[where].double() * scale.double()[..., None] - x[live].double()).abs()
+        assert bool((err <= torch.maximum(2.0 ** -4 * x[live].double().abs(), 2.0 ** -10 * scale.double()[..., None]) * (1 + 1e-5)).all())
+    ko, vo = (torch.full((tokens, heads, dim), 7.0, dtype=dt, device="cuda") for _ in range(2))
+    gpu.kv_load(kc, vc, slots.cuda(), ko, vo, ks, vs)
+    torch.cuda.synchronize()
+    for o, c, s in ((ko, kc, ks), (vo, vc, vs)):
+        want = torch.zeros((tokens, heads, dim), dtype=dt)
+        want[live] = (flat(c.float())[where] * (1.0 if s is None else flat(s)[where][..., None])).to(dt)
+        assert torch.equal(o.cpu(), want)
+
+
+def test_values_that_are_not_finite(gpu):
+    x = torch.ones((4, 1, 16), dtype=torch.bfloat16)
+    x[0, 0, 3] = math.nan
+    x[1, 0, 5] = math.inf
+    x[2] = math.nan
+    x[3] *= 1e-38
+    kc, vc, ks, vs = empty_cache(1, 1, 4, 16, TYPES["f8"])
+    slots = torch.arange(4, dtype=torch.int32).cuda()
+    gpu.kv_store(x.cuda(), x.cuda(), slots, kc, vc, ks, vs)
+    out, _ = gpu.kv_load(kc, vc, slots, torch.empty_like(x, device="cuda"), torch.empty_like(x, device="cuda"), ks, vs)
+    got = out.cpu().float()
+    others = torch.arange(16) != 3
+    assert math.isnan(got[0, 0, 3]) and bool((got[0, 0, others] == 1.0).all())
+    assert bool(torch.isnan(got[1]).all()) and bool(torch.isnan(got[2]).all())
+    assert bool(((got[3] - x[3].float()).abs() <= 2.0 ** -7 * 1e-38).all())
+
+
+def test_rows_as_slices_of_a_projection(gpu):
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn((50, 4 + 2 + 2, 64), generator=g).to(torch.bfloat16).cuda()
+    kc, vc, _, _ = empty_cache(2, 2, 32, 64, torch.bfloat16)
+    slots = torch.arange(50, dtype=torch.int32).cuda()
+    gpu.kv_store(qkv[:, 4:6], qkv[:, 6:], slots, kc, vc)
+    out = torch.zeros_like(qkv)
+    gpu.kv_load(kc, vc, slots, out[:, 4:6], out[:, 6:])
+    torch.cuda.synchronize()
+    assert torch.equal(out[:, 4:], qkv[:, 4:]) and bool((out[:, :4] == 0).all())
+
+
+# ---- attention over the cache --------------------------------------------------------------------------------
+
+def paged_case(seqs, lengths, heads, kv_heads, dim, page, dtype, cache, each, seed, token_major=False):
+    """A cache filled through kv_store, page lists in random order, NaN in every slot that holds no token."""
+    from lapis_amd import hip
+    g = torch.Generator().manual_seed(seed)
+    held = [-(-n // page) for n in lengths]
+    pages = sum(held) + 3
+    kc, vc, ks, vs = empty_cache(pages, kv_heads, page, dim, TYPES["f8"] if cache == "f8" else dtype, token_major)
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    at, tables, slots = 0, [], []
+    for n, h in zip(lengths, held):
+        tables.append(order[at:at + h])
+        t = torch.arange(n)
+        slots.append(order[at:at + h][t // page].long() * page + t % page if n else torch.zeros(0, dtype=torch.int64))
+        at += h
+    slots = torch.cat(slots).to(torch.int32).cuda()
+    k, v = (torch.randn((slots.numel(), kv_heads, dim), generator=g).to(dtype).cuda() for _ in range(2))
+    hip.kv_store(k, v, slots, kc, vc, ks, vs)
+    q = torch.randn((seqs, heads, dim), generator=g).to(dtype).cuda()
+    lists, tokens = [], []
+    for n, table in zip(lengths, tables):
+        for _ in range(kv_heads if each else 1):
+            if each and len(table) > 2:  # some pages and the last one
+                keep = torch.rand(len(table), generator=g) < 0.5
+                keep[-1] = True
+                lists.append(table[keep])
+                tokens.append(n - int((~keep).sum()) * page)
+            else:
+                lists.append(table)
+                tokens.append(n)
+    pos = torch.tensor([0] + [sum(len(x) for x in lists[:i + 1]) for i in range(len(lists))], dtype=torch.int32).cuda()
+    crd = torch.cat(lists).to(torch.int32).cuda()
+    return q, kc, vc, pos, crd, torch.tensor(tokens, dtype=torch.int32).cuda(), ks, vs
+
+
+def paged_reference(q, kc, vc, pos, crd, tokens, ks, vs, scale):
+    seqs, heads, dim = q.shape
+    kv_heads, page = kc.shape[1], kc.shape[2]
+    group = heads // kv_heads
+    K, V = read(kc, ks), read(vc, vs)
+    out, lse, bound, lse_bound = (torch.zeros((seqs, heads, dim), dtype=torch.float64), torch.full((seqs, heads), -math.inf, dtype=torch.float64),
+                                  torch.zeros((seqs, heads, dim), dtype=torch.float64), torch.zeros((seqs, heads), dtype=torch.float64))
+    p, c, t = pos.clamp(0, crd.numel()).tolist(), crd.cpu().long(), tokens.tolist()
+    u, tiny = ref.HALF_ULP[q.dtype], ref.TINY[q.dtype]
+    each = len(t) != seqs
+    Q = q.cpu().double()
+    for s in range(seqs):
+        for h in range(heads):
+            kh = h // group
+            row = s * kv_heads + kh if each else s
+            pages = c[p[row]:p[row + 1]]
+            there = ((pages >= 0) & (pages < kc.shape[0])).repeat_interleave(page)[:max(0, t[row])]
+            pages = pages.clamp(0, kc.shape[0] - 1)
+            kk, vv = (x[pages, kh].reshape(-1, dim)[:max(0, t[row])][there] for x in (K, V))
+            if kk.shape[0] == 0:
+                continue
+            score = scale * (kk @ Q[s, h])
+            weight = torch.softmax(score, 0)
+            ds = float((dim * 2.0 ** -23 * abs(scale) * (kk.abs() @ Q[s, h].abs())).max())
+            out[s, h] = weight @ vv
+            lse[s, h] = torch.logsumexp(score, 0)
+            # 8-bit codes are multiplied as they are, their scales go into the weights before these are rounded
+            bound[s, h] = u * out[s, h].abs() + (weight @ vv.abs()) * (u + 2 * ds + 2.0 ** -18) + tiny * vv.abs().sum(0)
+            lse_bound[s, h] = 2 * ds + 2.0 ** -18 + u / 4 + 2.0 ** -22 * lse[s, h].abs()
+    return out, lse, bound, lse_bound
+
+
+def check_paged(gpu, what, case, scale=None):
+    q, kc, vc, pos, crd, tokens, ks, vs = case
+    print("case", what, flush=True)
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    gpu.paged_attention(q, kc, vc, pos, crd, tokens, out, lse=lse, scale=scale, k_scale=ks, v_scale=vs)
+    torch.cuda.synchronize()
+    want, want_lse, bound, lse_bound = paged_reference(*case[:6], ks, vs, q.shape[2] ** -0.5 if scale is None else scale)
+    ref.assert_within(out, want, bound, what + ": out")
+    ref.assert_within(lse, want_lse, lse_bound, what + ": lse")
+    return out
+
+
+@pytest.mark.parametrize("cache", ["f8", "same"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [
+    ([1], 1, 1, 64, 64), ([0], 4, 2, 64, 16), ([17, 0, 16, 15, 1], 4, 4, 64, 16), ([300], 8, 1, 128, 32), ([64, 65, 63], 6, 2, 72, 64),
+    ([1000, 3, 129], 16, 2, 96, 128), ([257], 7, 1, 80, 8), ([200, 31], 32, 2, 40, 1), ([1500], 5, 5, 8, 16), ([700, 900], 12, 4, 256, 64),
+    ([513], 34, 2, 136, 256), ([2000], 3, 1, 200, 1024)])
+def test_paged_attention(gpu, lengths, heads, kv_heads, dim, page, dtype, cache):
+    case = paged_case(len(lengths), lengths, heads, kv_heads, dim, page, TYPES[dtype], cache, False, dim)
+    check_paged(gpu, "%s, %d heads over %d, %d x %d, %s %s" % (lengths, heads, kv_heads, page, dim, dtype, cache), case)
+
+
+@pytest.mark.parametrize("cache", ["f8", "same"])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_a_list_for_each_head(gpu, cache, token_major):
+    case = paged_case(3, [700, 5, 333], 12, 4, 64, 32, torch.bfloat16, cache, True, 3, token_major)
+    check_paged(gpu, "lists of each head", case)
+
+
+@pytest.mark.parametrize("cache", ["f8", "same"])
+def test_a_long_sequence_beside_short_ones(gpu, cache):
+    case = paged_case(5, [40000, 1, 70, 0, 9000], 8, 2, 128, 64, torch.bfloat16, cache, False, 3)
+    out = check_paged(gpu, "40000 tokens", case)
+    for _ in range(3):
+        again = torch.empty_like(out)
+        gpu.paged_attention(*case[:6], again, k_scale=case[6], v_scale=case[7])
+        assert torch.equal(out, again)
+
+
+def test_tokens_and_lists_that_disagree(gpu):
+    q, kc, vc, pos, crd, tokens, ks, vs = paged_case(3, [100, 100, 100], 4, 2, 64, 16, torch.bfloat16, "same", False, 8)
+    for slots in (kc, vc):
+        slots.copy_(torch.nan_to_num(slots, nan=0.5))
+    crd[3], crd[9] = -7, 1 << 29                                        # pages that do not exist are absent
+    tokens = torch.tensor([1000, -4, 50], dtype=torch.int32).cuda()     # more than listed, fewer than none, fewer than listed
+    check_paged(gpu, "disagreement", (q, kc, vc, pos, crd, tokens, ks, vs))
+    pos = torch.tensor([-3, 5, 2, 1 << 30], dtype=torch.int32).cuda()
+    check_paged(gpu, "positions", (q, kc, vc, pos, crd, torch.full((3,), 90, dtype=torch.int32).cuda(), ks, vs))
+
+
+def test_scores_of_hundreds_and_scales(gpu):
+    case = list(paged_case(2, [300, 40], 4, 2, 64, 16, torch.float16, "same", False, 8))
+    case[0] = case[0] * 12
+    check_paged(gpu, "large scores", case, scale=1.0)
+    check_paged(gpu, "scale 0", case, scale=0.0)
+
+
+def test_a_cache_beyond_32_bits(gpu):
+    """Pages 2^31 and more elements into the cache."""
+    pages, page, dim = 9000, 64, 256
+    kc = torch.empty((pages, 16, page, dim), dtype=torch.bfloat16, device="cuda")
+    assert kc.numel() > 1 << 31
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn((130, 16, dim), generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    slots = torch.cat([torch.arange(64) + 64 * 8999, torch.arange(64) + 64 * 8500, torch.arange(2) + 64 * 3]).to(torch.int32).cuda()
+    vc = torch.empty_like(kc)
+    gpu.kv_store(k, v, slots, kc, vc)
+    q = torch.randn((1, 16, dim), generator=g).to(torch.bfloat16).cuda()
+    pos, crd = torch.tensor([0, 3], dtype=torch.int32).cuda(), torch.tensor([8999, 8500, 3], dtype=torch.int32).cuda()
+    out, lse = torch.empty_like(q), torch.empty((1, 16), device="cuda")
+    gpu.paged_attention(q, kc, vc, pos, crd, torch.tensor([130], dtype=torch.int32).cuda(), out, lse=lse)
+    ko, vo = gpu.kv_load(kc, vc, slots, torch.empty_like(k), torch.empty_like(v))
+    torch.cuda.synchronize()
+    assert torch.equal(ko, k) and torch.equal(vo, v)
+    small = [x.transpose(0, 1)[None].reshape(1, 16, 130, dim) for x in (k, v)]
+    padded = [torch.nn.functional.pad(x, (0, 0, 0, 1024 - 130)) for x in small]
+    want = paged_reference(q, *padded, torch.tensor([0, 1]), torch.tensor([0]), torch.tensor([130]), None, None, dim ** -0.5)
+    ref.assert_within(out, want[0], want[2], "far pages: out")
+    ref.assert_within(lse, want[1], want[3], "far pages: lse")
+
+
+def test_another_stream_and_a_captured_graph(gpu):
+    q, kc, vc, pos, crd, tokens, ks, vs = case = paged_case(4, [3000, 10, 0, 900], 8, 2, 128, 64, torch.bfloat16, "f8", False, 5)
+    want = check_paged(gpu, "plain", case)
+    side = torch.cuda.Stream()
+    out = torch.empty_like(q)
+    gpu.paged_attention(q, kc, vc, pos, crd, tokens, out, k_scale=ks, v_scale=vs, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.paged_attention(q, kc, vc, pos, crd, tokens, out, k_scale=ks, v_scale=vs)
+    for _ in range(4):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        eager = torch.empty_like(out)
+        gpu.paged_attention(q, kc, vc, pos, crd, tokens, eager, k_scale=ks, v_scale=vs)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want)
+
+
+def test_the_c_entries_refuse(gpu):
+    k = torch.zeros((4, 1, 64), dtype=torch.bfloat16, device="cuda")
+    slots = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for pages, page, dim in ((1, 24, 64), (1, 2048, 64), (1, 16, 264), (1, 16, 12)):
+        kc, vc, _, _ = empty_cache(pages, 1, page, dim, torch.bfloat16)
+        x = torch.zeros((4, 1, dim), dtype=torch.bfloat16, device="cuda")
+        with pytest.raises(gpu.LapisHipError, match="INVALID_ARGUMENT"):
+            gpu.kv_store(x, x, slots, kc, vc)
+    flat = torch.empty(4 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 1, 64)
+    kc, vc, _, _ = empty_cache(1, 1, 16, 64, torch.bfloat16)
+    with pytest.raises(gpu.LapisHipError, match="16-byte"):
+        gpu.kv_store(flat, k, slots, kc, vc)
