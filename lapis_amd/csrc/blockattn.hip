@@ -1,61 +1,209 @@
 // Attention over the blocks that a CSR structure lists, forward.
 #include "blockattn.hpp"
+#include "mfma.hpp"
 
 namespace lapis {
 namespace {
 
-// One wavefront per query and head: a key per lane for the scores, elements of the row per lane for the sum.
-template <typename T>
-__global__ __launch_bounds__(64) void block_simple_kernel(BlockArgs a) {
+constexpr int kAbsent = 0x7fff0000;  // first key of sixteen that do not exist
+
+// Keys of a list in the order of its entries, sixteen at a time: blocks hold at least sixteen, so sixteen neighbouring
+// places of the list are sixteen neighbouring keys.
+__device__ __forceinline__ int first_key(const BlockArgs &a, int first, int count, int place) {
+  const int e = place >> a.block_n_log2;
+  if (e >= count) return kAbsent;
+  const int block = a.crd[first + e];
+  return (unsigned)block < (unsigned)a.columns ? (block << a.block_n_log2) + (place & ((1 << a.block_n_log2) - 1)) : kAbsent;
+}
+
+// Rows of a list are its queries times the heads of the group, heads first: row i is query i / group, head i % group.
+//
+// A workgroup takes 32 * NW rows of one list, a wavefront 32 of them.  Tiles of KT keys go through LDS (two buffers: the
+// next tile is loaded into registers while one is computed, and written before the barrier that ends it).
+// S^T = K Q^T has a query per lane, so maxima, sums and factors of the softmax are one register and need one exchange
+// between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
+template <typename T, int DP, int NW, int KT>
+__global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
-  const int lane = threadIdx.x, i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, kh = h / a.group;
-  __shared__ float q[kMaxBlockDim], weight[64];
-  const elem *qp = (const elem *)a.q.data + b * a.q.stride[0] + i * a.q.stride[1] + h * a.q.stride[2];
+  constexpr int PIECES = DP / 8, RP = NW * 64 / PIECES, PASSES = KT / RP, ST = KT / 32, DT = DP / 32, CH = KT / 16;
+  __shared__ __attribute__((aligned(16))) elem k_tile[2][KT * DP], v_tile[2][KT * DP];
+  __shared__ int bad_tile[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
+  const int list = block / tiles_of_list, part = block - list * tiles_of_list;
+  const int bh = list / a.rows, r = list - bh * a.rows, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
+  const int q0 = r * a.block_m, held = min(a.block_m, a.queries - q0), rows = held * a.group;
+  if (part * 32 * NW >= rows) return;  // the last block of queries is cut
+  int first, count;
+  entries_of(a, list, &first, &count);
+
+  const int row0 = part * 32 * NW + wave * 32, row = row0 + (lane & 31);
+  const bool live = row < rows;
+  const int query = q0 + row / a.group, head = kh * a.group + row % a.group;
+  const int limit = a.causal ? min(query + a.shift, a.keys - 1) : a.keys - 1;  // last key this row sees
+  const int row_last = min(row0 + 31, rows - 1);
+  const int low = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row0 / a.group + a.shift, a.keys - 1) : a.keys - 1);
+  const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
+  const int low_of_all = a.causal ? min(q0 + part * 32 * NW / a.group + a.shift, a.keys - 1) : a.keys - 1;
+
+  vec8<T> qf[DP / 16];
+  const elem *qp = (const elem *)a.q.data + b * a.q.stride[0] + query * a.q.stride[1] + head * a.q.stride[2];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int d = 16 * s + 8 * half;
+    v4i x = {0, 0, 0, 0};
+    if (live && d < a.dim) x = *(const v4i *)(qp + d);
+    qf[s] = __builtin_bit_cast(vec8<T>, x ^ flip);
+  }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  for (int d = lane; d < a.dim; d += 64) q[d] = (float)qp[d] * a.scale;
-  int first, count;
-  entries_of(a, ((long long)b * a.kv_heads + kh) * a.rows + i / a.block_m, &first, &count);
-  float m = -INFINITY, l = 0.f, acc[kMaxBlockDim / 64] = {};
+
+  const int tiles = a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + KT - 1) / KT) : 0;
+  const int place = tid % PIECES, my_row = tid / PIECES;
+  int next[CH], now[CH];
+  // Tile t on its way into buffer t & 1.  A key that is not there is read from the last one: its scores become -infinity,
+  // and a value that is no number is looked for below wherever a mask cuts.
+  const auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) next[i] = first_key(a, first, count, t * KT + 16 * i);
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int at = p * RP + my_row;
+      const int key0 = RP <= 16 ? next[p * RP / 16] : my_row < 16 ? next[p * RP / 16] : next[p * RP / 16 + (RP > 16)];
+      const long long key = min(key0 + (at & 15), a.keys - 1);
+      const unsigned to = __builtin_amdgcn_readfirstlane((p * NW + wave) * 1024);
+      const int kd = (place ^ row_turn<DP>(at)) * 8, vd = (place ^ column_turn<DP>(at)) * 8;
+      if (kd < a.dim) load_to_lds(kp + key * a.k.stride[1] + kd, lds_address(k_tile[t & 1]) + to);
+      if (vd < a.dim) load_to_lds(vp + key * a.v.stride[1] + vd, lds_address(v_tile[t & 1]) + to);
+    }
+  };
+
+  v16f acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = v16f{};
+  const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);  // scores in units of ln 2; never 0: masked ones are -inf
+  float m = -INFINITY, l = 0.f;  // of this row; l of this half's keys
+
+  if (tid < 2) bad_tile[tid] = 0;
+  if (a.dim < DP) {  // what no row fills stays zero
+    for (int i = tid; i < 2 * KT * PIECES; i += 64 * NW) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
+    __syncthreads();
+  }
+  if (tiles > 0) load(0);
+  lds_loads_done();
   __syncthreads();
-  const int block_n = 1 << a.block_n_log2;
-  for (int e = 0; e < count; ++e) {
-    const int block = a.crd[first + e];
-    if (block < 0 || block >= a.columns) continue;
-    for (int n0 = 0; n0 < block_n; n0 += 64) {
-      const int key = (block << a.block_n_log2) + n0 + lane;
-      float score = -INFINITY;
-      const bool live = n0 + lane < block_n && key < a.keys && (!a.causal || key <= i + a.shift);
-      if (live) {
-        score = 0.f;
-        for (int d = 0; d < a.dim; d += 8) {
-          float f[8];
-          widen<T>(*(const vec8<T> *)(kp + key * a.k.stride[1] + d), f);
-          for (int x = 0; x < 8; ++x) score += q[d + x] * f[x];
+  for (int t = 0; t < tiles; ++t) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) now[i] = next[i];
+    if (t + 1 < tiles) load(t + 1);
+    int lowest = now[0], top = now[0];
+#pragma unroll
+    for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
+    if (top + 15 > low_of_all) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
+      bool bad = false;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(v_tile[t & 1] + (p * NW * 64 + tid) * 8));
+      if (__any(bad) && lane == 0) bad_tile[t & 1] = t + 1;
+      __syncthreads();
+    }
+    if (lowest <= high) {
+      const elem *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+      v16f s[ST];
+#pragma unroll
+      for (int x = 0; x < ST; ++x) {
+        s[x] = v16f{};
+#pragma unroll
+        for (int y = 0; y < DP / 16; ++y) {
+          const vec8<T> kf = *(const vec8<T> *)(kt + by_row<DP>(32 * x + (lane & 31), 2 * y + half));
+          s[x] = mfma32(kf, qf[y], s[x]);
         }
       }
-      float top = score;
-      for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-      const float m_new = fmaxf(m, top), keep = m == m_new ? 1.f : expf(m - m_new);
-      const float p = !live || score == -INFINITY ? 0.f : expf(score - m_new);
-      l = l * keep + group_sum<64>(p);
-      m = m_new;
-      __syncthreads();
-      weight[lane] = p;
-      const unsigned long long use = __ballot(live);
-      __syncthreads();
-      for (int x = 0; x < kMaxBlockDim / 64; ++x) acc[x] *= keep;
-      for (int j = 0; j < 64; ++j) {
-        if (!(use >> j & 1)) continue;
-        for (int x = 0; x < kMaxBlockDim / 64; ++x)
-          if (x * 64 + lane < a.dim) acc[x] += weight[j] * (float)vp[(key - lane + j) * a.v.stride[1] + x * 64 + lane];
+      const bool cut = top + 15 > low;
+      if (cut) {
+#pragma unroll
+        for (int x = 0; x < ST; ++x)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = now[2 * x + (e >> 3)] + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
+            if (key > limit) s[x][e] = -INFINITY;
+          }
+      }
+      float best = s[0][0];
+#pragma unroll
+      for (int x = 0; x < ST; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) best = fmaxf(best, s[x][e]);
+      best = halves_max(best) * c;
+      // the maximum in use moves only when it is left behind by more than 2^8: P stays below that, exact in fp32
+      if (__any(best > m + 8.f)) {
+        const float to = fmaxf(m, best), keep = to == m ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] *= keep;
+      }
+      const float off = m == -INFINITY ? 0.f : m;
+      vec8<T> pf[2 * ST];
+#pragma unroll
+      for (int x = 0; x < ST; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], c, -off));
+          l += p;
+          pf[2 * x + (e >> 3)][e & 7] = (elem)p;
+        }
+      if (cut && bad_tile[t & 1] == t + 1) {
+        // the finite values as always; an infinity or NaN only to the rows that see its key
+#pragma unroll
+        for (int y = 0; y < 2 * ST; ++y)
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+            acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(vt, 16 * y, 32 * i, lane)), pf[y], acc[i]);
+#pragma unroll 1
+        for (int x = 0; x < KT; ++x) {
+          int key0 = now[0];
+#pragma unroll
+          for (int i = 1; i < CH; ++i) key0 = x >> 4 == i ? now[i] : key0;
+          const bool sees = key0 + (x & 15) <= limit;
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const vec4<T> v = *(const vec4<T> *)(vt + by_column<DP>(x, 4 * i + (e >> 2)) + 4 * half);
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const float f = (float)v[n];
+                if (sees && abs_bits(f) >= kInfBits) acc[i][e + n] += f;
+              }
+            }
+        }
+      } else {
+#pragma unroll
+        for (int y = 0; y < 2 * ST; ++y)
+#pragma unroll
+          for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP>(vt, 16 * y, 32 * i, lane), pf[y], acc[i]);
       }
     }
+    lds_loads_done();
+    __syncthreads();
   }
-  elem *op = (elem *)a.out.data + b * a.out.stride[0] + i * a.out.stride[1] + h * a.out.stride[2];
-  for (int x = 0; x < kMaxBlockDim / 64; ++x)
-    if (x * 64 + lane < a.dim) op[x * 64 + lane] = (elem)(l == 0.f ? 0.f : acc[x] / l);
-  if (a.lse && lane == 0) a.lse[((long long)b * a.heads + h) * a.queries + i] = l == 0.f ? -INFINITY : m + logf(l);
+
+  l = halves_sum(l);
+  const float factor = l == 0.f ? 0.f : 1.f / l;
+  if (!live) return;
+  elem *op = (elem *)a.out.data + b * a.out.stride[0] + query * a.out.stride[1] + head * a.out.stride[2];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * i + 2 * e + 4 * half;
+      vec4<T> x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = (elem)(l == 0.f ? 0.f : acc[i][e + j] * factor);
+      if (d < a.dim) *(vec4<T> *)(op + d) = x;
+    }
+  if (a.lse && half == 0)
+    a.lse[((long long)b * a.heads + head) * a.queries + query] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 int read_view(const char *what, const lapis_hip_rows &r, View *v) {
@@ -64,6 +212,21 @@ int read_view(const char *what, const lapis_hip_rows &r, View *v) {
   v->data = static_cast<char *>(r.data);
   for (int i = 0; i < 3; ++i) v->stride[i] = r.stride[i];
   return LAPIS_HIP_OK;
+}
+
+template <typename T, int DP, int NW, int KT>
+int launch_wide(const BlockArgs &a, hipStream_t st) {
+  const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)min(a.block_m, a.queries) * a.group, 32 * NW);
+  LAPIS_REQUIRE(lists * tiles * 64 * NW < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
+  hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT>), dim3((unsigned)(lists * tiles)), dim3(64 * NW), 0, st, a, (int)tiles,
+                     a.scale < 0.f ? (int)0x80008000u : 0);
+  LAPIS_LAUNCH_CHECK();
+  return LAPIS_HIP_OK;
+}
+
+template <typename T>
+int launch_forward(const BlockArgs &a, hipStream_t st) {
+  return a.dim <= 64 ? launch_wide<T, 64, 4, 64>(a, st) : launch_wide<T, 128, 4, 64>(a, st);
 }
 
 }  // namespace
@@ -132,8 +295,5 @@ extern "C" int lapis_hip_block_attention(const lapis_hip_block_args *args, lapis
   const int rc = read_block("block_attention", args, false, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   if (a.batch == 0 || a.queries == 0 || a.heads == 0) return LAPIS_HIP_OK;
-  const auto kernel = args->dtype == LAPIS_HIP_BF16 ? block_simple_kernel<Bf16> : block_simple_kernel<F16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.queries, (unsigned)a.heads, (unsigned)a.batch), dim3(64), 0, as_stream(stream), a);
-  LAPIS_LAUNCH_CHECK();
-  return LAPIS_HIP_OK;
+  return args->dtype == LAPIS_HIP_BF16 ? launch_forward<Bf16>(a, as_stream(stream)) : launch_forward<F16>(a, as_stream(stream));
 }
