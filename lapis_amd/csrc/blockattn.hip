@@ -1,20 +1,8 @@
 // Attention over the blocks that a CSR structure lists, forward.
 #include "blockattn.hpp"
-#include "mfma.hpp"
 
 namespace lapis {
 namespace {
-
-constexpr int kAbsent = 0x7fff0000;  // first key of sixteen that do not exist
-
-// Keys of a list in the order of its entries, sixteen at a time: blocks hold at least sixteen, so sixteen neighbouring
-// places of the list are sixteen neighbouring keys.
-__device__ __forceinline__ int first_key(const BlockArgs &a, int first, int count, int place) {
-  const int e = place >> a.block_n_log2;
-  if (e >= count) return kAbsent;
-  const int block = a.crd[first + e];
-  return (unsigned)block < (unsigned)a.columns ? (block << a.block_n_log2) + (place & ((1 << a.block_n_log2) - 1)) : kAbsent;
-}
 
 // Rows of a list are its queries times the heads of the group, heads first: row i is query i / group, head i % group.
 //
@@ -25,7 +13,7 @@ __device__ __forceinline__ int first_key(const BlockArgs &a, int first, int coun
 template <typename T, int DP, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
-  constexpr int PIECES = DP / 8, RP = NW * 64 / PIECES, PASSES = KT / RP, ST = KT / 32, DT = DP / 32, CH = KT / 16;
+  constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
   __shared__ __attribute__((aligned(16))) elem k_tile[2][KT * DP], v_tile[2][KT * DP];
   __shared__ int bad_tile[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
@@ -55,28 +43,9 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     if (live && d < a.dim) x = *(const v4i *)(qp + d);
     qf[s] = __builtin_bit_cast(vec8<T>, x ^ flip);
   }
-  const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
-  const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-
-  const int tiles = a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + KT - 1) / KT) : 0;
-  const int place = tid % PIECES, my_row = tid / PIECES;
+  const KeyTiles<T, DP, NW, KT, true> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  const int tiles = keys.tiles();
   int next[CH], now[CH];
-  // Tile t on its way into buffer t & 1.  A key that is not there is read from the last one: its scores become -infinity,
-  // and a value that is no number is looked for below wherever a mask cuts.
-  const auto load = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) next[i] = first_key(a, first, count, t * KT + 16 * i);
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int at = p * RP + my_row;
-      const int key0 = RP <= 16 ? next[p * RP / 16] : my_row < 16 ? next[p * RP / 16] : next[p * RP / 16 + (RP > 16)];
-      const long long key = min(key0 + (at & 15), a.keys - 1);
-      const unsigned to = __builtin_amdgcn_readfirstlane((p * NW + wave) * 1024);
-      const int kd = (place ^ row_turn<DP>(at)) * 8, vd = (place ^ column_turn<DP>(at)) * 8;
-      if (kd < a.dim) load_to_lds(kp + key * a.k.stride[1] + kd, lds_address(k_tile[t & 1]) + to);
-      if (vd < a.dim) load_to_lds(vp + key * a.v.stride[1] + vd, lds_address(v_tile[t & 1]) + to);
-    }
-  };
 
   v16f acc[DT];
 #pragma unroll
@@ -89,13 +58,13 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     for (int i = tid; i < 2 * KT * PIECES; i += 64 * NW) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
     __syncthreads();
   }
-  if (tiles > 0) load(0);
+  if (tiles > 0) keys.load(0, next);
   lds_loads_done();
   __syncthreads();
   for (int t = 0; t < tiles; ++t) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) now[i] = next[i];
-    if (t + 1 < tiles) load(t + 1);
+    if (t + 1 < tiles) keys.load(t + 1, next);
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
@@ -114,7 +83,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
         s[x] = v16f{};
 #pragma unroll
         for (int y = 0; y < DP / 16; ++y) {
-          const vec8<T> kf = *(const vec8<T> *)(kt + by_row<DP>(32 * x + (lane & 31), 2 * y + half));
+          const vec8<T> kf = *(const vec8<T> *)(kt + place_of<DP>(32 * x + (lane & 31), 2 * y + half));
           s[x] = mfma32(kf, qf[y], s[x]);
         }
       }
@@ -158,7 +127,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
         for (int y = 0; y < 2 * ST; ++y)
 #pragma unroll
           for (int i = 0; i < DT; ++i)
-            acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(vt, 16 * y, 32 * i, lane)), pf[y], acc[i]);
+            acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP, true>(vt, 16 * y, 32 * i, lane)), pf[y], acc[i]);
 #pragma unroll 1
         for (int x = 0; x < KT; ++x) {
           int key0 = now[0];
@@ -169,7 +138,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
           for (int i = 0; i < DT; ++i)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-              const vec4<T> v = *(const vec4<T> *)(vt + by_column<DP>(x, 4 * i + (e >> 2)) + 4 * half);
+              const vec4<T> v = *(const vec4<T> *)(vt + place_of<DP, true>(x, 4 * i + (e >> 2)) + 4 * half);
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
                 const float f = (float)v[n];
@@ -181,7 +150,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
 #pragma unroll
         for (int y = 0; y < 2 * ST; ++y)
 #pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP>(vt, 16 * y, 32 * i, lane), pf[y], acc[i]);
+          for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP, true>(vt, 16 * y, 32 * i, lane), pf[y], acc[i]);
       }
     }
     lds_loads_done();
@@ -253,7 +222,7 @@ int read_block(const char *what, const lapis_hip_block_args *p, bool backward, B
   a->kv_heads = (int)p->kv_heads;
   a->group = p->kv_heads ? (int)(p->heads / p->kv_heads) : 0;
   a->dim = (int)p->dim;
-  a->block_m = (int)p->block_m;
+  a->block_m = (int)min(p->block_m, max(p->queries, (int64_t)1));  // a longer block has no more queries
   a->block_n_log2 = __builtin_ctz((unsigned)p->block_n);
   a->rows = (int)ceil_div(p->queries, p->block_m);
   a->columns = (int)ceil_div(p->keys, p->block_n);

@@ -32,24 +32,23 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
 }
 
-// Tiles of rows of DP 16-bit elements in LDS, the 16-byte pieces of a row in an order of its own.
-// by_row: 16 lanes reading the same piece of 16 neighbouring rows (an operand whose lanes are rows) meet 64 different banks.
+// Tiles of rows of DP 16-bit elements in LDS, the 16-byte pieces of a row in an order of its own, so that two ways of reading
+// meet 64 different banks: 16 lanes that take the same piece of 16 neighbouring rows (an operand whose lanes are rows; the
+// turn is another one for each of the rows that would share banks), and 32 lanes that take the same 64 bytes of four
+// neighbouring rows (a transposing read; the turns of four rows differ in the bits that number 64 bytes).
 template <int DP>
-__device__ __forceinline__ int row_turn(int row) {
-  return DP >= 128 ? row & 15 : (row >> 1) & 7;
+__device__ __forceinline__ int turn(int row) {
+  return DP >= 128 ? (row & 3) << 2 | ((row >> 2) & 3) : ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
 }
-template <int DP>
-__device__ __forceinline__ int by_row(int row, int piece) {
-  return row * DP + ((piece ^ row_turn<DP>(row)) * 8);
-}
-// by_column: 32 lanes reading the same 64 bytes of four neighbouring rows (a transposing read) meet 64 different banks.
+// A tile that is only read by columns takes the part of it that serves that: rows eight apart have the same order then, one
+// address register fewer for each 32 columns (in the forward kernel the difference between spilling and not).
 template <int DP>
 __device__ __forceinline__ int column_turn(int row) {
   return DP >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
 }
-template <int DP>
-__device__ __forceinline__ int by_column(int row, int piece) {
-  return row * DP + ((piece ^ column_turn<DP>(row)) * 8);
+template <int DP, bool COLUMNS = false>
+__device__ __forceinline__ int place_of(int row, int piece) {
+  return row * DP + ((piece ^ (COLUMNS ? column_turn<DP>(row) : turn<DP>(row))) * 8);
 }
 
 // Transposing read: of the four rows and 16 columns that a group of 16 lanes points at (lane i: row i / 4, columns
@@ -65,13 +64,13 @@ __device__ __forceinline__ vec8<T> join(vec4<T> a, vec4<T> b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Operand of 32x32x16 whose lanes are columns d0 .. d0 + 31 of a by_column tile and whose contracted index is its rows r0 ..
-// r0 + 15 in the order of a 32x32 result: element j of half h is row 8 (j / 4) + 4 h + j % 4.
-template <typename T, int DP>
+// Operand of 32x32x16 whose lanes are columns d0 .. d0 + 31 of a tile and whose contracted index is its rows r0 .. r0 + 15
+// in the order of a 32x32 result: element j of half h is row 8 (j / 4) + 4 h + j % 4.
+template <typename T, int DP, bool COLUMNS = false>
 __device__ __forceinline__ vec8<T> columns_in_order(const typename T::elem *tile, int r0, int d0, int lane) {
-  const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2), d = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  const typename T::elem *p = tile + by_column<DP>(row, d >> 3) + (d & 7);
-  return join<T>(read_columns<T>(p), read_columns<T>(p + 8 * DP));  // row + 8 has the same order of pieces
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), d = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const typename T::elem *p = tile + r0 * DP;
+  return join<T>(read_columns<T>(p + place_of<DP, COLUMNS>(row, d >> 3) + (d & 7)), read_columns<T>(p + place_of<DP, COLUMNS>(row + 8, d >> 3) + (d & 7)));
 }
 
 // 16 bytes a lane from global memory straight into LDS, lane i's at `to` + 16 i: no registers between, so a tile can be on
