@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   }
   const KeyTiles<T, DP, NW, KT, true> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
   const int tiles = keys.tiles();
-  int next[CH], now[CH];
+  int now[CH], next[CH];  // first keys of each sixteen of this tile and the next
 
   v16f acc[DT];
 #pragma unroll
@@ -58,13 +58,22 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     for (int i = tid; i < 2 * KT * PIECES; i += 64 * NW) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
     __syncthreads();
   }
-  if (tiles > 0) keys.load(0, next);
+  int ahead = 0;
+  if (tiles > 0) {
+    ahead = keys.look_up(1);
+    keys.spread(keys.look_up(0), next);
+    keys.load(0, next);
+  }
   lds_loads_done();
   __syncthreads();
   for (int t = 0; t < tiles; ++t) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) now[i] = next[i];
-    if (t + 1 < tiles) keys.load(t + 1, next);
+    if (t + 1 < tiles) {
+      keys.spread(ahead, next);
+      ahead = keys.look_up(t + 2);
+      keys.load(t + 1, next);
+    }
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
@@ -226,13 +235,15 @@ int read_block(const char *what, const lapis_hip_block_args *p, bool backward, B
   a->block_n_log2 = __builtin_ctz((unsigned)p->block_n);
   a->rows = (int)ceil_div(p->queries, p->block_m);
   a->columns = (int)ceil_div(p->keys, p->block_n);
+  if (p->heads == 0) a->rows = 0, a->group = 1;
   a->causal = p->causal != 0;
   a->shift = (int)(p->keys - p->queries);
   a->scale = p->scale;
   a->pos = p->pos;
   a->crd = p->crd;
-  a->nnz = p->nnz;
+  a->nnz = a->rows ? p->nnz : 0;
   a->lse = p->lse;
+  LAPIS_REQUIRE(!backward || (double)p->batch * (double)p->heads * (double)p->queries < 2147483647.0, "%s: more queries times heads than 31 bits count", what);
   LAPIS_REQUIRE((double)p->batch * (double)p->kv_heads * (double)a->rows < 2147483647.0, "%s: more rows than 31 bits count", what);
   const bool some_queries = p->batch && p->queries && p->heads, some_keys = p->batch && p->keys && p->kv_heads;
   if (some_queries || (backward && some_keys && p->queries)) LAPIS_REQUIRE(p->pos && (p->crd || p->nnz == 0), "%s: null structure", what);

@@ -30,12 +30,11 @@ __device__ __forceinline__ void entries_of(const BlockArgs &a, long long row, in
 constexpr int kAbsent = 0x7fff0000;  // first key of sixteen that do not exist
 
 // Keys of a list in the order of its entries, sixteen at a time: blocks hold at least sixteen, so sixteen neighbouring
-// places of the list are sixteen neighbouring keys.
+// places of the list are sixteen neighbouring keys.  (The list has an entry.)
 __device__ __forceinline__ int first_key(const BlockArgs &a, int first, int count, int place) {
-  const int e = place >> a.block_n_log2;
-  if (e >= count) return kAbsent;
-  const int block = a.crd[first + e];
-  return (unsigned)block < (unsigned)a.columns ? (block << a.block_n_log2) + (place & ((1 << a.block_n_log2) - 1)) : kAbsent;
+  const int e = place >> a.block_n_log2, block = a.crd[first + min(e, count - 1)];
+  const int key = (block << a.block_n_log2) + (place & ((1 << a.block_n_log2) - 1));
+  return e < count && (unsigned)block < (unsigned)a.columns ? key : kAbsent;
 }
 
 // Tiles of KT keys and values of a list on their way into two LDS buffers each, a workgroup of NW wavefronts sharing the
@@ -63,10 +62,14 @@ struct KeyTiles {
     v_to = lds_address(v_tile) + wave * 1024;
   }
   __device__ __forceinline__ int tiles() const { return a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + KT - 1) / KT) : 0; }
-  // Tile t into buffer t & 1; `key0`: the first key of each sixteen of it.
-  __device__ __forceinline__ void load(int t, int (&key0)[CH]) const {
+  // The first key of each sixteen of tile t, one to a lane: asked for a tile before they are needed.
+  __device__ __forceinline__ int look_up(int t) const { return first_key(a, first, count, t * KT + 16 * (threadIdx.x % CH)); }
+  static __device__ __forceinline__ void spread(int of_lane, int (&key0)[CH]) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) key0[i] = __builtin_amdgcn_readfirstlane(first_key(a, first, count, t * KT + 16 * i));
+    for (int i = 0; i < CH; ++i) key0[i] = __builtin_amdgcn_readlane(of_lane, i);
+  }
+  // Tile t into buffer t & 1.
+  __device__ __forceinline__ void load(int t, const int (&key0)[CH]) const {
     const unsigned buffer = (t & 1) * KT * DP * 2;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {

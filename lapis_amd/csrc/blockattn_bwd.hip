@@ -9,19 +9,21 @@ namespace lapis {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kParts = 8;  // of the units of work beside dK and dV, one to each XCD
 
 // ---- dQ --------------------------------------------------------------------------------------------------------
 
 // As the forward kernel: 32 rows a wavefront, a query per lane.  dS^T = P^T * (scale V dO^T - scale delta) feeds dQ^T = K^T dS^T
 // from its registers.  rowsum(dO * O) is computed here and left, times `scale`, for the other kernel.
 template <typename T, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta) {
+__global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, int *odd) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
   __shared__ __attribute__((aligned(16))) elem k_tile[2][KT * DP], v_tile[2][KT * DP];
   __shared__ int bad_tile[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
+  if (block == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
   const int list = block / tiles_of_list, part = block - list * tiles_of_list;
   const int bh = list / a.rows, r = list - bh * a.rows, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const int q0 = r * a.block_m, held = min(a.block_m, a.queries - q0), rows = held * a.group;
@@ -65,7 +67,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
   }
   const KeyTiles<T, DP, NW, KT, false> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
   const int tiles = keys.tiles();
-  int next[CH], now[CH];
+  int now[CH], next[CH];  // first keys of each sixteen of this tile and the next
   v16f acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = v16f{};
@@ -76,13 +78,22 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     for (int i = tid; i < 2 * KT * PIECES; i += 64 * NW) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
     __syncthreads();
   }
-  if (tiles > 0) keys.load(0, next);
+  int ahead = 0;
+  if (tiles > 0) {
+    ahead = keys.look_up(1);
+    keys.spread(keys.look_up(0), next);
+    keys.load(0, next);
+  }
   lds_loads_done();
   __syncthreads();
   for (int t = 0; t < tiles; ++t) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) now[i] = next[i];
-    if (t + 1 < tiles) keys.load(t + 1, next);
+    if (t + 1 < tiles) {
+      keys.spread(ahead, next);
+      ahead = keys.look_up(t + 2);
+      keys.load(t + 1, next);
+    }
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
@@ -150,10 +161,11 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
 
 // ---- the columns' lists ----------------------------------------------------------------------------------------
 
-// Which rows list a column, in ascending order (a row that lists it twice, twice).  Rows are cut into at most 32 chunks;
+// Which rows list a column, in ascending order (a row that lists it twice, twice).  Rows are cut into at most 64 chunks;
 // counts[column][chunk], summed over a (batch entry, head)'s columns and chunks, gives each chunk its places.
 struct Columns {
   int *odd;           // not 0: positions overlap or leave [0, nnz]; the lists are not used then
+  int *next;          // units taken from each part of them
   int *counts;        // lists x columns x chunks
   int *start, *end;   // of each column's rows
   int *unit;          // column of each unit of work, -1 = nothing to do
@@ -162,8 +174,12 @@ struct Columns {
   int chunks, chunk_rows, per_unit, units, lists, sub;
 };
 
-constexpr int kColumnsInLds = 8192;
+__global__ void clear_kernel(int *p) { p[threadIdx.x] = 0; }
 
+constexpr int kColumnsInLds = 8192, kRowsAtOnce = 16;
+
+// One wavefront per chunk takes its rows one after the other, so that the places of a column ascend with its rows; the
+// entries of sixteen rows are on their way at a time.
 template <bool FILL>
 __global__ __launch_bounds__(64) void columns_kernel(BlockArgs a, Columns t) {
   __shared__ int place[kColumnsInLds];
@@ -173,27 +189,40 @@ __global__ __launch_bounds__(64) void columns_kernel(BlockArgs a, Columns t) {
   __syncthreads();
   const int r_end = min(a.rows, (chunk + 1) * t.chunk_rows);
   bool odd = false;
-  for (int r = chunk * t.chunk_rows; r < r_end; ++r) {
-    const long long row = (long long)bh * a.rows + r;
-    int first, count;
-    entries_of(a, row, &first, &count);
-    odd |= a.pos[row] != first || (long long)a.pos[row + 1] != (long long)first + count;
-    // one wavefront, row after row: the places of a column ascend with its rows
-    for (int e = lane; e < count; e += 64) {
-      const int c = a.crd[first + e];
-      if ((unsigned)c < (unsigned)a.columns && c >= c0 && c < c0 + cs) {
-        const int at = atomicAdd(&place[c - c0], 1);
-        if (FILL && at < a.nnz) t.rows[at] = r;
+  const auto add = [&](int c, int r) {
+    if ((unsigned)c < (unsigned)a.columns && c >= c0 && c < c0 + cs) {
+      const int at = atomicAdd(&place[c - c0], 1);
+      if (FILL && at < a.nnz) t.rows[at] = r;
+    }
+  };
+  for (int r0 = chunk * t.chunk_rows; r0 < r_end; r0 += kRowsAtOnce) {
+    int first = 0, count = 0, entry[kRowsAtOnce];
+    if (lane < kRowsAtOnce && r0 + lane < r_end) {
+      const long long row = (long long)bh * a.rows + r0 + lane;
+      entries_of(a, row, &first, &count);
+      odd |= a.pos[row] != first || (long long)a.pos[row + 1] != (long long)first + count;
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      const int f = __builtin_amdgcn_readlane(first, i), n = __builtin_amdgcn_readlane(count, i);
+      entry[i] = lane < n ? a.crd[f + lane] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      const int f = __builtin_amdgcn_readlane(first, i), n = __builtin_amdgcn_readlane(count, i);
+      add(entry[i], r0 + i);
+      wave_lds_sync();
+      for (int e = 64 + lane; e - lane < n; e += 64) {
+        add(e < n ? a.crd[f + e] : -1, r0 + i);
+        wave_lds_sync();
       }
     }
-    __syncthreads();
   }
   if (FILL) return;
-  if (odd && lane == 0) atomicOr(t.odd, 1);
+  if (__any(odd) && lane == 0) atomicOr(t.odd, 1);
+  __syncthreads();
   for (int c = lane; c < cs; c += 64) t.counts[((long long)bh * a.columns + c0 + c) * t.chunks + chunk] = place[c];
 }
-
-__global__ void clear_kernel(int *p) { *p = 0; }
 
 // Where a list's entries start (positions are in order here).
 __device__ __forceinline__ int list_start(const BlockArgs &a, long long bh) {
@@ -251,261 +280,280 @@ __global__ __launch_bounds__(1024) void columns_scan_kernel(BlockArgs a, Columns
                            : bh + 1 < t.lists ? (long long)list_start(a, bh + 1ll) / t.per_unit + cc + 1
                                               : t.units;
     for (long long u = to; u < stop && u < t.units; ++u) t.unit[u] = u < to + needed ? cc : -1;
+    if (cc == 0)  // positions may start past 0
+      for (long long u = 0; u < to && u < t.units; ++u) t.unit[u] = -1;
   }
 }
 
 // ---- dK and dV -------------------------------------------------------------------------------------------------
 
-// A workgroup takes 32 * KG keys of a column and some of the rows that list it, their queries times heads packed into tiles of
-// 32: KG wavefronts share a tile, 4 / KG such groups take turns and add up at the end.  With a key per lane P and dS (queries x
-// keys) feed dV^T = dO^T P and dK^T = Q^T dS from their registers; K and V of a wavefront's keys stay in registers.
-// A tile's rows (where they lie, log-sums, deltas, last keys) are looked up while earlier ones are computed: place in the
-// list two tiles ahead, sums one and a half, so that no wait is left but the one at the end of a tile.
-template <typename T, int DP, int KG>
-__global__ __launch_bounds__(256, 1) void block_dkv_kernel(BlockArgs a, Columns cols, const float *__restrict__ delta) {
+constexpr int kMostEntries = 384;  // of a unit
+
+// A unit of work: 32 * KG keys of a column and some of the rows that list it, their queries times heads packed into tiles of
+// 32.  Two wavefronts share 32 keys, a key per lane, K or V of them in registers: one computes S and P (queries x keys), leaves
+// P in LDS for the other and feeds dV^T = dO^T P from its registers; the other computes dP meanwhile, and then dS, which
+// feeds dK^T = Q^T dS.  Both sums in one wavefront take 318 registers, one wavefront a SIMD and nothing to fill the waits
+// with (1.06 ms at 8k queries against X); split, four wavefronts a workgroup and two workgroups a compute unit fit.
+// Where keys are few (KG = 1) two pairs take turns with the tiles and add up at the end.
+// The rows of a column lie all over Q and dO, beyond L2 in large passes: S tiles are on their way or being computed, where a
+// tile's rows lie is worked out one tile earlier still, and no load but those into LDS is in the loop.
+// Columns are anything but equal (the first block is listed by all rows, the last by few): workgroups take units from a
+// counter, those of their XCD's part first, whose rows of Q and dO its L2 holds.
+template <typename T, int DP, int KG, int S>
+__global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns cols, const float *__restrict__ delta) {
   typedef typename T::elem elem;
-  constexpr int QG = 4 / KG, PIECES = DP / 8, RP = KG * 64 / PIECES, PASSES = 32 / RP, DT = DP / 32;
-  struct Info {
+  constexpr int QG = 2 / KG, TG = KG * 128, PIECES = DP / 8, RP = TG / PIECES, PASSES = 32 / RP, DT = DP / 32;
+  struct Info {  // where a tile's rows lie
     long long q[32], g[32];
-    float off[32], del[32];
-    int last[32];
+    int sums[32], last[32];
+    float times[32];  // how often the row lists the column, where every row is looked through
   };
-  __shared__ __attribute__((aligned(16))) elem tiles[QG][2][2][32 * DP];
-  __shared__ __attribute__((aligned(16))) Info infos[QG][3];
+  __shared__ __attribute__((aligned(16))) elem tiles[QG][S][2][32 * DP];
+  __shared__ __attribute__((aligned(16))) float weights[QG * KG][1024];
+  __shared__ __attribute__((aligned(16))) float sums[QG][S][2][32];  // log-sums and deltas of a tile's rows
+  __shared__ __attribute__((aligned(16))) Info infos[QG][S + 1];
+  __shared__ int rows_of_unit[kMostEntries], taken;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int kg = wave % KG, qg = wave / KG, gt = tid - qg * KG * 64;
-  const unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
-  const int u = block / cols.sub, sub = block - u * cols.sub;
+  const int role = wave & 1, kg = (wave >> 1) % KG, qg = (wave >> 1) / KG, gt = tid - qg * TG;  // role 0: dV, 1: dK
   const bool odd = *cols.odd != 0;
-  int cc, from = 0, n, start = 0;
-  bool several = false;
-  if (odd) {  // every row is looked through for the column
-    if (u >= cols.lists * a.columns) return;
-    cc = u;
-    n = a.rows;
-  } else {
-    cc = cols.unit[u];
-    if (cc < 0) return;
-    start = cols.start[cc];
-    const int rows = cols.end[cc] - start;
-    several = rows > cols.per_unit;
-    from = (u - (start / cols.per_unit + cc)) * cols.per_unit;
-    n = min(rows - from, cols.per_unit);
-  }
-  const int bh = cc / a.columns, column = cc - bh * a.columns, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
-  const int in_block = sub * 32 * KG + kg * 32;
-  const int key_low = (column << a.block_n_log2) + in_block, key = key_low + (lane & 31);
-  const bool live = in_block + (lane & 31) < (1 << a.block_n_log2) && key < a.keys;
-
-  vec8<T> kf[DP / 16], vf[DP / 16];
-  const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + key * a.k.stride[1] + kh * a.k.stride[2];
-  const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + key * a.v.stride[1] + kh * a.v.stride[2];
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const int d = 16 * s + 8 * half;
-    kf[s] = vf[s] = vec8<T>{};
-    if (live && d < a.dim) kf[s] = *(const vec8<T> *)(kp + d), vf[s] = *(const vec8<T> *)(vp + d);
-  }
-
-  // this lane's row of the tiles of its group: entry, query of the block and head of the group, moved on by 32 QG each tile
-  const int steps_h = 32 * QG % a.group, steps_q = 32 * QG / a.group % a.block_m, steps_e = 32 * QG / a.group / a.block_m;
-  const int slot0 = qg * 32 + (lane & 31);
-  int entry = slot0 / a.group / a.block_m, in = slot0 / a.group % a.block_m, hd = slot0 % a.group;
-  const auto on = [&] {
-    hd += steps_h;
-    in += steps_q;
-    entry += steps_e;
-    if (hd >= a.group) hd -= a.group, ++in;
-    if (in >= a.block_m) in -= a.block_m, ++entry;
-  };
-  const long long all = (long long)n * a.block_m * a.group;
-  const int tiles_n = (int)((all + 32 * QG - 1) / (32 * QG));
-
-  int row_next = 0;  // list row of the tile after the one whose sums are on their way
-  struct Row {
-    int query, head;
-    bool there;
-    float weight;
-  } now_row = {0, 0, false, 1.f};
-  float lse_next = 0.f, del_next = 0.f;
-  const auto fetch_row = [&] { row_next = odd || entry >= n ? entry : cols.rows[start + from + entry]; };
-  const auto fetch_sums = [&] {  // of the row that fetch_row found; then on to the next tile's
-    now_row.there = entry < n;
-    now_row.query = row_next * a.block_m + in;
-    now_row.there = now_row.there && now_row.query < a.queries;
-    if (!now_row.there) now_row.query = 0;
-    now_row.head = kh * a.group + hd;
-    now_row.weight = 0.f;
-    if (odd && now_row.there) {
-      int first, count, times = 0;
-      entries_of(a, (long long)bh * a.rows + row_next, &first, &count);
-      for (int e = 0; e < count; ++e) times += a.crd[first + e] == column;
-      now_row.weight = __builtin_amdgcn_logf((float)times);  // a row that does not list the column: -infinity, weight 0
-    }
-    const long long at = ((long long)b * a.heads + now_row.head) * a.queries + now_row.query;
-    lse_next = a.lse[at];
-    del_next = delta[at];
-    on();
-  };
-  const auto put_info = [&](int t) {
-    Info &i = infos[qg][t % 3];
-    if (kg != 0 || lane >= 32) return;
-    i.q[lane] = b * a.q.stride[0] + now_row.query * a.q.stride[1] + now_row.head * a.q.stride[2];
-    i.g[lane] = b * a.dout.stride[0] + now_row.query * a.dout.stride[1] + now_row.head * a.dout.stride[2];
-    i.off[lane] = !now_row.there || lse_next == -INFINITY ? INFINITY : lse_next * kLog2e - now_row.weight;
-    i.del[lane] = del_next;
-    i.last[lane] = !now_row.there ? -1 : a.causal ? min(now_row.query + a.shift, a.keys - 1) : a.keys - 1;
-  };
-  const int place = gt % PIECES, my_row = gt / PIECES;
-  const auto load = [&](int t) {
-    const Info &i = infos[qg][t % 3];
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int at = p * RP + my_row, d = (place ^ turn<DP>(at)) * 8;
-      const unsigned to = __builtin_amdgcn_readfirstlane((p * KG + kg) * 1024);
-      if (d < a.dim) {
-        load_to_lds((const elem *)a.q.data + i.q[at] + d, lds_address(tiles[qg][t & 1][0]) + to);
-        load_to_lds((const elem *)a.dout.data + i.g[at] + d, lds_address(tiles[qg][t & 1][1]) + to);
-      }
-    }
-  };
-
-  v16f dk[DT], dv[DT];
-#pragma unroll
-  for (int i = 0; i < DT; ++i) dk[i] = dv[i] = v16f{};
+  const int all_units = (odd ? cols.lists * a.columns : cols.units) * cols.sub;
   const float c = a.scale * kLog2e;
-  if (a.dim < DP)
-    for (int i = tid; i < QG * 4 * 32 * PIECES; i += 256) ((v4i *)tiles)[i] = v4i{0, 0, 0, 0};
-  if (tiles_n > 0) {
-    // tiles 0 and 1 looked up, tile 0 loaded, the sums of tile 2 and the row of tile 3 under way
-    fetch_row();
-    fetch_sums();
-    put_info(0);
-    fetch_row();
-    fetch_sums();
-    put_info(1);
-    fetch_row();
-    fetch_sums();
-    fetch_row();
+
+  for (int part = 0; part < kParts;) {
     __syncthreads();
-    load(0);
-  }
-  lds_loads_done();
-  __syncthreads();
-  for (int t = 0; t < tiles_n; ++t) {
-    put_info(t + 2);
-    fetch_sums();
-    fetch_row();
-    if (t + 1 < tiles_n) load(t + 1);
-    const Info &info = infos[qg][t % 3];
-    const elem *qt = tiles[qg][t & 1][0], *gt_ = tiles[qg][t & 1][1];
-    const int last = info.last[lane & 31];
-    if (__any(last >= key_low)) {
-      const bool cut = __any(last < key_low + 31);
-      v16f s = {}, g = {};
+    if (tid == 0) taken = atomicAdd(cols.next + (blockIdx.x + part) % kParts, 1);
+    __syncthreads();
+    const int mine = (blockIdx.x + part) % kParts;
+    const long long unit_l = (long long)all_units * mine / kParts + taken;
+    if (unit_l >= (long long)all_units * (mine + 1) / kParts) {
+      ++part;
+      continue;
+    }
+    const int u = (int)unit_l / cols.sub, sub = (int)unit_l - u * cols.sub;
+    int cc, from = 0, n, start = 0;
+    bool several = false;
+    if (odd) {  // every row is looked through for the column
+      cc = u;
+      n = a.rows;
+    } else {
+      cc = cols.unit[u];
+      if (cc < 0) continue;
+      start = cols.start[cc];
+      const int rows = cols.end[cc] - start;
+      several = rows > cols.per_unit;
+      from = (u - (start / cols.per_unit + cc)) * cols.per_unit;
+      n = min(rows - from, cols.per_unit);
+      for (int e = tid; e < n; e += 256) rows_of_unit[e] = cols.rows[start + from + e];
+    }
+    const int bh = cc / a.columns, column = cc - bh * a.columns, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
+    const int in_block = sub * 32 * KG + kg * 32;
+    const int key_low = (column << a.block_n_log2) + in_block, key = key_low + (lane & 31);
+    const bool live = in_block + (lane & 31) < (1 << a.block_n_log2) && key < a.keys;
+
+    const View &kv = role ? a.v : a.k;
+    vec8<T> kf[DP / 16];  // of this wavefront's keys: K, or V
+    const elem *kp = (const elem *)kv.data + b * kv.stride[0] + key * kv.stride[1] + kh * kv.stride[2];
 #pragma unroll
-      for (int y = 0; y < DP / 16; ++y) s = mfma32(*(const vec8<T> *)(qt + place_of<DP>(lane & 31, 2 * y + half)), kf[y], s);
-#pragma unroll
-      for (int y = 0; y < DP / 16; ++y) g = mfma32(*(const vec8<T> *)(gt_ + place_of<DP>(lane & 31, 2 * y + half)), vf[y], g);
-      vec8<T> pf[2], df[2];
-      bool bad = false;
-      if (cut) {  // 0 times an infinity or NaN must not count
-        for (int i = 0; i < PIECES / 2; ++i)
-          bad |= not_finite<T>(*(const vec8<T> *)(qt + (i * 64 + lane) * 8)) || not_finite<T>(*(const vec8<T> *)(gt_ + (i * 64 + lane) * 8));
-        bad = __any(bad);
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = 16 * s + 8 * half;
+      kf[s] = vec8<T>{};
+      if (live && d < a.dim) kf[s] = *(const vec8<T> *)(kp + d);
+    }
+
+    // this lane's row of the tiles of its group: entry, query of the block and head of the group, moved on by 32 QG each tile
+    const int steps_h = 32 * QG % a.group, steps_q = 32 * QG / a.group % a.block_m, steps_e = 32 * QG / a.group / a.block_m;
+    const int slot0 = qg * 32 + (lane & 31);
+    int entry = slot0 / a.group / a.block_m, in = slot0 / a.group % a.block_m, hd = slot0 % a.group;
+    const long long all = (long long)n * a.block_m * a.group;
+    const int tiles_n = (int)((all + 32 * QG - 1) / (32 * QG));
+    const auto put_info = [&](int t) {  // of the tiles in turn
+      if (role != 0 || kg != 0) return;
+      if (lane < 32) {
+        Info &i = infos[qg][t % (S + 1)];
+        int query = 0;
+        bool there = entry < n;
+        if (there) {
+          query = (odd ? entry : rows_of_unit[entry]) * a.block_m + in;
+          there = query < a.queries;
+        }
+        if (odd) {
+          int first = 0, count = 0, times = 0;
+          if (there) entries_of(a, (long long)bh * a.rows + entry, &first, &count);
+          for (int e = 0; e < count; ++e) times += a.crd[first + e] == column;
+          i.times[lane] = (float)times;
+        }
+        query = there ? query : 0;
+        const int head = kh * a.group + hd;
+        i.q[lane] = b * a.q.stride[0] + query * a.q.stride[1] + head * a.q.stride[2];
+        i.g[lane] = b * a.dout.stride[0] + query * a.dout.stride[1] + head * a.dout.stride[2];
+        i.sums[lane] = (b * a.heads + head) * a.queries + query;
+        i.last[lane] = !there ? -1 : a.causal ? min(query + a.shift, a.keys - 1) : a.keys - 1;
       }
+      hd += steps_h;
+      in += steps_q;
+      entry += steps_e;
+      if (hd >= a.group) hd -= a.group, ++in;
+      if (in >= a.block_m) in -= a.block_m, ++entry;
+    };
+    const int place = gt % PIECES, my_row = gt / PIECES, in_group = wave - qg * KG * 2;
+    constexpr int LOADS = 2 * PASSES;  // at least that many a tile and wavefront
+    const auto load = [&](int t) {
+      const Info &i = infos[qg][t % (S + 1)];
+      const int slot = t % S;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v4f off = *(const v4f *)(info.off + 8 * j + 4 * half), del = *(const v4f *)(info.del + 8 * j + 4 * half);
-        const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -off[e]));
-          float ds = p * __builtin_fmaf(g[4 * j + e], a.scale, -del[e]);
-          if (bad && abs_bits(g[4 * j + e]) >= kInfBits) p = __builtin_nanf("");  // its row of dO is taken as zeros below
-          if (cut && key > lim[e]) p = ds = 0.f;
-          pf[j >> 1][(4 * j + e) & 7] = (elem)p;
-          df[j >> 1][(4 * j + e) & 7] = (elem)ds;
+      for (int p = 0; p < PASSES; ++p) {
+        const int at = p * RP + my_row, d = (place ^ turn<DP>(at)) * 8;
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds_address(tiles[qg][slot][0]) + (p * KG * 2 + in_group) * 1024);
+        if (d < a.dim) {
+          load_to_lds((const elem *)a.q.data + i.q[at] + d, to);
+          load_to_lds((const elem *)a.dout.data + i.g[at] + d, to + 64 * DP);
         }
       }
-      if (bad) {
+      if (role == 0 && kg == 0 && lane < 32) {
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds_address(sums[qg][slot][0]));
+        load_word_to_lds(a.lse + i.sums[lane], to);
+        load_word_to_lds(delta + i.sums[lane], to + 128);
+      }
+    };
+
+    v16f acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i] = v16f{};
+    if (a.dim < DP)  // what no row fills stays zero
+      for (int i = tid; i < QG * S * 2 * 32 * PIECES; i += 256) ((v4i *)tiles)[i] = v4i{0, 0, 0, 0};
+    __syncthreads();
+    for (int t = 0; t < S; ++t) put_info(t);
+    __syncthreads();
+    for (int t = 0; t < S - 1; ++t)
+      if (t < tiles_n) load(t);
+    lds_loads_done();
+    __syncthreads();
+    for (int t = 0; t < tiles_n; ++t) {
+      put_info(t + S);
+      if (t + S - 1 < tiles_n) load(t + S - 1);
+      const Info &info = infos[qg][t % (S + 1)];
+      const elem *by_row = tiles[qg][t % S][role], *by_column = tiles[qg][t % S][1 - role];
+      float *w = weights[qg * KG + kg] + lane * 4;  // element e of this lane at (e / 4) * 256 + lane * 4 + e % 4
+      const int last = info.last[lane & 31];
+      const bool some = __any(last >= key_low), cut = odd || __any(last < key_low + 31);
+      v16f s = {};  // S, or dP
+      unsigned bad = 0;
+      if (some) {
+#pragma unroll
+        for (int y = 0; y < DP / 16; ++y) s = mfma32(*(const vec8<T> *)(by_row + place_of<DP>(lane & 31, 2 * y + half)), kf[y], s);
+        if (cut) {  // 0 times an infinity or NaN must not count: which rows of the other operand hold one?
+#pragma unroll 1
+          for (int i = 0; i < PIECES / 2; ++i) {
+            const unsigned long long lanes = __ballot(not_finite<T>(*(const vec8<T> *)(by_column + (i * 64 + lane) * 8)));
+            if (lanes == 0) continue;
+#pragma unroll
+            for (int x = 0; x < 64 / PIECES; ++x)
+              if (lanes >> (x * PIECES) & ((1u << PIECES) - 1)) bad |= 1u << (i * (64 / PIECES) + x);
+          }
+        }
+      }
+      vec8<T> f[2];
+      if (role == 0 && some) {
+        const float *lse = sums[qg][t % S][0];
+        if (!cut) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
+            v4f p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+              f[j >> 1][(4 * j + e) & 7] = (elem)p[e];
+            }
+            *(v4f *)(w + 256 * j) = p;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
+            const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
+            v4f p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = 8 * j + 4 * half + e;
+              const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+              const float times = odd ? info.times[row] : 1.f;
+              const bool seen = key <= lim[e] && times != 0.f;  // a row without an entry (log-sum -infinity) sees no key
+              p[e] = seen ? x * times : 0.f;
+              f[j >> 1][(4 * j + e) & 7] = (elem)(seen && (bad >> row & 1) ? __builtin_nanf("") : p[e]);  // its dO is taken as zeros below
+            }
+            *(v4f *)(w + 256 * j) = p;
+          }
+        }
+      }
+      __syncthreads();
+      if (role == 1 && some) {
+        const float *dl = sums[qg][t % S][1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const v4f p = *(const v4f *)(w + 256 * j), del = *(const v4f *)(dl + 8 * j + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float ds = p[e] * __builtin_fmaf(s[4 * j + e], a.scale, -del[e]);
+            if (cut) ds = p[e] == 0.f ? 0.f : ds;
+            f[j >> 1][(4 * j + e) & 7] = (elem)ds;
+          }
+        }
+      }
+      if (some) {
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int i = 0; i < DT; ++i) {
-            dv[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(gt_, 16 * y, 32 * i, lane)), pf[y], dv[i]);
-            dk[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(qt, 16 * y, 32 * i, lane)), df[y], dk[i]);
+            vec8<T> x = columns_in_order<T, DP>(by_column, 16 * y, 32 * i, lane);
+            if (bad) x = finite_only<T>(x);
+            acc[i] = mfma32(x, f[y], acc[i]);
           }
-      } else {
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-#pragma unroll
-          for (int i = 0; i < DT; ++i) dv[i] = mfma32(columns_in_order<T, DP>(gt_, 16 * y, 32 * i, lane), pf[y], dv[i]);
-#pragma unroll
-          for (int i = 0; i < DT; ++i) dk[i] = mfma32(columns_in_order<T, DP>(qt, 16 * y, 32 * i, lane), df[y], dk[i]);
-        }
       }
+      if (t + S - 1 < tiles_n) lds_loads_done<(S - 2) * LOADS>();
+      else lds_loads_done();
+      __syncthreads();
     }
-    lds_loads_done();
-    __syncthreads();
-  }
 
-  // the groups' sums, in their order, with the tiles' memory between them
-  if (QG > 1) {
-    float *sums = (float *)tiles;  // (group - 1, key group): 2 DT 16 values of 64 lanes
-    constexpr int EACH = 2 * DT * 16 * 64;
-    static_assert((QG - 1) * KG * EACH / 2 * 4 <= (int)sizeof(tiles), "the groups' sums fit");
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {  // dk, then dv
-      if (part) __syncthreads();
+    if (QG > 1) {  // the second pair's sums to the first, with the tiles' memory between them
+      float *between = (float *)tiles + role * DT * 1024;
       if (qg > 0) {
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sums[((qg - 1) * KG + kg) * (EACH / 2) + (i * 16 + e) * 64 + lane] = part ? dv[i][e] : dk[i][e];
+          for (int e = 0; e < 16; ++e) between[(i * 16 + e) * 64 + lane] = acc[i][e];
       }
       __syncthreads();
-      if (qg == 0)
-        for (int x = 0; x < QG - 1; ++x)
+      if (qg == 0) {
 #pragma unroll
-          for (int i = 0; i < DT; ++i)
+        for (int i = 0; i < DT; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float f = sums[(x * KG + kg) * (EACH / 2) + (i * 16 + e) * 64 + lane];
-              if (part) dv[i][e] += f;
-              else dk[i][e] += f;
-            }
+          for (int e = 0; e < 16; ++e) acc[i][e] += between[(i * 16 + e) * 64 + lane];
+      }
     }
-  }
-  if (qg > 0 || !live) return;
-  if (several) {
-    const long long slot = 2ll * (start / cols.per_unit) + from / cols.per_unit;
-    float *to = cols.partial + (slot * 2 << a.block_n_log2) * DP + (long long)(in_block + (lane & 31)) * DP;
-    float *to_v = to + ((long long)DP << a.block_n_log2);
+    if (qg > 0 || !live) continue;
+    if (several) {
+      const long long slot = 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << a.block_n_log2;
+      float *to = cols.partial + (slot * 2 + 1 - role) * each + (long long)(in_block + (lane & 31)) * DP;
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *(v4f *)(to + 32 * i + 2 * e + 4 * half) = v4f{acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]};
+      continue;
+    }
+    const View &dkv = role ? a.dk : a.dv;
+    elem *to = (elem *)dkv.data + b * dkv.stride[0] + key * dkv.stride[1] + kh * dkv.stride[2];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const int d = 32 * i + 2 * e + 4 * half;
-        *(v4f *)(to + d) = v4f{dk[i][e], dk[i][e + 1], dk[i][e + 2], dk[i][e + 3]};
-        *(v4f *)(to_v + d) = v4f{dv[i][e], dv[i][e + 1], dv[i][e + 2], dv[i][e + 3]};
+        vec4<T> x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (elem)acc[i][e + j];
+        if (d < a.dim) *(vec4<T> *)(to + d) = x;
       }
-    return;
   }
-  elem *kd = (elem *)a.dk.data + b * a.dk.stride[0] + key * a.dk.stride[1] + kh * a.dk.stride[2];
-  elem *vd = (elem *)a.dv.data + b * a.dv.stride[0] + key * a.dv.stride[1] + kh * a.dv.stride[2];
-#pragma unroll
-  for (int i = 0; i < DT; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int d = 32 * i + 2 * e + 4 * half;
-      if (d >= a.dim) continue;
-      vec4<T> x, y;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (elem)dk[i][e + j], y[j] = (elem)dv[i][e + j];
-      *(vec4<T> *)(kd + d) = x;
-      *(vec4<T> *)(vd + d) = y;
-    }
 }
 
 // Columns of several units: their sums, in the order of the units.
@@ -520,7 +568,7 @@ __global__ __launch_bounds__(256) void join_units_kernel(BlockArgs a, Columns co
   const int bh = cc / a.columns, column = cc - bh * a.columns, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const long long each = (long long)DP << a.block_n_log2;
   const float *from = cols.partial + 2ll * (start / cols.per_unit) * 2 * each;
-  for (long long x = threadIdx.x * 4; x < 2 * each; x += 1024) {
+  for (long long x = (blockIdx.y * 256 + threadIdx.x) * 4; x < 2 * each; x += 4096) {
     const bool is_v = x >= each;
     const int at = (int)(is_v ? x - each : x), d = at % DP, key = (column << a.block_n_log2) + at / DP;
     if (key >= a.keys || d >= a.dim) continue;
@@ -549,11 +597,12 @@ Layout layout_of(const BlockArgs &a) {
   Layout l = {};
   Columns &c = l.columns;
   c.lists = a.batch * a.kv_heads;
-  c.chunk_rows = (int)max((int64_t)64, ceil_div(a.rows, 32));
+  c.chunk_rows = (int)max((int64_t)kRowsAtOnce, ceil_div(ceil_div(a.rows, 64), kRowsAtOnce) * kRowsAtOnce);
   c.chunks = (int)max((int64_t)1, ceil_div(a.rows, c.chunk_rows));
-  // 4096 queries times heads a unit: a sixteenth of what a compute unit does in a large pass, so long columns do not stand alone
+  // 8192 queries times heads a unit, an eighth of what a compute unit does in a large pass: long columns do not stand alone,
+  // and those of ordinary length need no join
   const int64_t rows_of_entry = (int64_t)min(a.block_m, max(a.queries, 1)) * max(a.group, 1);
-  c.per_unit = (int)max((int64_t)1, 4096 / rows_of_entry);
+  c.per_unit = (int)min((int64_t)kMostEntries, max((int64_t)1, 8192 / rows_of_entry));
   c.units = (int)(a.nnz / c.per_unit + (int64_t)c.lists * a.columns);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -562,7 +611,7 @@ Layout layout_of(const BlockArgs &a) {
     return here;
   };
   l.delta = take(4ll * a.batch * a.heads * a.queries);
-  l.odd = take(4);
+  l.odd = take(4 * (1 + kParts));
   l.counts = take(4ll * c.lists * a.columns * c.chunks);
   l.start = take(4ll * c.lists * a.columns);
   l.end = take(4ll * c.lists * a.columns);
@@ -574,11 +623,12 @@ Layout layout_of(const BlockArgs &a) {
   return l;
 }
 
-template <typename T, int DP, int KG>
+template <typename T, int DP, int KG, int S>
 void launch_dkv(const BlockArgs &a, const Columns &c, const float *delta, hipStream_t st) {
   Columns cols = c;
   cols.sub = (int)ceil_div(1 << a.block_n_log2, 32 * KG);
-  hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG>), dim3((unsigned)c.units * (unsigned)cols.sub), dim3(256), 0, st, a, cols, delta);
+  const int64_t grid = min((int64_t)2 * device_cu_count(), (int64_t)c.units * cols.sub);
+  hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG, S>), dim3((unsigned)grid), dim3(256), 0, st, a, cols, delta);
 }
 
 template <typename T, int DP>
@@ -587,27 +637,28 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   Columns &c = l.columns;
   float *delta = reinterpret_cast<float *>(work + l.delta);
   c.odd = reinterpret_cast<int *>(work + l.odd);
+  c.next = c.odd + 1;
   c.counts = reinterpret_cast<int *>(work + l.counts);
   c.start = reinterpret_cast<int *>(work + l.start);
   c.end = reinterpret_cast<int *>(work + l.end);
   c.unit = reinterpret_cast<int *>(work + l.unit);
   c.rows = reinterpret_cast<int *>(work + l.rows);
   c.partial = reinterpret_cast<float *>(work + l.partial);
-  if (a.queries && a.heads) {
+  if (a.rows) {
     const long long lists = (long long)c.lists * a.rows, tiles = ceil_div((long long)min(a.block_m, a.queries) * a.group, 128);
     LAPIS_REQUIRE(lists * tiles * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld rows of the structure", lists);
-    hipLaunchKernelGGL((block_dq_kernel<T, DP, 4, 64>), dim3((unsigned)(lists * tiles)), dim3(256), 0, st, a, (int)tiles, delta);
+    hipLaunchKernelGGL((block_dq_kernel<T, DP, 4, 64>), dim3((unsigned)(lists * tiles)), dim3(256), 0, st, a, (int)tiles, delta, c.odd);
   }
   if (c.lists && a.columns) {
-    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1), 0, st, c.odd);
+    if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
     const dim3 grid((unsigned)c.chunks, (unsigned)ceil_div(a.columns, kColumnsInLds), (unsigned)c.lists);
-    LAPIS_REQUIRE(c.lists <= 65535 && (int64_t)c.units * 8 * 256 < (INT64_C(1) << 32), "block_attention_backward: %d lists, %d units", c.lists, c.units);
+    LAPIS_REQUIRE(c.lists <= 65535 && (int64_t)c.units * 8 <= INT32_MAX, "block_attention_backward: %d lists, %d units", c.lists, c.units);
     hipLaunchKernelGGL(columns_kernel<false>, grid, dim3(64), 0, st, a, c);
     hipLaunchKernelGGL(columns_scan_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
     hipLaunchKernelGGL(columns_kernel<true>, grid, dim3(64), 0, st, a, c);
-    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1>(a, c, delta, st);
-    else launch_dkv<T, DP, 2>(a, c, delta, st);
-    hipLaunchKernelGGL((join_units_kernel<T, DP>), dim3((unsigned)(c.lists * a.columns)), dim3(256), 0, st, a, c);
+    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, 2>(a, c, delta, st);
+    else launch_dkv<T, DP, 2, 4>(a, c, delta, st);
+    hipLaunchKernelGGL((join_units_kernel<T, DP>), dim3((unsigned)(c.lists * a.columns), 4), dim3(256), 0, st, a, c);
   }
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;

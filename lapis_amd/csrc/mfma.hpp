@@ -79,23 +79,26 @@ __device__ __forceinline__ vec8<T> columns_in_order(const typename T::elem *tile
 __device__ __forceinline__ void load_to_lds(const void *from, unsigned to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
-__device__ __forceinline__ void lds_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void load_word_to_lds(const void *from, unsigned to) {  // 4 bytes a lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+}
+// all but the last N loads of this wavefront
+template <int N = 0>
+__device__ __forceinline__ void lds_loads_done() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 template <typename E>
 __device__ __forceinline__ unsigned lds_address(const E *p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) E *)p;
 }
 
-// Any element that is infinite or NaN?
+// Any element that is infinite or NaN?  (An exponent of all ones, two elements a word: one more than that reaches the sign's bit.)
 template <typename T>
 __device__ __forceinline__ bool not_finite(vec8<T> x) {
-  const unsigned mask = std::is_same<T, Bf16>::value ? 0x7f80u : 0x7c00u;
-  const u16x8 b = __builtin_bit_cast(u16x8, x);
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= (b[i] & mask) == mask;
-  return bad;
+  const unsigned mask = std::is_same<T, Bf16>::value ? 0x7f807f80u : 0x7c007c00u, one = std::is_same<T, Bf16>::value ? 0x00800080u : 0x04000400u;
+  const v4u w = __builtin_bit_cast(v4u, x);
+  return ((((w[0] & mask) + one) | ((w[1] & mask) + one) | ((w[2] & mask) + one) | ((w[3] & mask) + one)) & 0x80008000u) != 0;
 }
-
 template <typename T>
 __device__ __forceinline__ vec8<T> finite_only(vec8<T> x) {
   const unsigned mask = std::is_same<T, Bf16>::value ? 0x7f80u : 0x7c00u;

@@ -124,6 +124,17 @@ def test_lists_out_of_order_twice_over_and_outside(gpu):
     check(gpu, "disorder", t, pos, crd, 32, 32, False)
 
 
+def test_positions_that_start_past_the_first_entry_and_end_before_the_last(gpu):
+    """Only what the rows name counts of a coordinate buffer that holds more; many entries in front, so that units of work
+    come before the first column's."""
+    t = make(1, 96, 200, 32, 1, 64, torch.float16, 3)
+    front = 3000
+    pos = (torch.tensor([0, 2, 2, 5], dtype=torch.int32) + front).cuda()
+    crd = torch.zeros(front + 5 + 700, dtype=torch.int32)
+    crd[front:front + 5] = torch.tensor([1, 4, 0, 3, 6])
+    check(gpu, "positions from 3000", t, pos, crd.cuda(), 32, 32, False)
+
+
 def test_positions_that_make_no_sense_are_not_followed(gpu):
     t = make(1, 96, 200, 2, 1, 64, torch.float16, 3)
     pos = torch.tensor([-5, 2, 1, 1000], dtype=torch.int32).cuda()  # rows [0, 2), nothing, [1, 4)
