@@ -51,6 +51,12 @@ __device__ __forceinline__ int place_of(int row, int piece) {
   return row * DP + ((piece ^ (COLUMNS ? column_turn<DP>(row) : turn<DP>(row))) * 8);
 }
 
+// The same for transposing reads of 16 columns, 32 lanes meeting the same 32 bytes of eight neighbouring rows.
+template <int DP>
+__device__ __forceinline__ int turn16(int row) {
+  return DP >= 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
+}
+
 // Transposing read: of the four rows and 16 columns that a group of 16 lanes points at (lane i: row i / 4, columns
 // 4 (i % 4) ..), lane i gets column i of the four rows.
 template <typename T>

@@ -1,5 +1,5 @@
 // Attention of one new token of each sequence over the pages of a cache that a CSR row lists.
-#include "attn.hpp"
+#include "mfma.hpp"
 
 namespace lapis {
 namespace {
@@ -12,90 +12,356 @@ struct PagedArgs {
   const float *k_scale, *v_scale;
   long long stride[3], scale_stride[3];
   long long pages, nnz;
-  int seqs, heads, kv_heads, dim, page_log2;
+  int seqs, lists, heads, kv_heads, group, dim, page_log2;
   bool each;  // a list per key-value head
   const int *pos, *crd, *tokens;
   float *lse;
   float scale;
+  int chunk, units, head_tiles;  // pages a unit, units of all lists, tiles of 16 heads
+  float *partial, *sums;         // of each unit: 16 x DP, and 16 maxima and sums
 };
 
 // Pages that a row lists and tokens that count in them, whatever pos and tokens hold.
 __device__ __forceinline__ void list_of(const PagedArgs &a, long long row, int *first, int *tokens) {
   const long long lo = min(max((long long)a.pos[row], 0ll), a.nnz), hi = min(max((long long)a.pos[row + 1], lo), a.nnz);
   *first = (int)lo;
-  *tokens = (int)max(0ll, min((long long)a.tokens[row], (hi - lo) << a.page_log2));
+  *tokens = a.pages > 0 ? (int)max(0ll, min((long long)a.tokens[row], (hi - lo) << a.page_log2)) : 0;
 }
 
-// One wavefront per (sequence, head): 64 tokens at a time, a token per lane for the scores, then elements of the row
-// per lane for the sum.
-template <typename T, bool F8>
-__global__ __launch_bounds__(64) void paged_simple_kernel(PagedArgs a) {
-  typedef typename T::elem elem;
-  const int lane = threadIdx.x, s = blockIdx.y, h = blockIdx.x, kh = h / (a.heads / a.kv_heads);
-  __shared__ float q[kMaxDim], weight[64];
-  __shared__ long long at[64];
-  const elem *qp = (const elem *)a.q + s * a.q_stride[0] + h * a.q_stride[1];
-  for (int d = lane; d < a.dim; d += 64) q[d] = (float)qp[d] * a.scale;
-  int first, tokens;
-  list_of(a, a.each ? (long long)s * a.kv_heads + kh : s, &first, &tokens);
-  float m = -INFINITY, l = 0.f, acc[kMaxDim / 64] = {};
-  __syncthreads();
-  for (int t0 = 0; t0 < tokens; t0 += 64) {
-    const int t = t0 + lane;
-    float score = -INFINITY;
-    long long from = -1;
-    float vs = 1.f;
-    if (t < tokens) {
-      const int page = a.crd[first + (t >> a.page_log2)];
-      if (page >= 0 && page < a.pages) {
-        const int in = t & ((1 << a.page_log2) - 1);
-        from = page * a.stride[0] + kh * a.stride[1] + in * a.stride[2];
-        float dot = 0.f, ks = 1.f;
-        if (F8) {
-          const long long sc = page * a.scale_stride[0] + kh * a.scale_stride[1] + in * a.scale_stride[2];
-          ks = a.k_scale[sc], vs = a.v_scale[sc];
-        }
-        for (int d = 0; d < a.dim; d += 8) {
-          float f[8];
-          if (F8) widen_f8(*(const v2i *)(a.k + from + d), f);
-          else widen<T>(*(const vec8<T> *)((const elem *)a.k + from + d), f);
-          for (int e = 0; e < 8; ++e) dot += q[d + e] * f[e];
-        }
-        score = dot * ks;
-      }
-    }
-    float top = score;
-    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float m_new = fmaxf(m, top), keep = m == m_new ? 1.f : expf(m - m_new);
-    const float p = score == -INFINITY ? 0.f : expf(score - m_new);
-    l = l * keep + group_sum<64>(p);
-    m = m_new;
-    __syncthreads();
-    weight[lane] = p * vs;
-    at[lane] = from;
-    __syncthreads();
-    for (int i = 0; i < kMaxDim / 64; ++i) acc[i] *= keep;
-    for (int j = 0; j < min(64, tokens - t0); ++j) {
-      if (at[j] < 0) continue;
-      for (int i = 0; i < kMaxDim / 64; ++i) {
-        const int d = i * 64 + lane;
-        if (d >= a.dim) continue;
-        const float x = F8 ? __builtin_amdgcn_cvt_f32_fp8((int)(unsigned char)a.v[at[j] + d], 0) : (float)((const elem *)a.v)[at[j] + d];
-        acc[i] += weight[j] * x;
-      }
+// Lists are cut into units of `chunk` pages.  Unit numbers start at pos[row] / chunk + row for each list, which leaves it at
+// least the units it needs, so they are known without a sum over the lists before; those left over do nothing.
+__device__ __forceinline__ long long unit_start(const PagedArgs &a, long long row) {
+  return min(max((long long)a.pos[row], 0ll), a.nnz) / a.chunk + row;
+}
+
+// The list that unit u belongs to (the last one that starts at or before it): 64 candidates a step.
+__device__ __forceinline__ int list_of_unit(const PagedArgs &a, int u, int lane) {
+  int lo = 0, n = a.lists;
+  while (n > 1) {
+    const int step = (n + 63) / 64, at = lo + lane * step;
+    const unsigned long long before = __ballot(lane * step < n && unit_start(a, at) <= u);
+    // positions that do not ascend may give any pattern: the highest candidate at or before u, or the first
+    const int pick = before ? 63 - __clzll(before) : 0;
+    lo += pick * step;
+    n = min(step, n - pick * step);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float rows_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  const unsigned a = p[0], b = p[1];
+  return halves_max(fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  const unsigned a = p[0], b = p[1];
+  return halves_sum(__builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+}
+
+// Eight e4m3 codes as eight numbers of a 16-bit type: exact.
+template <typename T>
+__device__ __forceinline__ vec8<T> codes_to(v2i x) {
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (std::is_same<T, Bf16>::value) {
+      r[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[i], 1.0f, false));
+      r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[i], 1.0f, true));
+    } else {
+      r[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)x[i], 1.0f, false));
+      r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)x[i], 1.0f, true));
     }
   }
-  elem *op = (elem *)a.out + s * a.out_stride[0] + h * a.out_stride[1];
-  for (int i = 0; i < kMaxDim / 64; ++i)
-    if (i * 64 + lane < a.dim) op[i * 64 + lane] = (elem)(l == 0.f ? 0.f : acc[i] / l);
-  if (a.lse && lane == 0) a.lse[(long long)s * a.heads + h] = l == 0.f ? -INFINITY : m + logf(l);
+  return __builtin_bit_cast(vec8<T>, r);
+}
+
+// A unit: up to 16 heads of a group against a stretch of a list.  Its four wavefronts take tiles of 32 tokens in turn, each by
+// itself; their maxima, sums and results are joined through LDS.
+//   S^T = K Q^T (16x16x32, a head per lane): K goes from memory into the operand's registers, each lane a piece of one token.
+//   O^T = V^T P^T: P^T stays in its registers, V goes through LDS, where it is read by columns.
+// The next tile is loaded into the same registers as soon as they have been used, so all but the first products of a tile
+// run under its successor's loads; eight wavefronts a compute unit have 64 KB (8-bit cache) to 128 KB on their way.
+// 8-bit codes are multiplied as they are (exact in 16 bits); a key's scale multiplies its score, a value's scale its weight.
+template <typename T, bool F8, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs a) {
+  typedef typename T::elem elem;
+  typedef typename std::conditional<F8, v2i, v4i>::type raw;  // eight elements
+  constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8, RP = 64 / PIECES, PASSES = 32 / RP, WIDTH = F8 ? 1 : 2;
+  struct Tokens {
+    long long at[32];     // element offsets of the tile's rows
+    float ks[32], vs[32];
+  };
+  union Own {  // of a wavefront
+    elem v[32 * DP];
+    float out[16][DP + 4];
+  };
+  __shared__ __attribute__((aligned(16))) Own own[4];
+  __shared__ __attribute__((aligned(16))) Tokens tokens_of[4][2];
+  __shared__ float top[4][16], total[4][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
+  unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
+  const int ht = block % a.head_tiles;
+  block /= a.head_tiles;
+  int kh = 0;
+  if (!a.each) {
+    kh = block % a.kv_heads;
+    block /= a.kv_heads;
+  }
+  const int u = block, row = list_of_unit(a, u, lane);
+  const int seq = a.each ? row / a.kv_heads : row;
+  if (a.each) kh = row - seq * a.kv_heads;
+  int first, count;
+  list_of(a, row, &first, &count);
+  const int part = (int)(u - unit_start(a, row));
+  const int chunk = a.chunk << a.page_log2;  // tokens
+  const long long from_l = (long long)part * chunk;
+  if (part < 0 || (from_l >= count && part != 0)) return;  // a unit number left over (a list without tokens still writes its zeros)
+  const int from = (int)from_l, n = min(chunk, count - from), tiles = (n + 31) / 32;
+  const int head0 = kh * a.group + ht * 16, heads = min(16, a.group - ht * 16);
+
+  // element j of step s of this lane's operands stands for dimension 32 s + 8 quarter + j
+  vec8<T> qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = 32 * s + 8 * quarter;
+    qf[s] = vec8<T>{};
+    if (col < heads && d < a.dim) qf[s] = *(const vec8<T> *)((const elem *)a.q + seq * a.q_stride[0] + (head0 + col) * a.q_stride[1] + d);
+  }
+  const float c = a.scale * 1.4426950408889634f;
+
+  Own &mine = own[wave];
+  int page = -1;  // of token `lane & 31` of the tile after the one being loaded
+  const auto page_of = [&](int t) {
+    const int x = t * 32 + (lane & 31);
+    page = t < tiles && x < n ? a.crd[first + ((from + x) >> a.page_log2)] : -1;
+  };
+  unsigned there_next = 0;
+  const auto put_tokens = [&](int t) {  // pages into places of rows, for lanes 0 .. 31
+    Tokens &x = tokens_of[wave][(t / 4) & 1];
+    const bool there = (unsigned)page < (unsigned long long)a.pages;
+    there_next = (unsigned)__ballot(there);
+    const int in = (from + t * 32 + (lane & 31)) & ((1 << a.page_log2) - 1);
+    if (lane < 32) {
+      x.at[lane] = there ? page * a.stride[0] + kh * a.stride[1] + in * a.stride[2] : 0;
+      if (F8) {
+        const long long s = there ? page * a.scale_stride[0] + kh * a.scale_stride[1] + in * a.scale_stride[2] : 0;
+        x.ks[lane] = there ? a.k_scale[s] : 0.f;
+        x.vs[lane] = there ? a.v_scale[s] : 0.f;
+      }
+    }
+    wave_lds_sync();
+  };
+  raw kr[2][KS], vr[PASSES];
+  const auto load = [&](int t) {
+    const Tokens &x = tokens_of[wave][(t / 4) & 1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char *k = a.k + x.at[16 * i + col] * WIDTH;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = 32 * s + 8 * quarter;
+        kr[i][s] = *(const raw *)(k + (d < a.dim ? d : 0) * WIDTH);
+        if (a.dim < 32 * s + 32 && d >= a.dim) kr[i][s] = raw{};
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int d = (lane % PIECES) * 8;
+      vr[p] = *(const raw *)(a.v + (x.at[p * RP + lane / PIECES] + (d < a.dim ? d : 0)) * WIDTH);
+    }
+  };
+
+  v4f acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f, unit = 0x1p-126f;  // `unit`: what acc's weights are counted in (8-bit cache, float16)
+  page_of(wave);
+  put_tokens(wave);
+  unsigned there = there_next;
+  if (wave < tiles) load(wave);
+  page_of(wave + 4);
+  for (int t = wave; t < tiles; t += 4) {
+    const Tokens &tok = tokens_of[wave][(t / 4) & 1];
+    v4f s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        vec8<T> k;
+        if constexpr (F8) k = codes_to<T>(kr[i][x]);
+        else k = __builtin_bit_cast(vec8<T>, kr[i][x]);
+        s[i] = mfma16(k, qf[x], s[i]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int r = p * RP + lane / PIECES, piece = lane % PIECES;
+      vec8<T> v;
+      if constexpr (F8) v = codes_to<T>(vr[p]);
+      else v = __builtin_bit_cast(vec8<T>, vr[p]);
+      if (there != 0xffffffffu && !(there >> r & 1)) v = vec8<T>{};  // whatever an unused slot holds: 0 times it must be 0
+      *(vec8<T> *)(mine.v + r * DP + ((piece ^ turn16<DP>(r)) * 8)) = v;
+    }
+    const unsigned now = there;
+    float ks[8], vs[8];
+    if (F8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const v4f k4 = *(const v4f *)(tok.ks + 16 * i + 4 * quarter), v4 = *(const v4f *)(tok.vs + 16 * i + 4 * quarter);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ks[4 * i + e] = k4[e], vs[4 * i + e] = v4[e];
+      }
+    }
+    float unit_to = unit;
+    if (F8 && std::is_same<T, F16>::value) {
+      // weights times scales could leave float16's range: they are counted in the largest scale so far, a power of two
+      const float most = rows_max(__builtin_bit_cast(float, group_max<16>(__builtin_bit_cast(unsigned, fmaxf(tok.vs[lane & 31], 0.f)))));
+      if (most > unit) unit_to = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, most) & 0x7f800000u) + 0x00800000u);
+    }
+    put_tokens(t + 4);
+    there = there_next;
+    if (t + 4 < tiles) load(t + 4);
+    page_of(t + 8);
+
+    float best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = s[i][e] * (F8 ? c * ks[4 * i + e] : c);
+        if (now != 0xffffffffu && !(now >> (16 * i + 4 * quarter + e) & 1)) x = -INFINITY;
+        s[i][e] = x;
+        best = fmaxf(best, x);
+      }
+    best = rows_max(best);
+    // the maximum in use moves only when it is left behind by more than 2^8
+    if (__any(best > m + 8.f) || unit_to != unit) {
+      const float to = fmaxf(m, best), keep = to == m ? 1.f : __builtin_amdgcn_exp2f(m - to);
+      const float by = unit_to == unit ? keep : keep * (unit / unit_to);
+      m = to;
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] *= by;
+      unit = unit_to;
+    }
+    const float off = m == -INFINITY ? 0.f : m, per_unit = 1.f / unit;
+    vec8<T> pf;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(s[i][e] - off);
+        l += p;
+        float w = p;
+        if (F8) w = std::is_same<T, F16>::value ? p * (vs[4 * i + e] * per_unit) : p * vs[4 * i + e];
+        pf[4 * i + e] = (elem)w;
+      }
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      const int r = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
+      const elem *p = mine.v + r * DP + ((d >> 3) ^ turn16<DP>(r)) * 8 + (d & 7);  // row + 16 has the same order of pieces
+      acc[i] = mfma16(join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP)), pf, acc[i]);
+    }
+    wave_lds_sync();
+  }
+  l = rows_sum(l);
+  if (F8 && std::is_same<T, F16>::value) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i] *= unit;
+  }
+  if (quarter == 0) top[wave][col] = m, total[wave][col] = l;
+#pragma unroll
+  for (int i = 0; i < DT; ++i) *(v4f *)(&mine.out[col][16 * i + 4 * quarter]) = acc[i];
+  __syncthreads();
+
+  const bool whole = count <= chunk;
+  const long long unit_id = (long long)(a.each ? u : u * a.kv_heads + kh) * a.head_tiles + ht;
+  for (int x = tid; x < 16 * PIECES; x += 256) {
+    const int h = x / PIECES, d = (x % PIECES) * 8;
+    if (h >= heads || d >= a.dim) continue;
+    float most = top[0][h], sum = 0.f, o[8] = {};
+#pragma unroll
+    for (int w = 1; w < 4; ++w) most = fmaxf(most, top[w][h]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = top[w][h] == most ? 1.f : __builtin_amdgcn_exp2f(top[w][h] - most);
+      sum += by * total[w][h];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += by * own[w].out[h][d + e];
+    }
+    if (whole) {
+      const float by = 1.f / sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = sum == 0.f ? 0.f : o[e] * by;
+      *(vec8<T> *)((elem *)a.out + seq * a.out_stride[0] + (head0 + h) * a.out_stride[1] + d) = narrow<T>(o);
+      if (a.lse && d == 0)
+        a.lse[(long long)seq * a.heads + head0 + h] = sum == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    } else {
+      float *to = a.partial + (unit_id * 16 + h) * DP + d;
+      *(v4f *)to = v4f{o[0], o[1], o[2], o[3]};
+      *(v4f *)(to + 4) = v4f{o[4], o[5], o[6], o[7]};
+      if (d == 0) *(v2f *)(a.sums + (unit_id * 16 + h) * 2) = v2f{most, sum};
+    }
+  }
+}
+
+// Lists of several units: one workgroup per (sequence, head), the units in their order.
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs a) {
+  typedef typename T::elem elem;
+  const int lane = threadIdx.x, seq = blockIdx.y, head = blockIdx.x, kh = head / a.group, in = head - kh * a.group;
+  const long long row = a.each ? (long long)seq * a.kv_heads + kh : seq;
+  int first, count;
+  list_of(a, row, &first, &count);
+  const int chunk = a.chunk << a.page_log2, needed = (int)(((long long)count + chunk - 1) / chunk);
+  if (needed <= 1) return;
+  const long long u0 = unit_start(a, row);
+  const int units = (int)min((long long)needed, a.units - u0);  // fewer only where positions descend
+  const auto id = [&](int x) { return ((a.each ? u0 + x : (u0 + x) * a.kv_heads + kh) * a.head_tiles + in / 16) * 16 + in % 16; };
+  float most = -INFINITY;
+  for (int x = lane; x < units; x += 64) most = fmaxf(most, a.sums[id(x) * 2]);
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+  float sum = 0.f, o[DP / 64] = {};
+  for (int x = 0; x < units; ++x) {
+    const v2f s = *(const v2f *)(a.sums + id(x) * 2);
+    const float by = s[0] == most ? 1.f : __builtin_amdgcn_exp2f(s[0] - most);
+    sum += by * s[1];
+    const float *from = a.partial + id(x) * DP;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) o[i] += i * 64 + lane < a.dim ? by * from[i * 64 + lane] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < DP / 64; ++i)
+    if (i * 64 + lane < a.dim) ((elem *)a.out)[seq * a.out_stride[0] + head * a.out_stride[1] + i * 64 + lane] = (elem)(sum == 0.f ? 0.f : o[i] / sum);
+  if (a.lse && lane == 0) a.lse[(long long)seq * a.heads + head] = sum == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+}
+
+template <typename T, bool F8, int DP>
+int launch_paged(const PagedArgs &a, hipStream_t st) {
+  const long long blocks = (long long)a.units * (a.each ? 1 : a.kv_heads) * a.head_tiles;
+  LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "paged_attention: %lld units of work", blocks);
+  hipLaunchKernelGGL((paged_kernel<T, F8, DP>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  LAPIS_LAUNCH_CHECK();
+  if (a.nnz > a.chunk) {  // some list may have several units
+    hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(64), 0, st, a);
+    LAPIS_LAUNCH_CHECK();
+  }
+  return LAPIS_HIP_OK;
+}
+
+template <typename T, bool F8>
+int launch_paged(const PagedArgs &a, hipStream_t st) {
+  return a.dim <= 64 ? launch_paged<T, F8, 64>(a, st) : a.dim <= 128 ? launch_paged<T, F8, 128>(a, st) : launch_paged<T, F8, 256>(a, st);
 }
 
 int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_paged_args *p, PagedArgs *a) {
   const int rc = check_cache(what, c);
   if (rc != LAPIS_HIP_OK) return rc;
   LAPIS_REQUIRE(p, "%s: null arguments", what);
-  LAPIS_REQUIRE(p->seqs >= 0 && p->seqs <= 65535 * 16 && p->heads >= 0 && p->heads <= 65535 && p->heads % c->heads == 0,
+  LAPIS_REQUIRE(p->seqs >= 0 && p->seqs <= 65535 && p->heads >= 0 && p->heads <= 65535 && p->heads % c->heads == 0,
                 "%s: %lld sequences and %lld heads over a cache of %d", what, (long long)p->seqs, (long long)p->heads, c->heads);
   LAPIS_REQUIRE(p->lists == p->seqs || p->lists == p->seqs * c->heads, "%s: %lld lists of pages for %lld sequences", what,
                 (long long)p->lists, (long long)p->seqs);
@@ -124,7 +390,24 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
   a->tokens = p->tokens;
   a->lse = p->lse;
   a->scale = p->scale;
+  a->lists = (int)p->lists;
+  a->group = a->heads / c->heads;
+  a->head_tiles = (int)ceil_div(max(a->group, 1), 16);
+  // Units for two workgroups a compute unit, of 128 to 1024 tokens: shorter ones cost more than they spread (a partial result
+  // and its join), longer ones leave compute units waiting for the last.
+  const int64_t copies = (int64_t)a->head_tiles * (a->each ? 1 : c->heads), wanted = max(2 * device_cu_count(), 1);
+  const int64_t tokens = min(max(p->nnz * c->page * copies / wanted, (int64_t)128), (int64_t)1024);
+  a->chunk = (int)max(tokens / c->page, (int64_t)1);
+  a->units = (int)(p->nnz / a->chunk + p->lists);
   return LAPIS_HIP_OK;
+}
+
+// bytes of the partial results, and where the sums lie behind them
+int64_t partial_bytes(const PagedArgs &a, int64_t *sums_at) {
+  const int dp = a.dim <= 64 ? 64 : a.dim <= 128 ? 128 : 256;
+  const int64_t ids = (int64_t)a.units * (a.each ? 1 : a.kv_heads) * a.head_tiles * 16;
+  *sums_at = ids * dp * 4;
+  return a.nnz > a.chunk ? ids * (dp + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -137,7 +420,8 @@ extern "C" int lapis_hip_paged_attention_work(const lapis_hip_kv_cache *cache, c
   const int rc = read_paged("paged_attention", cache, args, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   LAPIS_REQUIRE(bytes, "paged_attention: null result");
-  *bytes = 0;
+  int64_t sums_at;
+  *bytes = partial_bytes(a, &sums_at);
   return LAPIS_HIP_OK;
 }
 
@@ -149,11 +433,14 @@ extern "C" int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const 
   LAPIS_REQUIRE(a.q && a.out && a.pos && a.tokens && (a.crd || a.nnz == 0), "paged_attention: null operands");
   LAPIS_REQUIRE(aligned16(a.q) && aligned16(a.out) && strides_of_8(args->q.stride, 3) && strides_of_8(args->out.stride, 3),
                 "paged_attention: queries or results that are not on 16-byte boundaries or strides that are no multiples of 8");
+  int64_t sums_at;
+  if (partial_bytes(a, &sums_at) > 0) {
+    LAPIS_REQUIRE(args->work && aligned16(args->work), "paged_attention: work that is null or not on a 16-byte boundary");
+    a.partial = static_cast<float *>(args->work);
+    a.sums = reinterpret_cast<float *>(static_cast<char *>(args->work) + sums_at);
+  }
   const bool f8 = cache->dtype == LAPIS_HIP_F8E4M3, bf16 = args->dtype == LAPIS_HIP_BF16;
-  const auto kernel = bf16 ? (f8 ? paged_simple_kernel<Bf16, true> : paged_simple_kernel<Bf16, false>)
-                           : (f8 ? paged_simple_kernel<F16, true> : paged_simple_kernel<F16, false>);
-  LAPIS_REQUIRE(a.seqs <= 65535, "paged_attention: %d sequences", a.seqs);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(64), 0, as_stream(stream), a);
-  LAPIS_LAUNCH_CHECK();
-  return LAPIS_HIP_OK;
+  const hipStream_t st = as_stream(stream);
+  if (bf16) return f8 ? launch_paged<Bf16, true>(a, st) : launch_paged<Bf16, false>(a, st);
+  return f8 ? launch_paged<F16, true>(a, st) : launch_paged<F16, false>(a, st);
 }
