@@ -308,11 +308,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
   }
 }
 
-// Lists of several units: one workgroup per (sequence, head), the units in their order.
+// Lists of several units: one workgroup per (sequence, head), 64 units at a time, a quarter of them to each wavefront and
+// four of those on their way (one after the other they took 45 us for 64 units); always in the same order.
 template <typename T, int DP>
-__global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   typedef typename T::elem elem;
-  const int lane = threadIdx.x, seq = blockIdx.y, head = blockIdx.x, kh = head / a.group, in = head - kh * a.group;
+  constexpr int E = DP / 64;
+  typedef float vec __attribute__((ext_vector_type(E)));
+  __shared__ float factor[64];
+  __shared__ __attribute__((aligned(16))) float part[3][DP];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.y, head = blockIdx.x, kh = head / a.group, in = head - kh * a.group;
   const long long row = a.each ? (long long)seq * a.kv_heads + kh : seq;
   int first, count;
   list_of(a, row, &first, &count);
@@ -324,18 +329,45 @@ __global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs a) {
   float most = -INFINITY;
   for (int x = lane; x < units; x += 64) most = fmaxf(most, a.sums[id(x) * 2]);
   for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-  float sum = 0.f, o[DP / 64] = {};
-  for (int x = 0; x < units; ++x) {
-    const v2f s = *(const v2f *)(a.sums + id(x) * 2);
-    const float by = s[0] == most ? 1.f : __builtin_amdgcn_exp2f(s[0] - most);
-    sum += by * s[1];
-    const float *from = a.partial + id(x) * DP;
+  float sum = 0.f, o[E] = {};
+  for (int x0 = 0; x0 < units; x0 += 64) {
+    float by = 0.f, s1 = 0.f;
+    if (x0 + lane < units) {
+      const v2f s = *(const v2f *)(a.sums + id(x0 + lane) * 2);
+      by = s[0] == most ? 1.f : __builtin_amdgcn_exp2f(s[0] - most);
+      s1 = s[1];
+    }
+    sum += group_sum<64>(by * s1);
+    __syncthreads();
+    if (wave == 0) factor[lane] = by;
+    __syncthreads();
+    const int n = min(64, units - x0);
+    for (int x = wave; x < n; x += 16) {
+      vec f[4];
 #pragma unroll
-    for (int i = 0; i < DP / 64; ++i) o[i] += i * 64 + lane < a.dim ? by * from[i * 64 + lane] : 0.f;
+      for (int i = 0; i < 4; ++i) f[i] = *(const vec *)(a.partial + id(x0 + min(x + 4 * i, n - 1)) * DP + lane * E);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = x + 4 * i < n ? factor[x + 4 * i] : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += x + 4 * i < n ? w * f[i][e] : 0.f;
+      }
+    }
   }
+  if (wave > 0) {
 #pragma unroll
-  for (int i = 0; i < DP / 64; ++i)
-    if (i * 64 + lane < a.dim) ((elem *)a.out)[seq * a.out_stride[0] + head * a.out_stride[1] + i * 64 + lane] = (elem)(sum == 0.f ? 0.f : o[i] / sum);
+    for (int e = 0; e < E; ++e) part[wave - 1][lane * E + e] = o[e];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = lane * E + e;
+    o[e] += part[0][d];
+    o[e] += part[1][d];
+    o[e] += part[2][d];
+    if (d < a.dim) ((elem *)a.out)[seq * a.out_stride[0] + head * a.out_stride[1] + d] = (elem)(sum == 0.f ? 0.f : o[e] / sum);
+  }
   if (a.lse && lane == 0) a.lse[(long long)seq * a.heads + head] = sum == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
@@ -346,7 +378,7 @@ int launch_paged(const PagedArgs &a, hipStream_t st) {
   hipLaunchKernelGGL((paged_kernel<T, F8, DP>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   LAPIS_LAUNCH_CHECK();
   if (a.nnz > a.chunk) {  // some list may have several units
-    hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(64), 0, st, a);
+    hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(256), 0, st, a);
     LAPIS_LAUNCH_CHECK();
   }
   return LAPIS_HIP_OK;
