@@ -95,18 +95,30 @@ struct SelectArgs {
   long long list_entries;  // of one list, where every list has the same
 };
 
-__host__ __device__ inline long long floor_div(long long a, long long b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+// 64-bit division takes a hundred instructions on the device; most operands here fit 32 bits.
+__host__ __device__ inline long long quotient(long long a, long long b) {  // both non-negative
+  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+__host__ __device__ inline long long floor_div(long long a, long long b) { return a >= 0 ? quotient(a, b) : -quotient(-a + b - 1, b); }
 
 // sum over i < n of floor((a i + b) / m), all non-negative, by the steps of Euclid's algorithm
 __host__ __device__ inline long long floor_sum(long long n, long long m, long long a, long long b) {
   long long total = 0;
   while (n > 0) {
-    if (a >= m) total += (n - 1) * n / 2 * (a / m), a %= m;
-    if (b >= m) total += n * (b / m), b %= m;
+    if (a >= m) {
+      const long long q = quotient(a, m);
+      total += (n - 1) * n / 2 * q;
+      a -= q * m;
+    }
+    if (b >= m) {
+      const long long q = quotient(b, m);
+      total += n * q;
+      b -= q * m;
+    }
     const long long top = a * n + b;
     if (top < m) break;
-    n = top / m;
-    b = top % m;
+    n = quotient(top, m);
+    b = top - n * m;
     const long long t = m;
     m = a;
     a = t;
@@ -150,97 +162,215 @@ __device__ __forceinline__ unsigned sortable(float x) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-// One wavefront per row; `key(j)` gives block j's score.  A candidate's bits are found from the top: the largest
-// threshold that still leaves `need` blocks at or above it.
-template <typename Key>
-__device__ __forceinline__ void take_best(const SelectArgs &a, long long seen, int *out, int lane, Key key,
-                                          const int *__restrict__ table) {
-  const long long need = seen < a.count ? seen : a.count;
-  unsigned threshold = 0;
-  if (need < seen) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned candidate = threshold | (1u << bit);
-      int n = 0;
-      for (long long j = lane; j < seen; j += 64) n += key(j) >= candidate;
-      n = group_sum<64>(n);
-      if (n >= need) threshold = candidate;
-    }
+// What a row may see, and where its entries go.
+struct RowPlace {
+  int seen;
+  int first;
+};
+
+// Of the rows r0 .. of a list, lane i's.  (All lanes of a wavefront call.)
+__device__ __forceinline__ RowPlace place_of_row(const SelectArgs &a, long long list, long long r0, int lane) {
+  const long long b = list / a.heads, h = list - b * a.heads, r = r0 + lane;
+  if (a.blocks) {
+    long long before = 0;
+    for (long long i = lane; i < b; i += 64) before += min(max(0ll, min((long long)a.blocks[i], a.columns)), a.count);
+    for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o, 64);
+    const long long seen = max(0ll, min((long long)a.blocks[b], a.columns));
+    return {(int)seen, (int)(before * a.heads * a.rows + (h * a.rows + r) * min(seen, a.count))};
   }
-  long long above = 0;
-  if (need < seen) {
+  const long long seen = r < a.rows ? blocks_seen(a, r) : 0;
+  int mine = (int)min(seen, a.count), upto = mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += x;
+  }
+  return {(int)seen, (int)(list * a.list_entries + entries_before(a, r0)) + upto - mine};
+}
+
+// The page or block that column j of list (b, h) stands for; -1: none.
+__device__ __forceinline__ long long row_of_codes(const SelectArgs &a, long long b, long long j) {
+  if (!a.table) return j;
+  const long long page = a.table[b * a.table_width + j];
+  return page >= 0 && page < a.pages ? page : -1;
+}
+
+// The `need` best of `seen` keys, fewer than seen; `key(i)` is this lane's key of block 64 i + lane (0 from `seen` on), NV > 0: i
+// below NV, from registers.  Bit by bit from the first one in which the keys differ: the largest threshold that leaves at least
+// `need` blocks at or above it, or one that leaves just as many.  Equal keys at the threshold are taken from the lowest block on.
+template <int NV, typename Key>
+__device__ __forceinline__ void take_best(int seen, int need, int *out, int lane, const int *__restrict__ table, Key key) {
+  const int steps = NV ? NV : (seen + 63) / 64;
+  unsigned most = 0, least = 0xffffffffu;
+#pragma unroll NV ? NV : 1
+  for (int i = 0; i < steps; ++i) {
+    most = max(most, key(i));
+    least = min(least, i * 64 + lane < seen ? key(i) : 0xffffffffu);
+  }
+  most = group_max<64>(most);
+  least = ~group_max<64>(~least);
+  const int top = most == least ? -1 : 31 - __clz(most ^ least);
+  unsigned threshold = top < 0 ? most : top == 31 ? 0u : most >> (top + 1) << (top + 1);  // what all have in common
+  int at_or_above = seen;
+  for (int bit = top; bit >= 0 && at_or_above != need; --bit) {
+    const unsigned candidate = threshold | (1u << bit);
     int n = 0;
-    for (long long j = lane; j < seen; j += 64) n += key(j) > threshold;
-    above = group_sum<64>(n);
+#pragma unroll NV ? NV : 1
+    for (int i = 0; i < steps; ++i) n += __popcll(__ballot(key(i) >= candidate));
+    if (n >= need) threshold = candidate, at_or_above = n;
   }
-  long long equal_left = need - above, at = 0;
-  for (long long j0 = 0; j0 < seen && at < need; j0 += 64) {
-    const long long j = j0 + lane;
-    bool take = j < seen;
-    if (need < seen) {
-      const unsigned k = take ? key(j) : 0u;
-      const bool equal = take && k == threshold;
-      const unsigned long long ties = __ballot(equal);
-      const int before = __popcll(ties & ((1ull << lane) - 1));
-      take = take && (k > threshold || (equal && before < equal_left));
-      equal_left -= min((long long)__popcll(ties), equal_left);
-    }
+  int equal_left = need;  // of the blocks at the threshold itself
+  if (at_or_above != need) {
+    int above = 0;
+#pragma unroll NV ? NV : 1
+    for (int i = 0; i < steps; ++i) above += __popcll(__ballot(key(i) > threshold));
+    equal_left = need - above;
+  }
+  int at = 0;
+#pragma unroll NV ? NV : 1
+  for (int i = 0; i < steps; ++i) {
+    const int j = i * 64 + lane;
+    const bool equal = j < seen && key(i) == threshold;
+    const unsigned long long ties = __ballot(equal), below = (1ull << lane) - 1;
+    const bool take = j < seen && (key(i) > threshold || (equal && __popcll(ties & below) < equal_left));
+    equal_left -= min(__popcll(ties), equal_left);
     const unsigned long long taken = __ballot(take);
-    if (take) out[at + __popcll(taken & ((1ull << lane) - 1))] = table ? table[j] : (int)j;
+    if (take) out[at + __popcll(taken & below)] = table ? table[j] : j;
     at += __popcll(taken);
   }
 }
 
-__device__ __forceinline__ float block_score(const SelectArgs &a, long long b, long long h, const signed char *q, long long j) {
-  long long page = j;
-  const signed char *k = a.k + h * a.k_stride[1];
-  const float *s = a.scales + h * a.scale_stride[1];
-  if (a.table) {
-    page = a.table[b * a.table_width + j];
-    if (page < 0 || page >= a.pages) return __builtin_nanf("");
-  } else {
-    k += b * a.k_stride[0];
-    s += b * a.scale_stride[0];
-  }
-  k += page * a.k_stride[2];
-  int dot = 0;
-  for (int d = 0; d < a.dim; d += 8) {
-    const v2i x = *(const v2i *)(q + d), y = *(const v2i *)(k + d);
-    dot = __builtin_amdgcn_sdot4(x[0], y[0], dot, false);
-    dot = __builtin_amdgcn_sdot4(x[1], y[1], dot, false);
-  }
-  return (float)dot * s[page * a.scale_stride[2]];
+__device__ __forceinline__ void take_all(int seen, int *out, int lane, const int *__restrict__ table) {
+  for (int j = lane; j < seen; j += 64) out[j] = table ? table[j] : j;
 }
 
-__global__ __launch_bounds__(64) void block_select_kernel(SelectArgs a, unsigned *scores) {
-  const long long row = linear_block();
-  const int lane = threadIdx.x;
-  const long long lists = a.batch * a.heads;
-  if (row >= lists * a.rows) return;
-  const long long list = row / a.rows, r = row - list * a.rows, b = list / a.heads, h = list - b * a.heads;
-  long long seen, first;
-  if (a.blocks) {
-    long long before = 0;
-    for (long long i = lane; i < b; i += 64) {
-      const long long n = max(0ll, min((long long)a.blocks[i], a.columns));
-      before += min(n, a.count);
+// A workgroup takes 16 rows of a list.  Scores come from matrix instructions (16 rows x 16 blocks, 64 codes a step; the
+// queries' codes stay in registers), go to LDS as sortable numbers and are taken by a wavefront per row, NV a lane.  The search
+// is one chain of compare, count and branch: it takes many wavefronts to fill the time between, and 64 rows a workgroup, which
+// read the codes of K a quarter as often, left room for a quarter of them (174 us against 96 for 131 072 rows of up to 256).
+template <int NV, int KC>
+__global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long long tiles_of_list) {
+  constexpr int RT = 16, STRIDE = NV * 64 + 4;  // rows four apart start 16 banks apart
+  __shared__ unsigned keys[RT][STRIDE];
+  __shared__ RowPlace places[RT];
+  __shared__ int most_seen;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+  const long long block = xcd_contiguous_block(linear_block(), gridDim.x * gridDim.y);
+  const long long list = block / tiles_of_list, r0 = (block - list * tiles_of_list) * RT, b = list / a.heads, h = list - b * a.heads;
+  if (list >= a.batch * a.heads) return;
+  const int rows = (int)min((long long)RT, a.rows - r0);
+  if (wave == 0) {
+    const RowPlace p = place_of_row(a, list, r0, lane);
+    if (lane < RT) places[lane] = p;
+    const unsigned top = group_max<64>(lane < rows ? (unsigned)p.seen : 0u);
+    if (lane == 0) most_seen = (int)top;
+    const long long row = list * a.rows + r0 + lane;
+    if (lane < rows) {
+      a.pos[row] = p.first;
+      if (row == a.batch * a.heads * a.rows - 1) a.pos[row + 1] = p.first + (int)min((long long)p.seen, a.count);
     }
-    for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o, 64);
-    seen = max(0ll, min((long long)a.blocks[b], a.columns));
-    first = before * a.heads * a.rows + (h * a.rows + r) * min(seen, a.count);
-  } else {
-    seen = blocks_seen(a, r);
-    first = list * a.list_entries + entries_before(a, r);
   }
-  if (lane == 0) {
-    a.pos[row] = (int)first;
-    if (row == lists * a.rows - 1) a.pos[row + 1] = (int)(first + min(seen, a.count));
-  }
-  unsigned *mine = scores + row * a.columns;
-  if (seen > a.count)
-    for (long long j = lane; j < seen; j += 64)
-      mine[j] = j < a.sink || j >= seen - a.local ? 0xffffffffu : sortable(block_score(a, b, h, a.q + row * a.dim, j));
+  v4i qf[RT / 16][KC];
+#pragma unroll
+  for (int x = 0; x < RT / 16; ++x)
+#pragma unroll
+    for (int s = 0; s < KC; ++s) {
+      const int r = 16 * x + col, d = 64 * s + 16 * quarter;
+      qf[x][s] = v4i{0, 0, 0, 0};
+      if (r < rows) {
+        const signed char *q = a.q + (list * a.rows + r0 + r) * a.dim + d;
+        if (d < a.dim) *(v2i *)&qf[x][s] = *(const v2i *)q;
+        if (d + 8 < a.dim) ((v2i *)&qf[x][s])[1] = *(const v2i *)(q + 8);
+      }
+    }
+  __syncthreads();
+  const int seen_all = most_seen;
+  if (seen_all > a.count)  // else every row takes what it sees
+    for (int j0 = wave * 16; j0 < seen_all; j0 += 64) {
+      const int j = j0 + col;
+      const long long from = j < seen_all ? row_of_codes(a, b, j) : -1;
+      float scale = __builtin_nanf("");
+      v4i kf[KC];
+#pragma unroll
+      for (int s = 0; s < KC; ++s) kf[s] = v4i{0, 0, 0, 0};
+      if (from >= 0) {
+        const signed char *k = a.k + h * a.k_stride[1] + from * a.k_stride[2] + (a.table ? 0 : b * a.k_stride[0]);
+        scale = a.scales[h * a.scale_stride[1] + from * a.scale_stride[2] + (a.table ? 0 : b * a.scale_stride[0])];
+#pragma unroll
+        for (int s = 0; s < KC; ++s) {
+          const int d = 64 * s + 16 * quarter;
+          if (d < a.dim) *(v2i *)&kf[s] = *(const v2i *)(k + d);
+          if (d + 8 < a.dim) ((v2i *)&kf[s])[1] = *(const v2i *)(k + d + 8);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < RT / 16; ++x) {
+        v4i dot = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KC; ++s) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[x][s], kf[s], dot, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keys[16 * x + 4 * quarter + e][j] = sortable((float)dot[e] * scale);
+      }
+    }
+  __syncthreads();
   const int *table = a.table ? a.table + b * a.table_width : nullptr;
-  take_best(a, seen, a.crd + first, lane, [&](long long j) { return mine[j]; }, table);
+  for (int r = wave; r < rows; r += 4) {
+    const int seen = places[r].seen, need = (int)min((long long)seen, a.count);
+    int *out = a.crd + places[r].first;
+    if (need == seen) {
+      take_all(seen, out, lane, table);
+      continue;
+    }
+    unsigned k[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = i * 64 + lane;
+      k[i] = j >= seen ? 0u : j < a.sink || j >= seen - a.local ? 0xffffffffu : keys[r][j];
+    }
+    take_best<NV>(seen, need, out, lane, table, [&](int i) { return k[i]; });
+  }
+}
+
+// Rows of more blocks or longer codes than that: scores go through memory, one wavefront per row.
+__global__ __launch_bounds__(64) void block_select_long_kernel(SelectArgs a, unsigned *scores, long long row0) {
+  const long long at = linear_block(), row = row0 + at;
+  const int lane = threadIdx.x;
+  if (row >= a.batch * a.heads * a.rows) return;
+  const long long list = row / a.rows, b = list / a.heads, h = list - b * a.heads;
+  RowPlace p = place_of_row(a, list, row - list * a.rows, lane);
+  p.seen = __builtin_amdgcn_readfirstlane(p.seen);
+  p.first = __builtin_amdgcn_readfirstlane(p.first);
+  const int need = (int)min((long long)p.seen, a.count);
+  if (lane == 0) {
+    a.pos[row] = p.first;
+    if (row == a.batch * a.heads * a.rows - 1) a.pos[row + 1] = p.first + need;
+  }
+  const int *table = a.table ? a.table + b * a.table_width : nullptr;
+  if (need == p.seen) {
+    take_all(p.seen, a.crd + p.first, lane, table);
+    return;
+  }
+  unsigned *mine = scores + at * a.columns;  // a lane reads what it has written itself
+  const signed char *q = a.q + row * a.dim;
+  for (long long j = lane; j < p.seen; j += 64) {
+    unsigned key = 0xffffffffu;
+    if (j >= a.sink && j < p.seen - a.local) {
+      const long long from = row_of_codes(a, b, j);
+      float score = __builtin_nanf("");
+      if (from >= 0) {
+        const signed char *k = a.k + h * a.k_stride[1] + from * a.k_stride[2] + (a.table ? 0 : b * a.k_stride[0]);
+        int dot = 0;
+        for (int d = 0; d < a.dim; d += 8) {
+          const v2i x = *(const v2i *)(q + d), y = *(const v2i *)(k + d);
+          dot = __builtin_amdgcn_sdot4(x[0], y[0], dot, false);
+          dot = __builtin_amdgcn_sdot4(x[1], y[1], dot, false);
+        }
+        score = (float)dot * a.scales[h * a.scale_stride[1] + from * a.scale_stride[2] + (a.table ? 0 : b * a.scale_stride[0])];
+      }
+      key = sortable(score);
+    }
+    mine[j] = key;
+  }
+  take_best<0>(p.seen, need, a.crd + p.first, lane, table, [&](int i) { return i * 64 + lane < p.seen ? mine[i * 64 + lane] : 0u; });
 }
 
 __global__ void empty_positions_kernel(int *pos) { pos[0] = 0; }
@@ -330,12 +460,35 @@ extern "C" int lapis_hip_block_select_entries(const lapis_hip_select_args *args,
   return LAPIS_HIP_OK;
 }
 
+namespace lapis {
+namespace {
+
+constexpr int kShortColumns = 2048, kShortDim = 256;
+constexpr int64_t kScoreBytes = INT64_C(256) << 20;  // of rows that go through memory at a time
+
+bool short_rows(const SelectArgs &a) { return a.columns <= kShortColumns && a.dim <= kShortDim; }
+
+// Rows at a time of those that go through memory.
+long long rows_at_once(const SelectArgs &a) { return max(1ll, min(a.batch * a.heads * a.rows, kScoreBytes / (4 * max(a.columns, 1ll)))); }
+
+template <int NV>
+void launch_select(const SelectArgs &a, hipStream_t st) {
+  const long long tiles = ceil_div(a.rows, 16);
+  const dim3 grid = grid_of(a.batch * a.heads * tiles);
+  if (a.dim <= 64) hipLaunchKernelGGL((block_select_kernel<NV, 1>), grid, dim3(256), 0, st, a, tiles);
+  else if (a.dim <= 128) hipLaunchKernelGGL((block_select_kernel<NV, 2>), grid, dim3(256), 0, st, a, tiles);
+  else hipLaunchKernelGGL((block_select_kernel<NV, 4>), grid, dim3(256), 0, st, a, tiles);
+}
+
+}  // namespace
+}  // namespace lapis
+
 extern "C" int lapis_hip_block_select_work(const lapis_hip_select_args *args, int64_t *bytes) {
   SelectArgs a;
   const int rc = read_select("block_select", args, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   LAPIS_REQUIRE(bytes, "block_select: null result");
-  *bytes = 4 * a.batch * a.heads * a.rows * a.columns;
+  *bytes = short_rows(a) ? 0 : 4 * a.columns * rows_at_once(a);
   return LAPIS_HIP_OK;
 }
 
@@ -353,11 +506,24 @@ extern "C" int lapis_hip_block_select(const lapis_hip_select_args *args, lapis_h
       return LAPIS_HIP_OK;
     }
   } else {
-    LAPIS_REQUIRE(a.q && a.k && a.scales && a.crd && args->work, "block_select: null operands");
+    LAPIS_REQUIRE(a.q && a.k && a.scales && a.crd && (args->work || short_rows(a)), "block_select: null operands");
     const uintptr_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k);
     LAPIS_REQUIRE((low & 7u) == 0 && strides_of_8(args->k_stride, 3), "block_select: codes that are not on 8-byte boundaries or strides that are no multiples of 8");
   }
-  hipLaunchKernelGGL(block_select_kernel, grid_of(rows), dim3(64), 0, as_stream(stream), a, static_cast<unsigned *>(args->work));
+  const hipStream_t st = as_stream(stream);
+  if (!short_rows(a)) {
+    const long long some = rows_at_once(a);
+    for (long long row0 = 0; row0 < rows; row0 += some)
+      hipLaunchKernelGGL(block_select_long_kernel, grid_of(min(some, rows - row0)), dim3(64), 0, st, a, static_cast<unsigned *>(args->work), row0);
+  } else if (a.columns <= 256) {
+    launch_select<4>(a, st);
+  } else if (a.columns <= 512) {
+    launch_select<8>(a, st);
+  } else if (a.columns <= 1024) {
+    launch_select<16>(a, st);
+  } else {
+    launch_select<32>(a, st);
+  }
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
 }
