@@ -184,6 +184,187 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     a.lse[((long long)b * a.heads + head) * a.queries + query] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
+// Lists of few rows (queries of their own lists: a row block of one query has a row for each head of the group).  16 rows a
+// wavefront, which reads its keys and values by itself: K from memory into the operand's registers (16x16x32, S^T = K Q^T, a
+// row per lane), V through LDS, where it is read by columns, 32 keys at a time, the next ones loaded as soon as the
+// registers are free.  SPLIT wavefronts share the keys of one list, by tiles in turn, and join through LDS.
+template <typename T, int DP, int SPLIT>
+__global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(BlockArgs a, int tiles_of_list, int flip) {
+  typedef typename T::elem elem;
+  constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8, RP = 64 / PIECES, PASSES = 32 / RP;
+  union Own {  // of a wavefront
+    elem v[32 * DP];
+    float out[16][DP + 4];
+  };
+  __shared__ __attribute__((aligned(16))) Own own[4];
+  __shared__ float tops[4][16], totals[4][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
+  const int block = (int)(xcd_contiguous_block(blockIdx.x, gridDim.x) * (4 / SPLIT)) + wave / SPLIT, share = wave % SPLIT;
+  const int list = block / tiles_of_list, part = block - list * tiles_of_list;
+  const int lists = a.batch * a.kv_heads * a.rows;
+  const bool any = list < lists;
+  if (SPLIT == 1 && !any) return;  // no barrier below then
+  const int bh = any ? list / a.rows : 0, r = any ? list - bh * a.rows : 0, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
+  const int q0 = r * a.block_m, rows = min(a.block_m, a.queries - q0) * a.group;
+  int first = 0, count = 0;
+  if (any && part * 16 < rows) entries_of(a, list, &first, &count);
+  const int row0 = part * 16, row = row0 + col, row_last = min(row0 + 15, rows - 1);
+  const bool live = any && row < rows;
+  const int query = q0 + row / a.group, head = kh * a.group + row % a.group;
+  const int limit = a.causal ? min(query + a.shift, a.keys - 1) : a.keys - 1;
+  const int low = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row0 / a.group + a.shift, a.keys - 1) : a.keys - 1);
+  const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
+
+  vec8<T> qf[KS];
+  const elem *qp = (const elem *)a.q.data + b * a.q.stride[0] + query * a.q.stride[1] + head * a.q.stride[2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = 32 * s + 8 * quarter;
+    v4i x = {0, 0, 0, 0};
+    if (live && d < a.dim) x = *(const v4i *)(qp + d);
+    qf[s] = __builtin_bit_cast(vec8<T>, x ^ flip);
+  }
+  const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
+  const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
+  const int tiles = a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + 31) / 32) : 0;
+  const int piece = lane % PIECES, v_row = lane / PIECES, vd = piece * 8 < a.dim ? piece * 8 : 0;
+  v4i kr[2][KS], vr[PASSES];
+  const auto load = [&](const int (&key0)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int from = min(key0[i], a.keys - 1), room = a.keys - 1 - from;
+      const elem *k = kp + from * a.k.stride[1] + min(col, room) * a.k.stride[1];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = 32 * s + 8 * quarter;
+        kr[i][s] = *(const v4i *)(k + (d < a.dim ? d : 0));
+        if (a.dim < 32 * s + 32 && d >= a.dim) kr[i][s] = v4i{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int p = i * PASSES / 2; p < (i + 1) * PASSES / 2; ++p)
+        vr[p] = *(const v4i *)(vp + from * a.v.stride[1] + min((p * RP & 15) + v_row, room) * a.v.stride[1] + vd);
+    }
+  };
+  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, t * 32 + 16 * (lane & 1)) : kAbsent; };
+
+  v4f acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+  float m = -INFINITY, l = 0.f;
+  elem *mine = own[wave].v;
+  int now[2], next[2], ahead = look_up(share);
+  next[0] = __builtin_amdgcn_readlane(ahead, 0), next[1] = __builtin_amdgcn_readlane(ahead, 1);
+  if (share < tiles) load(next);
+  ahead = look_up(share + SPLIT);
+  for (int t = share; t < tiles; t += SPLIT) {
+    now[0] = next[0], now[1] = next[1];
+    v4f s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) s[i] = mfma16(__builtin_bit_cast(vec8<T>, kr[i][x]), qf[x], s[i]);
+    }
+    const bool cut = max(now[0], now[1]) + 15 > low, skip = min(now[0], now[1]) > high;
+    bool bad = false;
+    if (cut) {  // 0 times an infinity or NaN must not count
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(__builtin_bit_cast(vec8<T>, vr[p]));
+      bad = __any(bad);
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int at = p * RP + v_row;
+      *(v4i *)(mine + at * DP + ((piece ^ turn16<DP>(at)) * 8)) = vr[p];
+    }
+    next[0] = __builtin_amdgcn_readlane(ahead, 0), next[1] = __builtin_amdgcn_readlane(ahead, 1);
+    if (t + SPLIT < tiles) load(next);
+    ahead = look_up(t + 2 * SPLIT);
+    if (skip) continue;
+    float best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (cut && now[i] + 4 * quarter + e > limit) s[i][e] = -INFINITY;
+        best = fmaxf(best, s[i][e]);
+      }
+    best = rows_max(best) * c;
+    if (__any(best > m + 8.f)) {  // as in the kernel above
+      const float to = fmaxf(m, best), keep = to == m ? 1.f : __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] *= keep;
+    }
+    const float off = m == -INFINITY ? 0.f : m;
+    vec8<T> pf;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], c, -off));
+        l += p;
+        pf[4 * i + e] = (elem)p;
+      }
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      const int x = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
+      const elem *p = mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7);  // row + 16 has the same order of pieces
+      vec8<T> v = join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP));
+      if (bad) v = finite_only<T>(v);
+      acc[i] = mfma16(v, pf, acc[i]);
+    }
+    if (bad)  // an infinity or NaN only to the rows that see its key
+#pragma unroll 1
+      for (int x = 0; x < 32; ++x) {
+        const bool sees = (x < 16 ? now[0] : now[1]) + (x & 15) <= limit;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const int d = 16 * i + 4 * quarter;
+          const vec4<T> v = *(const vec4<T> *)(mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (sees && abs_bits((float)v[e]) >= kInfBits) acc[i][e] += (float)v[e];
+        }
+      }
+    wave_lds_sync();
+  }
+  l = rows_sum(l);
+  if (quarter == 0) tops[wave][col] = m, totals[wave][col] = l;
+#pragma unroll
+  for (int i = 0; i < DT; ++i) *(v4f *)(&own[wave].out[col][16 * i + 4 * quarter]) = acc[i];
+  if (SPLIT == 1) wave_lds_sync();
+  else __syncthreads();
+  if (!any) return;
+  // a piece of a row per lane, from all wavefronts that share the list
+  constexpr int W0 = SPLIT == 1 ? 0 : 1;
+  const int w0 = SPLIT == 1 ? wave : 0;
+  for (int x = SPLIT == 1 ? lane : tid; x < 16 * PIECES; x += SPLIT * 64) {
+    const int h = x / PIECES, d = (x % PIECES) * 8;
+    if (row0 + h >= rows || d >= a.dim) continue;
+    float most = tops[w0][h], sum = 0.f, o[8] = {};
+#pragma unroll
+    for (int w = W0; w < SPLIT; ++w) most = fmaxf(most, tops[w0 + w][h]);
+#pragma unroll
+    for (int w = 0; w < SPLIT; ++w) {
+      const float by = tops[w0 + w][h] == most ? 1.f : __builtin_amdgcn_exp2f(tops[w0 + w][h] - most);
+      sum += by * totals[w0 + w][h];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += by * own[w0 + w].out[h][d + e];
+    }
+    const float by = 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = sum == 0.f ? 0.f : o[e] * by;
+    const int i = q0 + (row0 + h) / a.group, to = kh * a.group + (row0 + h) % a.group;
+    *(vec8<T> *)((elem *)a.out.data + b * a.out.stride[0] + i * a.out.stride[1] + to * a.out.stride[2] + d) = narrow<T>(o);
+    if (a.lse && d == 0)
+      a.lse[((long long)b * a.heads + to) * a.queries + i] = sum == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+  }
+}
+
 int read_view(const char *what, const lapis_hip_rows &r, View *v) {
   LAPIS_REQUIRE(r.data && aligned16(r.data) && strides_of_8(r.stride, 3),
                 "%s: an operand that is null, not on a 16-byte boundary or with strides that are no multiples of 8", what);
@@ -202,8 +383,27 @@ int launch_wide(const BlockArgs &a, hipStream_t st) {
   return LAPIS_HIP_OK;
 }
 
+template <typename T, int DP, int SPLIT>
+int launch_narrow(const BlockArgs &a, hipStream_t st) {
+  const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)a.block_m * a.group, 16);
+  const long long blocks = ceil_div(lists * tiles * SPLIT, 4);
+  LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
+  hipLaunchKernelGGL((block_narrow_kernel<T, DP, SPLIT>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, a.scale < 0.f ? (int)0x80008000u : 0);
+  LAPIS_LAUNCH_CHECK();
+  return LAPIS_HIP_OK;
+}
+
 template <typename T>
 int launch_forward(const BlockArgs &a, hipStream_t st) {
+  // Up to 32 rows a list the 128-row workgroup mostly waits for its own tiles (16 rows, 4096 queries, 4 lists of 512 keys each, dim
+  // 64: 498 us against 169; 32 rows: 257 against 167; 48 rows: 37.5 against 41.7), and while there are fewer of them than half
+  // the compute units, 16 rows of four wavefronts spread further (128 rows, 64 workgroups: 10.5 against 8.2).
+  const int64_t rows = (int64_t)a.block_m * a.group, lists = (int64_t)a.batch * a.kv_heads * a.rows, waves = ceil_div(rows, 16) * lists;
+  if (rows <= 32 || ceil_div(rows, 128) * lists < device_cu_count() / 2) {
+    const bool many = waves >= 8 * device_cu_count();  // two wavefronts a SIMD without sharing lists
+    if (a.dim <= 64) return many ? launch_narrow<T, 64, 1>(a, st) : launch_narrow<T, 64, 4>(a, st);
+    return many ? launch_narrow<T, 128, 1>(a, st) : launch_narrow<T, 128, 4>(a, st);
+  }
   return a.dim <= 64 ? launch_wide<T, 64, 4, 64>(a, st) : launch_wide<T, 128, 4, 64>(a, st);
 }
 

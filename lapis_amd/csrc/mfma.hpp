@@ -32,6 +32,17 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
 }
 
+__device__ __forceinline__ float rows_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  const unsigned a = p[0], b = p[1];
+  return halves_max(fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  const unsigned a = p[0], b = p[1];
+  return halves_sum(__builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+}
+
 // Tiles of rows of DP 16-bit elements in LDS, the 16-byte pieces of a row in an order of its own, so that two ways of reading
 // meet 64 different banks: 16 lanes that take the same piece of 16 neighbouring rows (an operand whose lanes are rows; the
 // turn is another one for each of the rows that would share banks), and 32 lanes that take the same 64 bytes of four

@@ -48,17 +48,6 @@ __device__ __forceinline__ int list_of_unit(const PagedArgs &a, int u, int lane)
   return lo;
 }
 
-__device__ __forceinline__ float rows_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
-  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
-  const unsigned a = p[0], b = p[1];
-  return halves_max(fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
-}
-__device__ __forceinline__ float rows_sum(float x) {
-  const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
-  const unsigned a = p[0], b = p[1];
-  return halves_sum(__builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
-}
-
 // Eight e4m3 codes as eight numbers of a 16-bit type: exact.
 template <typename T>
 __device__ __forceinline__ vec8<T> codes_to(v2i x) {
