@@ -290,10 +290,10 @@ __global__ __launch_bounds__(1024) void columns_scan_kernel(BlockArgs a, Columns
 constexpr int kMostEntries = 384;  // of a unit
 
 // A unit of work: 32 * KG keys of a column and some of the rows that list it, their queries times heads packed into tiles of
-// 32.  Two wavefronts share 32 keys, a key per lane, K or V of them in registers: one computes S and P (queries x keys), leaves
-// P in LDS for the other and feeds dV^T = dO^T P from its registers; the other computes dP meanwhile, and then dS, which
-// feeds dK^T = Q^T dS.  Both sums in one wavefront take 318 registers, one wavefront a SIMD and nothing to fill the waits
-// with (1.06 ms at 8k queries against X); split, four wavefronts a workgroup and two workgroups a compute unit fit.
+// 32.  Two wavefronts share 32 keys, a key per lane, K and V of them in registers: one computes S and P (queries x keys), which
+// feeds dV^T = dO^T P from its registers; the other S, P, dP and dS, which feeds dK^T = Q^T dS.  Both sums in one wavefront take
+// 318 registers, one wavefront a SIMD and nothing to fill the waits with (1.06 ms at 8k queries); P handed over
+// through LDS saves a product of five, but its barrier in the middle of every tile costs more (0.69 ms).
 // Where keys are few (KG = 1) two pairs take turns with the tiles and add up at the end.
 // The rows of a column lie all over Q and dO, beyond L2 in large passes: S tiles are on their way or being computed, where a
 // tile's rows lie is worked out one tile earlier still, and no load but those into LDS is in the loop.
@@ -309,12 +309,11 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
     float times[32];  // how often the row lists the column, where every row is looked through
   };
   __shared__ __attribute__((aligned(16))) elem tiles[QG][S][2][32 * DP];
-  __shared__ __attribute__((aligned(16))) float weights[QG * KG][1024];
   __shared__ __attribute__((aligned(16))) float sums[QG][S][2][32];  // log-sums and deltas of a tile's rows
   __shared__ __attribute__((aligned(16))) Info infos[QG][S + 1];
   __shared__ int rows_of_unit[kMostEntries], taken;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const int role = wave & 1, kg = (wave >> 1) % KG, qg = (wave >> 1) / KG, gt = tid - qg * TG;  // role 0: dV, 1: dK
+  const int role = (wave ^ blockIdx.x / kParts) & 1, kg = (wave >> 1) % KG, qg = (wave >> 1) / KG, gt = tid - qg * TG;  // role 0: dV, 1: dK
   const bool odd = *cols.odd != 0;
   const int all_units = (odd ? cols.lists * a.columns : cols.units) * cols.sub;
   const float c = a.scale * kLog2e;
@@ -350,14 +349,15 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
     const int key_low = (column << a.block_n_log2) + in_block, key = key_low + (lane & 31);
     const bool live = in_block + (lane & 31) < (1 << a.block_n_log2) && key < a.keys;
 
-    const View &kv = role ? a.v : a.k;
-    vec8<T> kf[DP / 16];  // of this wavefront's keys: K, or V
-    const elem *kp = (const elem *)kv.data + b * kv.stride[0] + key * kv.stride[1] + kh * kv.stride[2];
+    vec8<T> kf[DP / 16], vf[DP / 16];
+    const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + key * a.k.stride[1] + kh * a.k.stride[2];
+    const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + key * a.v.stride[1] + kh * a.v.stride[2];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       const int d = 16 * s + 8 * half;
-      kf[s] = vec8<T>{};
+      kf[s] = vf[s] = vec8<T>{};
       if (live && d < a.dim) kf[s] = *(const vec8<T> *)(kp + d);
+      if (role && live && d < a.dim) vf[s] = *(const vec8<T> *)(vp + d);
     }
 
     // this lane's row of the tiles of its group: entry, query of the block and head of the group, moved on by 32 QG each tile
@@ -432,16 +432,37 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
       put_info(t + S);
       if (t + S - 1 < tiles_n) load(t + S - 1);
       const Info &info = infos[qg][t % (S + 1)];
-      const elem *by_row = tiles[qg][t % S][role], *by_column = tiles[qg][t % S][1 - role];
-      float *w = weights[qg * KG + kg] + lane * 4;  // element e of this lane at (e / 4) * 256 + lane * 4 + e % 4
+      const elem *qt = tiles[qg][t % S][0], *dt = tiles[qg][t % S][1], *by_column = tiles[qg][t % S][1 - role];
       const int last = info.last[lane & 31];
-      const bool some = __any(last >= key_low), cut = odd || __any(last < key_low + 31);
-      v16f s = {};  // S, or dP
-      unsigned bad = 0;
-      if (some) {
+      if (__any(last >= key_low)) {
+        const bool cut = odd || __any(last < key_low + 31);
+        const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
+        v16f s = {}, g = {};
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) s = mfma32(*(const vec8<T> *)(by_row + place_of<DP>(lane & 31, 2 * y + half)), kf[y], s);
-        if (cut) {  // 0 times an infinity or NaN must not count: which rows of the other operand hold one?
+        for (int y = 0; y < DP / 16; ++y) s = mfma32(*(const vec8<T> *)(qt + place_of<DP>(lane & 31, 2 * y + half)), kf[y], s);
+        if (role) {
+#pragma unroll
+          for (int y = 0; y < DP / 16; ++y) g = mfma32(*(const vec8<T> *)(dt + place_of<DP>(lane & 31, 2 * y + half)), vf[y], g);
+        }
+        vec8<T> f[2];
+        unsigned bad = 0;
+        if (!cut) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+          }
+          if (role) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const v4f del = *(const v4f *)(dl + 8 * j + 4 * half);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[4 * j + e] *= __builtin_fmaf(g[4 * j + e], a.scale, -del[e]);
+            }
+          }
+        } else {
+          // 0 times an infinity or NaN must not count: which rows of the last product's operand hold one?
 #pragma unroll 1
           for (int i = 0; i < PIECES / 2; ++i) {
             const unsigned long long lanes = __ballot(not_finite<T>(*(const vec8<T> *)(by_column + (i * 64 + lane) * 8)));
@@ -450,65 +471,39 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
             for (int x = 0; x < 64 / PIECES; ++x)
               if (lanes >> (x * PIECES) & ((1u << PIECES) - 1)) bad |= 1u << (i * (64 / PIECES) + x);
           }
-        }
-      }
-      vec8<T> f[2];
-      if (role == 0 && some) {
-        const float *lse = sums[qg][t % S][0];
-        if (!cut) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
-            v4f p;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
-              f[j >> 1][(4 * j + e) & 7] = (elem)p[e];
-            }
-            *(v4f *)(w + 256 * j) = p;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
+            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half), del = *(const v4f *)(dl + 8 * j + 4 * half);
             const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
-            v4f p;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int row = 8 * j + 4 * half + e;
-              const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+              float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+              if (role) x *= __builtin_fmaf(g[4 * j + e], a.scale, -del[e]);
+              else if (bad >> row & 1) x = __builtin_nanf("");  // its dO is taken as zeros below
               const float times = odd ? info.times[row] : 1.f;
-              const bool seen = key <= lim[e] && times != 0.f;  // a row without an entry (log-sum -infinity) sees no key
-              p[e] = seen ? x * times : 0.f;
-              f[j >> 1][(4 * j + e) & 7] = (elem)(seen && (bad >> row & 1) ? __builtin_nanf("") : p[e]);  // its dO is taken as zeros below
+              // a row without an entry (log-sum -infinity) sees no key
+              s[4 * j + e] = key <= lim[e] && times != 0.f ? x * times : 0.f;
             }
-            *(v4f *)(w + 256 * j) = p;
           }
         }
-      }
-      __syncthreads();
-      if (role == 1 && some) {
-        const float *dl = sums[qg][t % S][1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const v4f p = *(const v4f *)(w + 256 * j), del = *(const v4f *)(dl + 8 * j + 4 * half);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float ds = p[e] * __builtin_fmaf(s[4 * j + e], a.scale, -del[e]);
-            if (cut) ds = p[e] == 0.f ? 0.f : ds;
-            f[j >> 1][(4 * j + e) & 7] = (elem)ds;
-          }
-        }
-      }
-      if (some) {
+        for (int e = 0; e < 16; ++e) f[e >> 3][e & 7] = (elem)s[e];
+        vec8<T> x[2][DT];
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            vec8<T> x = columns_in_order<T, DP>(by_column, 16 * y, 32 * i, lane);
-            if (bad) x = finite_only<T>(x);
-            acc[i] = mfma32(x, f[y], acc[i]);
-          }
+          for (int i = 0; i < DT; ++i) x[y][i] = columns_in_order<T, DP>(by_column, 16 * y, 32 * i, lane);
+        if (bad) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < DT; ++i) x[y][i] = finite_only<T>(x[y][i]);
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int i = 0; i < DT; ++i) acc[i] = mfma32(x[y][i], f[y], acc[i]);
       }
       if (t + S - 1 < tiles_n) lds_loads_done<(S - 2) * LOADS>();
       else lds_loads_done();
@@ -599,10 +594,11 @@ Layout layout_of(const BlockArgs &a) {
   c.lists = a.batch * a.kv_heads;
   c.chunk_rows = (int)max((int64_t)kRowsAtOnce, ceil_div(ceil_div(a.rows, 64), kRowsAtOnce) * kRowsAtOnce);
   c.chunks = (int)max((int64_t)1, ceil_div(a.rows, c.chunk_rows));
-  // 8192 queries times heads a unit, an eighth of what a compute unit does in a large pass: long columns do not stand alone,
-  // and those of ordinary length need no join
+  // Up to 8192 queries times heads a unit, so that long columns do not stand alone and those of ordinary length need no join; in
+  // small passes what gives every workgroup one (the first block's column is all there is to wait for otherwise).
   const int64_t rows_of_entry = (int64_t)min(a.block_m, max(a.queries, 1)) * max(a.group, 1);
-  c.per_unit = (int)min((int64_t)kMostEntries, max((int64_t)1, 8192 / rows_of_entry));
+  const int64_t rows_of_unit = min(max(a.nnz * rows_of_entry / max(2 * device_cu_count(), 1), (int64_t)256), (int64_t)8192);
+  c.per_unit = (int)min((int64_t)kMostEntries, max((int64_t)1, rows_of_unit / rows_of_entry));
   c.units = (int)(a.nnz / c.per_unit + (int64_t)c.lists * a.columns);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
