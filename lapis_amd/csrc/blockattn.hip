@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   }
   const KeyTiles<T, DP, NW, KT, true> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
   const int tiles = keys.tiles();
-  int now[CH], next[CH];  // first keys of each sixteen of this tile and the next
+  v4i now, next;  // first keys of each sixteen of this tile and the next
 
   v16f acc[DT];
 #pragma unroll
@@ -61,18 +61,18 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   int ahead = 0;
   if (tiles > 0) {
     ahead = keys.look_up(1);
-    keys.spread(keys.look_up(0), next);
-    keys.load(0, next);
+    next = keys.spread(keys.look_up(0));
+    keys.template load<0>(next);
   }
   lds_loads_done();
   __syncthreads();
-  for (int t = 0; t < tiles; ++t) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) now[i] = next[i];
+  const auto step = [&](int t, auto which) {
+    constexpr int buffer = decltype(which)::value;  // t & 1, known where addresses are made
+    now = next;
     if (t + 1 < tiles) {
-      keys.spread(ahead, next);
+      next = keys.spread(ahead);
       ahead = keys.look_up(t + 2);
-      keys.load(t + 1, next);
+      keys.template load<1 - buffer>(next);
     }
     int lowest = now[0], top = now[0];
 #pragma unroll
@@ -80,12 +80,12 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     if (top + 15 > low_of_all) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
       bool bad = false;
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(v_tile[t & 1] + (p * NW * 64 + tid) * 8));
-      if (__any(bad) && lane == 0) bad_tile[t & 1] = t + 1;
+      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(v_tile[buffer] + (p * NW * 64 + tid) * 8));
+      if (__any(bad) && lane == 0) bad_tile[buffer] = t + 1;
       __syncthreads();
     }
     if (lowest <= high) {
-      const elem *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+      const elem *kt = k_tile[buffer], *vt = v_tile[buffer];
       v16f s[ST];
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
@@ -125,12 +125,20 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
 #pragma unroll
       for (int x = 0; x < ST; ++x)
 #pragma unroll
+        for (int e = 0; e < 16; ++e) s[x][e] = __builtin_fmaf(s[x][e], c, -off);
+#pragma unroll
+      for (int x = 0; x < ST; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[x][e] = __builtin_amdgcn_exp2f(s[x][e]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < ST; ++x)
+#pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], c, -off));
-          l += p;
-          pf[2 * x + (e >> 3)][e & 7] = (elem)p;
+          l += s[x][e];
+          pf[2 * x + (e >> 3)][e & 7] = (elem)s[x][e];
         }
-      if (cut && bad_tile[t & 1] == t + 1) {
+      if (cut && bad_tile[buffer] == t + 1) {
         // the finite values as always; an infinity or NaN only to the rows that see its key
 #pragma unroll
         for (int y = 0; y < 2 * ST; ++y)
@@ -164,6 +172,10 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     }
     lds_loads_done();
     __syncthreads();
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 1 < tiles) step(t + 1, std::integral_constant<int, 1>());
   }
 
   l = halves_sum(l);

@@ -64,13 +64,15 @@ struct KeyTiles {
   __device__ __forceinline__ int tiles() const { return a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + KT - 1) / KT) : 0; }
   // The first key of each sixteen of tile t, one to a lane: asked for a tile before they are needed.
   __device__ __forceinline__ int look_up(int t) const { return first_key(a, first, count, t * KT + 16 * (threadIdx.x % CH)); }
-  static __device__ __forceinline__ void spread(int of_lane, int (&key0)[CH]) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) key0[i] = __builtin_amdgcn_readlane(of_lane, i);
+  static __device__ __forceinline__ v4i spread(int of_lane) {
+    static_assert(CH == 4, "tiles of 64 keys");
+    return v4i{__builtin_amdgcn_readlane(of_lane, 0), __builtin_amdgcn_readlane(of_lane, 1), __builtin_amdgcn_readlane(of_lane, 2),
+               __builtin_amdgcn_readlane(of_lane, 3)};
   }
-  // Tile t into buffer t & 1.
-  __device__ __forceinline__ void load(int t, const int (&key0)[CH]) const {
-    const unsigned buffer = (t & 1) * KT * DP * 2;
+  // The tile of these keys into one of the buffers.
+  template <int BUFFER>
+  __device__ __forceinline__ void load(v4i key0) const {
+    constexpr unsigned buffer = BUFFER * KT * DP * 2;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int at = RP == 16 ? key0[p] : __builtin_amdgcn_readfirstlane(my_row < 16 ? key0[p * RP / 16] : key0[p * RP / 16 + (RP > 16)]);

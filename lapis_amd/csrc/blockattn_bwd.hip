@@ -14,9 +14,9 @@ constexpr int kParts = 8;  // of the units of work beside dK and dV, one to each
 // ---- dQ --------------------------------------------------------------------------------------------------------
 
 // As the forward kernel: 32 rows a wavefront, a query per lane.  dS^T = P^T * (scale V dO^T - scale delta) feeds dQ^T = K^T dS^T
-// from its registers.  rowsum(dO * O) is computed here and left, times `scale`, for the other kernel.
+// from its registers.  rowsum(dO * O), times `scale`, and the log-sums in units of ln 2 are left for the other kernel.
 template <typename T, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, int *odd) {
+__global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
   __shared__ __attribute__((aligned(16))) elem k_tile[2][KT * DP], v_tile[2][KT * DP];
@@ -63,11 +63,11 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     const long long at = ((long long)b * a.heads + head) * a.queries + query;
     const float lse = a.lse[at];
     off = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    if (half == 0) delta[at] = del;
+    if (half == 0) delta[at] = del, logs[at] = off;
   }
   const KeyTiles<T, DP, NW, KT, false> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
   const int tiles = keys.tiles();
-  int now[CH], next[CH];  // first keys of each sixteen of this tile and the next
+  v4i now, next;  // first keys of each sixteen of this tile and the next
   v16f acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = v16f{};
@@ -81,18 +81,18 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
   int ahead = 0;
   if (tiles > 0) {
     ahead = keys.look_up(1);
-    keys.spread(keys.look_up(0), next);
-    keys.load(0, next);
+    next = keys.spread(keys.look_up(0));
+    keys.template load<0>(next);
   }
   lds_loads_done();
   __syncthreads();
-  for (int t = 0; t < tiles; ++t) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) now[i] = next[i];
+  const auto step = [&](int t, auto which) {
+    constexpr int buffer = decltype(which)::value;  // t & 1, known where addresses are made
+    now = next;
     if (t + 1 < tiles) {
-      keys.spread(ahead, next);
+      next = keys.spread(ahead);
       ahead = keys.look_up(t + 2);
-      keys.load(t + 1, next);
+      keys.template load<1 - buffer>(next);
     }
     int lowest = now[0], top = now[0];
 #pragma unroll
@@ -100,14 +100,14 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     if (top + 15 > low_of_all) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
       bool bad = false;
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(k_tile[t & 1] + (p * NW * 64 + tid) * 8));
-      if (__any(bad) && lane == 0) bad_tile[t & 1] = t + 1;
+      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(k_tile[buffer] + (p * NW * 64 + tid) * 8));
+      if (__any(bad) && lane == 0) bad_tile[buffer] = t + 1;
       __syncthreads();
     }
     if (lowest <= high) {
-      const elem *kt = k_tile[t & 1], *vt = v_tile[t & 1];
+      const elem *kt = k_tile[buffer], *vt = v_tile[buffer];
       const bool cut = top + 15 > low;
-      const bool bad = cut && bad_tile[t & 1] == t + 1;
+      const bool bad = cut && bad_tile[buffer] == t + 1;
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
         v16f s = {}, g = {};
@@ -144,6 +144,10 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     }
     lds_loads_done();
     __syncthreads();
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 1 < tiles) step(t + 1, std::integral_constant<int, 1>());
   }
   if (!live) return;
   elem *dp = (elem *)a.dq.data + b * a.dq.stride[0] + query * a.dq.stride[1] + head * a.dq.stride[2];
@@ -293,14 +297,14 @@ constexpr int kMostEntries = 384;  // of a unit
 // 32.  Two wavefronts share 32 keys, a key per lane, K and V of them in registers: one computes S and P (queries x keys), which
 // feeds dV^T = dO^T P from its registers; the other S, P, dP and dS, which feeds dK^T = Q^T dS.  Both sums in one wavefront take
 // 318 registers, one wavefront a SIMD and nothing to fill the waits with (1.06 ms at 8k queries); P handed over
-// through LDS saves a product of five, but its barrier in the middle of every tile costs more (0.69 ms).
+// through LDS saves a product of five, but its barrier in the middle of every tile costs more (0.67 ms against 0.57).
 // Where keys are few (KG = 1) two pairs take turns with the tiles and add up at the end.
 // The rows of a column lie all over Q and dO, beyond L2 in large passes: S tiles are on their way or being computed, where a
 // tile's rows lie is worked out one tile earlier still, and no load but those into LDS is in the loop.
 // Columns are anything but equal (the first block is listed by all rows, the last by few): workgroups take units from a
 // counter, those of their XCD's part first, whose rows of Q and dO its L2 holds.
 template <typename T, int DP, int KG, int S>
-__global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns cols, const float *__restrict__ delta) {
+__global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns cols, const float *__restrict__ delta, const float *__restrict__ logs) {
   typedef typename T::elem elem;
   constexpr int QG = 2 / KG, TG = KG * 128, PIECES = DP / 8, RP = TG / PIECES, PASSES = 32 / RP, DT = DP / 32;
   struct Info {  // where a tile's rows lie
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
       }
       if (role == 0 && kg == 0 && lane < 32) {
         const unsigned to = __builtin_amdgcn_readfirstlane(lds_address(sums[qg][slot][0]));
-        load_word_to_lds(a.lse + i.sums[lane], to);
+        load_word_to_lds(logs + i.sums[lane], to);
         load_word_to_lds(delta + i.sums[lane], to + 128);
       }
     };
@@ -438,11 +442,23 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
         const bool cut = odd || __any(last < key_low + 31);
         const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
         v16f s = {}, g = {};
+        // operands are read a product ahead of their use at least: left to itself the compiler reads each one just before
+        vec8<T> qa[DP / 16], ga[DP / 16];
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) s = mfma32(*(const vec8<T> *)(qt + place_of<DP>(lane & 31, 2 * y + half)), kf[y], s);
+        for (int y = 0; y < DP / 16; ++y) qa[y] = *(const vec8<T> *)(qt + place_of<DP>(lane & 31, 2 * y + half));
+        __builtin_amdgcn_sched_barrier(0);
         if (role) {
 #pragma unroll
-          for (int y = 0; y < DP / 16; ++y) g = mfma32(*(const vec8<T> *)(dt + place_of<DP>(lane & 31, 2 * y + half)), vf[y], g);
+          for (int y = 0; y < DP / 16; ++y) {
+            s = mfma32(qa[y], kf[y], s);
+            ga[y] = *(const vec8<T> *)(dt + place_of<DP>(lane & 31, 2 * y + half));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int y = 0; y < DP / 16; ++y) g = mfma32(ga[y], vf[y], g);
+        } else {
+#pragma unroll
+          for (int y = 0; y < DP / 16; ++y) s = mfma32(qa[y], kf[y], s);
         }
         vec8<T> f[2];
         unsigned bad = 0;
@@ -451,7 +467,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
           for (int j = 0; j < 4; ++j) {
             const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+            for (int e = 0; e < 4; ++e) s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -off[e]));
           }
           if (role) {
 #pragma unroll
@@ -478,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int row = 8 * j + 4 * half + e;
-              float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -kLog2e * off[e]));
+              float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -off[e]));
               if (role) x *= __builtin_fmaf(g[4 * j + e], a.scale, -del[e]);
               else if (bad >> row & 1) x = __builtin_nanf("");  // its dO is taken as zeros below
               const float times = odd ? info.times[row] : 1.f;
@@ -584,7 +600,7 @@ __global__ __launch_bounds__(256) void join_units_kernel(BlockArgs a, Columns co
 // ---- host ------------------------------------------------------------------------------------------------------
 
 struct Layout {
-  int64_t delta, odd, counts, start, end, unit, rows, partial, bytes;
+  int64_t delta, logs, odd, counts, start, end, unit, rows, partial, bytes;
   Columns columns;
 };
 
@@ -597,7 +613,7 @@ Layout layout_of(const BlockArgs &a) {
   // Up to 8192 queries times heads a unit, so that long columns do not stand alone and those of ordinary length need no join; in
   // small passes what gives every workgroup one (the first block's column is all there is to wait for otherwise).
   const int64_t rows_of_entry = (int64_t)min(a.block_m, max(a.queries, 1)) * max(a.group, 1);
-  const int64_t rows_of_unit = min(max(a.nnz * rows_of_entry / max(2 * device_cu_count(), 1), (int64_t)256), (int64_t)8192);
+  const int64_t rows_of_unit = min(max(a.nnz * rows_of_entry / max(device_cu_count(), 1), (int64_t)256), (int64_t)8192);
   c.per_unit = (int)min((int64_t)kMostEntries, max((int64_t)1, rows_of_unit / rows_of_entry));
   c.units = (int)(a.nnz / c.per_unit + (int64_t)c.lists * a.columns);
   int64_t at = 0;
@@ -607,6 +623,7 @@ Layout layout_of(const BlockArgs &a) {
     return here;
   };
   l.delta = take(4ll * a.batch * a.heads * a.queries);
+  l.logs = take(4ll * a.batch * a.heads * a.queries);
   l.odd = take(4 * (1 + kParts));
   l.counts = take(4ll * c.lists * a.columns * c.chunks);
   l.start = take(4ll * c.lists * a.columns);
@@ -620,18 +637,18 @@ Layout layout_of(const BlockArgs &a) {
 }
 
 template <typename T, int DP, int KG, int S>
-void launch_dkv(const BlockArgs &a, const Columns &c, const float *delta, hipStream_t st) {
+void launch_dkv(const BlockArgs &a, const Columns &c, const float *delta, const float *logs, hipStream_t st) {
   Columns cols = c;
   cols.sub = (int)ceil_div(1 << a.block_n_log2, 32 * KG);
   const int64_t grid = min((int64_t)2 * device_cu_count(), (int64_t)c.units * cols.sub);
-  hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG, S>), dim3((unsigned)grid), dim3(256), 0, st, a, cols, delta);
+  hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG, S>), dim3((unsigned)grid), dim3(256), 0, st, a, cols, delta, logs);
 }
 
 template <typename T, int DP>
 int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   Layout l = layout_of(a);
   Columns &c = l.columns;
-  float *delta = reinterpret_cast<float *>(work + l.delta);
+  float *delta = reinterpret_cast<float *>(work + l.delta), *logs = reinterpret_cast<float *>(work + l.logs);
   c.odd = reinterpret_cast<int *>(work + l.odd);
   c.next = c.odd + 1;
   c.counts = reinterpret_cast<int *>(work + l.counts);
@@ -643,7 +660,7 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   if (a.rows) {
     const long long lists = (long long)c.lists * a.rows, tiles = ceil_div((long long)min(a.block_m, a.queries) * a.group, 128);
     LAPIS_REQUIRE(lists * tiles * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld rows of the structure", lists);
-    hipLaunchKernelGGL((block_dq_kernel<T, DP, 4, 64>), dim3((unsigned)(lists * tiles)), dim3(256), 0, st, a, (int)tiles, delta, c.odd);
+    hipLaunchKernelGGL((block_dq_kernel<T, DP, 4, 64>), dim3((unsigned)(lists * tiles)), dim3(256), 0, st, a, (int)tiles, delta, logs, c.odd);
   }
   if (c.lists && a.columns) {
     if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
@@ -652,8 +669,8 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
     hipLaunchKernelGGL(columns_kernel<false>, grid, dim3(64), 0, st, a, c);
     hipLaunchKernelGGL(columns_scan_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
     hipLaunchKernelGGL(columns_kernel<true>, grid, dim3(64), 0, st, a, c);
-    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, 2>(a, c, delta, st);
-    else launch_dkv<T, DP, 2, 4>(a, c, delta, st);
+    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, 2>(a, c, delta, logs, st);
+    else launch_dkv<T, DP, 2, 4>(a, c, delta, logs, st);
     hipLaunchKernelGGL((join_units_kernel<T, DP>), dim3((unsigned)(c.lists * a.columns), 4), dim3(256), 0, st, a, c);
   }
   LAPIS_LAUNCH_CHECK();
