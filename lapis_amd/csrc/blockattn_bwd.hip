@@ -163,6 +163,157 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     }
 }
 
+// Lists of few rows, as in the forward pass: 16 rows a wavefront, K and V from memory into the operands' registers, K through LDS
+// for the product by columns.  SPLIT wavefronts share the keys of one list and add up, in their order, through LDS.
+template <typename T, int DP, int SPLIT>
+__global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta,
+                                                                               float *__restrict__ logs, int *odd) {
+  typedef typename T::elem elem;
+  constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8;
+  union Own {  // of a wavefront
+    elem k[32 * DP];
+    float out[16][DP + 4];
+  };
+  __shared__ __attribute__((aligned(16))) Own own[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
+  if (blockIdx.x == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
+  const int block = (int)(xcd_contiguous_block(blockIdx.x, gridDim.x) * (4 / SPLIT)) + wave / SPLIT, share = wave % SPLIT;
+  const int list = block / tiles_of_list, part = block - list * tiles_of_list;
+  const bool any = list < a.batch * a.kv_heads * a.rows;
+  if (SPLIT == 1 && !any) return;  // no barrier below then
+  const int bh = any ? list / a.rows : 0, r = any ? list - bh * a.rows : 0, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
+  const int q0 = r * a.block_m, rows = min(a.block_m, a.queries - q0) * a.group;
+  int first = 0, count = 0;
+  if (any && part * 16 < rows) entries_of(a, list, &first, &count);
+  const int row0 = part * 16, row = row0 + col, row_last = min(row0 + 15, rows - 1);
+  const bool live = any && row < rows;
+  const int query = q0 + row / a.group, head = kh * a.group + row % a.group;
+  const int limit = a.causal ? min(query + a.shift, a.keys - 1) : a.keys - 1;
+  const int low = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row0 / a.group + a.shift, a.keys - 1) : a.keys - 1);
+  const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
+
+  vec8<T> qf[KS], gf[KS];
+  float off = INFINITY, del = 0.f;  // of a row without entries: weights 0
+  const elem *qp = (const elem *)a.q.data + b * a.q.stride[0] + query * a.q.stride[1] + head * a.q.stride[2];
+  const elem *gp = (const elem *)a.dout.data + b * a.dout.stride[0] + query * a.dout.stride[1] + head * a.dout.stride[2];
+  const elem *op = (const elem *)a.out.data + b * a.out.stride[0] + query * a.out.stride[1] + head * a.out.stride[2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = 32 * s + 8 * quarter;
+    vec8<T> o = {};
+    qf[s] = gf[s] = vec8<T>{};
+    if (live && d < a.dim) {
+      qf[s] = *(const vec8<T> *)(qp + d);
+      gf[s] = *(const vec8<T> *)(gp + d);
+      o = *(const vec8<T> *)(op + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) del += (float)gf[s][j] * (float)o[j];
+  }
+  del = rows_sum(del) * a.scale;
+  if (live) {
+    const long long at = ((long long)b * a.heads + head) * a.queries + query;
+    const float lse = a.lse[at];
+    off = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    if (quarter == 0 && share == 0) delta[at] = del, logs[at] = off;
+  }
+  const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
+  const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
+  const int tiles = a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + 31) / 32) : 0;
+  v4i kr[2][KS], vr[2][KS];
+  const auto load = [&](int key0, int key1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int from = min(i ? key1 : key0, a.keys - 1), in = min(col, a.keys - 1 - from);
+      const elem *k = kp + from * a.k.stride[1] + in * a.k.stride[1], *v = vp + from * a.v.stride[1] + in * a.v.stride[1];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = 32 * s + 8 * quarter;
+        kr[i][s] = *(const v4i *)(k + (d < a.dim ? d : 0));
+        vr[i][s] = *(const v4i *)(v + (d < a.dim ? d : 0));
+        if (a.dim < 32 * s + 32 && d >= a.dim) kr[i][s] = vr[i][s] = v4i{0, 0, 0, 0};
+      }
+    }
+  };
+  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, t * 32 + 16 * (lane & 1)) : kAbsent; };
+
+  v4f acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  const float c = a.scale * kLog2e;
+  elem *mine = own[wave].k;
+  int ahead = look_up(share), next0 = __builtin_amdgcn_readlane(ahead, 0), next1 = __builtin_amdgcn_readlane(ahead, 1);
+  if (share < tiles) load(next0, next1);
+  ahead = look_up(share + SPLIT);
+  for (int t = share; t < tiles; t += SPLIT) {
+    const int now0 = next0, now1 = next1;
+    v4f s[2], g[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = g[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        s[i] = mfma16(__builtin_bit_cast(vec8<T>, kr[i][x]), qf[x], s[i]);
+        g[i] = mfma16(__builtin_bit_cast(vec8<T>, vr[i][x]), gf[x], g[i]);
+      }
+    }
+    const bool cut = max(now0, now1) + 15 > low, skip = min(now0, now1) > high;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const int at = 16 * i + col, piece = 4 * x + quarter;
+        if (cut) bad |= not_finite<T>(__builtin_bit_cast(vec8<T>, kr[i][x]));  // 0 times an infinity or NaN must not count
+        *(v4i *)(mine + at * DP + ((piece ^ turn16<DP>(at)) * 8)) = kr[i][x];
+      }
+    bad = cut && __any(bad);
+    next0 = __builtin_amdgcn_readlane(ahead, 0), next1 = __builtin_amdgcn_readlane(ahead, 1);
+    if (t + SPLIT < tiles) load(next0, next1);
+    ahead = look_up(t + 2 * SPLIT);
+    if (skip) continue;
+    vec8<T> df;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], c, -off));
+        float ds = p * __builtin_fmaf(g[i][e], a.scale, -del);
+        if (cut && (i ? now1 : now0) + 4 * quarter + e > limit) ds = 0.f;
+        df[4 * i + e] = (elem)ds;
+      }
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      const int x = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
+      const elem *p = mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7);  // row + 16 has the same order of pieces
+      vec8<T> k = join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP));
+      if (bad) k = finite_only<T>(k);
+      acc[i] = mfma16(k, df, acc[i]);
+    }
+    wave_lds_sync();
+  }
+#pragma unroll
+  for (int i = 0; i < DT; ++i) *(v4f *)(&own[wave].out[col][16 * i + 4 * quarter]) = acc[i];
+  if (SPLIT == 1) wave_lds_sync();
+  else __syncthreads();
+  if (!any) return;
+  const int w0 = SPLIT == 1 ? wave : 0;
+  for (int x = SPLIT == 1 ? lane : tid; x < 16 * PIECES; x += SPLIT * 64) {
+    const int h = x / PIECES, d = (x % PIECES) * 8;
+    if (row0 + h >= rows || d >= a.dim) continue;
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = own[w0].out[h][d + e];
+#pragma unroll
+    for (int w = 1; w < SPLIT; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += own[w0 + w].out[h][d + e];
+    const int i = q0 + (row0 + h) / a.group, to = kh * a.group + (row0 + h) % a.group;
+    *(vec8<T> *)((elem *)a.dq.data + b * a.dq.stride[0] + i * a.dq.stride[1] + to * a.dq.stride[2] + d) = narrow<T>(o);
+  }
+}
+
 // ---- the columns' lists ----------------------------------------------------------------------------------------
 
 // Which rows list a column, in ascending order (a row that lists it twice, twice).  Rows are cut into at most 64 chunks;
@@ -658,9 +809,13 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   c.rows = reinterpret_cast<int *>(work + l.rows);
   c.partial = reinterpret_cast<float *>(work + l.partial);
   if (a.rows) {
-    const long long lists = (long long)c.lists * a.rows, tiles = ceil_div((long long)min(a.block_m, a.queries) * a.group, 128);
-    LAPIS_REQUIRE(lists * tiles * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld rows of the structure", lists);
-    hipLaunchKernelGGL((block_dq_kernel<T, DP, 4, 64>), dim3((unsigned)(lists * tiles)), dim3(256), 0, st, a, (int)tiles, delta, logs, c.odd);
+    const long long lists = (long long)c.lists * a.rows, rows = (long long)a.block_m * a.group;
+    // the forward pass's rule: short lists, or few of them
+    const bool few = rows <= 32 || ceil_div(rows, 128) * lists < device_cu_count() / 2, many = ceil_div(rows, 16) * lists >= 8 * device_cu_count();
+    const long long tiles = ceil_div(rows, few ? 16 : 128), blocks = few ? ceil_div(lists * tiles * (many ? 1 : 4), 4) : lists * tiles;
+    LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld rows of the structure", lists);
+    const auto kernel = !few ? block_dq_kernel<T, DP, 4, 64> : many ? block_dq_narrow_kernel<T, DP, 1> : block_dq_narrow_kernel<T, DP, 4>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, delta, logs, c.odd);
   }
   if (c.lists && a.columns) {
     if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
