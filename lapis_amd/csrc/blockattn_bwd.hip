@@ -379,6 +379,16 @@ __global__ __launch_bounds__(64) void columns_kernel(BlockArgs a, Columns t) {
   for (int c = lane; c < cs; c += 64) t.counts[((long long)bh * a.columns + c0 + c) * t.chunks + chunk] = place[c];
 }
 
+// The units of work of a column: the places start / per_unit + column leave each column at least as many as it needs, so they
+// are known without a sum over the columns before.  `next`: where the entries of the column after it start.
+__device__ __forceinline__ void put_units(const Columns &t, int cc, int start, int rows, int next, bool last) {
+  const int needed = max(1, (rows + t.per_unit - 1) / t.per_unit);
+  const long long to = (long long)start / t.per_unit + cc, stop = last ? t.units : (long long)next / t.per_unit + cc + 1;
+  for (long long u = to; u < stop && u < t.units; ++u) t.unit[u] = u < to + needed ? cc : -1;
+  if (cc == 0)  // positions may start past 0
+    for (long long u = 0; u < to && u < t.units; ++u) t.unit[u] = -1;
+}
+
 // Where a list's entries start (positions are in order here).
 __device__ __forceinline__ int list_start(const BlockArgs &a, long long bh) {
   return a.rows ? (int)min(max((long long)a.pos[bh * a.rows], 0ll), a.nnz) : 0;
@@ -427,17 +437,82 @@ __global__ __launch_bounds__(1024) void columns_scan_kernel(BlockArgs a, Columns
   __threadfence_block();
   __syncthreads();
   for (int c = tid; c < a.columns; c += 1024) {
-    const int cc = bh * a.columns + c, start = t.start[cc], rows = t.end[cc] - start;
-    const int needed = max(1, (rows + t.per_unit - 1) / t.per_unit);
-    // the places start / per_unit + column leave each column at least as many units as it needs
-    const long long to = (long long)start / t.per_unit + cc;
-    const long long stop = c + 1 < a.columns  ? (long long)t.end[cc] / t.per_unit + cc + 1
-                           : bh + 1 < t.lists ? (long long)list_start(a, bh + 1ll) / t.per_unit + cc + 1
-                                              : t.units;
-    for (long long u = to; u < stop && u < t.units; ++u) t.unit[u] = u < to + needed ? cc : -1;
-    if (cc == 0)  // positions may start past 0
-      for (long long u = 0; u < to && u < t.units; ++u) t.unit[u] = -1;
+    const int cc = bh * a.columns + c, start = t.start[cc], end = t.end[cc];
+    put_units(t, cc, start, end - start, c + 1 < a.columns ? end : list_start(a, bh + 1ll), c + 1 == a.columns && bh + 1 == t.lists);
   }
+}
+
+// All of it in one workgroup per (batch entry, key-value head) where rows and columns are few: a chunk of rows to each of its
+// wavefronts, the counts in LDS.  (Three launches less two: 14 us become 6 at 128 rows and columns.)
+constexpr int kFewColumns = 1024, kFewRows = 512;
+__global__ __launch_bounds__(1024) void few_columns_kernel(BlockArgs a, Columns t) {
+  __shared__ int place[kFewColumns * 16];  // [column][wavefront]
+  __shared__ int wave_sum[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bh = blockIdx.x;
+  const int rows_each = (a.rows + 15) / 16, r0 = wave * rows_each, r1 = min(a.rows, r0 + rows_each);  // at most 32
+  for (int i = tid; i < a.columns * 16; i += 1024) place[i] = 0;
+  int first = 0, count = 0;
+  bool odd = false;
+  if (lane < rows_each && r0 + lane < r1) {
+    const long long row = (long long)bh * a.rows + r0 + lane;
+    entries_of(a, row, &first, &count);
+    odd = a.pos[row] != first || (long long)a.pos[row + 1] != (long long)first + count;
+  }
+  if (__any(odd) && lane == 0) atomicOr(t.odd, 1);
+  __syncthreads();
+  const auto pass = [&](bool fill) {  // a wavefront's rows one after the other, their first entries asked for eight at a time
+    for (int i0 = 0; i0 < r1 - r0; i0 += 8) {
+      int entry[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int f = __builtin_amdgcn_readlane(first, (i0 + i) & 63), n = i0 + i < r1 - r0 ? __builtin_amdgcn_readlane(count, (i0 + i) & 63) : 0;
+        entry[i] = lane < n ? a.crd[f + lane] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int f = __builtin_amdgcn_readlane(first, (i0 + i) & 63), n = i0 + i < r1 - r0 ? __builtin_amdgcn_readlane(count, (i0 + i) & 63) : 0;
+        for (int e = lane; e - lane < n; e += 64) {
+          const int c = e < 64 ? entry[i] : e < n ? a.crd[f + e] : -1;
+          if ((unsigned)c < (unsigned)a.columns) {
+            const int at = atomicAdd(&place[c * 16 + wave], 1);
+            if (fill && at < a.nnz) t.rows[at] = r0 + i0 + i;
+          }
+          wave_lds_sync();
+        }
+      }
+    }
+  };
+  pass(false);
+  __syncthreads();
+  // a column to a thread: its sixteen counts, and the sum over the columns before
+  int sum = 0;
+  if (tid < a.columns)
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += place[tid * 16 + w];
+  int upto = sum;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 63) wave_sum[wave] = upto;
+  __syncthreads();
+  int start = list_start(a, bh) + upto - sum;
+  for (int w = 0; w < wave; ++w) start += wave_sum[w];
+  if (tid < a.columns) {
+    int at = start;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const int n = place[tid * 16 + w];
+      place[tid * 16 + w] = at;
+      at += n;
+    }
+    const int cc = bh * a.columns + tid;
+    t.start[cc] = start;
+    t.end[cc] = at;
+    put_units(t, cc, start, sum, tid + 1 < a.columns ? at : list_start(a, bh + 1ll), tid + 1 == a.columns && bh + 1 == t.lists);
+  }
+  __syncthreads();
+  pass(true);
 }
 
 // ---- dK and dV -------------------------------------------------------------------------------------------------
@@ -473,17 +548,39 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
   const int all_units = (odd ? cols.lists * a.columns : cols.units) * cols.sub;
   const float c = a.scale * kLog2e;
 
-  for (int part = 0; part < kParts;) {
-    __syncthreads();
-    if (tid == 0) taken = atomicAdd(cols.next + (blockIdx.x + part) % kParts, 1);
-    __syncthreads();
-    const int mine = (blockIdx.x + part) % kParts;
-    const long long unit_l = (long long)all_units * mine / kParts + taken;
-    if (unit_l >= (long long)all_units * (mine + 1) / kParts) {
-      ++part;
-      continue;
+  // One unit for each workgroup, or units from the counters: those of the own part, then of whichever part has some left.
+  const bool one_each = all_units <= (int)gridDim.x;
+  const auto part_start = [&](int p) { return (int)((long long)all_units * p / kParts); };
+  int part = blockIdx.x % kParts;
+  for (bool more = true; more;) {
+    int unit_l;
+    if (one_each) {
+      unit_l = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
+      if (unit_l >= all_units) return;
+      more = false;
+    } else {
+      __syncthreads();
+      if (tid == 0) taken = atomicAdd(cols.next + part, 1);
+      __syncthreads();
+      unit_l = part_start(part) + taken;
+      if (unit_l >= part_start(part + 1)) {
+        bool left = false;
+        if (lane < kParts) {
+          const int p = (part + lane) % kParts;
+          left = part_start(p) + __hip_atomic_load(cols.next + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < part_start(p + 1);
+        }
+        __syncthreads();
+        if (wave == 0) {
+          const unsigned long long some = __ballot(left);
+          if (lane == 0) taken = some ? (part + __ffsll((long long)some) - 1) % kParts : -1;
+        }
+        __syncthreads();
+        part = taken;
+        more = part >= 0;
+        continue;
+      }
     }
-    const int u = (int)unit_l / cols.sub, sub = (int)unit_l - u * cols.sub;
+    const int u = unit_l / cols.sub, sub = unit_l - u * cols.sub;
     int cc, from = 0, n, start = 0;
     bool several = false;
     if (odd) {  // every row is looked through for the column
@@ -821,10 +918,14 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
     if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
     const dim3 grid((unsigned)c.chunks, (unsigned)ceil_div(a.columns, kColumnsInLds), (unsigned)c.lists);
     LAPIS_REQUIRE(c.lists <= 65535 && (int64_t)c.units * 8 <= INT32_MAX, "block_attention_backward: %d lists, %d units", c.lists, c.units);
-    hipLaunchKernelGGL(columns_kernel<false>, grid, dim3(64), 0, st, a, c);
-    hipLaunchKernelGGL(columns_scan_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
-    hipLaunchKernelGGL(columns_kernel<true>, grid, dim3(64), 0, st, a, c);
-    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, 2>(a, c, delta, logs, st);
+    if (a.columns <= kFewColumns && a.rows <= kFewRows) {
+      hipLaunchKernelGGL(few_columns_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
+    } else {
+      hipLaunchKernelGGL(columns_kernel<false>, grid, dim3(64), 0, st, a, c);
+      hipLaunchKernelGGL(columns_scan_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
+      hipLaunchKernelGGL(columns_kernel<true>, grid, dim3(64), 0, st, a, c);
+    }
+    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, DP == 64 ? 4 : 2>(a, c, delta, logs, st);
     else launch_dkv<T, DP, 2, 4>(a, c, delta, logs, st);
     hipLaunchKernelGGL((join_units_kernel<T, DP>), dim3((unsigned)(c.lists * a.columns), 4), dim3(256), 0, st, a, c);
   }

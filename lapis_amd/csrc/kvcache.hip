@@ -36,24 +36,34 @@ CacheView view_of(const lapis_hip_kv_cache *c) {
   return v;
 }
 
-// Group of L lanes per (token, head); blockIdx.z: keys or values.
-template <typename T, bool F8, int L>
+// Group of L lanes per (token, head) and of N of them, 256 / L rows apart; blockIdx.z: keys or values.
+template <typename T, bool F8, int L, int N>
 __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, long long rows, const int *__restrict__ slots) {
   typedef typename T::elem elem;
-  const long long row = ((long long)linear_block() * 256 + threadIdx.x) / L;
+  const long long row0 = (long long)linear_block() * (256 / L * N) + threadIdx.x / L;
   const int d = (threadIdx.x % L) * 8, which = blockIdx.z;
+  vec8<T> read[N];
+  int slot_of[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned row = (unsigned)min(row0 + i * (256 / L), rows - 1), t = row / (unsigned)c.heads, h = row - t * c.heads;
+    slot_of[i] = slots[t];
+    read[i] = vec8<T>{};
+    if (d < c.dim) read[i] = load_stream((const vec8<T> *)((const elem *)x.data[which] + t * x.stride[which][0] + h * x.stride[which][1] + d));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+  const long long row = row0 + i * (256 / L);
   if (row >= rows) return;
-  const long long t = row / c.heads;
-  const int h = (int)(row - t * c.heads);
-  const long long slot = slots[t];
-  if (slot < 0 || slot >= c.slots) return;
+  const int h = (int)((unsigned)row % (unsigned)c.heads);
+  const long long slot = slot_of[i];
+  if (slot < 0 || slot >= c.slots) continue;
   const long long page = slot >> c.page_log2, in = slot & ((1 << c.page_log2) - 1);
   const long long to = page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d;
-  vec8<T> e = {};
-  if (d < c.dim) e = *(const vec8<T> *)((const elem *)x.data[which] + t * x.stride[which][0] + h * x.stride[which][1] + d);
+  const vec8<T> e = read[i];
   if (!F8) {
     if (d < c.dim) *(vec8<T> *)((elem *)c.data[which] + to) = e;
-    return;
+    continue;
   }
   float f[8];
   widen<T>(e, f);
@@ -68,33 +78,47 @@ __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, 
   }
   if (d < c.dim) *(v2i *)(c.data[which] + to) = narrow_f8(f);
   if (d == 0) c.scale[which][page * c.scale_stride[0] + h * c.scale_stride[1] + in * c.scale_stride[2]] = scale;
+  }
 }
 
-template <typename T, bool F8, int L>
+template <typename T, bool F8, int L, int N>
 __global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, long long rows, const int *__restrict__ slots) {
   typedef typename T::elem elem;
-  const long long row = ((long long)linear_block() * 256 + threadIdx.x) / L;
+  typedef typename std::conditional<F8, v2i, v4i>::type raw;  // eight elements
+  const long long row0 = (long long)linear_block() * (256 / L * N) + threadIdx.x / L;
   const int d = (threadIdx.x % L) * 8, which = blockIdx.z;
-  if (row >= rows || d >= c.dim) return;
-  const long long t = row / c.heads;
-  const int h = (int)(row - t * c.heads);
-  const long long slot = slots[t];
-  vec8<T> e = {};
-  if (slot >= 0 && slot < c.slots) {
-    const long long page = slot >> c.page_log2, in = slot & ((1 << c.page_log2) - 1);
-    const long long from = page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d;
-    if (F8) {
-      float f[8];
-      widen_f8(*(const v2i *)(c.data[which] + from), f);
-      const float scale = c.scale[which][page * c.scale_stride[0] + h * c.scale_stride[1] + in * c.scale_stride[2]];
+  if (d >= c.dim) return;
+  raw read[N];
+  float scale[N];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * scale;
-      e = narrow<T>(f);
-    } else {
-      e = *(const vec8<T> *)((const elem *)c.data[which] + from);
+  for (int i = 0; i < N; ++i) {
+    const unsigned row = (unsigned)min(row0 + i * (256 / L), rows - 1), t = row / (unsigned)c.heads, h = row - t * c.heads;
+    const long long slot = slots[t];
+    read[i] = raw{};
+    scale[i] = 0.f;
+    if (slot >= 0 && slot < c.slots) {
+      const long long page = slot >> c.page_log2, in = slot & ((1 << c.page_log2) - 1);
+      read[i] = load_stream((const raw *)(c.data[which] + (page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d) * (F8 ? 1 : 2)));
+      if (F8) scale[i] = c.scale[which][page * c.scale_stride[0] + h * c.scale_stride[1] + in * c.scale_stride[2]];
     }
   }
-  *(vec8<T> *)((elem *)x.data[which] + t * x.stride[which][0] + h * x.stride[which][1] + d) = e;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const long long row = row0 + i * (256 / L);
+    if (row >= rows) return;
+    const unsigned t = (unsigned)row / (unsigned)c.heads, h = (unsigned)row - t * c.heads;
+    vec8<T> e;
+    if constexpr (F8) {
+      float f[8];
+      widen_f8(read[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = f[j] * scale[i];
+      e = narrow<T>(f);
+    } else {
+      e = __builtin_bit_cast(vec8<T>, read[i]);
+    }
+    *(vec8<T> *)((elem *)x.data[which] + t * x.stride[which][0] + h * x.stride[which][1] + d) = e;
+  }
 }
 
 template <bool STORE>
@@ -108,27 +132,32 @@ int kv_move(const char *what, const lapis_hip_kv_cache *cache, int64_t tokens, c
   const long long rows = tokens * cache->heads;
   if (rows == 0) return LAPIS_HIP_OK;
   LAPIS_REQUIRE(slots, "%s: null slots", what);
-  LAPIS_REQUIRE(tokens <= INT32_MAX && rows <= (INT64_C(1) << 33), "%s: %lld tokens", what, (long long)tokens);
+  LAPIS_REQUIRE(tokens <= INT32_MAX && rows < (INT64_C(1) << 31), "%s: %lld tokens", what, (long long)tokens);
   for (const lapis_hip_rows *r : {k, v})
     LAPIS_REQUIRE(r->data && aligned16(r->data) && strides_of_8(r->stride + 1, 2),
                   "%s: rows that are null, not on a 16-byte boundary or with strides that are no multiples of 8", what);
   const CacheView c = view_of(cache);
   RowsView x = {{static_cast<char *>(k->data), static_cast<char *>(v->data)}, {{k->stride[1], k->stride[2]}, {v->stride[1], v->stride[2]}}};
   const bool f8 = cache->dtype == LAPIS_HIP_F8E4M3, bf16 = dtype == LAPIS_HIP_BF16;
-  const auto go = [&](auto lanes) {
-    constexpr int L = decltype(lanes)::value;
+  const auto go = [&](auto lanes, auto times) {
+    constexpr int L = decltype(lanes)::value, N = decltype(times)::value;
     const auto pick = [&](auto type) {
       typedef decltype(type) T;
-      if (STORE) return f8 ? kv_store_kernel<T, true, L> : kv_store_kernel<T, false, L>;
-      return f8 ? kv_load_kernel<T, true, L> : kv_load_kernel<T, false, L>;
+      if (STORE) return f8 ? kv_store_kernel<T, true, L, N> : kv_store_kernel<T, false, L, N>;
+      return f8 ? kv_load_kernel<T, true, L, N> : kv_load_kernel<T, false, L, N>;
     };
-    dim3 grid = grid_of(ceil_div(rows * L, 256));
+    dim3 grid = grid_of(ceil_div(rows * L, 256 * N));
     grid.z = 2;
     hipLaunchKernelGGL((bf16 ? pick(Bf16()) : pick(F16())), grid, dim3(256), 0, as_stream(stream), c, x, rows, slots);
   };
-  if (cache->dim <= 64) go(std::integral_constant<int, 8>());
-  else if (cache->dim <= 128) go(std::integral_constant<int, 16>());
-  else go(std::integral_constant<int, 32>());
+  const auto with = [&](auto lanes) {
+    // four rows a thread only where that leaves every compute unit its workgroups
+    if (rows * decltype(lanes)::value >= 256 * 16 * device_cu_count()) go(lanes, std::integral_constant<int, 4>());
+    else go(lanes, std::integral_constant<int, 1>());
+  };
+  if (cache->dim <= 64) with(std::integral_constant<int, 8>());
+  else if (cache->dim <= 128) with(std::integral_constant<int, 16>());
+  else with(std::integral_constant<int, 32>());
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
 }
