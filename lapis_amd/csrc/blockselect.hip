@@ -7,6 +7,10 @@
 namespace lapis {
 namespace {
 
+// 64-bit division takes a hundred instructions on the device; most operands here fit 32 bits.
+__host__ __device__ inline long long quotient(long long a, long long b) {  // both non-negative
+  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
 // ---- pooling --------------------------------------------------------------------------------------------------
 
 struct PoolArgs {
@@ -36,18 +40,21 @@ __global__ __launch_bounds__(256) void block_pool_kernel(PoolArgs a) {
   if (d < a.dim) {
     const typename T::elem *x = (const typename T::elem *)a.x + b * a.stride[0] + d;
     const long long n = held * a.group;
-    // row i of the block is token i / group, head i % group
-    long long t = part / a.group;
-    int h = part % a.group;
-    for (long long i = part; i < n; i += PARTS) {
-      float f[8];
-      widen<T>(*(const vec8<T> *)(x + (t0 + t) * a.stride[1] + (h0 + h) * a.stride[2]), f);
+    // row i of the block is token i / group, head i % group; four rows on their way at a time
+    const auto at_row = [&](long long i) {
+      const long long t = a.group == 1 ? i : quotient(i, a.group);
+      return x + (t0 + t) * a.stride[1] + (h0 + (int)(i - t * a.group)) * a.stride[2];
+    };
+    for (long long i = part; i < n; i += 4 * PARTS) {
+      vec8<T> read[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += f[e];
-      h += PARTS;
-      while (h >= a.group) {
-        h -= a.group;
-        ++t;
+      for (int u = 0; u < 4; ++u) read[u] = i + u * PARTS < n ? load_stream((const vec8<T> *)at_row(i + u * PARTS)) : vec8<T>{};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float f[8];
+        widen<T>(read[u], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += f[e];
       }
     }
   }
@@ -95,10 +102,6 @@ struct SelectArgs {
   long long list_entries;  // of one list, where every list has the same
 };
 
-// 64-bit division takes a hundred instructions on the device; most operands here fit 32 bits.
-__host__ __device__ inline long long quotient(long long a, long long b) {  // both non-negative
-  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
-}
 __host__ __device__ inline long long floor_div(long long a, long long b) { return a >= 0 ? quotient(a, b) : -quotient(-a + b - 1, b); }
 
 // sum over i < n of floor((a i + b) / m), all non-negative, by the steps of Euclid's algorithm
