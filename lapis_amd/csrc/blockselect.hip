@@ -197,29 +197,53 @@ __device__ __forceinline__ long long row_of_codes(const SelectArgs &a, long long
   return page >= 0 && page < a.pages ? page : -1;
 }
 
+constexpr unsigned kTaken = 0xffffffffu;  // key of a block that is taken whatever it scores
+
 // The `need` best of `seen` keys, fewer than seen; `key(i)` is this lane's key of block 64 i + lane (0 from `seen` on), NV > 0: i
-// below NV, from registers.  Bit by bit from the first one in which the keys differ: the largest threshold that leaves at least
-// `need` blocks at or above it, or one that leaves just as many.  Equal keys at the threshold are taken from the lowest block on.
+// below NV, from registers.  A threshold that leaves `need` blocks at or above it is searched for from the best score down,
+// half an octave, two, eight ... of scores away, then by halving; the largest that leaves more, if none leaves as many.  (Bit
+// by bit over the whole range took twice as many steps: most of them went through exponents that no score has.)
+// Equal keys at the threshold are taken from the lowest block on.
 template <int NV, typename Key>
 __device__ __forceinline__ void take_best(int seen, int need, int *out, int lane, const int *__restrict__ table, Key key) {
   const int steps = NV ? NV : (seen + 63) / 64;
   unsigned most = 0, least = 0xffffffffu;
 #pragma unroll NV ? NV : 1
   for (int i = 0; i < steps; ++i) {
-    most = max(most, key(i));
-    least = min(least, i * 64 + lane < seen ? key(i) : 0xffffffffu);
+    const unsigned k = key(i);
+    most = max(most, k == kTaken ? 0u : k);
+    least = min(least, i * 64 + lane < seen ? k : 0xffffffffu);
   }
-  most = group_max<64>(most);
-  least = ~group_max<64>(~least);
-  const int top = most == least ? -1 : 31 - __clz(most ^ least);
-  unsigned threshold = top < 0 ? most : top == 31 ? 0u : most >> (top + 1) << (top + 1);  // what all have in common
-  int at_or_above = seen;
-  for (int bit = top; bit >= 0 && at_or_above != need; --bit) {
-    const unsigned candidate = threshold | (1u << bit);
+  most = __builtin_amdgcn_readfirstlane(group_max<64>(most));
+  least = __builtin_amdgcn_readfirstlane(~group_max<64>(~least));
+  const auto at_least = [&](unsigned candidate) {
     int n = 0;
 #pragma unroll NV ? NV : 1
     for (int i = 0; i < steps; ++i) n += __popcll(__ballot(key(i) >= candidate));
-    if (n >= need) threshold = candidate, at_or_above = n;
+    return n;
+  };
+  unsigned threshold = least, beyond = most + 1;  // too few are at or above `beyond`, or just as many
+  int at_or_above = seen;
+  const int taken_anyway = at_least(beyond);
+  if (taken_anyway >= need) {
+    threshold = beyond;
+    at_or_above = need;
+  } else {
+    for (unsigned step = 1u << 22; step != 0 && most > least && most - least > step; step <<= 2) {
+      const int n = at_least(most - step);
+      if (n >= need) {
+        threshold = most - step;
+        at_or_above = n;
+        break;
+      }
+      beyond = most - step;
+    }
+    while (at_or_above != need && beyond - threshold > 1) {
+      const unsigned middle = threshold + (beyond - threshold) / 2;
+      const int n = at_least(middle);
+      if (n >= need) threshold = middle, at_or_above = n;
+      else beyond = middle;
+    }
   }
   int equal_left = need;  // of the blocks at the threshold itself
   if (at_or_above != need) {
@@ -327,7 +351,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long lo
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = i * 64 + lane;
-      k[i] = j >= seen ? 0u : j < a.sink || j >= seen - a.local ? 0xffffffffu : keys[r][j];
+      k[i] = j >= seen ? 0u : j < a.sink || j >= seen - a.local ? kTaken : keys[r][j];
     }
     take_best<NV>(seen, need, out, lane, table, [&](int i) { return k[i]; });
   }
@@ -355,7 +379,7 @@ __global__ __launch_bounds__(64) void block_select_long_kernel(SelectArgs a, uns
   unsigned *mine = scores + at * a.columns;  // a lane reads what it has written itself
   const signed char *q = a.q + row * a.dim;
   for (long long j = lane; j < p.seen; j += 64) {
-    unsigned key = 0xffffffffu;
+    unsigned key = kTaken;
     if (j >= a.sink && j < p.seen - a.local) {
       const long long from = row_of_codes(a, b, j);
       float score = __builtin_nanf("");
