@@ -100,6 +100,9 @@ struct SelectArgs {
   long long table_width, pages;
   int *pos, *crd;
   long long list_entries;  // of one list, where every list has the same
+  // entries_before()'s stretches, the same for all rows; step_rows > 0: block_n is a multiple of block_m, and then
+  // floor((block_m i + c) / block_n) is floor((i + shift) / step_rows)
+  long long first_row, full_row, shift, step_rows, steps_before;
 };
 
 __host__ __device__ inline long long floor_div(long long a, long long b) { return a >= 0 ? quotient(a, b) : -quotient(-a + b - 1, b); }
@@ -129,12 +132,19 @@ __host__ __device__ inline long long floor_sum(long long n, long long m, long lo
   return total;
 }
 
-// Blocks that row r may see (causal or all of `columns`).
+// Blocks that row r may see (causal or all of `columns`).  Queries and keys are counted with 31 bits.
 __host__ __device__ inline long long blocks_seen(const SelectArgs &a, long long r) {
   if (!a.causal) return a.columns;
-  const long long end = (r + 1) * a.block_m, last = (end < a.queries ? end : a.queries) - 1;
-  const long long n = floor_div(last + a.keys - a.queries, a.block_n) + 1;
-  return n < 0 ? 0 : n < a.columns ? n : a.columns;
+  const long long end = (r + 1) * a.block_m, last = (end < a.queries ? end : a.queries) - 1 + a.keys - a.queries;
+  if (last < 0) return 0;
+  const long long n = (unsigned)last / (unsigned)a.block_n + 1;
+  return n < a.columns ? n : a.columns;
+}
+
+// Sum over x below y of floor(x / q).
+__host__ __device__ inline long long stairs(long long y, long long q) {
+  const long long k = quotient(y, q);
+  return q * (k * (k - 1) / 2) + k * (y - k * q);
 }
 
 // Entries of the rows before row r of a list: min(count, seen) grows with r in three stretches (none, floor((block_m i +
@@ -144,18 +154,32 @@ __host__ __device__ inline long long entries_before(const SelectArgs &a, long lo
   if (!a.causal) return r * cap;
   if (r <= 0) return 0;
   const long long before = r < a.rows ? r : a.rows - 1;  // the last row's end is cut: it is added by itself
-  const long long c = a.block_m - 1 + a.keys - a.queries + a.block_n;
-  long long i0 = -floor_div(c - a.block_n, a.block_m), i1 = -floor_div(c - cap * a.block_n, a.block_m);
-  i0 = i0 < 0 ? 0 : i0;
-  i1 = i1 < i0 ? i0 : i1;
-  const long long stop = before < i1 ? before : i1;
-  long long total = stop > i0 ? floor_sum(stop - i0, a.block_n, a.block_m, a.block_m * i0 + c) : 0;
-  if (before > i1) total += (before - i1) * cap;
+  const long long stop = before < a.full_row ? before : a.full_row;
+  long long total = 0;
+  if (stop > a.first_row) {
+    if (a.step_rows > 0) total = stairs(stop + a.shift, a.step_rows) - a.steps_before;
+    else total = floor_sum(stop - a.first_row, a.block_n, a.block_m, a.block_m * (a.first_row + 1) - 1 + a.keys - a.queries + a.block_n);
+  }
+  if (before > a.full_row) total += (before - a.full_row) * cap;
   if (r == a.rows) {
     const long long seen = blocks_seen(a, r - 1);
     total += seen < cap ? seen : cap;
   }
   return total;
+}
+
+// The stretches: the first row that sees a block, and the first that sees `cap`.
+inline void set_stretches(SelectArgs *a) {
+  const long long cap = a->count < a->columns ? a->count : a->columns, c = a->block_m - 1 + a->keys - a->queries + a->block_n;
+  a->first_row = -floor_div(c - a->block_n, a->block_m);
+  a->full_row = -floor_div(c - cap * a->block_n, a->block_m);
+  if (a->first_row < 0) a->first_row = 0;
+  if (a->full_row < a->first_row) a->full_row = a->first_row;
+  a->step_rows = a->block_n % a->block_m == 0 ? a->block_n / a->block_m : 0;
+  a->shift = floor_div(c, a->block_m);
+  // from first_row on every term is at least 1, so i + shift is not negative there
+  if (a->step_rows > 0 && a->first_row + a->shift >= 0) a->steps_before = stairs(a->first_row + a->shift, a->step_rows);
+  else a->step_rows = 0;
 }
 
 // Scores as unsigned numbers in the same order, NaN first.
@@ -173,7 +197,7 @@ struct RowPlace {
 
 // Of the rows r0 .. of a list, lane i's.  (All lanes of a wavefront call.)
 __device__ __forceinline__ RowPlace place_of_row(const SelectArgs &a, long long list, long long r0, int lane) {
-  const long long b = list / a.heads, h = list - b * a.heads, r = r0 + lane;
+  const long long b = (unsigned)list / (unsigned)a.heads, h = list - b * a.heads, r = r0 + lane;
   if (a.blocks) {
     long long before = 0;
     for (long long i = lane; i < b; i += 64) before += min(max(0ll, min((long long)a.blocks[i], a.columns)), a.count);
@@ -282,7 +306,9 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long lo
   __shared__ int most_seen;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
   const long long block = xcd_contiguous_block(linear_block(), gridDim.x * gridDim.y);
-  const long long list = block / tiles_of_list, r0 = (block - list * tiles_of_list) * RT, b = list / a.heads, h = list - b * a.heads;
+  // (the grid has fewer than 2^32 workgroups)
+  const long long list = (unsigned)block / (unsigned)tiles_of_list, r0 = (block - list * tiles_of_list) * RT;
+  const long long b = (unsigned)list / (unsigned)a.heads, h = list - b * a.heads;
   if (list >= a.batch * a.heads) return;
   const int rows = (int)min((long long)RT, a.rows - r0);
   if (wave == 0) {
@@ -437,6 +463,7 @@ int read_select(const char *what, const lapis_hip_select_args *p, SelectArgs *a)
   a->pos = p->pos;
   a->crd = p->crd;
   LAPIS_REQUIRE(a->columns >= 0 && a->columns <= INT32_MAX, "%s: %lld blocks", what, (long long)a->columns);
+  set_stretches(a);
   a->list_entries = a->rows ? entries_before(*a, a->rows) : 0;
   const double lists = (double)p->batch * (double)p->heads;
   LAPIS_REQUIRE(lists * (double)a->rows < 2147483647.0 && lists * (double)a->list_entries < 2147483647.0,
