@@ -183,11 +183,11 @@ inline void set_stretches(SelectArgs *a) {
 }
 
 // Scores as unsigned numbers in the same order, NaN first.
-__device__ __forceinline__ unsigned sortable(float x) {
-  if (x != x) return 0u;
-  const unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);  // -0 becomes 0
-  return b >> 31 ? ~b : b | 0x80000000u;
+__device__ __forceinline__ unsigned sortable_number(float x) {  // not NaN
+  const int b = __builtin_bit_cast(int, x + 0.0f);  // -0 becomes 0
+  return (unsigned)(b ^ (b >> 31 | (int)0x80000000));
 }
+__device__ __forceinline__ unsigned sortable(float x) { return x != x ? 0u : sortable_number(x); }
 
 // What a row may see, and where its entries go.
 struct RowPlace {
@@ -221,6 +221,19 @@ __device__ __forceinline__ long long row_of_codes(const SelectArgs &a, long long
   return page >= 0 && page < a.pages ? page : -1;
 }
 
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+  v = group_max<16>(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  const unsigned a = max((unsigned)p[0], (unsigned)p[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return max((unsigned)q[0], (unsigned)q[1]);
+}
+
+// Set bits of a mask below this lane's.
+__device__ __forceinline__ int lanes_below(unsigned long long mask) {
+  return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
+}
+
 constexpr unsigned kTaken = 0xffffffffu;  // key of a block that is taken whatever it scores
 
 // The `need` best of `seen` keys, fewer than seen; `key(i)` is this lane's key of block 64 i + lane (0 from `seen` on), NV > 0: i
@@ -231,29 +244,27 @@ constexpr unsigned kTaken = 0xffffffffu;  // key of a block that is taken whatev
 template <int NV, typename Key>
 __device__ __forceinline__ void take_best(int seen, int need, int *out, int lane, const int *__restrict__ table, Key key) {
   const int steps = NV ? NV : (seen + 63) / 64;
-  unsigned most = 0, least = 0xffffffffu;
+  unsigned most = 0;
 #pragma unroll NV ? NV : 1
   for (int i = 0; i < steps; ++i) {
     const unsigned k = key(i);
     most = max(most, k == kTaken ? 0u : k);
-    least = min(least, i * 64 + lane < seen ? k : 0xffffffffu);
   }
-  most = __builtin_amdgcn_readfirstlane(group_max<64>(most));
-  least = __builtin_amdgcn_readfirstlane(~group_max<64>(~least));
+  most = __builtin_amdgcn_readfirstlane(wave_max(most));
   const auto at_least = [&](unsigned candidate) {
     int n = 0;
 #pragma unroll NV ? NV : 1
     for (int i = 0; i < steps; ++i) n += __popcll(__ballot(key(i) >= candidate));
     return n;
   };
-  unsigned threshold = least, beyond = most + 1;  // too few are at or above `beyond`, or just as many
+  unsigned threshold = 0, beyond = most + 1;  // too few are at or above `beyond`, or just as many
   int at_or_above = seen;
   const int taken_anyway = at_least(beyond);
   if (taken_anyway >= need) {
     threshold = beyond;
     at_or_above = need;
   } else {
-    for (unsigned step = 1u << 22; step != 0 && most > least && most - least > step; step <<= 2) {
+    for (unsigned step = 1u << 22; step != 0 && most > step; step <<= 2) {
       const int n = at_least(most - step);
       if (n >= need) {
         threshold = most - step;
@@ -269,24 +280,32 @@ __device__ __forceinline__ void take_best(int seen, int need, int *out, int lane
       else beyond = middle;
     }
   }
-  int equal_left = need;  // of the blocks at the threshold itself
-  if (at_or_above != need) {
-    int above = 0;
-#pragma unroll NV ? NV : 1
-    for (int i = 0; i < steps; ++i) above += __popcll(__ballot(key(i) > threshold));
-    equal_left = need - above;
-  }
   int at = 0;
+  const auto put = [&](bool take, int i) {
+    const unsigned long long taken = __ballot(take);
+    if (take) {
+      const int j = i * 64 + lane;
+      out[at + lanes_below(taken)] = table ? table[j] : j;
+    }
+    at += __popcll(taken);
+  };
+  if (at_or_above == need && threshold > 0) {
+#pragma unroll NV ? NV : 1
+    for (int i = 0; i < steps; ++i) put(key(i) >= threshold, i);
+    return;
+  }
+  int above = 0;
+#pragma unroll NV ? NV : 1
+  for (int i = 0; i < steps; ++i) above += __popcll(__ballot(key(i) > threshold));
+  int equal_left = need - above;  // of the blocks at the threshold itself
 #pragma unroll NV ? NV : 1
   for (int i = 0; i < steps; ++i) {
-    const int j = i * 64 + lane;
-    const bool equal = j < seen && key(i) == threshold;
-    const unsigned long long ties = __ballot(equal), below = (1ull << lane) - 1;
-    const bool take = j < seen && (key(i) > threshold || (equal && __popcll(ties & below) < equal_left));
+    const unsigned k = key(i);
+    const bool equal = i * 64 + lane < seen && k == threshold;
+    const unsigned long long ties = __ballot(equal);
+    const bool take = k > threshold || (equal && lanes_below(ties) < equal_left);
     equal_left -= min(__popcll(ties), equal_left);
-    const unsigned long long taken = __ballot(take);
-    if (take) out[at + __popcll(taken & below)] = table ? table[j] : j;
-    at += __popcll(taken);
+    put(take, i);
   }
 }
 
@@ -360,8 +379,13 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long lo
         v4i dot = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KC; ++s) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[x][s], kf[s], dot, 0, 0, 0);
+        if (__any(abs_bits(scale) >= kInfBits)) {  // only then is there a NaN
 #pragma unroll
-        for (int e = 0; e < 4; ++e) keys[16 * x + 4 * quarter + e][j] = sortable((float)dot[e] * scale);
+          for (int e = 0; e < 4; ++e) keys[16 * x + 4 * quarter + e][j] = sortable((float)dot[e] * scale);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) keys[16 * x + 4 * quarter + e][j] = sortable_number((float)dot[e] * scale);
+        }
       }
     }
   __syncthreads();
@@ -373,12 +397,12 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long lo
       take_all(seen, out, lane, table);
       continue;
     }
+    const int sink = (int)a.sink, local = (int)a.local;
+    for (int x = lane; x < sink + local; x += 64) keys[r][x < sink ? x : seen - local + x - sink] = kTaken;
+    wave_lds_sync();
     unsigned k[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = i * 64 + lane;
-      k[i] = j >= seen ? 0u : j < a.sink || j >= seen - a.local ? kTaken : keys[r][j];
-    }
+    for (int i = 0; i < NV; ++i) k[i] = i * 64 + lane < seen ? keys[r][i * 64 + lane] : 0u;
     take_best<NV>(seen, need, out, lane, table, [&](int i) { return k[i]; });
   }
 }
