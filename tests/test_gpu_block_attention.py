@@ -329,3 +329,88 @@ def test_the_c_entries_refuse(gpu):
     odd = torch.empty((1, 32, 2, 65), dtype=q.dtype, device="cuda")[..., :64]
     with pytest.raises(gpu.LapisHipError, match="multiples of 8"):
         gpu.block_attention(odd, k, v, pos, crd, out, lse, block_m=32, block_n=32)
+
+
+# ---- many rows: workgroups of 128 rows, units from counters, the lists of columns in three launches ---------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("queries,keys,heads,block_m,block_n,dim,causal", [
+    (300, 300, 8, 40, 16, 64, True), (300, 211, 8, 64, 32, 128, True), (257, 500, 16, 64, 64, 40, True),
+    (300, 300, 24, 100, 128, 104, True), (200, 700, 8, 33, 256, 128, False), (330, 90, 16, 128, 64, 72, True)])
+def test_many_rows(gpu, queries, keys, heads, block_m, block_n, dim, causal, dtype):
+    # 8 key-value heads times 4 batch entries times two to ten rows of blocks: more than half a workgroup to a compute unit
+    t = make(4, queries, keys, heads, 8, dim, TYPES[dtype], queries + dim)
+    pos, crd = random_lists(32, -(-queries // block_m), -(-keys // block_n), 9, dim, empty=0.1)
+    check(gpu, "%s %d x %d, %d heads, blocks %d x %d, dim %d" % (dtype, queries, keys, heads, block_m, block_n, dim), t, pos, crd, block_m,
+          block_n, causal)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
+@pytest.mark.parametrize("block_n", [16, 64, 128])
+def test_many_rows_beside_what_nothing_attends_to(gpu, bad, block_n):
+    """Keys past every compared query's position, inside listed blocks and in unlisted ones, may hold anything."""
+    q, k, v, dout = make(4, 160, 160, 16, 8, 64, torch.bfloat16, 9)
+    rows, columns = 5, -(-160 // block_n)
+    listed = [[c for c in range(columns) if c * block_n <= 32 * r + 31] for r in range(rows)] * 32
+    pos = torch.tensor([0] + [len(x) for x in listed], dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
+    crd = torch.tensor(sum(listed, []), dtype=torch.int32).cuda()
+    sizes = dict(block_m=32, block_n=block_n, causal=True)
+    w = ref.pair_weights(pos, crd, 4, 8, 160, 160, 32, block_n, True)
+    want, want_lse, bound, _ = ref.forward(q, k, v, w, 64 ** -0.5)
+    for at in (150, 33):
+        bk, bv = k.clone(), v.clone()
+        bk[:, at:], bv[:, at:] = bad, bad
+        out, lse = run_forward(gpu, q, bk, bv, pos, crd, **sizes)
+        dq, _, _ = run_backward(gpu, dout, q, bk, bv, out, lse, pos, crd, **sizes)
+        torch.cuda.synchronize()
+        ref.assert_within(out[:, :at], want[:, :at], bound[:, :at], "rows before %d, %r" % (at, bad))
+        seen = w.clone()
+        seen[:, :, at:] = 0  # the rows from `at` on are not compared
+        wants, bounds = ref.backward(dout, q, k, v, torch.where(torch.isfinite(out), out, 0.0), torch.where(torch.isfinite(lse), lse, 0.0), seen, 64 ** -0.5)
+        ref.assert_within(dq[:, :at], wants[0][:, :at], bounds[0][:, :at], "dq before %d, %r" % (at, bad))
+
+
+def test_lists_of_many_blocks(gpu):
+    """A few hundred entries to a row, in any order: more than a wavefront looks up at a time."""
+    t = make(4, 96, 4100, 8, 8, 64, torch.bfloat16, 77)
+    pos, crd = random_lists(32, 2, 257, 250, 3, empty=0.0, ordered=False)
+    check(gpu, "long lists", t, pos, crd, 64, 16, True)
+
+
+@pytest.mark.parametrize("queries,keys,block_m,block_n", [(1100, 1100, 2, 16), (60, 16500, 4, 16), (1030, 16500, 2, 16)])
+def test_more_rows_or_columns_than_one_workgroup_lists(gpu, queries, keys, block_m, block_n):
+    t = make(1, queries, keys, 1, 1, 16, torch.float16, queries)
+    pos, crd = random_lists(1, -(-queries // block_m), -(-keys // block_n), 30, keys, empty=0.2)
+    check(gpu, "%d rows, %d columns" % (pos.numel() - 1, -(-keys // block_n)), t, pos, crd, block_m, block_n, True)
+
+
+def test_one_column_that_every_row_names(gpu):
+    """Its entries are several units of work, added up afterwards; most columns have none."""
+    t = make(1, 4000, 640, 4, 2, 64, torch.bfloat16, 5)
+    rows = 63
+    g = torch.Generator().manual_seed(2)
+    other = torch.randint(1, 10, (2 * rows,), generator=g)
+    crd = torch.stack([torch.zeros_like(other), other], 1).reshape(-1).to(torch.int32).cuda()
+    pos = (torch.arange(2 * rows + 1) * 2).to(torch.int32).cuda()
+    check(gpu, "a column of 63 entries", t, pos, crd, 64, 64, False)
+
+
+def test_many_rows_the_same_bits_again_and_in_a_graph(gpu):
+    q, k, v, dout = make(4, 500, 500, 16, 8, 64, torch.bfloat16, 21)
+    pos, crd = random_lists(32, 8, 16, 12, 7)
+    sizes = dict(block_m=64, block_n=32, causal=True)
+    want = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    want += tuple(run_backward(gpu, dout, q, k, v, *want, pos, crd, **sizes))
+    torch.cuda.synchronize()
+    got = [torch.empty_like(x) for x in want]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.block_attention(q, k, v, pos, crd, *got[:2], **sizes)
+        gpu.block_attention_backward(dout, q, k, v, *got[:2], pos, crd, *got[2:], **sizes)
+    for _ in range(4):
+        for x in got:
+            x.fill_(5.0)
+        graph.replay()
+        again = run_forward(gpu, q, k, v, pos, crd, **sizes)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(again, want))

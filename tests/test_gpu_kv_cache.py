@@ -290,3 +290,34 @@ def test_the_c_entries_refuse(gpu):
     kc, vc, _, _ = empty_cache(1, 1, 16, 64, torch.bfloat16)
     with pytest.raises(gpu.LapisHipError, match="16-byte"):
         gpu.kv_store(flat, k, slots, kc, vc)
+
+
+@pytest.mark.parametrize("cache", ["f8", "same"])
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "f16"), (168, "bf16")])
+def test_many_rows_move_as_few_do(gpu, cache, dim, dtype):
+    """Enough rows for four to a thread, an odd number of them: the same bits as in calls of fewer
+    rows, which the tests above hold to the formulas."""
+    heads, tokens, page = 8, 70001 if dim == 64 else 35003, 64
+    dt = TYPES[dtype]
+    pages = -(-tokens // page) + 1
+    g = torch.Generator().manual_seed(dim)
+    k, v = (torch.randn((tokens, heads, dim), generator=g).to(dt).cuda() for _ in range(2))
+    slots = torch.randperm(pages * page, generator=g)[:tokens].to(torch.int32)
+    slots[5::1000] = -1
+    slots = slots.cuda()
+    print("case", cache, dim, dtype, flush=True)
+    stored, loaded = [], []
+    for step in (tokens, 4001):
+        c = empty_cache(pages, heads, page, dim, TYPES["f8"] if cache == "f8" else dt)
+        ko, vo = (torch.full_like(k, 7.0) for _ in range(2))
+        for i in range(0, tokens, step):
+            gpu.kv_store(k[i:i + step], v[i:i + step], slots[i:i + step], *c)
+            gpu.kv_load(*c[:2], slots[i:i + step], ko[i:i + step], vo[i:i + step], *c[2:])
+        torch.cuda.synchronize()
+        stored.append([x.view(torch.uint8) for x in c if x is not None])
+        loaded.append((ko, vo))
+    assert all(torch.equal(x, y) for x, y in zip(*stored)) and all(torch.equal(x, y) for x, y in zip(*loaded))
+    live = slots >= 0
+    assert bool((loaded[0][0][~live] == 0).all()) and bool((loaded[0][1][~live] == 0).all())
+    if cache == "same":
+        assert torch.equal(loaded[0][0][live], k[live]) and torch.equal(loaded[0][1][live], v[live])
