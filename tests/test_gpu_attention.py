@@ -1,0 +1,113 @@
+"""The operators of block-sparse attention put together: gradients through chosen blocks, a cache that grows token by token."""
+import pytest
+import torch
+
+import attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def attention(gpu):
+    from lapis_amd import attention
+    return attention
+
+
+def test_gradients_through_chosen_blocks(attention):
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(s, generator=g).to(torch.bfloat16).cuda().requires_grad_() for s in ((2, 200, 4, 64), (2, 200, 2, 64), (2, 200, 2, 64)))
+    blocks = attention.choose_blocks(q, k, 4, 32, 16)
+    out = attention.attend(q, k, v, blocks, 0.2)
+    weight = torch.randn((2, 200, 64, 4), generator=g).to(torch.bfloat16).cuda().transpose(2, 3)  # a gradient that is not contiguous
+    (out * weight).sum().backward()
+    w = ref.pair_weights(blocks.pos, blocks.crd, 2, 2, 200, 200, 32, 16, True)
+    assert int(w.amax()) == 1 and bool((w[:, :, torch.arange(200), torch.arange(200)] == 1).all())  # a query's own block is listed
+    want, lse, bound, _ = ref.forward(q, k, v, w, 0.2)
+    ref.assert_within(out, want, bound, "out")
+    lse = lse.float().cuda()
+    wants, bounds = ref.backward(weight, q, k, v, out, lse, w, 0.2)
+    for name, x, y, z in zip(("dq", "dk", "dv"), (q, k, v), wants, bounds):
+        ref.assert_within(x.grad, y, z, name)
+    # a sum's gradient is a broadcast one
+    q.grad = None
+    attention.attend(q, k, v, blocks).sum().backward()
+    assert bool(torch.isfinite(q.grad).all())
+
+
+@pytest.mark.parametrize("f8", [False, True], ids=["bf16", "f8"])
+def test_a_cache_that_grows(attention, f8):
+    """Three sequences of different lengths, one of them empty at first; all pages are read, so that the answer is that of
+    attention over everything."""
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
+    cache = attention.PagedCache(3, 30, 160, 2, 64, page=16, f8=f8)
+    history = []
+    for s, n in enumerate((37, 0, 64)):
+        k, v = r(n, 2, 64), r(n, 2, 64)
+        if n:
+            cache.prefill(s, k, v)
+        history.append([k, v])
+    for step in range(40):
+        q, k, v = r(3, 4, 64), r(3, 2, 64), r(3, 2, 64)
+        out = cache.step(q, k, v, count=10)
+        for s in range(3):
+            history[s] = [torch.cat([history[s][0], k[s:s + 1]]), torch.cat([history[s][1], v[s:s + 1]])]
+            if step % 13 == 0 or step == 39:
+                hk, hv = history[s]
+                if f8:
+                    hk, hv = (codes(x) for x in (hk, hv))
+                keys = hk.shape[0]
+                want, _, bound, _ = ref.forward(q[s:s + 1, None], hk[None], hv[None], torch.ones((1, 2, 1, keys), dtype=torch.float64), 64 ** -0.5)
+                ref.assert_within(out[s:s + 1, None], want, bound, "step %d, sequence %d" % (step, s))
+    assert cache.lengths == [77, 40, 104] == cache.length.tolist()
+
+
+def codes(x):
+    """What an e4m3 cache holds of x; on the CPU, whose division by a number is a division."""
+    x = x.cpu()
+    scale = x.float().abs().amax(-1, keepdim=True) / 448.0
+    return (x.float() / scale).to(torch.float8_e4m3fn).double() * scale.double()
+
+
+def test_few_pages_of_a_long_sequence(attention):
+    """The page a query is made for is found, and what it reads is attention over the chosen pages."""
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
+    cache = attention.PagedCache(1, 70, 1100, 1, 64, page=16)
+    k, v = r(1001, 1, 64) * 0.1, r(1001, 1, 64)
+    k[320:336] += 3.0 * r(1, 1, 64)
+    cache.prefill(0, k, v)
+    q = (k[325:326] * 2).expand(1, 2, 64).contiguous()
+    nk, nv = r(1, 1, 64), r(1, 1, 64)
+    out = cache.step(q, nk, nv, count=1 + 2 + 1)
+    k, v = torch.cat([k, nk]), torch.cat([v, nv])
+    # the first page, page 20 and the last two (the last holds 10 tokens)
+    listed = torch.cat([torch.arange(16), torch.arange(320, 336), torch.arange(976, 1002)])
+    w = torch.zeros((1, 1, 1, 1002), dtype=torch.float64)
+    w[..., listed] = 1
+    want, _, bound, _ = ref.forward(q[:, None], k[None], v[None], w, 64 ** -0.5)
+    ref.assert_within(out[:, None], want, bound, "four pages")
+
+
+def test_pages_run_out_and_come_back(attention):
+    cache = attention.PagedCache(2, 4, 64, 1, 64, page=16)
+    x = torch.ones((33, 1, 64), dtype=torch.bfloat16, device="cuda")
+    cache.prefill(0, x, x)
+    with pytest.raises(ValueError, match="holds 33 tokens"):
+        cache.prefill(0, x, x)
+    with pytest.raises(RuntimeError, match="2 more pages for sequence 1, 1 are free"):
+        cache.prefill(1, x[:17], x[:17])
+    assert cache.lengths == [33, 0] and len(cache.free) == 1
+    cache.release(0)
+    cache.prefill(1, x, x)
+    assert len(cache.free) == 1 and cache.lengths == [0, 33]
+    with pytest.raises(ValueError, match="local = 0"):
+        cache.step(x[:2], x[:2], x[:2], 2, local=0)
+
+
+def test_the_example(attention):
+    lines = []
+    losses, difference, answered = attention.main(tokens=1024, asked=64, steps=12, count=16, log=lines.append)
+    assert losses[-1] < losses[0] and lines
+    # both sides round to bf16 once or twice, of answers below 8 in size
+    assert difference < (8 * 2.0 ** -8) ** 2 and answered == answered
