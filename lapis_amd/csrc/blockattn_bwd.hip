@@ -525,14 +525,38 @@ constexpr int kMostEntries = 384;  // of a unit
 // 318 registers, one wavefront a SIMD and nothing to fill the waits with (1.06 ms at 8k queries); P handed over
 // through LDS saves a product of five, but its barrier in the middle of every tile costs more (0.67 ms against 0.57).
 // Where keys are few (KG = 1) two pairs take turns with the tiles and add up at the end.
-// The rows of a column lie all over Q and dO, beyond L2 in large passes: S tiles are on their way or being computed, where a
-// tile's rows lie is worked out one tile earlier still, and no load but those into LDS is in the loop.
+// An iteration turns the scores of its tile into weights, then multiplies by them and computes the scores of the next tile in
+// turn, three chains of products that do not wait for each other; where the rows of four tiles lie is worked out by 128
+// threads at once, and what an iteration needs from LDS is asked for a stage before its use.  (A single workgroup, 64 keys,
+// dim 128: 1.35 us an iteration with one chain after the other, 1.10 so; 8192 queries, 32 heads over 8, 16 blocks of 64
+// a row: 630 us to 549, in a trace.)  It is bound by what an iteration of a wavefront waits for: the products alone are 128 us.
+// The rows of a column lie all over Q and dO, beyond L2 in large passes (16 tiles of 128 KB rows each read them: 2.1 GB, 290 us
+// by themselves): S tiles are on their way or being computed, and no load but those into LDS is in the loop.
 // Columns are anything but equal (the first block is listed by all rows, the last by few): workgroups take units from a
 // counter, those of their XCD's part first, whose rows of Q and dO its L2 holds.
+// The kernel's arguments are more than the scalar registers hold beside the loop, and a spilled one in the loop is worse than slow:
+// the wait for it waits for the tiles on their way too (each load one after the other, 3 us a tile).  So whatever the loop does
+// not need all the time is read from the arguments again where it is used.
+struct DkvArgs {
+  BlockArgs a;
+  Columns cols;
+  const float *delta, *logs;
+};
+typedef const __attribute__((address_space(4))) DkvArgs *DkvArgsAgain;
+__device__ __forceinline__ DkvArgsAgain again() {
+  DkvArgsAgain p = (DkvArgsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+// What all lanes of a wavefront agree on, said so that the compiler branches on it and does not walk through both sides.
+__device__ __forceinline__ bool same(bool x) { return __builtin_amdgcn_readfirstlane((int)x) != 0; }
+
 template <typename T, int DP, int KG, int S>
-__global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns cols, const float *__restrict__ delta, const float *__restrict__ logs) {
+__global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
   typedef typename T::elem elem;
-  constexpr int QG = 2 / KG, TG = KG * 128, PIECES = DP / 8, RP = TG / PIECES, PASSES = 32 / RP, DT = DP / 32;
+  constexpr int QG = 2 / KG, TG = KG * 128, PIECES = DP / 8, RP = TG / PIECES, PASSES = 32 / RP, DT = DP / 32, BATCH = 4;
+  static_assert(S <= BATCH, "what is loaded is looked up a batch before");
   struct Info {  // where a tile's rows lie
     long long q[32], g[32];
     int sums[32], last[32];
@@ -540,13 +564,15 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
   };
   __shared__ __attribute__((aligned(16))) elem tiles[QG][S][2][32 * DP];
   __shared__ __attribute__((aligned(16))) float sums[QG][S][2][32];  // log-sums and deltas of a tile's rows
-  __shared__ __attribute__((aligned(16))) Info infos[QG][S + 1];
+  __shared__ __attribute__((aligned(16))) Info infos[QG][2 * BATCH];
   __shared__ int rows_of_unit[kMostEntries], taken;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int role = (wave ^ blockIdx.x / kParts) & 1, kg = (wave >> 1) % KG, qg = (wave >> 1) / KG, gt = tid - qg * TG;  // role 0: dV, 1: dK
-  const bool odd = *cols.odd != 0;
-  const int all_units = (odd ? cols.lists * a.columns : cols.units) * cols.sub;
-  const float c = a.scale * kLog2e;
+  const bool odd = same(*args.cols.odd != 0);
+  const int all_units = (odd ? args.cols.lists * args.a.columns : args.cols.units) * args.cols.sub;
+  const float scale = args.a.scale, c = scale * kLog2e;
+  const int dim = args.a.dim;
+  const elem *const all_q = (const elem *)args.a.q.data, *const all_g = (const elem *)args.a.dout.data;
 
   // One unit for each workgroup, or units from the counters: those of the own part, then of whichever part has some left.
   const bool one_each = all_units <= (int)gridDim.x;
@@ -560,14 +586,15 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
       more = false;
     } else {
       __syncthreads();
-      if (tid == 0) taken = atomicAdd(cols.next + part, 1);
+      int *const next = again()->cols.next;
+      if (tid == 0) taken = atomicAdd(next + part, 1);
       __syncthreads();
       unit_l = part_start(part) + taken;
       if (unit_l >= part_start(part + 1)) {
         bool left = false;
         if (lane < kParts) {
           const int p = (part + lane) % kParts;
-          left = part_start(p) + __hip_atomic_load(cols.next + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < part_start(p + 1);
+          left = part_start(p) + __hip_atomic_load(next + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < part_start(p + 1);
         }
         __syncthreads();
         if (wave == 0) {
@@ -580,6 +607,9 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
         continue;
       }
     }
+    const DkvArgsAgain at_start = again();
+    const auto &a = at_start->a;
+    const auto &cols = at_start->cols;
     const int u = unit_l / cols.sub, sub = unit_l - u * cols.sub;
     int cc, from = 0, n, start = 0;
     bool several = false;
@@ -601,27 +631,20 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
     const int key_low = (column << a.block_n_log2) + in_block, key = key_low + (lane & 31);
     const bool live = in_block + (lane & 31) < (1 << a.block_n_log2) && key < a.keys;
 
-    vec8<T> kf[DP / 16], vf[DP / 16];
-    const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + key * a.k.stride[1] + kh * a.k.stride[2];
-    const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + key * a.v.stride[1] + kh * a.v.stride[2];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      const int d = 16 * s + 8 * half;
-      kf[s] = vf[s] = vec8<T>{};
-      if (live && d < a.dim) kf[s] = *(const vec8<T> *)(kp + d);
-      if (role && live && d < a.dim) vf[s] = *(const vec8<T> *)(vp + d);
-    }
-
-    // this lane's row of the tiles of its group: entry, query of the block and head of the group, moved on by 32 QG each tile
-    const int steps_h = 32 * QG % a.group, steps_q = 32 * QG / a.group % a.block_m, steps_e = 32 * QG / a.group / a.block_m;
-    const int slot0 = qg * 32 + (lane & 31);
+    // Where rows lie is worked out for four tiles of a group at a time, a row to each of 128 threads: one wavefront doing it in
+    // every iteration is what all others wait for.  A thread's row: entry, query of the block and head of the group.
+    const int looks_up = KG == 2 ? (role ? 128 : kg * 64 + lane) : gt, steps = BATCH * 32 * QG;
+    const int steps_h = steps % a.group, steps_q = steps / a.group % a.block_m, steps_e = steps / a.group / a.block_m;
+    const int slot0 = ((looks_up >> 5) * QG + qg) * 32 + (looks_up & 31);
     int entry = slot0 / a.group / a.block_m, in = slot0 / a.group % a.block_m, hd = slot0 % a.group;
     const long long all = (long long)n * a.block_m * a.group;
     const int tiles_n = (int)((all + 32 * QG - 1) / (32 * QG));
-    const auto put_info = [&](int t) {  // of the tiles in turn
-      if (role != 0 || kg != 0) return;
-      if (lane < 32) {
-        Info &i = infos[qg][t % (S + 1)];
+    const auto put_info = [&](int t) {  // of tiles t .. t + 3, batches in turn
+      if (looks_up >= 128) return;
+      const auto &a = again()->a;
+      {
+        Info &i = infos[qg][(t + (looks_up >> 5)) % (2 * BATCH)];
+        const int lane = looks_up & 31;
         int query = 0;
         bool there = entry < n;
         if (there) {
@@ -630,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
         }
         if (odd) {
           int first = 0, count = 0, times = 0;
-          if (there) entries_of(a, (long long)bh * a.rows + entry, &first, &count);
+          if (there) entries_of(a.pos, a.nnz, (long long)bh * a.rows + entry, &first, &count);
           for (int e = 0; e < count; ++e) times += a.crd[first + e] == column;
           i.times[lane] = (float)times;
         }
@@ -649,131 +672,188 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
     };
     const int place = gt % PIECES, my_row = gt / PIECES, in_group = wave - qg * KG * 2;
     constexpr int LOADS = 2 * PASSES;  // at least that many a tile and wavefront
-    const auto load = [&](int t) {
-      const Info &i = infos[qg][t % (S + 1)];
+    struct Places {  // of what this thread loads of a tile
+      long long q[PASSES], g[PASSES];
+      int sums;
+    };
+    const auto look = [&](int t) {
+      const Info &i = infos[qg][t % (2 * BATCH)];
+      Places at;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) at.q[p] = i.q[p * RP + my_row], at.g[p] = i.g[p * RP + my_row];
+      at.sums = i.sums[lane & 31];
+      return at;
+    };
+    const auto load = [&](int t, const Places &from) {
       const int slot = t % S;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
-        const int at = p * RP + my_row, d = (place ^ turn<DP>(at)) * 8;
+        const int d = (place ^ turn<DP>(p * RP + my_row)) * 8;
         const unsigned to = __builtin_amdgcn_readfirstlane(lds_address(tiles[qg][slot][0]) + (p * KG * 2 + in_group) * 1024);
-        if (d < a.dim) {
-          load_to_lds((const elem *)a.q.data + i.q[at] + d, to);
-          load_to_lds((const elem *)a.dout.data + i.g[at] + d, to + 64 * DP);
+        if (d < dim) {
+          load_to_lds(all_q + from.q[p] + d, to);
+          load_to_lds(all_g + from.g[p] + d, to + 64 * DP);
         }
       }
       if (role == 0 && kg == 0 && lane < 32) {
         const unsigned to = __builtin_amdgcn_readfirstlane(lds_address(sums[qg][slot][0]));
-        load_word_to_lds(logs + i.sums[lane], to);
-        load_word_to_lds(delta + i.sums[lane], to + 128);
+        load_word_to_lds(args.logs + from.sums, to);
+        load_word_to_lds(args.delta + from.sums, to + 128);
       }
     };
 
     v16f acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[i] = v16f{};
-    if (a.dim < DP)  // what no row fills stays zero
-      for (int i = tid; i < QG * S * 2 * 32 * PIECES; i += 256) ((v4i *)tiles)[i] = v4i{0, 0, 0, 0};
-    __syncthreads();
-    for (int t = 0; t < S; ++t) put_info(t);
-    __syncthreads();
-    for (int t = 0; t < S - 1; ++t)
-      if (t < tiles_n) load(t);
-    lds_loads_done();
-    __syncthreads();
-    for (int t = 0; t < tiles_n; ++t) {
-      put_info(t + S);
-      if (t + S - 1 < tiles_n) load(t + S - 1);
-      const Info &info = infos[qg][t % (S + 1)];
-      const elem *qt = tiles[qg][t % S][0], *dt = tiles[qg][t % S][1], *by_column = tiles[qg][t % S][1 - role];
-      const int last = info.last[lane & 31];
-      if (__any(last >= key_low)) {
-        const bool cut = odd || __any(last < key_low + 31);
-        const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
-        v16f s = {}, g = {};
-        // operands are read a product ahead of their use at least: left to itself the compiler reads each one just before
-        vec8<T> qa[DP / 16], ga[DP / 16];
+    // The two roles have a loop of their own each, the same barriers in both: what one of them keeps in registers is not kept
+    // free in the other.
+    const auto run = [&](auto with_g) {
+      constexpr bool G = decltype(with_g)::value;
+      vec8<T> kf[DP / 16], vf[DP / 16];
+      const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + key * a.k.stride[1] + kh * a.k.stride[2];
+      const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + key * a.v.stride[1] + kh * a.v.stride[2];
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) qa[y] = *(const vec8<T> *)(qt + place_of<DP>(lane & 31, 2 * y + half));
-        __builtin_amdgcn_sched_barrier(0);
-        if (role) {
+      for (int s = 0; s < DP / 16; ++s) {
+        const int d = 16 * s + 8 * half;
+        kf[s] = vf[s] = vec8<T>{};
+        if (live && d < dim) kf[s] = *(const vec8<T> *)(kp + d);
+        if (G && live && d < dim) vf[s] = *(const vec8<T> *)(vp + d);
+      }
+
+      if (dim < DP)  // what no row fills stays zero
+        for (int i = tid; i < QG * S * 2 * 32 * PIECES; i += 256) ((v4i *)tiles)[i] = v4i{0, 0, 0, 0};
+      __syncthreads();
+      put_info(0);
+      put_info(BATCH);
+      __syncthreads();
+      for (int t = 0; t < S - 1; ++t)
+        if (t < tiles_n) load(t, look(t));
+      lds_loads_done();
+      __syncthreads();
+      // An iteration turns the scores of its tile into weights, then multiplies by them and computes the next tile's scores: three
+      // chains of products that do not wait for each other.
+      int place_lane = lane;  // made anew in each iteration, or the compiler keeps the places of all operands in registers
+      const auto rows_of = [&](const elem *tile, int y) { return *(const vec8<T> *)(tile + place_of<DP>(place_lane & 31, 2 * y + (place_lane >> 5))); };
+      const auto last_of = [&](int t) { return infos[qg][t % (2 * BATCH)].last[lane & 31]; };
+      v16f s = {}, g = {};
+      int last = last_of(0);
+      bool now = tiles_n > 0 && same(__any(last >= key_low));
+      constexpr int N = DP / 16;
 #pragma unroll
-          for (int y = 0; y < DP / 16; ++y) {
-            s = mfma32(qa[y], kf[y], s);
-            ga[y] = *(const vec8<T> *)(dt + place_of<DP>(lane & 31, 2 * y + half));
-          }
-          __builtin_amdgcn_sched_barrier(0);
+      for (int y = 0; y < N; ++y) s = mfma32(rows_of(tiles[qg][0][0], y), kf[y], s);
+      if (G) {
 #pragma unroll
-          for (int y = 0; y < DP / 16; ++y) g = mfma32(ga[y], vf[y], g);
-        } else {
-#pragma unroll
-          for (int y = 0; y < DP / 16; ++y) s = mfma32(qa[y], kf[y], s);
-        }
-        vec8<T> f[2];
+        for (int y = 0; y < N; ++y) g = mfma32(rows_of(tiles[qg][0][1], y), vf[y], g);
+      }
+      for (int t = 0; t < tiles_n; ++t) {
+        asm volatile("" : "+v"(place_lane));
+        if (t % BATCH == 0 && t > 0 && t + BATCH < tiles_n) put_info(t + BATCH);
+        // asked for here, used after the weights
+        const int last_next = last_of(t + 1);
+        const Places from = look(t + S - 1);
+        const elem *qt = tiles[qg][(t + 1) % S][0], *dt = tiles[qg][(t + 1) % S][1], *by_column = tiles[qg][t % S][G ? 0 : 1];
+        vec8<T> f[2] = {};
         unsigned bad = 0;
-        if (!cut) {
+        if (now) {
+          const Info &info = infos[qg][t % (2 * BATCH)];
+          const bool cut = odd || same(__any(last < key_low + 31));
+          const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const v4f off = *(const v4f *)(lse + 8 * j + 4 * half);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * j + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -off[e]));
           }
-          if (role) {
+          if (G) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const v4f del = *(const v4f *)(dl + 8 * j + 4 * half);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * j + e] *= __builtin_fmaf(g[4 * j + e], a.scale, -del[e]);
+              for (int e = 0; e < 4; ++e) s[4 * j + e] *= __builtin_fmaf(g[4 * j + e], scale, -del[e]);
             }
           }
-        } else {
-          // 0 times an infinity or NaN must not count: which rows of the last product's operand hold one?
+          if (cut) {
+            // 0 times an infinity or NaN must not count: which rows of the last product's operand hold one?
 #pragma unroll 1
-          for (int i = 0; i < PIECES / 2; ++i) {
-            const unsigned long long lanes = __ballot(not_finite<T>(*(const vec8<T> *)(by_column + (i * 64 + lane) * 8)));
-            if (lanes == 0) continue;
+            for (int i = 0; i < PIECES / 2; ++i) {
+              const unsigned long long lanes = __ballot(not_finite<T>(*(const vec8<T> *)(by_column + (i * 64 + lane) * 8)));
+              if (lanes == 0) continue;
 #pragma unroll
-            for (int x = 0; x < 64 / PIECES; ++x)
-              if (lanes >> (x * PIECES) & ((1u << PIECES) - 1)) bad |= 1u << (i * (64 / PIECES) + x);
+              for (int x = 0; x < 64 / PIECES; ++x)
+                if (lanes >> (x * PIECES) & ((1u << PIECES) - 1)) bad |= 1u << (i * (64 / PIECES) + x);
+            }
+            bad = __builtin_amdgcn_readfirstlane(bad);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int row = 8 * j + 4 * half + e;
+                float x = s[4 * j + e];
+                if (!G && (bad >> row & 1)) x = __builtin_nanf("");  // its dO is taken as zeros below
+                const float times = odd ? info.times[row] : 1.f;
+                // a row without an entry (log-sum -infinity) sees no key
+                s[4 * j + e] = key <= lim[e] && times != 0.f ? x * times : 0.f;
+              }
+            }
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v4f off = *(const v4f *)(lse + 8 * j + 4 * half), del = *(const v4f *)(dl + 8 * j + 4 * half);
-            const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
+          for (int e = 0; e < 16; ++e) f[e >> 3][e & 7] = (elem)s[e];
+        }
+        if (t + S - 1 < tiles_n) load(t + S - 1, from);
+        const bool next = t + 1 < tiles_n && same(__any(last_next >= key_low));
+        last = last_next;
+        s = v16f{};
+        g = v16f{};
+        const auto column = [&](int y) { return columns_in_order<T, DP>(by_column, 16 * (y / DT), 32 * (y % DT), place_lane); };
+        // Either of two ways through, but not as two sides of one branch: the sums would be kept twice.
+        const bool fast = now && bad == 0;
+        if (fast) {  // (scores of a tile that no row sees are not used)
+          // operands are read some products ahead of their use: left to itself the compiler reads each one just before
+          constexpr int AHEAD = 2;
+          static_assert(2 * DT == N, "as many products of weights as of a score");
+          vec8<T> qa[N], ga[N], x[N];
+          const auto read = [&](int y) {
+            qa[y] = rows_of(qt, y);
+            if (G) ga[y] = rows_of(dt, y);
+            x[y] = column(y);
+          };
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int row = 8 * j + 4 * half + e;
-              float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + e], c, -off[e]));
-              if (role) x *= __builtin_fmaf(g[4 * j + e], a.scale, -del[e]);
-              else if (bad >> row & 1) x = __builtin_nanf("");  // its dO is taken as zeros below
-              const float times = odd ? info.times[row] : 1.f;
-              // a row without an entry (log-sum -infinity) sees no key
-              s[4 * j + e] = key <= lim[e] && times != 0.f ? x * times : 0.f;
+          for (int y = 0; y < AHEAD; ++y) read(y);
+#pragma unroll
+          for (int y = 0; y < N; ++y) {
+            if (y + AHEAD < N) read(y + AHEAD);
+            s = mfma32(qa[y], kf[y], s);
+            if (G) g = mfma32(ga[y], vf[y], g);
+            acc[y % DT] = mfma32(x[y], f[y / DT], acc[y % DT]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        int slow = !fast;
+        asm volatile("" : "+v"(slow));
+        if (__builtin_amdgcn_readfirstlane(slow)) {
+          if (now) {
+#pragma unroll
+            for (int y = 0; y < N; ++y) acc[y % DT] = mfma32(finite_only<T>(column(y)), f[y / DT], acc[y % DT]);
+          }
+          if (next) {
+#pragma unroll
+            for (int y = 0; y < N; ++y) s = mfma32(rows_of(qt, y), kf[y], s);
+            if (G) {
+#pragma unroll
+              for (int y = 0; y < N; ++y) g = mfma32(rows_of(dt, y), vf[y], g);
             }
           }
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) f[e >> 3][e & 7] = (elem)s[e];
-        vec8<T> x[2][DT];
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int i = 0; i < DT; ++i) x[y][i] = columns_in_order<T, DP>(by_column, 16 * y, 32 * i, lane);
-        if (bad) {
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int i = 0; i < DT; ++i) x[y][i] = finite_only<T>(x[y][i]);
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] = mfma32(x[y][i], f[y], acc[i]);
+        now = next;
+        // the tile after the next one has to be there
+        if (t + S - 1 < tiles_n) lds_loads_done<(S - 3) * LOADS>();
+        else lds_loads_done();
+        __syncthreads();
       }
-      if (t + S - 1 < tiles_n) lds_loads_done<(S - 2) * LOADS>();
-      else lds_loads_done();
-      __syncthreads();
-    }
-
+    };
+    if (role) run(std::true_type());
+    else run(std::false_type());
     if (QG > 1) {  // the second pair's sums to the first, with the tiles' memory between them
       float *between = (float *)tiles + role * DT * 1024;
       if (qg > 0) {
@@ -791,8 +871,10 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
       }
     }
     if (qg > 0 || !live) continue;
+    const DkvArgsAgain at_end = again();
     if (several) {
-      const long long slot = 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << a.block_n_log2;
+      const auto &cols = at_end->cols;
+      const long long slot = 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << at_end->a.block_n_log2;
       float *to = cols.partial + (slot * 2 + 1 - role) * each + (long long)(in_block + (lane & 31)) * DP;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -800,7 +882,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
         for (int e = 0; e < 16; e += 4) *(v4f *)(to + 32 * i + 2 * e + 4 * half) = v4f{acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]};
       continue;
     }
-    const View &dkv = role ? a.dk : a.dv;
+    const auto &dkv = role ? at_end->a.dk : at_end->a.dv;
     elem *to = (elem *)dkv.data + b * dkv.stride[0] + key * dkv.stride[1] + kh * dkv.stride[2];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -810,7 +892,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(BlockArgs a, Columns 
         vec4<T> x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = (elem)acc[i][e + j];
-        if (d < a.dim) *(vec4<T> *)(to + d) = x;
+        if (d < dim) *(vec4<T> *)(to + d) = x;
       }
   }
 }
@@ -889,7 +971,7 @@ void launch_dkv(const BlockArgs &a, const Columns &c, const float *delta, const 
   Columns cols = c;
   cols.sub = (int)ceil_div(1 << a.block_n_log2, 32 * KG);
   const int64_t grid = min((int64_t)2 * device_cu_count(), (int64_t)c.units * cols.sub);
-  hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG, S>), dim3((unsigned)grid), dim3(256), 0, st, a, cols, delta, logs);
+  hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG, S>), dim3((unsigned)grid), dim3(256), 0, st, DkvArgs{a, cols, delta, logs});
 }
 
 template <typename T, int DP>
@@ -925,7 +1007,7 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
       hipLaunchKernelGGL(columns_scan_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
       hipLaunchKernelGGL(columns_kernel<true>, grid, dim3(64), 0, st, a, c);
     }
-    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, DP == 64 ? 4 : 2>(a, c, delta, logs, st);
+    if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, DP == 64 ? 4 : 3>(a, c, delta, logs, st);
     else launch_dkv<T, DP, 2, 4>(a, c, delta, logs, st);
     hipLaunchKernelGGL((join_units_kernel<T, DP>), dim3((unsigned)(c.lists * a.columns), 4), dim3(256), 0, st, a, c);
   }

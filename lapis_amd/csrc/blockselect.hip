@@ -23,6 +23,8 @@ struct PoolArgs {
   float *scales;
 };
 
+// Bound by memory: 32 768 tokens of 8 heads, dim 128, bf16, blocks of 64: 12.5 us in a trace for 67 MB that the last-level
+// cache partly holds.
 // A wavefront takes 64 / (L * PARTS) blocks: groups of L lanes hold a row (8 elements each), PARTS of them share a block's
 // rows.  The rows of a block are summed in fp32, part by part, then over the parts.
 template <typename T, int L, int PARTS>
@@ -317,6 +319,7 @@ __device__ __forceinline__ void take_all(int seen, int *out, int lane, const int
 // queries' codes stay in registers), go to LDS as sortable numbers and are taken by a wavefront per row, NV a lane.  The search
 // is one chain of compare, count and branch: it takes many wavefronts to fill the time between, and 64 rows a workgroup, which
 // read the codes of K a quarter as often, left room for a quarter of them (174 us against 96 for 131 072 rows of up to 256).
+// Since then 79 us for those rows, dim 128: bound by vector instructions, about 300 a row, 72 % of the cycles.
 template <int NV, int KC>
 __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long long tiles_of_list) {
   constexpr int RT = 16, STRIDE = NV * 64 + 4;  // rows four apart start 16 banks apart
