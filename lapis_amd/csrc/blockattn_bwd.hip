@@ -530,13 +530,13 @@ constexpr int kMostEntries = 384;  // of a unit
 // threads at once, and what an iteration needs from LDS is asked for a stage before its use.  (A single workgroup, 64 keys,
 // dim 128: 1.35 us an iteration with one chain after the other, 1.10 so; 8192 queries, 32 heads over 8, 16 blocks of 64
 // a row: 630 us to 549, in a trace.)  It is bound by what an iteration of a wavefront waits for: the products alone are 128 us.
-// The rows of a column lie all over Q and dO, beyond L2 in large passes (16 tiles of 128 KB rows each read them: 2.1 GB, 290 us
+// The rows of a column lie all over Q and dO, beyond L2 in large passes (16 columns read each block of rows: 2.1 GB, 290 us
 // by themselves): S tiles are on their way or being computed, and no load but those into LDS is in the loop.
 // Columns are anything but equal (the first block is listed by all rows, the last by few): workgroups take units from a
 // counter, those of their XCD's part first, whose rows of Q and dO its L2 holds.
-// The kernel's arguments are more than the scalar registers hold beside the loop, and a spilled one in the loop is worse than slow:
-// the wait for it waits for the tiles on their way too (each load one after the other, 3 us a tile).  So whatever the loop does
-// not need all the time is read from the arguments again where it is used.
+// The kernel's arguments are more than the scalar registers hold beside the loop (148 spilled, and a wait for a spilled register in
+// the loop waits for the tiles on their way too), so whatever the loop does not need all the time is read from the arguments
+// again where it is used (54 spilled, none in the loop).
 struct DkvArgs {
   BlockArgs a;
   Columns cols;
