@@ -15,6 +15,8 @@ constexpr int kParts = 8;  // of the units of work beside dK and dV, one to each
 
 // As the forward kernel: 32 rows a wavefront, a query per lane.  dS^T = P^T * (scale V dO^T - scale delta) feeds dQ^T = K^T dS^T
 // from its registers.  rowsum(dO * O), times `scale`, and the log-sums in units of ln 2 are left for the other kernel.
+// 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 319 us in a trace (356 with 24 registers spilled and the products
+// one chain after the other), 590 TFLOP/s; bound by what a wavefront waits for between its chains of products.
 template <typename T, int DP, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
@@ -110,11 +112,26 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
       const bool bad = cut && bad_tile[buffer] == t + 1;
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
+        int place_lane = lane;  // made anew each time, or the compiler keeps the places of all operands in registers
+        asm volatile("" : "+v"(place_lane));
+        // two chains of products that do not wait for each other, their operands read two products ahead
+        constexpr int N = DP / 16, AHEAD = 2;
         v16f s = {}, g = {};
+        vec8<T> ka[N], va[N];
+        const auto read = [&](int y) {
+          const int at = place_of<DP>(32 * x + (place_lane & 31), 2 * y + (place_lane >> 5));
+          ka[y] = *(const vec8<T> *)(kt + at);
+          va[y] = *(const vec8<T> *)(vt + at);
+        };
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) s = mfma32(*(const vec8<T> *)(kt + place_of<DP>(32 * x + (lane & 31), 2 * y + half)), qf[y], s);
+        for (int y = 0; y < AHEAD; ++y) read(y);
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) g = mfma32(*(const vec8<T> *)(vt + place_of<DP>(32 * x + (lane & 31), 2 * y + half)), gf[y], g);
+        for (int y = 0; y < N; ++y) {
+          if (y + AHEAD < N) read(y + AHEAD);
+          s = mfma32(ka[y], qf[y], s);
+          g = mfma32(va[y], gf[y], g);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         vec8<T> df[2];
         // dS is rounded to the operands' type for the product, with `scale` in it: smaller by its factor in float16's range
 #pragma unroll
@@ -128,17 +145,20 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
           df[e >> 3][e & 7] = (elem)ds;
         }
         // a row that sees a key with an infinity or NaN has NaN in its score; the others take the key as zeros
-        if (bad) {
+        int clean = !bad;  // either way, but not as two sides of one branch: the sums would be kept twice
+        if (clean) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, place_lane), df[y], acc[i]);
+        }
+        asm volatile("" : "+v"(clean));
+        if (__builtin_amdgcn_readfirstlane(clean) == 0) {
 #pragma unroll
           for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int i = 0; i < DT; ++i)
-              acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, lane)), df[y], acc[i]);
-        } else {
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, lane), df[y], acc[i]);
+              acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, place_lane)), df[y], acc[i]);
         }
       }
     }
