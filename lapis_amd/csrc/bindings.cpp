@@ -8,7 +8,6 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/from_blob.h>
-#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -697,16 +696,25 @@ lapis_hip_rows rows_of(const char *what, const char *name, const at::Tensor &t, 
   return r;
 }
 
-// Device memory for the length of a call on `stream`: torch's allocator hands it on once that stream is done with it.
+// Device memory for the length of a call on `stream`, from the allocator's memory of that stream: what was freed on another one
+// may still be used by work queued there, and nothing makes `stream` wait for it.  Its next owner is on `stream` too.
 struct Scratch {
   at::Tensor held;
   Scratch(int64_t bytes, lapis_hip_stream_t stream) {
     if (bytes <= 0) return;
-    const auto current = c10::hip::getCurrentHIPStream();
-    held = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, current.device_index())));
-    if (stream != (lapis_hip_stream_t)current.stream())
-      c10::hip::HIPCachingAllocator::recordStream(held.storage().data_ptr(),
-                                                  c10::hip::getStreamFromExternal((hipStream_t)stream, current.device_index()));
+    struct Current {
+      const c10::hip::HIPStream before = c10::hip::getCurrentHIPStream();
+      bool moved = false;
+      ~Current() {
+        if (moved) c10::hip::setCurrentHIPStream(before);
+      }
+    } current;
+    const auto device = current.before.device_index();
+    if (stream != (lapis_hip_stream_t)current.before.stream()) {
+      c10::hip::setCurrentHIPStream(c10::hip::getStreamFromExternal((hipStream_t)stream, device));
+      current.moved = true;
+    }
+    held = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, device)));
   }
   void *data() const { return held.defined() ? held.data_ptr() : nullptr; }
 };

@@ -414,3 +414,55 @@ def test_many_rows_the_same_bits_again_and_in_a_graph(gpu):
         again = run_forward(gpu, q, k, v, pos, crd, **sizes)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(again, want))
+
+
+# ---- scratch memory and streams ------------------------------------------------------------------------------------------
+
+def side_by_side(call, outputs):
+    """``call(outputs, stream)`` queued several times on the current stream and, while these run, on another one that only waits
+    for the inputs: both get what a call by itself gives."""
+    call(outputs, None)
+    torch.cuda.synchronize()
+    want = [x.clone() for x in outputs]
+    here, there = ([torch.empty_like(x) for x in outputs] for _ in range(2))
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        for x in here + there:
+            x.zero_()
+        ready = torch.cuda.Event()
+        ready.record()
+        side.wait_event(ready)
+        for _ in range(4):
+            call(here, None)
+            call(there, stream)
+        torch.cuda.synchronize()
+        for name, got in (("the current stream", here), ("the other stream", there)):
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), "results on " + name
+
+
+def test_scratch_of_calls_on_two_streams_is_not_shared(gpu):
+    q, k, v, dout = make(2, 2000, 2000, 8, 2, 64, torch.bfloat16, 21)
+    pos, crd = random_lists(4, 32, 63, 12, 7)
+    sizes = dict(block_m=64, block_n=32, causal=True)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    side_by_side(lambda grads, stream: gpu.block_attention_backward(dout, q, k, v, out, lse, pos, crd, *grads, stream=stream, **sizes),
+                 [torch.zeros_like(x) for x in (q, k, v)])
+
+
+def test_scratch_on_the_default_stream_while_another_one_is_current(gpu):
+    q, k, v, dout = make(2, 2000, 2000, 8, 2, 64, torch.float16, 22)
+    pos, crd = random_lists(4, 32, 63, 12, 8)
+    sizes = dict(block_m=64, block_n=32, causal=True)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    want = run_backward(gpu, dout, q, k, v, out, lse, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [[torch.empty_like(x) for x in want] for _ in range(2)]
+        side.synchronize()
+        for _ in range(4):
+            for grads, stream in zip(got, (None, 0)):
+                gpu.block_attention_backward(dout, q, k, v, out, lse, pos, crd, *grads, stream=stream, **sizes)
+        assert torch.cuda.current_stream() == side  # the calls leave it as it was
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for grads in got for x, y in zip(grads, want))

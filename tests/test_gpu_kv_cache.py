@@ -321,3 +321,20 @@ def test_many_rows_move_as_few_do(gpu, cache, dim, dtype):
     assert bool((loaded[0][0][~live] == 0).all()) and bool((loaded[0][1][~live] == 0).all())
     if cache == "same":
         assert torch.equal(loaded[0][0][live], k[live]) and torch.equal(loaded[0][1][live], v[live])
+
+
+def test_partial_results_of_calls_on_two_streams_are_not_shared(gpu):
+    """Both calls cut their lists into units and join them, at the same time on two streams."""
+    case = paged_case(3, [40000, 9000, 20000], 8, 2, 128, 64, torch.bfloat16, "f8", False, 3)
+    q, kc, vc, pos, crd, tokens, ks, vs = case
+    want = check_paged(gpu, "by itself", case)
+    other = (q.float() * 0.5).to(q.dtype)
+    want_other = check_paged(gpu, "other queries", (other,) + case[1:])
+    got, got_other = torch.zeros_like(q), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(8):
+        gpu.paged_attention(q, kc, vc, pos, crd, tokens, got, k_scale=ks, v_scale=vs)
+        gpu.paged_attention(other, kc, vc, pos, crd, tokens, got_other, k_scale=ks, v_scale=vs, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(got_other, want_other)
