@@ -439,6 +439,8 @@ int lapis_hip_normalize_mom2_f64(int64_t n, const double *mom1, const double *mo
  * codes on 8-byte ones, strides (in elements) are multiples of 8.  Outputs must not overlap inputs.
  * Structures: positions and coordinates int32.  A coordinate outside [0, columns) (of pages: outside [0, pages))
  * and positions outside [0, nnz] are never followed: such an entry counts as absent.  Coordinates need not ascend.
+ * Positions do; where they descend nothing outside the operands is read or written, rows overlap and are taken as they stand, each
+ * with all its entries (positions that nobody wrote may make that rows times nnz of them).
  * Rows without an entry give zeros, and -infinity as the logarithm of their sum.
  * No entry point below allocates or synchronises: where scratch memory is needed the caller passes `work` of at least
  * the bytes the matching _work call says. */
@@ -545,7 +547,8 @@ int lapis_hip_block_attention(const lapis_hip_block_args *args, lapis_hip_stream
 /* Gradients of the forward call whose out and lse these are: dv = P^T dout, dS = P * (dout v^T - rowsum(dout * out)),
  * dq = scale dS k, dk = scale dS^T q, with P = exp(scale q k^T - lse) on the listed blocks.  Every element of dq, dk and
  * dv is written; a group's heads add up into their key-value head's gradient.  Sums are taken in a fixed order: the same
- * inputs give the same bits. */
+ * inputs give the same bits.  With positions that descend, dk and dv of a block of keys that more than 384 rows name are NaN, and
+ * all of dk and dv where positions descend more than 16 times. */
 int lapis_hip_block_attention_backward_work(const lapis_hip_block_args *args, int64_t *bytes);
 int lapis_hip_block_attention_backward(const lapis_hip_block_args *args, lapis_hip_stream_t stream);
 

@@ -339,10 +339,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
 // Which rows list a column, in ascending order (a row that lists it twice, twice).  Rows are cut into at most 64 chunks;
 // counts[column][chunk], summed over a (batch entry, head)'s columns and chunks, gives each chunk its places.
 struct Columns {
-  int *odd;           // not 0: positions overlap or leave [0, nnz]; the lists are not used then
+  int *odd;           // rows whose positions descend: with one of them rows overlap, and the lists are not made
   int *next;          // units taken from each part of them
   int *counts;        // lists x columns x chunks
-  int *start, *end;   // of each column's rows
+  int *start, *end;   // of each column's rows; with positions that descend, end < 0: they were not found
   int *unit;          // column of each unit of work, -1 = nothing to do
   int *rows;          // nnz
   float *partial;     // of columns of several units: dk and dv of each
@@ -353,30 +353,36 @@ __global__ void clear_kernel(int *p) { p[threadIdx.x] = 0; }
 
 constexpr int kColumnsInLds = 8192, kRowsAtOnce = 16;
 
+__device__ __forceinline__ long long position(const BlockArgs &a, long long row) { return min(max((long long)a.pos[row], 0ll), a.nnz); }
+
 // One wavefront per chunk takes its rows one after the other, so that the places of a column ascend with its rows; the
 // entries of sixteen rows are on their way at a time.
 template <bool FILL>
 __global__ __launch_bounds__(64) void columns_kernel(BlockArgs a, Columns t) {
   __shared__ int place[kColumnsInLds];
+  if (FILL && *t.odd) return;
   const int lane = threadIdx.x, chunk = blockIdx.x, bh = blockIdx.z;
   const int c0 = blockIdx.y * kColumnsInLds, cs = min(kColumnsInLds, a.columns - c0);
   for (int c = lane; c < cs; c += 64) place[c] = FILL ? t.counts[((long long)bh * a.columns + c0 + c) * t.chunks + chunk] : 0;
   __syncthreads();
   const int r_end = min(a.rows, (chunk + 1) * t.chunk_rows);
-  bool odd = false;
+  int odd = 0;
   const auto add = [&](int c, int r) {
     if ((unsigned)c < (unsigned)a.columns && c >= c0 && c < c0 + cs) {
       const int at = atomicAdd(&place[c - c0], 1);
-      if (FILL && at < a.nnz) t.rows[at] = r;
+      if (FILL && (unsigned)at < (unsigned long long)a.nnz) t.rows[at] = r;
     }
   };
   for (int r0 = chunk * t.chunk_rows; r0 < r_end; r0 += kRowsAtOnce) {
     int first = 0, count = 0, entry[kRowsAtOnce];
+    bool descends = false;
     if (lane < kRowsAtOnce && r0 + lane < r_end) {
       const long long row = (long long)bh * a.rows + r0 + lane;
       entries_of(a, row, &first, &count);
-      odd |= a.pos[row] != first || (long long)a.pos[row + 1] != (long long)first + count;
+      descends = position(a, row + 1) < first;
     }
+    odd += __popcll(__ballot(descends));
+    if (odd) continue;  // rows that overlap may name more entries than 32 bits count
 #pragma unroll
     for (int i = 0; i < kRowsAtOnce; ++i) {
       const int f = __builtin_amdgcn_readlane(first, i), n = __builtin_amdgcn_readlane(count, i);
@@ -394,7 +400,7 @@ __global__ __launch_bounds__(64) void columns_kernel(BlockArgs a, Columns t) {
     }
   }
   if (FILL) return;
-  if (__any(odd) && lane == 0) atomicOr(t.odd, 1);
+  if (odd && lane == 0 && c0 == 0) atomicAdd(t.odd, odd);
   __syncthreads();
   for (int c = lane; c < cs; c += 64) t.counts[((long long)bh * a.columns + c0 + c) * t.chunks + chunk] = place[c];
 }
@@ -410,13 +416,12 @@ __device__ __forceinline__ void put_units(const Columns &t, int cc, int start, i
 }
 
 // Where a list's entries start (positions are in order here).
-__device__ __forceinline__ int list_start(const BlockArgs &a, long long bh) {
-  return a.rows ? (int)min(max((long long)a.pos[bh * a.rows], 0ll), a.nnz) : 0;
-}
+__device__ __forceinline__ int list_start(const BlockArgs &a, long long bh) { return a.rows ? (int)position(a, bh * a.rows) : 0; }
 
 // One workgroup per (batch entry, key-value head): counts become places, columns get their ranges and their units of work.
 __global__ __launch_bounds__(1024) void columns_scan_kernel(BlockArgs a, Columns t) {
   __shared__ int wave_sum[16], total;
+  if (*t.odd) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bh = blockIdx.x;
   if (tid == 0) total = list_start(a, bh);
   const long long n = (long long)a.columns * t.chunks;
@@ -476,10 +481,11 @@ __global__ __launch_bounds__(1024) void few_columns_kernel(BlockArgs a, Columns 
   if (lane < rows_each && r0 + lane < r1) {
     const long long row = (long long)bh * a.rows + r0 + lane;
     entries_of(a, row, &first, &count);
-    odd = a.pos[row] != first || (long long)a.pos[row + 1] != (long long)first + count;
+    odd = position(a, row + 1) < first;
   }
-  if (__any(odd) && lane == 0) atomicOr(t.odd, 1);
-  __syncthreads();
+  const int descents = __popcll(__ballot(odd));
+  if (descents && lane == 0) atomicAdd(t.odd, descents);
+  if (__syncthreads_or(odd)) return;
   const auto pass = [&](bool fill) {  // a wavefront's rows one after the other, their first entries asked for eight at a time
     for (int i0 = 0; i0 < r1 - r0; i0 += 8) {
       int entry[8];
@@ -495,7 +501,7 @@ __global__ __launch_bounds__(1024) void few_columns_kernel(BlockArgs a, Columns 
           const int c = e < 64 ? entry[i] : e < n ? a.crd[f + e] : -1;
           if ((unsigned)c < (unsigned)a.columns) {
             const int at = atomicAdd(&place[c * 16 + wave], 1);
-            if (fill && at < a.nnz) t.rows[at] = r0 + i0 + i;
+            if (fill && (unsigned)at < (unsigned long long)a.nnz) t.rows[at] = r0 + i0 + i;
           }
           wave_lds_sync();
         }
@@ -538,6 +544,7 @@ __global__ __launch_bounds__(1024) void few_columns_kernel(BlockArgs a, Columns 
 // ---- dK and dV -------------------------------------------------------------------------------------------------
 
 constexpr int kMostEntries = 384;  // of a unit
+constexpr int kMostDescents = 16;  // of positions: 17 times the entries at most
 
 // A unit of work: 32 * KG keys of a column and some of the rows that list it, their queries times heads packed into tiles of
 // 32.  Two wavefronts share 32 keys, a key per lane, K and V of them in registers: one computes S and P (queries x keys), which
@@ -572,24 +579,82 @@ __device__ __forceinline__ DkvArgsAgain again() {
 // What all lanes of a wavefront agree on, said so that the compiler branches on it and does not walk through both sides.
 __device__ __forceinline__ bool same(bool x) { return __builtin_amdgcn_readfirstlane((int)x) != 0; }
 
+// Where positions descend rows overlap and there are no lists of columns: the rows that name column cc (counted through all lists)
+// are looked for, by a workgroup of 256.  Rows whose positions ascend hold neighbouring entries, which are compared 256 at a time; each
+// descent may bring all entries once more.  Returns how many there are, in order, in `rows`; -1: more than that holds, or
+// descents without end.
+__device__ __forceinline__ int rows_that_name(const BlockArgs &a, int cc, int descents, int *rows, int *found) {
+  if (descents > kMostDescents) return -1;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bh = cc / a.columns, column = cc - bh * a.columns;
+  const long long row0 = (long long)bh * a.rows;
+  const auto threads_that = [&](bool x, int *before) {  // say so, and how many of them come before this one
+    const unsigned long long these = __ballot(x);
+    __syncthreads();
+    if (lane == 0) found[wave] = __popcll(these);
+    __syncthreads();
+    int all = 0;
+    *before = __popcll(these & ((1ull << lane) - 1));
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) *before += found[w];
+      all += found[w];
+    }
+    return __builtin_amdgcn_readfirstlane(all);
+  };
+  int n = 0, before;
+  for (int r0 = 0, r1; r0 < a.rows; r0 = r1) {
+    r1 = min(r0 + 256, a.rows);
+    const long long r = row0 + min(r0 + tid, r1 - 1);
+    if (threads_that(position(a, r + 1) < position(a, r), &before) > 0) r1 = r0 + 1;
+    const long long end = position(a, row0 + r1);
+    for (long long e0 = position(a, row0 + r0); e0 < end; e0 += 256) {
+      const long long e = e0 + tid;
+      const bool names = e < end && a.crd[e] == column;
+      const int more = threads_that(names, &before);
+      if (n + more > kMostEntries) return -1;
+      if (names) {
+        int lo = r0, hi = r1;  // row lo starts at or before entry e, row hi behind it
+        while (hi - lo > 1) {
+          const int middle = lo + (hi - lo) / 2;
+          if (position(a, row0 + middle) <= e) lo = middle;
+          else hi = middle;
+        }
+        rows[n + before] = lo;
+      }
+      n += more;
+    }
+  }
+  return n;
+}
+
 template <typename T, int DP, int KG, int S>
-__global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
-  typedef typename T::elem elem;
-  constexpr int QG = 2 / KG, TG = KG * 128, PIECES = DP / 8, RP = TG / PIECES, PASSES = 32 / RP, DT = DP / 32, BATCH = 4;
-  static_assert(S <= BATCH, "what is loaded is looked up a batch before");
+struct DkvShared {
+  static constexpr int QG = 2 / KG, BATCH = 4;
   struct Info {  // where a tile's rows lie
     long long q[32], g[32];
     int sums[32], last[32];
-    float times[32];  // how often the row lists the column, where every row is looked through
   };
-  __shared__ __attribute__((aligned(16))) elem tiles[QG][S][2][32 * DP];
-  __shared__ __attribute__((aligned(16))) float sums[QG][S][2][32];  // log-sums and deltas of a tile's rows
-  __shared__ __attribute__((aligned(16))) Info infos[QG][2 * BATCH];
-  __shared__ int rows_of_unit[kMostEntries], taken;
+  __attribute__((aligned(16))) typename T::elem tiles[QG][S][2][32 * DP];
+  __attribute__((aligned(16))) float sums[QG][S][2][32];  // log-sums and deltas of a tile's rows
+  __attribute__((aligned(16))) Info infos[QG][2 * BATCH];
+  int rows_of_unit[kMostEntries], taken, found[4];
+};
+
+// ODD: positions descend.  A body of its own, as the kernel's own look for rows among its units costs the loop registers (8192 queries, 16
+// blocks of 64: 547 us against 510).
+template <typename T, int DP, int KG, int S, bool ODD>
+__device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, KG, S> &mem) {
+  typedef typename T::elem elem;
+  typedef typename DkvShared<T, DP, KG, S>::Info Info;
+  constexpr int QG = 2 / KG, TG = KG * 128, PIECES = DP / 8, RP = TG / PIECES, PASSES = 32 / RP, DT = DP / 32, BATCH = 4;
+  static_assert(S <= BATCH, "what is loaded is looked up a batch before");
+  auto &tiles = mem.tiles;
+  auto &sums = mem.sums;
+  auto &infos = mem.infos;
+  auto &rows_of_unit = mem.rows_of_unit;
+  int &taken = mem.taken;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int role = (wave ^ blockIdx.x / kParts) & 1, kg = (wave >> 1) % KG, qg = (wave >> 1) / KG, gt = tid - qg * TG;  // role 0: dV, 1: dK
-  const bool odd = same(*args.cols.odd != 0);
-  const int all_units = (odd ? args.cols.lists * args.a.columns : args.cols.units) * args.cols.sub;
+  const int all_units = (ODD ? args.cols.lists * args.a.columns : args.cols.units) * args.cols.sub;
   const float scale = args.a.scale, c = scale * kLog2e;
   const int dim = args.a.dim;
   const elem *const all_q = (const elem *)args.a.q.data, *const all_g = (const elem *)args.a.dout.data;
@@ -631,11 +696,13 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
     const auto &a = at_start->a;
     const auto &cols = at_start->cols;
     const int u = unit_l / cols.sub, sub = unit_l - u * cols.sub;
-    int cc, from = 0, n, start = 0;
+    int cc, from = 0, n = 0, start = 0;
     bool several = false;
-    if (odd) {  // every row is looked through for the column
+    if (ODD) {
       cc = u;
-      n = a.rows;
+      n = rows_that_name(*(const BlockArgs *)&at_start->a, cc, *cols.odd, rows_of_unit, mem.found);
+      if (tid == 0) cols.end[cc] = n;
+      if (n < 0) continue;  // NaN: the next kernel
     } else {
       cc = cols.unit[u];
       if (cc < 0) continue;
@@ -668,14 +735,8 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
         int query = 0;
         bool there = entry < n;
         if (there) {
-          query = (odd ? entry : rows_of_unit[entry]) * a.block_m + in;
+          query = rows_of_unit[entry] * a.block_m + in;
           there = query < a.queries;
-        }
-        if (odd) {
-          int first = 0, count = 0, times = 0;
-          if (there) entries_of(a.pos, a.nnz, (long long)bh * a.rows + entry, &first, &count);
-          for (int e = 0; e < count; ++e) times += a.crd[first + e] == column;
-          i.times[lane] = (float)times;
         }
         query = there ? query : 0;
         const int head = kh * a.group + hd;
@@ -776,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
         unsigned bad = 0;
         if (now) {
           const Info &info = infos[qg][t % (2 * BATCH)];
-          const bool cut = odd || same(__any(last < key_low + 31));
+          const bool cut = same(__any(last < key_low + 31));
           const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -811,9 +872,7 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
                 const int row = 8 * j + 4 * half + e;
                 float x = s[4 * j + e];
                 if (!G && (bad >> row & 1)) x = __builtin_nanf("");  // its dO is taken as zeros below
-                const float times = odd ? info.times[row] : 1.f;
-                // a row without an entry (log-sum -infinity) sees no key
-                s[4 * j + e] = key <= lim[e] && times != 0.f ? x * times : 0.f;
+                s[4 * j + e] = key <= lim[e] ? x : 0.f;
               }
             }
           }
@@ -917,14 +976,21 @@ __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
   }
 }
 
-// Columns of several units: their sums, in the order of the units.
+template <typename T, int DP, int KG, int S>
+__global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
+  __shared__ DkvShared<T, DP, KG, S> mem;
+  if (same(*args.cols.odd != 0)) dkv_units<T, DP, KG, S, true>(args, mem);
+  else dkv_units<T, DP, KG, S, false>(args, mem);
+}
+
+// Columns of several units: their sums, in the order of the units.  NaN where the rows of a column were not found.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void join_units_kernel(BlockArgs a, Columns cols) {
   typedef typename T::elem elem;
   const int cc = blockIdx.x;
-  if (*cols.odd) return;
-  const int start = cols.start[cc], rows = cols.end[cc] - start;
-  if (rows <= cols.per_unit) return;
+  const bool odd = *cols.odd != 0, lost = odd && cols.end[cc] < 0;
+  const int start = odd ? 0 : cols.start[cc], rows = odd ? 0 : cols.end[cc] - start;
+  if (rows <= cols.per_unit && !lost) return;
   const int units = (rows + cols.per_unit - 1) / cols.per_unit;
   const int bh = cc / a.columns, column = cc - bh * a.columns, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const long long each = (long long)DP << a.block_n_log2;
@@ -933,7 +999,8 @@ __global__ __launch_bounds__(256) void join_units_kernel(BlockArgs a, Columns co
     const bool is_v = x >= each;
     const int at = (int)(is_v ? x - each : x), d = at % DP, key = (column << a.block_n_log2) + at / DP;
     if (key >= a.keys || d >= a.dim) continue;
-    v4f sum = {0.f, 0.f, 0.f, 0.f};
+    const float none = lost ? __builtin_nanf("") : 0.f;
+    v4f sum = {none, none, none, none};
     for (int j = 0; j < units; ++j) {
       const v4f y = *(const v4f *)(from + j * 2 * each + x);
 #pragma unroll

@@ -466,3 +466,92 @@ def test_scratch_on_the_default_stream_while_another_one_is_current(gpu):
         assert torch.cuda.current_stream() == side  # the calls leave it as it was
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for grads in got for x, y in zip(grads, want))
+
+
+# ---- positions that descend --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("queries,block_m,columns", [(480, 16, 12), (1100, 2, 12), (480, 16, 1100)])
+def test_rows_that_overlap(gpu, queries, block_m, columns):
+    """Positions that go back twice within a list and once from one list to the next, in structures that one workgroup lists and
+    in larger ones: the rows share entries, and each counts."""
+    rows = -(-queries // block_m)
+    t = make(2, queries, columns * 16, 2, 1, 64, torch.float16, rows)
+    pos, crd = random_lists(2, rows, columns, 4, rows, empty=0.1)
+    pos = pos.cpu()
+    third = rows // 3
+    pos[third] = max(0, int(pos[third]) - 20)
+    pos[2 * third] = max(0, int(pos[2 * third]) - 9)
+    pos[rows] = max(0, int(pos[rows]) - 30)
+    assert 1 <= int((pos[1:] < pos[:-1]).sum()) <= 16
+    check(gpu, "%d rows, %d columns" % (rows, columns), t, pos.cuda(), crd, block_m, 16, False)
+
+
+def test_a_block_that_too_many_rows_name_where_rows_overlap(gpu):
+    """Every row names block 0, each of the others a few: the gradient of block 0 says that it was not computed."""
+    rows = 500
+    t = make(1, rows, 160, 1, 1, 64, torch.bfloat16, 4)
+    crd = torch.stack([torch.zeros(rows, dtype=torch.int32), torch.arange(rows, dtype=torch.int32) % 9 + 1], 1).reshape(-1).cuda()
+    pos = torch.arange(rows + 1, dtype=torch.int32) * 2
+    pos[200] -= 8
+    pos, sizes = pos.cuda(), dict(block_m=1, block_n=16, causal=False)
+    q, k, v, dout = t
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    dq, dk, dv = run_backward(gpu, dout, q, k, v, out, lse, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    w = ref.pair_weights(pos, crd, 1, 1, rows, 160, 1, 16, False)
+    wants, bounds = ref.backward(dout, q, k, v, out, lse, w, 64 ** -0.5)
+    ref.assert_within(dq, wants[0], bounds[0], "dq")
+    for name, g, x, y in (("dk", dk, wants[1], bounds[1]), ("dv", dv, wants[2], bounds[2])):
+        assert bool(torch.isnan(g[:, :16]).all()), name
+        ref.assert_within(g[:, 16:], x[:, 16:], y[:, 16:], name)
+
+
+def block_args(**values):
+    """The C structure of the entries' operands: tensors batch x tokens x heads x dim as rows, the rest as it is."""
+    import ctypes
+
+    class Rows(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3)]
+
+    class Args(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_int64) for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim", "block_m", "block_n", "nnz")] +
+                    [("causal", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_float), ("pos", ctypes.c_void_p), ("crd", ctypes.c_void_p)] +
+                    [(n, Rows) for n in ("q", "k", "v", "out")] + [("lse", ctypes.c_void_p)] + [(n, Rows) for n in ("dout", "dq", "dk", "dv")] +
+                    [("work", ctypes.c_void_p)])
+    a = Args()
+    for name, x in values.items():
+        if not torch.is_tensor(x):
+            setattr(a, name, x)
+        elif x.dim() == 4:
+            getattr(a, name).data = x.data_ptr()
+            getattr(a, name).stride[:] = x.stride()[:3]
+        else:
+            setattr(a, name, x.data_ptr())
+    return a
+
+
+@pytest.mark.parametrize("queries,block_m,columns,entries", [(40, 1, 8, 30), (512, 1, 8, 1 << 24), (8192, 1, 8, 1 << 20), (600, 1, 9000, 1 << 20)])
+def test_positions_that_go_up_and_down_write_nothing_outside(gpu, queries, block_m, columns, entries):
+    """Rows that name all entries in turn with rows that name none: more entries together than 32 bits count.  Scratch
+    memory stands between bytes that nothing may change."""
+    import ctypes
+    q, k, v, dout = make(1, queries, columns * 16, 1, 1, 8, torch.bfloat16, 5)
+    pos = torch.zeros(queries + 1, dtype=torch.int32)
+    pos[1::2] = entries
+    crd = (torch.arange(entries, dtype=torch.int32) % columns).cuda()
+    pos = pos.cuda()
+    out, lse = torch.zeros_like(q), torch.full((1, 1, queries), 20.0, device="cuda")
+    dq, dk, dv = (torch.full_like(x, 7.0) for x in (q, k, v))
+    a = block_args(batch=1, queries=queries, keys=columns * 16, heads=1, kv_heads=1, dim=8, block_m=block_m, block_n=16, nnz=entries, causal=0,
+                   dtype=0, scale=0.3, pos=pos, crd=crd, q=q, k=k, v=v, out=out, lse=lse, dout=dout, dq=dq, dk=dk, dv=dv)
+    lib, bytes_ = gpu.load(), ctypes.c_int64()
+    gpu.check(lib.lapis_hip_block_attention_backward_work(ctypes.byref(a), ctypes.byref(bytes_)))
+    margin = 1 << 24
+    work = torch.full((bytes_.value + 2 * margin,), 0xa5, dtype=torch.uint8, device="cuda")
+    a.work = work.data_ptr() + margin
+    torch.cuda.synchronize()
+    gpu.check(lib.lapis_hip_block_attention_backward(ctypes.byref(a), None))
+    torch.cuda.synchronize()
+    assert bool((work[:margin] == 0xa5).all()) and bool((work[margin + bytes_.value:] == 0xa5).all())
+    assert bool(torch.isnan(dk).all()) and bool(torch.isnan(dv).all())
+    assert bool(torch.isfinite(dq).all()) and bool((dq[:, 1::2] == 0).all())  # rows that name nothing
