@@ -410,11 +410,11 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a, long lo
   }
 }
 
-// Rows of more blocks or longer codes than that: scores go through memory, one wavefront per row.
-__global__ __launch_bounds__(64) void block_select_long_kernel(SelectArgs a, unsigned *scores, long long row0) {
+// Rows of more blocks or longer codes than that: scores go through memory, one wavefront per row, `rows` of them from row0 on.
+__global__ __launch_bounds__(64) void block_select_long_kernel(SelectArgs a, unsigned *scores, long long row0, long long rows) {
   const long long at = linear_block(), row = row0 + at;
   const int lane = threadIdx.x;
-  if (row >= a.batch * a.heads * a.rows) return;
+  if (at >= rows) return;  // workgroups past the count asked for have no scores of their own
   const long long list = row / a.rows, b = list / a.heads, h = list - b * a.heads;
   RowPlace p = place_of_row(a, list, row - list * a.rows, lane);
   p.seen = __builtin_amdgcn_readfirstlane(p.seen);
@@ -594,8 +594,10 @@ extern "C" int lapis_hip_block_select(const lapis_hip_select_args *args, lapis_h
   const hipStream_t st = as_stream(stream);
   if (!short_rows(a)) {
     const long long some = rows_at_once(a);
-    for (long long row0 = 0; row0 < rows; row0 += some)
-      hipLaunchKernelGGL(block_select_long_kernel, grid_of(min(some, rows - row0)), dim3(64), 0, st, a, static_cast<unsigned *>(args->work), row0);
+    for (long long row0 = 0; row0 < rows; row0 += some) {
+      const long long here = min(some, rows - row0);
+      hipLaunchKernelGGL(block_select_long_kernel, grid_of(here), dim3(64), 0, st, a, static_cast<unsigned *>(args->work), row0, here);
+    }
   } else if (a.columns <= 256) {
     launch_select<4>(a, st);
   } else if (a.columns <= 512) {

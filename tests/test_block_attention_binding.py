@@ -126,6 +126,14 @@ def test_calls_before_init_report_not_initialized():
         assert lib.lapis_hip_status_name(rc) == b"LAPIS_HIP_ERR_NOT_INITIALIZED"
 
 
+class SelectArgs(ctypes.Structure):
+    """lapis_hip_select_args"""
+    _fields_ = ([(n, ctypes.c_int64) for n in ("batch", "heads", "queries", "keys", "dim", "block_m", "block_n", "count", "sink", "local")] +
+                [("causal", ctypes.c_int)] + [(n, ctypes.c_void_p) for n in ("q_codes", "k_codes", "k_scales")] +
+                [("k_stride", ctypes.c_int64 * 3), ("scale_stride", ctypes.c_int64 * 3), ("table", ctypes.c_void_p), ("blocks", ctypes.c_void_p),
+                 ("table_width", ctypes.c_int64), ("pages", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("pos", "crd", "work")])
+
+
 def test_entries_of_a_selection_are_counted_without_a_gpu():
     """The closed form against a count row by row."""
     class Args(ctypes.Structure):

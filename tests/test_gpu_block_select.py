@@ -155,3 +155,43 @@ def test_the_c_entries_refuse(gpu):
     for dim, count, more in ((12, 1, {}), (1032, 1, {}), (8, 0, {}), (8, 1, {"sink": 1, "local": 1}), (8, 1, {"sink": -1})):
         with pytest.raises(gpu.LapisHipError, match="INVALID_ARGUMENT"):
             call(dim, count, **more)
+
+
+def best_on_the_device(q, k, s, count, sink, local):
+    """Columns of each row (rows x dim against columns x dim, every row sees all) by a stable sort: whole-number products are exact."""
+    best = []
+    for part in q.split(max(1, (1 << 27) // k.shape[0])):
+        score = (part.float() @ k.float().T.contiguous()) * s
+        score[:, :sink], score[:, k.shape[0] - local:] = math.inf, math.inf
+        best.append(score.sort(dim=1, descending=True, stable=True).indices[:, :count].sort(dim=1).values)
+    return torch.cat(best)
+
+
+@pytest.mark.parametrize("rows,columns,dim,count", [(2000, 70001, 64, 5), (9_700_000, 7, 264, 3)])
+def test_rows_whose_scores_take_several_launches(gpu, rows, columns, dim, count):
+    """256 MB of scores at a time: rows of the second and third launch; and launches of so many rows that their grid is rounded up,
+    with bytes behind the scratch memory that nothing may change."""
+    import ctypes
+    from test_block_attention_binding import SelectArgs
+    assert rows * columns * 4 > 1 << 28
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    q = torch.randint(-127, 128, (rows, dim), dtype=torch.int8, device="cuda", generator=g)
+    k = torch.randint(-127, 128, (columns, dim), dtype=torch.int8, device="cuda", generator=g)
+    s = torch.rand(columns, device="cuda", generator=g) + 0.01
+    pos = torch.full((rows + 1,), -9, dtype=torch.int32, device="cuda")
+    crd = torch.full((rows * count,), -9, dtype=torch.int32, device="cuda")
+    a = SelectArgs(batch=1, heads=1, queries=rows, keys=columns, dim=dim, block_m=1, block_n=1, count=count, sink=1, local=1, causal=0,
+                   q_codes=q.data_ptr(), k_codes=k.data_ptr(), k_scales=s.data_ptr(), k_stride=(columns * dim, columns * dim, dim),
+                   scale_stride=(columns, columns, 1), pos=pos.data_ptr(), crd=crd.data_ptr())
+    gpu.init()
+    lib, bytes_ = gpu.load(), ctypes.c_int64()
+    gpu.check(lib.lapis_hip_block_select_work(ctypes.byref(a), ctypes.byref(bytes_)))
+    assert bytes_.value <= 1 << 28
+    work = torch.full((bytes_.value + (1 << 28),), 0xa5, dtype=torch.uint8, device="cuda")
+    a.work = work.data_ptr()
+    torch.cuda.synchronize()
+    gpu.check(lib.lapis_hip_block_select(ctypes.byref(a), None))
+    torch.cuda.synchronize()
+    assert bool((work[bytes_.value:] == 0xa5).all())
+    assert torch.equal(pos, torch.arange(0, rows * count + 1, count, dtype=torch.int32, device="cuda"))
+    assert torch.equal(crd.view(rows, count).long(), best_on_the_device(q, k, s, count, 1, 1))
