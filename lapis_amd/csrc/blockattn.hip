@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
   }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  const int tiles = a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + 31) / 32) : 0;
+  const int tiles = tiles_of<32>(a, count);
   const int piece = lane % PIECES, v_row = lane / PIECES, vd = piece * 8 < a.dim ? piece * 8 : 0;
   v4i kr[2][KS], vr[PASSES];
   const auto load = [&](const int (&key0)[2]) {
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
         vr[p] = *(const v4i *)(vp + from * a.v.stride[1] + min((p * RP & 15) + v_row, room) * a.v.stride[1] + vd);
     }
   };
-  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, t * 32 + 16 * (lane & 1)) : kAbsent; };
+  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, 32ll * t + 16 * (lane & 1)) : kAbsent; };
 
   v4f acc[DT];
 #pragma unroll

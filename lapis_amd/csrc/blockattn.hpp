@@ -31,11 +31,18 @@ __device__ __forceinline__ void entries_of(const BlockArgs &a, long long row, in
 constexpr int kAbsent = 0x7fff0000;  // first key of sixteen that do not exist
 
 // Keys of a list in the order of its entries, sixteen at a time: blocks hold at least sixteen, so sixteen neighbouring
-// places of the list are sixteen neighbouring keys.  (The list has an entry.)
-__device__ __forceinline__ int first_key(const BlockArgs &a, int first, int count, int place) {
-  const int e = place >> a.block_n_log2, block = a.crd[first + min(e, count - 1)];
-  const int key = (block << a.block_n_log2) + (place & ((1 << a.block_n_log2) - 1));
+// places of the list are sixteen neighbouring keys.  (The list has an entry; with blocks listed over and over its places pass 31 bits.)
+__device__ __forceinline__ int first_key(const BlockArgs &a, int first, int count, long long place) {
+  const long long e = place >> a.block_n_log2;
+  const int block = a.crd[first + (int)min(e, count - 1ll)];
+  const int key = (int)((unsigned)block << a.block_n_log2) + ((int)place & ((1 << a.block_n_log2) - 1));
   return e < count && (unsigned)block < (unsigned)a.columns ? key : kAbsent;
+}
+
+// Tiles of KT keys that a list has.  They are numbered with 31 bits: more would be 2^36 keys of one list, of the 2^30 there are.
+template <int KT>
+__device__ __forceinline__ int tiles_of(const BlockArgs &a, int count) {
+  return a.keys > 0 ? (int)min((((long long)count << a.block_n_log2) + KT - 1) / KT, 0x7fffff00ll) : 0;
 }
 
 // Tiles of KT keys and values of a list on their way into two LDS buffers each, a workgroup of NW wavefronts sharing the
@@ -62,9 +69,9 @@ struct KeyTiles {
     k_to = lds_address(k_tile) + wave * 1024;
     v_to = lds_address(v_tile) + wave * 1024;
   }
-  __device__ __forceinline__ int tiles() const { return a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + KT - 1) / KT) : 0; }
+  __device__ __forceinline__ int tiles() const { return tiles_of<KT>(a, count); }
   // The first key of each sixteen of tile t, one to a lane: asked for a tile before they are needed.
-  __device__ __forceinline__ int look_up(int t) const { return first_key(a, first, count, t * KT + 16 * (threadIdx.x % CH)); }
+  __device__ __forceinline__ int look_up(int t) const { return first_key(a, first, count, (long long)t * KT + 16 * (threadIdx.x % CH)); }
   static __device__ __forceinline__ v4i spread(int of_lane) {
     static_assert(CH == 4, "tiles of 64 keys");
     return v4i{__builtin_amdgcn_readlane(of_lane, 0), __builtin_amdgcn_readlane(of_lane, 1), __builtin_amdgcn_readlane(of_lane, 2),

@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
   }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  const int tiles = a.keys > 0 ? (int)((((long long)count << a.block_n_log2) + 31) / 32) : 0;
+  const int tiles = tiles_of<32>(a, count);
   v4i kr[2][KS], vr[2][KS];
   const auto load = [&](int key0, int key1) {
 #pragma unroll
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
       }
     }
   };
-  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, t * 32 + 16 * (lane & 1)) : kAbsent; };
+  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, 32ll * t + 16 * (lane & 1)) : kAbsent; };
 
   v4f acc[DT];
 #pragma unroll

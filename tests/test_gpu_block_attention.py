@@ -555,3 +555,22 @@ def test_positions_that_go_up_and_down_write_nothing_outside(gpu, queries, block
     assert bool((work[:margin] == 0xa5).all()) and bool((work[margin + bytes_.value:] == 0xa5).all())
     assert bool(torch.isnan(dk).all()) and bool(torch.isnan(dv).all())
     assert bool(torch.isfinite(dq).all()) and bool((dq[:, 1::2] == 0).all())  # rows that name nothing
+
+
+def test_a_list_whose_keys_pass_31_bits(gpu):
+    """Eight million entries of blocks that do not exist, then one that does: 2^31 keys into the list."""
+    q, k, v, _ = make(1, 3, 600, 1, 1, 8, torch.bfloat16, 6)
+    entries = (1 << 23) + 2
+    crd = torch.full((entries,), -1, dtype=torch.int32)
+    crd[-1] = 1
+    pos = torch.tensor([0, entries], dtype=torch.int32).cuda()
+    out, lse = run_forward(gpu, q, k, v, pos, crd.cuda(), block_m=3, block_n=256, causal=False)
+    only = run_forward(gpu, q, k, v, torch.tensor([0, 1], dtype=torch.int32).cuda(), torch.ones(1, dtype=torch.int32).cuda(), block_m=3, block_n=256,
+                       causal=False)
+    torch.cuda.synchronize()
+    w = torch.zeros((1, 1, 3, 600), dtype=torch.float64)
+    w[..., 256:512] = 1
+    want, want_lse, bound, lse_bound = ref.forward(q, k, v, w, 8 ** -0.5)
+    for o, l in ((out, lse), only):
+        ref.assert_within(o, want, bound, "out")
+        ref.assert_within(l, want_lse, lse_bound, "lse")
