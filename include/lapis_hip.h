@@ -548,7 +548,10 @@ int lapis_hip_block_attention(const lapis_hip_block_args *args, lapis_hip_stream
  * dq = scale dS k, dk = scale dS^T q, with P = exp(scale q k^T - lse) on the listed blocks.  Every element of dq, dk and
  * dv is written; a group's heads add up into their key-value head's gradient.  Sums are taken in a fixed order: the same
  * inputs give the same bits.  With positions that descend, dk and dv of a block of keys that more than 384 rows name are NaN, and
- * all of dk and dv where positions descend more than 16 times. */
+ * all of dk and dv where positions descend more than 16 times.
+ * Fewer than 2^24 blocks of keys, of all batch entries and key-value heads together.  The scratch memory may take 16 * block_n *
+ * dim bytes an entry (dim rounded up to 64 or 128: 256 KB at block_n = dim = 128) where a block's queries times heads / kv_heads
+ * reach 8192; entries of fewer share it.  _work answers after lapis_hip_init: it goes by the number of compute units. */
 int lapis_hip_block_attention_backward_work(const lapis_hip_block_args *args, int64_t *bytes);
 int lapis_hip_block_attention_backward(const lapis_hip_block_args *args, lapis_hip_stream_t stream);
 

@@ -1021,8 +1021,26 @@ struct Layout {
   Columns columns;
 };
 
-Layout layout_of(const BlockArgs &a) {
-  Layout l = {};
+// How dQ is launched.
+struct DqGrid {
+  bool few, many;
+  long long tiles, blocks;
+};
+
+DqGrid dq_grid(const BlockArgs &a) {
+  const long long lists = (long long)a.batch * a.kv_heads * a.rows, rows = (long long)a.block_m * a.group;
+  // the forward pass's rule: short lists, or few of them
+  const bool few = rows <= 32 || ceil_div(rows, 128) * lists < device_cu_count() / 2, many = ceil_div(rows, 16) * lists >= 8 * device_cu_count();
+  const long long tiles = ceil_div(rows, few ? 16 : 128);
+  return {few, many, tiles, few ? ceil_div(lists * tiles * (many ? 1 : 4), 4) : lists * tiles};
+}
+
+int layout_of(const BlockArgs &a, Layout *layout) {
+  const int64_t lists = (int64_t)a.batch * a.kv_heads, columns = lists * a.columns;
+  LAPIS_REQUIRE(lists <= 65535 && columns * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld lists of %d columns", (long long)lists, a.columns);
+  LAPIS_REQUIRE(a.rows == 0 || dq_grid(a).blocks * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld rows of the structure",
+                (long long)lists * a.rows);
+  Layout &l = *layout = {};
   Columns &c = l.columns;
   c.lists = a.batch * a.kv_heads;
   c.chunk_rows = (int)max((int64_t)kRowsAtOnce, ceil_div(ceil_div(a.rows, 64), kRowsAtOnce) * kRowsAtOnce);
@@ -1032,7 +1050,9 @@ Layout layout_of(const BlockArgs &a) {
   const int64_t rows_of_entry = (int64_t)min(a.block_m, max(a.queries, 1)) * max(a.group, 1);
   const int64_t rows_of_unit = min(max(a.nnz * rows_of_entry / max(device_cu_count(), 1), (int64_t)256), (int64_t)8192);
   c.per_unit = (int)min((int64_t)kMostEntries, max((int64_t)1, rows_of_unit / rows_of_entry));
-  c.units = (int)(a.nnz / c.per_unit + (int64_t)c.lists * a.columns);
+  const int64_t units = a.nnz / c.per_unit + columns;
+  LAPIS_REQUIRE(units * 8 <= INT32_MAX, "block_attention_backward: %lld units of work", (long long)units);  // of up to eight parts each
+  c.units = (int)units;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -1050,7 +1070,7 @@ Layout layout_of(const BlockArgs &a) {
   const int dp = a.dim <= 64 ? 64 : 128;
   l.partial = take(2 * (a.nnz / c.per_unit) * 2 * ((int64_t)dp << a.block_n_log2) * 4);
   l.bytes = at;
-  return l;
+  return LAPIS_HIP_OK;
 }
 
 template <typename T, int DP, int KG, int S>
@@ -1063,7 +1083,9 @@ void launch_dkv(const BlockArgs &a, const Columns &c, const float *delta, const 
 
 template <typename T, int DP>
 int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
-  Layout l = layout_of(a);
+  Layout l;
+  const int rc = layout_of(a, &l);
+  if (rc != LAPIS_HIP_OK) return rc;
   Columns &c = l.columns;
   float *delta = reinterpret_cast<float *>(work + l.delta), *logs = reinterpret_cast<float *>(work + l.logs);
   c.odd = reinterpret_cast<int *>(work + l.odd);
@@ -1075,18 +1097,13 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   c.rows = reinterpret_cast<int *>(work + l.rows);
   c.partial = reinterpret_cast<float *>(work + l.partial);
   if (a.rows) {
-    const long long lists = (long long)c.lists * a.rows, rows = (long long)a.block_m * a.group;
-    // the forward pass's rule: short lists, or few of them
-    const bool few = rows <= 32 || ceil_div(rows, 128) * lists < device_cu_count() / 2, many = ceil_div(rows, 16) * lists >= 8 * device_cu_count();
-    const long long tiles = ceil_div(rows, few ? 16 : 128), blocks = few ? ceil_div(lists * tiles * (many ? 1 : 4), 4) : lists * tiles;
-    LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "block_attention_backward: %lld rows of the structure", lists);
-    const auto kernel = !few ? block_dq_kernel<T, DP, 4, 64> : many ? block_dq_narrow_kernel<T, DP, 1> : block_dq_narrow_kernel<T, DP, 4>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, delta, logs, c.odd);
+    const DqGrid g = dq_grid(a);
+    const auto kernel = !g.few ? block_dq_kernel<T, DP, 4, 64> : g.many ? block_dq_narrow_kernel<T, DP, 1> : block_dq_narrow_kernel<T, DP, 4>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)g.blocks), dim3(256), 0, st, a, (int)g.tiles, delta, logs, c.odd);
   }
   if (c.lists && a.columns) {
     if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
     const dim3 grid((unsigned)c.chunks, (unsigned)ceil_div(a.columns, kColumnsInLds), (unsigned)c.lists);
-    LAPIS_REQUIRE(c.lists <= 65535 && (int64_t)c.units * 8 <= INT32_MAX, "block_attention_backward: %d lists, %d units", c.lists, c.units);
     if (a.columns <= kFewColumns && a.rows <= kFewRows) {
       hipLaunchKernelGGL(few_columns_kernel, dim3((unsigned)c.lists), dim3(1024), 0, st, a, c);
     } else {
@@ -1108,12 +1125,15 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
 using namespace lapis;
 
 extern "C" int lapis_hip_block_attention_backward_work(const lapis_hip_block_args *args, int64_t *bytes) {
+  LAPIS_CHECK_INIT();  // the size goes by the number of compute units
   BlockArgs a;
-  const int rc = read_block("block_attention_backward", args, true, &a);
+  int rc = read_block("block_attention_backward", args, true, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   LAPIS_REQUIRE(bytes, "block_attention_backward: null result");
-  *bytes = layout_of(a).bytes;
-  return LAPIS_HIP_OK;
+  Layout l;
+  rc = layout_of(a, &l);
+  *bytes = l.bytes;
+  return rc;
 }
 
 extern "C" int lapis_hip_block_attention_backward(const lapis_hip_block_args *args, lapis_hip_stream_t stream) {

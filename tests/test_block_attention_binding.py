@@ -157,3 +157,13 @@ def test_entries_of_a_selection_are_counted_without_a_gpu():
                                 seen = min(max((last + keys - queries) // n + 1, 0), columns) if causal else columns
                                 want += min(seen, count)
                             assert got.value == want, (queries, keys, m, n, count, causal)
+
+
+def test_scratch_sizes_are_asked_for_after_init():
+    """They go by the number of compute units."""
+    lib = hip.load()
+    if hip._initialized:
+        pytest.skip("another test has initialised the library")
+    buffer, bytes_ = ctypes.create_string_buffer(1024), ctypes.c_int64(-1)
+    for rc in (lib.lapis_hip_block_attention_backward_work(buffer, ctypes.byref(bytes_)), lib.lapis_hip_paged_attention_work(buffer, buffer, ctypes.byref(bytes_))):
+        assert lib.lapis_hip_status_name(rc) == b"LAPIS_HIP_ERR_NOT_INITIALIZED" and bytes_.value == -1

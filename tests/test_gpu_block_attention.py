@@ -574,3 +574,25 @@ def test_a_list_whose_keys_pass_31_bits(gpu):
     for o, l in ((out, lse), only):
         ref.assert_within(o, want, bound, "out")
         ref.assert_within(l, want_lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(batch=64, heads=64, kv_heads=64, keys=1 << 30, block_n=16), "4096 lists of 67108864 columns"),       # 2^38 columns: 0 in 32 bits
+    (dict(batch=300, heads=300, kv_heads=300), "90000 lists"),
+    (dict(queries=1 << 30, block_m=1, heads=1), "67108864|rows of the structure"),
+    (dict(nnz=2147483647, block_m=1 << 20, queries=1 << 20), "2147483649 units of work")])
+def test_sizes_that_numbers_do_not_hold_are_refused_before_anything_is_launched(gpu, change, what):
+    import ctypes
+    x, lse = torch.full((1, 8, 1, 8), 7.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(8, device="cuda")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    sizes = dict(batch=1, queries=8, keys=32, heads=1, kv_heads=1, dim=8, block_m=8, block_n=16, nnz=0, causal=0, dtype=0, scale=1.0)
+    a = block_args(**dict(sizes, **change), pos=pos, crd=pos, q=x, k=x, v=x, out=x, lse=lse, dout=x, dq=x, dk=x, dv=x)
+    a.work = x.data_ptr()
+    gpu.init()
+    lib, bytes_ = gpu.load(), ctypes.c_int64(-1)
+    for call in (lambda: lib.lapis_hip_block_attention_backward_work(ctypes.byref(a), ctypes.byref(bytes_)),
+                 lambda: lib.lapis_hip_block_attention_backward(ctypes.byref(a), None)):
+        with pytest.raises(gpu.LapisHipError, match=what):
+            gpu.check(call())
+    torch.cuda.synchronize()
+    assert bool((x == 7.0).all())
