@@ -48,22 +48,25 @@ __device__ __forceinline__ int list_of_unit(const PagedArgs &a, int u, int lane)
   return lo;
 }
 
-// Eight e4m3 codes as eight numbers of a 16-bit type: exact.
+// Eight e4m3 codes as eight numbers of a 16-bit type: exact, times a power of two: exact but for float16's subnormal numbers, and
+// those are rounded once, to nearest even.
 template <typename T>
-__device__ __forceinline__ vec8<T> codes_to(v2i x) {
+__device__ __forceinline__ vec8<T> codes_to(v2i x, float by = 1.0f) {
   v4u r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if constexpr (std::is_same<T, Bf16>::value) {
-      r[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[i], 1.0f, false));
-      r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[i], 1.0f, true));
+      r[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[i], by, false));
+      r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)x[i], by, true));
     } else {
-      r[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)x[i], 1.0f, false));
-      r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)x[i], 1.0f, true));
+      r[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)x[i], by, false));
+      r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)x[i], by, true));
     }
   }
   return __builtin_bit_cast(vec8<T>, r);
 }
+
+__device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0x7f800000u); }
 
 // A unit: up to 16 heads of a group against a stretch of a list.  Its four wavefronts take tiles of 32 tokens in turn, each by
 // itself; their maxima, sums and results are joined through LDS.
@@ -71,17 +74,22 @@ __device__ __forceinline__ vec8<T> codes_to(v2i x) {
 //   O^T = V^T P^T: P^T stays in its registers, V goes through LDS, where it is read by columns.
 // The next tile is loaded into the same registers as soon as they have been used, so all but the first products of a tile
 // run under its successor's loads; eight wavefronts a compute unit have 64 KB (8-bit cache) to 128 KB on their way.
-// 8-bit codes are multiplied as they are (exact in 16 bits); a key's scale multiplies its score, a value's scale its weight.
+// 8-bit codes are multiplied as they are (exact in 16 bits); a key's scale multiplies its score, a value's scale its weight.  With
+// float16 only the scale's mantissa does: a weight times a whole scale would leave its range, and in units of the largest scale one large row
+// of little weight would push all others' weights below it.  The scale's power of two goes to the value's codes, in units of 2^-7 of the
+// largest so far: exact for scales down to 2^-22 of that one, rounded to multiples of 2^-24 units below.
 // Bound by memory: 64 sequences of up to 8192 tokens, 32 heads over 8, dim 128, 8-bit cache: 153 us at 4.5 TB/s (a large copy
-// reaches 4.75); one sequence of 16 384 tokens, bf16: 22.4 us, 16.9 of them here (4.0 TB/s) and 5.4 for the join.
+// reaches 4.75), 160 with float16 queries; one sequence of 16 384 tokens, bf16: 22.4 us, 16.9 of them here (4.0 TB/s) and 5.4 for the join.
 template <typename T, bool F8, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(PagedArgs a) {
   typedef typename T::elem elem;
   typedef typename std::conditional<F8, v2i, v4i>::type raw;  // eight elements
   constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8, RP = 64 / PIECES, PASSES = 32 / RP, WIDTH = F8 ? 1 : 2;
+  constexpr bool SCALED = F8 && std::is_same<T, F16>::value;
   struct Tokens {
     long long at[32];     // element offsets of the tile's rows
-    float ks[32], vs[32];
+    float ks[32], vs[32]; // SCALED: vs holds mantissas, and vp powers of two, those of a lane's rows side by side
+    float vp[SCALED ? 32 : 4];
   };
   union Own {  // of a wavefront
     elem v[32 * DP];
@@ -138,7 +146,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
       if (F8) {
         const long long s = there ? page * a.scale_stride[0] + kh * a.scale_stride[1] + in * a.scale_stride[2] : 0;
         x.ks[lane] = there ? a.k_scale[s] : 0.f;
-        x.vs[lane] = there ? a.v_scale[s] : 0.f;
+        const float vs = there ? a.v_scale[s] : 0.f;
+        x.vs[lane] = SCALED ? 2.f * __builtin_amdgcn_frexp_mantf(vs) : vs;  // (of an infinity or NaN: itself, and its power is infinite)
+        if (SCALED) x.vp[lane % RP * PASSES + lane / RP] = power_of_two(vs);
       }
     }
     wave_lds_sync();
@@ -166,7 +176,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
   v4f acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f, unit = 0x1p-126f;  // `unit`: what acc's weights are counted in (8-bit cache, float16)
+  float m = -INFINITY, l = 0.f;
+  float unit = 0x1p-126f;  // what acc is counted in, a power of two (SCALED)
   page_of(wave);
   put_tokens(wave);
   unsigned there = there_next;
@@ -186,35 +197,40 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
         s[i] = mfma16(k, qf[x], s[i]);
       }
     }
+    float unit_to = unit, per_unit = 1.f;
+    if constexpr (SCALED) {
+      const float most = rows_max(__builtin_bit_cast(float, group_max<16>(__builtin_bit_cast(unsigned, tok.vp[lane & 31]))));
+      unit_to = fmaxf(unit, most * 0x1p-7f);
+      per_unit = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(unsigned, unit_to));
+    }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int r = p * RP + lane / PIECES, piece = lane % PIECES;
       vec8<T> v;
-      if constexpr (F8) v = codes_to<T>(vr[p]);
+      if constexpr (SCALED) v = codes_to<T>(vr[p], tok.vp[lane / PIECES * PASSES + p] * per_unit);
+      else if constexpr (F8) v = codes_to<T>(vr[p]);
       else v = __builtin_bit_cast(vec8<T>, vr[p]);
       if (there != 0xffffffffu && !(there >> r & 1)) v = vec8<T>{};  // whatever an unused slot holds: 0 times it must be 0
       *(vec8<T> *)(mine.v + r * DP + ((piece ^ turn16<DP>(r)) * 8)) = v;
     }
     const unsigned now = there;
+    put_tokens(t + 4);
+    there = there_next;
+    if (t + 4 < tiles) load(t + 4);
+    page_of(t + 8);
+
     float ks[8], vs[8];
     if (F8) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const v4f k4 = *(const v4f *)(tok.ks + 16 * i + 4 * quarter), v4 = *(const v4f *)(tok.vs + 16 * i + 4 * quarter);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ks[4 * i + e] = k4[e], vs[4 * i + e] = v4[e];
+        for (int e = 0; e < 4; ++e) {
+          ks[4 * i + e] = k4[e];
+          vs[4 * i + e] = v4[e];
+        }
       }
     }
-    float unit_to = unit;
-    if (F8 && std::is_same<T, F16>::value) {
-      // weights times scales could leave float16's range: they are counted in the largest scale so far, a power of two
-      const float most = rows_max(__builtin_bit_cast(float, group_max<16>(__builtin_bit_cast(unsigned, fmaxf(tok.vs[lane & 31], 0.f)))));
-      if (most > unit) unit_to = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, most) & 0x7f800000u) + 0x00800000u);
-    }
-    put_tokens(t + 4);
-    there = there_next;
-    if (t + 4 < tiles) load(t + 4);
-    page_of(t + 8);
 
     float best = -INFINITY;
 #pragma unroll
@@ -230,14 +246,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
     // the maximum in use moves only when it is left behind by more than 2^8
     if (__any(best > m + 8.f) || unit_to != unit) {
       const float to = fmaxf(m, best), keep = to == m ? 1.f : __builtin_amdgcn_exp2f(m - to);
-      const float by = unit_to == unit ? keep : keep * (unit / unit_to);
+      const float by = SCALED ? keep * (unit * per_unit) : keep;
       m = to;
       l *= keep;
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i] *= by;
       unit = unit_to;
     }
-    const float off = m == -INFINITY ? 0.f : m, per_unit = 1.f / unit;
+    const float off = m == -INFINITY ? 0.f : m;
     vec8<T> pf;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -245,9 +261,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
       for (int e = 0; e < 4; ++e) {
         const float p = __builtin_amdgcn_exp2f(s[i][e] - off);
         l += p;
-        float w = p;
-        if (F8) w = std::is_same<T, F16>::value ? p * (vs[4 * i + e] * per_unit) : p * vs[4 * i + e];
-        pf[4 * i + e] = (elem)w;
+        pf[4 * i + e] = (elem)(F8 ? p * vs[4 * i + e] : p);
       }
     wave_lds_sync();
 #pragma unroll
@@ -259,7 +273,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_kernel(PagedArgs
     wave_lds_sync();
   }
   l = rows_sum(l);
-  if (F8 && std::is_same<T, F16>::value) {
+  if (SCALED) {
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[i] *= unit;
   }

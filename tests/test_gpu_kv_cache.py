@@ -338,3 +338,70 @@ def test_partial_results_of_calls_on_two_streams_are_not_shared(gpu):
         gpu.paged_attention(other, kc, vc, pos, crd, tokens, got_other, k_scale=ks, v_scale=vs, stream=side)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and torch.equal(got_other, want_other)
+
+
+@pytest.mark.parametrize("cache", ["f8", "same"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_large_values_of_no_weight_beside_many_small_ones(gpu, dtype, cache):
+    """In every stretch that a wavefront takes: one token of weight 1, one of next to none whose value row is 60000 in size, and a few
+    hundred ordinary ones of 2^-10.5 each, a sixth of the sum.  In an 8-bit cache the large row's scale must not cost theirs."""
+    tokens, heads, page, dim = 65536, 8, 64, 64
+    g = torch.Generator().manual_seed(3)
+    v = torch.randn((tokens, heads, dim), generator=g) + 1.0
+    score = torch.full((tokens,), -10.5 * math.log(2))
+    at = torch.arange(tokens)
+    first = (at // 32) % 32 < 4  # the first tile of each of four wavefronts in each 1024 tokens
+    score[first & (at % 32 == 5)] = 2.0 ** -9
+    score[first & (at % 32 == 17)] = -40.0
+    v[first & (at % 32 == 17)] = 60000.0
+    k = torch.zeros((tokens, heads, dim))
+    k[..., 0] = score[:, None]
+    k, v = (x.to(TYPES[dtype]).cuda() for x in (k, v))
+    kc, vc, ks, vs = empty_cache(tokens // page, heads, page, dim, TYPES["f8"] if cache == "f8" else TYPES[dtype])
+    gpu.kv_store(k, v, torch.arange(tokens, dtype=torch.int32).cuda(), kc, vc, ks, vs)
+    q = torch.zeros((1, heads, dim))
+    q[..., 0] = 1.0
+    pos, crd = torch.tensor([0, tokens // page], dtype=torch.int32).cuda(), torch.arange(tokens // page, dtype=torch.int32).cuda()
+    out = torch.empty((1, heads, dim), dtype=TYPES[dtype], device="cuda")
+    gpu.paged_attention(q.to(TYPES[dtype]).cuda(), kc, vc, pos, crd, torch.tensor([tokens], dtype=torch.int32).cuda(), out, scale=1.0,
+                        k_scale=ks, v_scale=vs)
+    torch.cuda.synchronize()
+    u, tiny = ref.HALF_ULP[TYPES[dtype]], ref.TINY[TYPES[dtype]]
+    for h in range(heads):
+        kk, vv = (read(x, s)[:, h].reshape(-1, dim) for x, s in ((kc, ks), (vc, vs)))
+        s = kk[:, 0]
+        p = torch.exp(s - s.max())
+        want, spread = p @ vv / p.sum(), p @ vv.abs() / p.sum()
+        # as everywhere: weights and results are rounded once to the type; a weight, 1 for the best token, also to a multiple of 2^-24
+        bound = u * want.abs() + spread * (u + 2 * dim * 2.0 ** -23 * 40 + 2.0 ** -18) + tiny * vv.abs().sum(0) / p.sum()
+        assert float((tiny * vv.abs().sum(0) / p.sum()).max()) < 0.01 and bool((spread < 4).all())
+        ref.assert_within(out[0, h], want, bound, "%s %s, head %d" % (dtype, cache, h))
+
+
+def test_scales_that_differ_by_powers_of_two_and_are_not_numbers(gpu):
+    """float16 with an 8-bit cache whose scales are 2^-15 to 2^7 in any order, each row the only one of a query: nothing is rounded, codes and
+    scales come out as they are.  Rows of zeros; an infinity and a NaN only where a sequence holds them."""
+    dim, page = 64, 16
+    g = torch.Generator().manual_seed(4)
+    sizes = 2.0 ** torch.tensor([0, 7, -15, 3, -9, 6, -12, 5, -3, -14, 4, 0, 2, -6, 1, -1], dtype=torch.float64)
+    every = torch.arange(127, dtype=torch.uint8).view(TYPES["f8"]).double()  # 0 to 448
+    v = every[torch.randint(0, 127, (3, 16, 1, dim), generator=g)] * torch.where(torch.rand((3, 16, 1, dim), generator=g) < 0.5, -1.0, 1.0)
+    v[..., 0] = 448.0
+    v *= sizes[None, :, None, None]
+    v[:, 11] = 0.0
+    v[1, 4, 0, 3], v[1, 9, 0, 5] = math.inf, math.nan
+    held, v = v[:, :, 0], v.to(torch.float16)
+    assert torch.equal(v[::2, :, 0].double(), held[::2])
+    k = torch.zeros((3, 16, 1, dim), dtype=torch.float16)
+    k[:, range(16), 0, range(16)] = 1.0
+    kc, vc, ks, vs = empty_cache(3, 1, page, dim, TYPES["f8"])
+    gpu.kv_store(k.reshape(48, 1, dim).cuda(), v.reshape(48, 1, dim).cuda(), torch.arange(48, dtype=torch.int32).cuda(), kc, vc, ks, vs)
+    q = torch.zeros((3, 16, dim), dtype=torch.float16)
+    q[:, range(16), range(16)] = 200.0  # a query for each key: the others' weights are 0
+    out = torch.empty((3, 16, dim), dtype=torch.float16, device="cuda")
+    gpu.paged_attention(q.cuda(), kc, vc, torch.arange(4, dtype=torch.int32).cuda(), torch.arange(3, dtype=torch.int32).cuda(),
+                        torch.full((3,), 16, dtype=torch.int32).cuda(), out, scale=1.0, k_scale=ks, v_scale=vs)
+    torch.cuda.synchronize()
+    for s in (0, 2):
+        assert torch.equal(out[s].cpu().double(), held[s])
+    assert bool(torch.isnan(out[1]).any())  # whatever a token holds that is no number, its sequence shows it
