@@ -868,16 +868,32 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
             for (int j = 0; j < 4; ++j) {
               const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int row = 8 * j + 4 * half + e;
-                float x = s[4 * j + e];
-                if (!G && (bad >> row & 1)) x = __builtin_nanf("");  // its dO is taken as zeros below
-                s[4 * j + e] = key <= lim[e] ? x : 0.f;
-              }
+              for (int e = 0; e < 4; ++e) s[4 * j + e] = key <= lim[e] ? s[4 * j + e] : 0.f;
             }
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) f[e >> 3][e & 7] = (elem)s[e];
+          // The operand's elements that are no numbers, for the keys that their rows see; the product below takes them as zeros.
+#pragma unroll 1
+          for (unsigned left = bad; left != 0; left &= left - 1) {
+            const int row = __builtin_ctz(left);
+            float w = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w = (row & ~4) == 8 * (e >> 2) + (e & 3) ? (float)f[e >> 3][e & 7] : w;
+            w = __shfl(w, (lane & 31) | (row & 4) << 3, 64);  // rows with this bit are in the other half's lanes
+            const bool sees = key <= infos[qg][t % (2 * BATCH)].last[row];
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                const vec4<T> x = *(const vec4<T> *)(by_column + place_of<DP>(row, 4 * i + (e >> 2)) + 4 * half);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                  const float y = (float)x[n];
+                  if (sees && abs_bits(y) >= kInfBits) acc[i][e + n] += w * y;
+                }
+              }
+          }
         }
         if (t + S - 1 < tiles_n) load(t + S - 1, from);
         const bool next = t + 1 < tiles_n && same(__any(last_next >= key_low));

@@ -596,3 +596,66 @@ def test_sizes_that_numbers_do_not_hold_are_refused_before_anything_is_launched(
             gpu.check(call())
     torch.cuda.synchronize()
     assert bool((x == 7.0).all())
+
+
+# ---- operands that are not finite, and all three gradients --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("batch,kv_heads,block_m,block_n,dim", [(1, 1, 32, 16, 64), (1, 1, 32, 64, 128), (4, 8, 40, 32, 96), (4, 8, 64, 128, 64)])
+def test_gradients_beside_queries_that_see_no_key(gpu, batch, kv_heads, block_m, block_n, dim, dtype, bad):
+    """More queries than keys: what the first ones, in front of the first key, hold in any operand takes no part."""
+    queries, keys, none = 170, 130, 40
+    q, k, v, dout = make(batch, queries, keys, 2 * kv_heads, kv_heads, dim, TYPES[dtype], dim)
+    rows, columns = -(-queries // block_m), -(-keys // block_n)
+    n = batch * kv_heads * rows
+    pos, crd = torch.arange(n + 1, dtype=torch.int32).cuda() * columns, torch.arange(columns, dtype=torch.int32).repeat(n).cuda()
+    sizes = dict(block_m=block_m, block_n=block_n, causal=True)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    bq, bd, bo = q.clone(), dout.clone(), out.clone()
+    for x in (bq, bd, bo):
+        x[:, :none] = bad
+    again, _ = run_forward(gpu, bq, k, v, pos, crd, **sizes)
+    grads = run_backward(gpu, bd, bq, k, v, bo, lse, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    assert torch.equal(again, out) and bool((out[:, :none] == 0).all())
+    w = ref.pair_weights(pos, crd, batch, kv_heads, queries, keys, block_m, block_n, True)
+    wants, bounds = ref.backward(dout, q, k, v, out, lse, w, dim ** -0.5)
+    for name, g, x, y in zip(("dq", "dk", "dv"), grads, wants, bounds):
+        ref.assert_within(g, x, y, name)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("batch,kv_heads,block_m,block_n,dim", [(1, 1, 32, 16, 64), (1, 1, 32, 64, 128), (4, 8, 40, 32, 96), (4, 8, 64, 128, 64)])
+def test_one_element_of_a_gradient_that_is_not_finite(gpu, batch, kv_heads, block_m, block_n, dim, dtype, bad):
+    """It shows in that element of dV of the keys its query sees, in all of dK of these, and in its own row of dQ; everywhere else the
+    gradients are as they would be.  Queries in tiles that the diagonal cuts, and one that sees whole tiles."""
+    n = 200
+    q, k, v, dout = make(batch, n, n, 2 * kv_heads, kv_heads, dim, TYPES[dtype], block_n)
+    rows, columns = -(-n // block_m), -(-n // block_n)
+    lists = batch * kv_heads * rows
+    pos, crd = torch.arange(lists + 1, dtype=torch.int32).cuda() * columns, torch.arange(columns, dtype=torch.int32).repeat(lists).cuda()
+    sizes = dict(block_m=block_m, block_n=block_n, causal=True)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    w = ref.pair_weights(pos, crd, batch, kv_heads, n, n, block_m, block_n, True)
+    for query, element in ((7, 3), (70, dim - 1), (150, 33)):
+        there, zeroed = dout.clone(), dout.clone()
+        there[:, query, 0, element], zeroed[:, query, 0, element] = bad, 0.0
+        dq, dk, dv = (x.cpu() for x in run_backward(gpu, there, q, k, v, out, lse, pos, crd, **sizes))
+        wants, bounds = ref.backward(zeroed, q, k, v, out, lse, w, dim ** -0.5)
+        # dQ: all of the query's row of that head, and nothing else
+        hit = torch.zeros(dq.shape, dtype=torch.bool)
+        hit[:, query, 0] = True
+        assert not bool(torch.isfinite(dq[hit]).any())  # dO v^T and the row sum, one from the other: NaN or infinite
+        ref.assert_within(torch.where(hit, 0.0, dq.float()).to(dq.dtype), torch.where(hit, 0.0, wants[0]), bounds[0], "dq, query %d" % query)
+        # dK: keys up to the query of that group; dV: that element of them
+        hit = torch.zeros(dk.shape, dtype=torch.bool)
+        hit[:, :query + 1, 0] = True
+        assert not bool(torch.isfinite(dk[hit]).any())  # dO v^T and the row sum, one from the other: NaN or infinite
+        ref.assert_within(torch.where(hit, 0.0, dk.float()).to(dk.dtype), torch.where(hit, 0.0, wants[1]), bounds[1], "dk, query %d" % query)
+        hit = torch.zeros(dv.shape, dtype=torch.bool)
+        hit[:, :query + 1, 0, element] = True
+        want = torch.full(dv[hit].shape, bad, dtype=dv.dtype)
+        assert torch.equal(dv[hit].nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+        ref.assert_within(torch.where(hit, 0.0, dv.float()).to(dv.dtype), torch.where(hit, 0.0, wants[2]), bounds[2], "dv, query %d" % query)
