@@ -485,7 +485,12 @@ __global__ __launch_bounds__(1024) void few_columns_kernel(BlockArgs a, Columns 
   }
   const int descents = __popcll(__ballot(odd));
   if (descents && lane == 0) atomicAdd(t.odd, descents);
-  if (__syncthreads_or(odd)) return;
+  if (lane == 0) wave_sum[wave] = descents;
+  __syncthreads();
+  int of_list = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) of_list |= wave_sum[w];
+  if (of_list) return;
   const auto pass = [&](bool fill) {  // a wavefront's rows one after the other, their first entries asked for eight at a time
     for (int i0 = 0; i0 < r1 - r0; i0 += 8) {
       int entry[8];
