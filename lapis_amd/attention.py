@@ -90,17 +90,22 @@ class PagedCache:
         self.held = [[] for _ in range(sequences)]
         self.free = list(range(pages))[::-1]
 
-    def _open(self, sequence, tokens):
-        """Pages for ``tokens`` more tokens; raises before anything changes where there are not enough."""
-        needed = -(-(self.lengths[sequence] + tokens) // self.page) - len(self.held[sequence])
-        if needed > len(self.free) or len(self.held[sequence]) + needed > self.table.shape[1]:
-            raise RuntimeError("PagedCache: %d more pages for sequence %d, %d are free, %d of %d held" % (
-                needed, sequence, len(self.free), len(self.held[sequence]), self.table.shape[1]))
-        new = [self.free.pop() for _ in range(needed)]
-        if new:
-            first = len(self.held[sequence])
-            self.table[sequence, first:first + needed] = torch.tensor(new, dtype=torch.int32).to(self.table.device)
-        self.held[sequence] += new
+    def _open(self, sequences, tokens):
+        """Pages for ``tokens`` more tokens of each of these sequences; raises before anything changes where there are not enough."""
+        free, needed = len(self.free), []
+        for s in sequences:
+            held = len(self.held[s])
+            needed.append(max(0, -(-(self.lengths[s] + tokens) // self.page) - held))
+            if needed[-1] > free or held + needed[-1] > self.table.shape[1]:
+                raise RuntimeError("PagedCache: %d more pages for sequence %d, %d are free, %d of %d held" % (
+                    needed[-1], s, free, held, self.table.shape[1]))
+            free -= needed[-1]
+        for s, n in zip(sequences, needed):
+            new = [self.free.pop() for _ in range(n)]
+            if new:
+                first = len(self.held[s])
+                self.table[s, first:first + n] = torch.tensor(new, dtype=torch.int32).to(self.table.device)
+            self.held[s] += new
 
     def _store(self, k, v, slots):
         hip.kv_store(k, v, slots, self.k, self.v, self.k_scale, self.v_scale)
@@ -115,7 +120,7 @@ class PagedCache:
         if self.lengths[sequence]:
             raise ValueError("PagedCache.prefill: sequence %d holds %d tokens" % (sequence, self.lengths[sequence]))
         tokens, page = k.shape[0], self.page
-        self._open(sequence, tokens)
+        self._open([sequence], tokens)
         t = torch.arange(tokens, device=k.device)
         slots = self.table[sequence][t // page] * page + t % page
         self._store(k, v, slots.to(torch.int32))
@@ -133,33 +138,37 @@ class PagedCache:
     def step(self, q, k, v, count, sink=1, local=2, scale=None):
         """One token more of every sequence (k, v: sequences x heads x dim), and what it reads (q: sequences x query heads x
         dim) from the ``count`` best pages of each sequence and key-value head; the last ``local`` (at least 1) and first
-        ``sink`` pages are always among them."""
+        ``sink`` pages are always among them.  A sequence that was released begins anew with its token.  Where the call raises, the
+        cache holds what it held before."""
         if local < 1:
             raise ValueError("PagedCache.step: the page of the token itself is always attended to: local = %d" % local)
+        if sink < 0 or count < sink + local:
+            raise ValueError("PagedCache.step: %d pages, the first %d and the last %d always among them" % (count, sink, local))
         page, sequences, groups = self.page, len(self.lengths), self.k.shape[1]
-        for s in range(sequences):
-            self._open(s, 1)
+        q_codes, _ = _means(q[:, None], 1, groups)
+        self._open(range(sequences), 1)
         at = self.table.gather(1, (self.length // page).long()[:, None])[:, 0]
         self._store(k, v, at * page + self.length % page)
-        self.length += 1
-        self.lengths = [n + 1 for n in self.lengths]
-        if any(n % page == 0 for n in self.lengths):  # pages that are full now
-            pages = torch.tensor([self.held[s][-1] for s, n in enumerate(self.lengths) if n % page == 0], device=q.device)
+        # the numbers of the cache itself change when all is done: what was written counts from then on
+        length, lengths = self.length + 1, [n + 1 for n in self.lengths]
+        if any(n % page == 0 for n in lengths):  # pages that are full now
+            pages = torch.tensor([self.held[s][n // page - 1] for s, n in enumerate(lengths) if n % page == 0], device=q.device)
             slots = (pages[:, None] * page + torch.arange(page, device=q.device)).to(torch.int32).reshape(-1)
             rows, unused = (torch.empty((slots.numel(), groups, q.shape[2]), dtype=self.dtype, device=q.device) for _ in range(2))
             hip.kv_load(self.k, self.v, slots, rows, unused, self.k_scale, self.v_scale)
             self._keep_means(pages, rows.reshape(-1, page, *rows.shape[1:]))
 
-        q_codes, _ = _means(q[:, None], 1, groups)
-        blocks = (self.length + (page - 1)) // page
+        blocks = (length + (page - 1)) // page
         pos = torch.empty(sequences * groups + 1, dtype=torch.int32, device=q.device)
         crd = torch.zeros(sequences * groups * min(count, self.table.shape[1]), dtype=torch.int32, device=q.device)
         hip.block_select(q_codes, self.codes, self.scales, count, pos, crd, 1, self.table.shape[1], 1, 1, False, sink, local,
                          self.table, blocks)
         # of the listed pages the last is the one the token is in
-        tokens = (blocks.clamp(max=count) * page - (blocks * page - self.length)).repeat_interleave(groups)
+        tokens = (blocks.clamp(max=count) * page - (blocks * page - length)).repeat_interleave(groups)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         hip.paged_attention(q, self.k, self.v, pos, crd, tokens, out, None, scale, self.k_scale, self.v_scale)
+        self.length.copy_(length)
+        self.lengths = lengths
         return out
 
 

@@ -111,3 +111,53 @@ def test_the_example(attention):
     assert losses[-1] < losses[0] and lines
     # both sides round to bf16 once or twice, of answers below 8 in size
     assert difference < (8 * 2.0 ** -8) ** 2 and answered == answered
+
+
+def test_a_step_that_is_refused_changes_nothing(attention):
+    """Two caches take the same tokens; one is asked for steps in between that are refused, just before a page is full and after."""
+    from lapis_amd import hip
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
+    caches = [attention.PagedCache(2, 14, 96, 2, 64, page=16) for _ in range(2)]
+    for s, n in enumerate((31, 14)):
+        k, v = r(n, 2, 64), r(n, 2, 64)
+        for c in caches:
+            c.prefill(s, k, v)
+    for step in range(4):
+        other = r(2, 4, 64), r(2, 2, 64), r(2, 2, 64)
+        before = list(caches[0].lengths), caches[0].length.tolist()
+        with pytest.raises(ValueError, match="2 pages, the first 1 and the last 2"):
+            caches[0].step(*other, count=2)
+        with pytest.raises(ValueError, match="the first -1"):
+            caches[0].step(*other, count=4, sink=-1)
+        with pytest.raises(TypeError):
+            caches[0].step(other[0].half(), *other[1:], count=4)       # queries of another type than the cache
+        with pytest.raises(TypeError):
+            caches[0].step(other[0], other[1].half(), other[2].half(), count=4)
+        with pytest.raises(ValueError):
+            caches[0].step(other[0], other[1], other[2][:1], count=4)
+        with pytest.raises(ValueError):
+            caches[0].step(other[0][:, :3], *other[1:], count=4)       # three heads over two
+        assert before == (caches[0].lengths, caches[0].length.tolist())
+        q, k, v = r(2, 4, 64), r(2, 2, 64), r(2, 2, 64)
+        out = [c.step(q, k, v, count=4) for c in caches]
+        assert torch.equal(*out)
+    assert caches[0].lengths == caches[1].lengths == [35, 18] == caches[0].length.tolist()
+
+
+def test_a_step_without_pages_gives_none_out(attention):
+    cache = attention.PagedCache(3, 4, 64, 1, 64, page=16)
+    x = torch.ones((16, 1, 64), dtype=torch.bfloat16, device="cuda")
+    for s in range(3):
+        cache.prefill(s, x, x)
+    with pytest.raises(RuntimeError, match="1 more pages for sequence 1, 0 are free"):
+        cache.step(x[:3], x[:3], x[:3], 4)
+    assert len(cache.free) == 1 and cache.lengths == [16, 16, 16] and [len(h) for h in cache.held] == [1, 1, 1]
+    # a released one gives its page back and begins anew with its next token
+    cache.release(2)
+    with pytest.raises(RuntimeError, match="1 more pages for sequence 2, 0 are free"):
+        cache.step(x[:3], x[:3], x[:3], 4)
+    assert len(cache.free) == 2 and cache.lengths == [16, 16, 0]
+    cache.release(1)
+    cache.step(x[:3], x[:3], x[:3], 4)
+    assert cache.lengths == [17, 1, 1] == cache.length.tolist() and len(cache.free) == 0
