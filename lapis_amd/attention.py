@@ -61,6 +61,7 @@ class _Attend(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable  # the gradient has none itself: asked for one it raises
     def backward(ctx, dout):
         q, k, v, out, lse, pos, crd = ctx.saved_tensors
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))

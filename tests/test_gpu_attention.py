@@ -161,3 +161,11 @@ def test_a_step_without_pages_gives_none_out(attention):
     cache.release(1)
     cache.step(x[:3], x[:3], x[:3], 4)
     assert cache.lengths == [17, 1, 1] == cache.length.tolist() and len(cache.free) == 0
+
+
+def test_second_derivatives_are_refused(attention):
+    q, k, v = (torch.randn((1, 64, 2, 64), device="cuda").to(torch.bfloat16).requires_grad_() for _ in range(3))
+    out = attention.attend(q, k, v, attention.choose_blocks(q, k, 4, 16, 16))
+    dq, = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.float().square().sum().backward()
