@@ -674,6 +674,12 @@ void contiguous(const char *what, const char *name, const at::Tensor &t) {
   if (!t.is_contiguous()) raise(PyExc_ValueError, "%s: %s is not contiguous", what, name);
 }
 
+// Tensors that a call has written: autograd notices where it has kept one of them for a gradient.
+void written(std::initializer_list<PyObject *> outputs) {
+  for (PyObject *o : outputs)
+    if (o != Py_None && !THPVariable_Unpack(o).is_inference()) THPVariable_Unpack(o).unsafeGetTensorImpl()->bump_version();
+}
+
 // The kernels read and write device memory only, of one device.
 void on_device(const char *what, PyObject *const *a, Py_ssize_t n) {
   int device = -1;
@@ -781,6 +787,8 @@ PyObject *kv_move(const char *what, bool store, PyObject *const *a, Py_ssize_t n
     on_device(what, a, n);
     const lapis_hip_stream_t st = stream_of(a[7]);
     check(store ? lapis_hip_kv_store(&c, k.size(0), &kr, &vr, dtype, s, st) : lapis_hip_kv_load(&c, k.size(0), s, &kr, &vr, dtype, st));
+    if (store) written({a[3], a[4], a[5], a[6]});
+    else written({a[3], a[4]});
     PyObject *result = PyTuple_Pack(2, a[3], a[4]);
     if (!result) throw Raised();
     return result;
@@ -835,6 +843,7 @@ LAPIS_PY(py_paged_attention) {
     const Scratch work(bytes, st);
     p.work = work.data();
     check(lapis_hip_paged_attention(&c, &p, st));
+    written({a[6], a[7]});
     return give(a[6]);
   });
 }
@@ -860,6 +869,7 @@ LAPIS_PY(py_block_pool) {
     on_device(what, a, n);
     check(lapis_hip_block_pool(x.size(0), x.size(1), x.size(2), groups, x.size(3), block, &r, dtype, static_cast<int8_t *>(codes.data_ptr()),
                                static_cast<float *>(scales.data_ptr()), stream_of(a[4])));
+    written({a[2], a[3]});
     PyObject *result = PyTuple_Pack(2, a[2], a[3]);
     if (!result) throw Raised();
     return result;
@@ -943,6 +953,7 @@ LAPIS_PY(py_block_select) {
     const Scratch work(bytes, st);
     c.p.work = work.data();
     check(lapis_hip_block_select(&c.p, st));
+    written({a[4], a[5]});
     PyObject *result = PyTuple_Pack(2, a[4], a[5]);
     if (!result) throw Raised();
     return result;
@@ -1004,6 +1015,7 @@ LAPIS_PY(py_block_attention) {
     const lapis_hip_block_args p = block_of(what, a[0], a[1], a[2], a[3], a[4], a[5], a[6], true, a + 7);
     on_device(what, a, n);
     check(lapis_hip_block_attention(&p, stream_of(a[11])));
+    written({a[5], a[6]});
     PyObject *result = PyTuple_Pack(2, a[5], a[6]);
     if (!result) throw Raised();
     return result;
@@ -1037,6 +1049,7 @@ LAPIS_PY(py_block_attention_backward) {
     const Scratch work(bytes, st);
     p.work = work.data();
     check(lapis_hip_block_attention_backward(&p, st));
+    written({a[8], a[9], a[10]});
     PyObject *result = PyTuple_Pack(3, a[8], a[9], a[10]);
     if (!result) throw Raised();
     return result;

@@ -528,7 +528,7 @@ def bspmm_csrv(n1, n2, pos, crd, val, V, out, stream=None):
 
 # ---- block-sparse attention ----------------------------------------------------------------------------------
 # Tensors of bfloat16 or float16, with any strides between rows; structures are int32.  Outputs are written in place
-# and returned.
+# (their versions say so) and returned.
 
 def kv_store(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None, stream=None):
     """New tokens' keys and values (tokens x heads x dim) into slots (page * page size + place) of a cache in pages

@@ -169,3 +169,47 @@ def test_second_derivatives_are_refused(attention):
     dq, = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dq.float().square().sum().backward()
+
+
+def test_a_structure_that_is_overwritten_before_the_gradient_is_noticed(attention):
+    from lapis_amd import hip
+    q, k, v = (torch.randn((1, 64, 2, 64), device="cuda").to(torch.bfloat16).requires_grad_() for _ in range(3))
+    codes, scales = torch.empty((1, 2, 4, 64), dtype=torch.int8, device="cuda"), torch.empty((1, 2, 4), device="cuda")
+    hip.block_pool(k.detach(), 16, codes, scales)
+    select = lambda b: hip.block_select(codes, codes, scales, 2, b.pos, b.crd, 64, 64, 16, 16)  # noqa: E731
+    for late in (False, True):
+        blocks = attention.choose_blocks(q, k, 2, 16, 16, sink=0, local=1)
+        out = attention.attend(q, k, v, blocks)
+        if not late:
+            out.sum().backward()
+            continue
+        select(blocks)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
+def test_every_output_counts_its_writes(attention):
+    from lapis_amd import hip
+    b = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    f = lambda *s: torch.zeros(s, device="cuda")  # noqa: E731
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    codes, more = torch.zeros((1, 1, 2, 64), dtype=torch.int8, device="cuda"), f(1, 1, 2)
+    q, out, lse, pos, crd, grads = b(1, 32, 1, 64), b(1, 32, 1, 64), f(1, 1, 32), i(3), i(4), [b(1, 32, 1, 64) for _ in range(3)]
+    caches, scales, rows = [b(2, 1, 16, 64).to(torch.float8_e4m3fn) for _ in range(2)], [f(2, 1, 16) for _ in range(2)], [b(3, 1, 64) for _ in range(2)]
+    one, sums = b(1, 1, 64), f(1, 1)
+    calls = [
+        (lambda: hip.block_pool(q, 16, codes, more), [codes, more]),
+        (lambda: hip.block_select(codes, codes, more, 2, pos, crd, 32, 32, 16, 16), [pos, crd]),
+        (lambda: hip.block_attention(q, q, q, pos, crd, out, lse, 16, 16), [out, lse]),
+        (lambda: hip.block_attention_backward(q, q, q, q, out, lse, pos, crd, *grads, 16, 16), grads),
+        (lambda: hip.kv_store(rows[0], rows[0], i(3) + torch.arange(3, dtype=torch.int32, device="cuda"), *caches, *scales), caches + scales),
+        (lambda: hip.kv_load(*caches, i(3), *rows, *scales), rows),
+        (lambda: hip.paged_attention(one, *caches, i(2), i(0), i(1), out[:1, :1, 0], sums, None, *scales), [sums])]
+    for call, outputs in calls:
+        before = [x._version for x in outputs]
+        call()
+        assert all(x._version == n + 1 for x, n in zip(outputs, before))
+    with torch.inference_mode():
+        kept = b(1, 32, 1, 64)
+    hip.block_attention(q, q, q, pos, crd, kept, lse, 16, 16)  # a tensor without a version is written as any other
+    torch.cuda.synchronize()
