@@ -513,8 +513,8 @@ extern "C" int lapis_hip_block_pool(int64_t batch, int64_t tokens, int64_t heads
   LAPIS_REQUIRE(is_16bit(dtype), "block_pool: rows of type %d", dtype);
   PoolArgs a = {static_cast<char *>(x->data), {x->stride[0], x->stride[1], x->stride[2]}, tokens, ceil_div(tokens, block),
                 batch * groups * ceil_div(tokens, block), block, (int)groups, (int)(heads / groups), (int)dim, (signed char *)codes, scales};
-  if (a.lists_blocks == 0 || heads == 0) return LAPIS_HIP_OK;
-  LAPIS_REQUIRE(codes && scales && x->data, "block_pool: null operands");
+  if (a.lists_blocks == 0) return LAPIS_HIP_OK;
+  LAPIS_REQUIRE(codes && scales && (x->data || heads == 0), "block_pool: null operands");  // the mean of no heads is not a number
   LAPIS_REQUIRE(aligned16(x->data) && strides_of_8(x->stride, 3) && (reinterpret_cast<uintptr_t>(codes) & 7u) == 0,
                 "block_pool: rows that are not on 16-byte boundaries, strides that are no multiples of 8, or codes that are not on an 8-byte boundary");
   LAPIS_REQUIRE(a.lists_blocks <= (INT64_C(1) << 33), "block_pool: %lld blocks", (long long)a.lists_blocks);

@@ -195,3 +195,13 @@ def test_rows_whose_scores_take_several_launches(gpu, rows, columns, dim, count)
     assert bool((work[bytes_.value:] == 0xa5).all())
     assert torch.equal(pos, torch.arange(0, rows * count + 1, count, dtype=torch.int32, device="cuda"))
     assert torch.equal(crd.view(rows, count).long(), best_on_the_device(q, k, s, count, 1, 1))
+
+
+@pytest.mark.parametrize("block", [1, 16])
+def test_pool_of_no_heads(gpu, block):
+    """The mean over no heads is not finite: codes 0, scales NaN, not what the outputs held."""
+    x = torch.empty((2, 32, 0, 64), dtype=torch.bfloat16, device="cuda")
+    codes, scales = torch.full((2, 3, 32 // block, 64), 9, dtype=torch.int8, device="cuda"), torch.full((2, 3, 32 // block), 7.0, device="cuda")
+    gpu.block_pool(x, block, codes, scales)
+    torch.cuda.synchronize()
+    assert not bool(codes.any()) and bool(torch.isnan(scales).all())
