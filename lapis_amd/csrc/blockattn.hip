@@ -4,6 +4,12 @@
 namespace lapis {
 namespace {
 
+// Factor of scores in units of ln 2 (the sign goes to the queries): never 0, as masked scores are -infinity; NaN stays.
+__device__ __forceinline__ float units_of_ln2(float scale) {
+  const float c = fabsf(scale) * 1.4426950408889634f;
+  return c < 1e-37f ? 1e-37f : c;
+}
+
 // Rows of a list are its queries times the heads of the group, heads first: row i is query i / group, head i % group.
 //
 // A workgroup takes 32 * NW rows of one list, a wavefront 32 of them.  Tiles of KT keys go through LDS (two buffers: the
@@ -52,7 +58,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   v16f acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = v16f{};
-  const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);  // scores in units of ln 2; never 0: masked ones are -inf
+  const float c = units_of_ln2(a.scale);
   float m = -INFINITY, l = 0.f;  // of this row; l of this half's keys
 
   if (tid < 2) bad_tile[tid] = 0;
@@ -265,7 +271,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
   v4f acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-  const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+  const float c = units_of_ln2(a.scale);
   float m = -INFINITY, l = 0.f;
   elem *mine = own[wave].v;
   int now[2], next[2], ahead = look_up(share);

@@ -659,3 +659,17 @@ def test_one_element_of_a_gradient_that_is_not_finite(gpu, batch, kv_heads, bloc
         want = torch.full(dv[hit].shape, bad, dtype=dv.dtype)
         assert torch.equal(dv[hit].nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
         ref.assert_within(torch.where(hit, 0.0, dv.float()).to(dv.dtype), torch.where(hit, 0.0, wants[2]), bounds[2], "dv, query %d" % query)
+
+
+@pytest.mark.parametrize("queries", [16, 4000])
+def test_a_scale_that_is_not_a_number_shows(gpu, queries):
+    q, k, v, dout = make(1, queries, 300, 2, 1, 64, torch.bfloat16, 3)
+    rows = -(-queries // 16)
+    pos, crd = torch.arange(rows + 1, dtype=torch.int32).cuda() * 2, torch.tensor([0, 3], dtype=torch.int32).repeat(rows).cuda()
+    sizes = dict(block_m=16, block_n=64, causal=False, scale=math.nan)
+    out, lse = run_forward(gpu, q, k, v, pos, crd, **sizes)
+    grads = run_backward(gpu, dout, q, k, v, out, lse, pos, crd, **sizes)
+    torch.cuda.synchronize()
+    assert all(bool(torch.isnan(x).all()) for x in (out, lse, grads[0]))
+    seen = [*range(64), *range(192, 256)]
+    assert all(bool(torch.isnan(x[:, seen]).all()) for x in grads[1:])
