@@ -396,7 +396,7 @@ int read_view(const char *what, const lapis_hip_rows &r, View *v) {
 
 template <typename T, int DP, int NW, int KT>
 int launch_wide(const BlockArgs &a, hipStream_t st) {
-  const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)min(a.block_m, a.queries) * a.group, 32 * NW);
+  const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)std::min(a.block_m, a.queries) * a.group, 32 * NW);
   LAPIS_REQUIRE(lists * tiles * 64 * NW < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
   hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT>), dim3((unsigned)(lists * tiles)), dim3(64 * NW), 0, st, a, (int)tiles,
                      a.scale < 0.f ? (int)0x80008000u : 0);
@@ -452,7 +452,7 @@ int read_block(const char *what, const lapis_hip_block_args *p, bool backward, B
   a->kv_heads = (int)p->kv_heads;
   a->group = p->kv_heads ? (int)(p->heads / p->kv_heads) : 0;
   a->dim = (int)p->dim;
-  a->block_m = (int)min(p->block_m, max(p->queries, (int64_t)1));  // a longer block has no more queries
+  a->block_m = (int)std::min(p->block_m, std::max(p->queries, INT64_C(1)));  // a longer block has no more queries
   a->block_n_log2 = __builtin_ctz((unsigned)p->block_n);
   a->rows = (int)ceil_div(p->queries, p->block_m);
   a->columns = (int)ceil_div(p->keys, p->block_n);

@@ -1064,13 +1064,13 @@ int layout_of(const BlockArgs &a, Layout *layout) {
   Layout &l = *layout = {};
   Columns &c = l.columns;
   c.lists = a.batch * a.kv_heads;
-  c.chunk_rows = (int)max((int64_t)kRowsAtOnce, ceil_div(ceil_div(a.rows, 64), kRowsAtOnce) * kRowsAtOnce);
-  c.chunks = (int)max((int64_t)1, ceil_div(a.rows, c.chunk_rows));
+  c.chunk_rows = (int)std::max<int64_t>(kRowsAtOnce, ceil_div(ceil_div(a.rows, 64), kRowsAtOnce) * kRowsAtOnce);
+  c.chunks = (int)std::max<int64_t>(1, ceil_div(a.rows, c.chunk_rows));
   // Up to 8192 queries times heads a unit, so that long columns do not stand alone and those of ordinary length need no join; in
   // small passes what gives every workgroup one (the first block's column is all there is to wait for otherwise).
-  const int64_t rows_of_entry = (int64_t)min(a.block_m, max(a.queries, 1)) * max(a.group, 1);
-  const int64_t rows_of_unit = min(max(a.nnz * rows_of_entry / max(device_cu_count(), 1), (int64_t)256), (int64_t)8192);
-  c.per_unit = (int)min((int64_t)kMostEntries, max((int64_t)1, rows_of_unit / rows_of_entry));
+  const int64_t rows_of_entry = (int64_t)std::min(a.block_m, std::max(a.queries, 1)) * std::max(a.group, 1);
+  const int64_t rows_of_unit = std::min<int64_t>(std::max<int64_t>(a.nnz * rows_of_entry / std::max(device_cu_count(), 1), 256), 8192);
+  c.per_unit = (int)std::min<int64_t>(kMostEntries, std::max<int64_t>(1, rows_of_unit / rows_of_entry));
   const int64_t units = a.nnz / c.per_unit + columns;
   LAPIS_REQUIRE(units * 8 <= INT32_MAX, "block_attention_backward: %lld units of work", (long long)units);  // of up to eight parts each
   c.units = (int)units;
@@ -1098,7 +1098,7 @@ template <typename T, int DP, int KG, int S>
 void launch_dkv(const BlockArgs &a, const Columns &c, const float *delta, const float *logs, hipStream_t st) {
   Columns cols = c;
   cols.sub = (int)ceil_div(1 << a.block_n_log2, 32 * KG);
-  const int64_t grid = min((int64_t)2 * device_cu_count(), (int64_t)c.units * cols.sub);
+  const int64_t grid = std::min<int64_t>(2 * device_cu_count(), (int64_t)c.units * cols.sub);
   hipLaunchKernelGGL((block_dkv_kernel<T, DP, KG, S>), dim3((unsigned)grid), dim3(256), 0, st, DkvArgs{a, cols, delta, logs});
 }
 

@@ -550,7 +550,7 @@ constexpr int64_t kScoreBytes = INT64_C(256) << 20;  // of rows that go through 
 bool short_rows(const SelectArgs &a) { return a.columns <= kShortColumns && a.dim <= kShortDim; }
 
 // Rows at a time of those that go through memory.
-long long rows_at_once(const SelectArgs &a) { return max(1ll, min(a.batch * a.heads * a.rows, kScoreBytes / (4 * max(a.columns, 1ll)))); }
+long long rows_at_once(const SelectArgs &a) { return std::max<int64_t>(1, std::min<int64_t>(a.batch * a.heads * a.rows, kScoreBytes / (4 * std::max(a.columns, 1ll)))); }
 
 template <int NV>
 void launch_select(const SelectArgs &a, hipStream_t st) {
@@ -595,7 +595,7 @@ extern "C" int lapis_hip_block_select(const lapis_hip_select_args *args, lapis_h
   if (!short_rows(a)) {
     const long long some = rows_at_once(a);
     for (long long row0 = 0; row0 < rows; row0 += some) {
-      const long long here = min(some, rows - row0);
+      const long long here = std::min(some, rows - row0);
       hipLaunchKernelGGL(block_select_long_kernel, grid_of(here), dim3(64), 0, st, a, static_cast<unsigned *>(args->work), row0, here);
     }
   } else if (a.columns <= 256) {

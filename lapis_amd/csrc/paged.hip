@@ -429,12 +429,12 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
   a->scale = p->scale;
   a->lists = (int)p->lists;
   a->group = a->heads / c->heads;
-  a->head_tiles = (int)ceil_div(max(a->group, 1), 16);
+  a->head_tiles = (int)ceil_div(std::max(a->group, 1), 16);
   // Units for two workgroups a compute unit, of 128 to 1024 tokens: shorter ones cost more than they spread (a partial result
   // and its join), longer ones leave compute units waiting for the last.
-  const int64_t copies = (int64_t)a->head_tiles * (a->each ? 1 : c->heads), wanted = max(2 * device_cu_count(), 1);
-  const int64_t tokens = min(max(p->nnz * c->page * copies / wanted, (int64_t)128), (int64_t)1024);
-  a->chunk = (int)max(tokens / c->page, (int64_t)1);
+  const int64_t copies = (int64_t)a->head_tiles * (a->each ? 1 : c->heads), wanted = std::max(2 * device_cu_count(), 1);
+  const int64_t tokens = std::min<int64_t>(std::max<int64_t>(p->nnz * c->page * copies / wanted, 128), 1024);
+  a->chunk = (int)std::max<int64_t>(tokens / c->page, 1);
   a->units = (int)(p->nnz / a->chunk + p->lists);
   return LAPIS_HIP_OK;
 }

@@ -673,3 +673,16 @@ def test_a_scale_that_is_not_a_number_shows(gpu, queries):
     assert all(bool(torch.isnan(x).all()) for x in (out, lse, grads[0]))
     seen = [*range(64), *range(192, 256)]
     assert all(bool(torch.isnan(x[:, seen]).all()) for x in grads[1:])
+
+
+def test_scratch_of_more_queries_times_entries_than_31_bits(gpu):
+    """2^30 entries of 512 queries: sixteen to a unit of work."""
+    import ctypes
+    x, pos = torch.zeros((1, 8, 1, 8), dtype=torch.bfloat16, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    a = block_args(batch=1, queries=512, keys=32, heads=1, kv_heads=1, dim=8, block_m=512, block_n=16, nnz=1 << 30, causal=0, dtype=0, scale=1.0,
+                   pos=pos, crd=pos, q=x, k=x, v=x, out=x, lse=x.view(-1), dout=x, dq=x, dk=x, dv=x)
+    gpu.init()
+    bytes_ = ctypes.c_int64(-1)
+    gpu.check(gpu.load().lapis_hip_block_attention_backward_work(ctypes.byref(a), ctypes.byref(bytes_)))
+    partial, rows, units = 2 * (1 << 26) * 2 * 16 * 64 * 4, 4 << 30, 4 * ((1 << 26) + 2)
+    assert partial + rows + units <= bytes_.value <= partial + rows + units + (1 << 20)

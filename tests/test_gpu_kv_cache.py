@@ -405,3 +405,24 @@ def test_scales_that_differ_by_powers_of_two_and_are_not_numbers(gpu):
     for s in (0, 2):
         assert torch.equal(out[s].cpu().double(), held[s])
     assert bool(torch.isnan(out[1]).any())  # whatever a token holds that is no number, its sequence shows it
+
+
+def test_partial_results_of_more_tokens_times_heads_than_31_bits(gpu):
+    """2^31 tokens of 1024 heads: units of 1024 tokens."""
+    import ctypes
+
+    class Rows(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3)]
+
+    class Cache(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("stride", ctypes.c_int64 * 3), ("scale_stride", ctypes.c_int64 * 3)] +
+                    [("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("heads", "page", "dim", "dtype")])
+
+    class Args(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_int64) for n in ("seqs", "lists", "heads", "nnz")] + [("q", Rows), ("out", Rows), ("dtype", ctypes.c_int)] +
+                    [(n, ctypes.c_void_p) for n in ("pos", "crd", "tokens", "lse")] + [("scale", ctypes.c_float), ("work", ctypes.c_void_p)])
+    gpu.init()
+    nnz, bytes_ = (1 << 31) - 1, ctypes.c_int64(-1)
+    cache, args = Cache(heads=1024, page=1, dim=8), Args(seqs=2, lists=2, heads=1024, nnz=nnz)
+    gpu.check(gpu.load().lapis_hip_paged_attention_work(ctypes.byref(cache), ctypes.byref(args), ctypes.byref(bytes_)))
+    assert bytes_.value == (nnz // 1024 + 2) * 1024 * 16 * (64 + 2) * 4
