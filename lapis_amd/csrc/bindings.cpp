@@ -859,7 +859,7 @@ LAPIS_PY(py_block_pool) {
     if (block < 1) raise(PyExc_ValueError, "%s: blocks of %lld tokens", what, (long long)block);
     of_type(what, "codes", codes, at::kChar);
     of_type(what, "scales", scales, at::kFloat);
-    const int64_t groups = codes.size(1), blocks = (x.size(1) + block - 1) / block;
+    const int64_t groups = codes.size(1), blocks = x.size(1) / block + (x.size(1) % block != 0);
     if (groups < 1 || x.size(2) % groups != 0) raise(PyExc_ValueError, "%s: %lld heads in %lld groups", what, (long long)x.size(2), (long long)groups);
     of_shape(what, "codes", codes, {x.size(0), groups, blocks, x.size(3)});
     of_shape(what, "scales", scales, {x.size(0), groups, blocks});

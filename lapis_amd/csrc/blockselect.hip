@@ -511,6 +511,7 @@ extern "C" int lapis_hip_block_pool(int64_t batch, int64_t tokens, int64_t heads
   LAPIS_REQUIRE(dim >= 8 && dim <= kMaxDim && dim % 8 == 0, "block_pool: rows of %lld elements (a multiple of 8 up to %d)", (long long)dim, kMaxDim);
   LAPIS_REQUIRE(block >= 1, "block_pool: blocks of %lld tokens", (long long)block);
   LAPIS_REQUIRE(is_16bit(dtype), "block_pool: rows of type %d", dtype);
+  block = std::min(block, std::max(tokens, INT64_C(1)));  // a longer one has no more tokens
   PoolArgs a = {static_cast<char *>(x->data), {x->stride[0], x->stride[1], x->stride[2]}, tokens, ceil_div(tokens, block),
                 batch * groups * ceil_div(tokens, block), block, (int)groups, (int)(heads / groups), (int)dim, (signed char *)codes, scales};
   if (a.lists_blocks == 0) return LAPIS_HIP_OK;

@@ -205,3 +205,15 @@ def test_pool_of_no_heads(gpu, block):
     gpu.block_pool(x, block, codes, scales)
     torch.cuda.synchronize()
     assert not bool(codes.any()) and bool(torch.isnan(scales).all())
+
+
+def test_pool_of_a_block_longer_than_any_number_of_tokens(gpu):
+    x = torch.randn((1, 40, 4, 64), device="cuda").to(torch.bfloat16)
+    results = []
+    for block in (40, 2 ** 62, 2 ** 63 - 1):
+        codes, scales = torch.full((1, 2, 1, 64), 9, dtype=torch.int8, device="cuda"), torch.full((1, 2, 1), 7.0, device="cuda")
+        gpu.block_pool(x, block, codes, scales)
+        results.append((codes, scales))
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, results[0][0]) and torch.equal(s, results[0][1]) for c, s in results)
+    assert int(results[0][0].abs().max()) == 127
