@@ -217,3 +217,59 @@ def test_pool_of_a_block_longer_than_any_number_of_tokens(gpu):
     torch.cuda.synchronize()
     assert all(torch.equal(c, results[0][0]) and torch.equal(s, results[0][1]) for c, s in results)
     assert int(results[0][0].abs().max()) == 127
+
+
+@pytest.mark.parametrize("dim", [40, 128, 256])
+@pytest.mark.parametrize("columns", [256, 257, 512, 513, 1024, 1025, 1500, 2048, 2049])
+def test_selection_at_the_widths_where_kernels_change(gpu, columns, dim):
+    """Rows that see all blocks and rows that see some, scores full of ties, scales that are NaN: one list each."""
+    rng = np.random.default_rng(columns + dim)
+    rows, count = 37, 50
+    q = rng.integers(-127, 128, (1, 3, rows, dim)).astype(np.int8)
+    k = rng.integers(-127, 128, (1, 3, columns, dim)).astype(np.int8)
+    s = rng.uniform(0.001, 0.1, (1, 3, columns)).astype(np.float32)
+    q[0, 1], k[0, 1], s[0, 1] = rng.integers(-1, 2, q[0, 1].shape), rng.integers(-1, 2, k[0, 1].shape), np.float32(0.01)
+    s[0, 2, rng.random(columns) < 0.97] = np.nan
+    t = [torch.from_numpy(x) for x in (q, k, s)]
+    for causal in (False, True):  # causal: the rows see from columns - 36 * m / n blocks to all of them
+        m = max(1, columns // 50)
+        queries = rows * m
+        pos, crd = run_select(gpu, *t, count, queries, columns, m, 1, causal, 2, 3)
+        at = 0
+        for h in range(3):
+            for r in range(rows):
+                seen = min(max((r + 1) * m + columns - queries, 0), columns) if causal else columns
+                want = reference(q[0, h, r], k[0, h], s[0, h], count, seen, 2, 3)
+                assert pos[h * rows + r] == at
+                assert crd[at:at + len(want)].tolist() == want, (causal, h, r)
+                at += len(want)
+        assert pos[-1] == at and bool((crd[at:] == -9).all())
+
+
+def test_selection_over_a_wide_table(gpu):
+    """1500 pages to a sequence, some of which do not exist; lengths that reach every one of the kernels' widths."""
+    rng = np.random.default_rng(9)
+    pages, heads, dim, width, count = 4000, 2, 128, 1500, 40
+    blocks = np.array([1500, 1025, 41, 40, 700, 2000], dtype=np.int32)
+    table = rng.integers(0, pages, (6, width)).astype(np.int32)
+    table[rng.random(table.shape) < 0.01] = -1
+    table[rng.random(table.shape) < 0.01] = pages
+    q = rng.integers(-127, 128, (6, heads, 1, dim)).astype(np.int8)
+    k = rng.integers(-127, 128, (pages, heads, dim)).astype(np.int8)
+    s = rng.uniform(0, 1, (pages, heads)).astype(np.float32)
+    pos = torch.full((6 * heads + 1,), -9, dtype=torch.int32, device="cuda")
+    crd = torch.full((6 * heads * count,), -9, dtype=torch.int32, device="cuda")
+    gpu.block_select(*(torch.from_numpy(x).cuda() for x in (q, k, s)), count, pos, crd, queries=1, keys=width, block_m=1, block_n=1,
+                     causal=False, sink=1, local=2, table=torch.from_numpy(table).cuda(), blocks=torch.from_numpy(blocks).cuda())
+    pos, crd = pos.cpu().numpy(), crd.cpu().numpy()
+    at = 0
+    for b in range(6):
+        for h in range(heads):
+            seen = min(max(int(blocks[b]), 0), width)
+            page = np.clip(table[b], 0, pages - 1)
+            scale = np.where((table[b] >= 0) & (table[b] < pages), s[page, h], np.nan).astype(np.float32)
+            want = reference(q[b, h, 0], k[page, h], scale, count, seen, 1, 2)
+            assert pos[b * heads + h] == at
+            assert crd[at:at + len(want)].tolist() == [int(table[b, j]) for j in want], (b, h)
+            at += len(want)
+    assert pos[-1] == at
