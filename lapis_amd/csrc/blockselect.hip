@@ -31,7 +31,7 @@ template <typename T, int L, int PARTS>
 __global__ __launch_bounds__(256) void block_pool_kernel(PoolArgs a) {
   const long long thread = (long long)linear_block() * 256 + threadIdx.x;
   const long long at = thread / (L * PARTS);
-  const int part = (int)(thread / L) % PARTS, d = (int)(thread % L) * 8;
+  const int part = (int)(thread / L % PARTS), d = (int)(thread % L) * 8;
   const bool live = at < a.lists_blocks;
   const long long list = live ? at / a.blocks : 0, j = live ? at - list * a.blocks : 0;
   const long long b = list / a.groups;

@@ -273,3 +273,15 @@ def test_selection_over_a_wide_table(gpu):
             assert crd[at:at + len(want)].tolist() == [int(table[b, j]) for j in want], (b, h)
             at += len(want)
     assert pos[-1] == at
+
+
+def test_pool_of_more_parts_of_blocks_than_31_bits(gpu):
+    """2^28 blocks and some, eight groups of lanes to each: one row of values, given 2^29 times over by a stride of 0."""
+    blocks = (1 << 28) + 3
+    x = torch.arange(1, 9, dtype=torch.bfloat16, device="cuda")
+    codes = torch.full((1, 1, blocks, 8), 99, dtype=torch.int8, device="cuda")
+    scales = torch.full((1, 1, blocks), 7.0, device="cuda")
+    gpu.block_pool(x.view(1, 1, 1, 8).expand(1, 2 * blocks, 1, 8), 2, codes, scales)
+    torch.cuda.synchronize()
+    want = torch.tensor([16, 32, 48, 64, 79, 95, 111, 127], dtype=torch.int8, device="cuda")  # 127 n / 8: 63.5 is a tie, to even
+    assert bool((codes == want).all()) and bool((scales == torch.tensor(8.0) / 127.0).all())
