@@ -132,10 +132,10 @@ int kv_move(const char *what, const lapis_hip_kv_cache *cache, int64_t tokens, c
   LAPIS_REQUIRE(k && v && tokens >= 0, "%s: null rows or a negative number of tokens", what);
   LAPIS_REQUIRE(is_16bit(dtype) && (cache->dtype == dtype || cache->dtype == LAPIS_HIP_F8E4M3),
                 "%s: rows of type %d and a cache of type %d", what, dtype, cache->dtype);
-  const long long rows = tokens * cache->heads;
-  if (rows == 0) return LAPIS_HIP_OK;
+  if (tokens == 0) return LAPIS_HIP_OK;
   LAPIS_REQUIRE(slots, "%s: null slots", what);
-  LAPIS_REQUIRE(tokens <= INT32_MAX && rows < (INT64_C(1) << 31), "%s: %lld tokens", what, (long long)tokens);
+  LAPIS_REQUIRE(tokens <= INT32_MAX / cache->heads, "%s: %lld tokens of %d heads", what, (long long)tokens, cache->heads);
+  const long long rows = tokens * cache->heads;
   for (const lapis_hip_rows *r : {k, v})
     LAPIS_REQUIRE(r->data && aligned16(r->data) && strides_of_8(r->stride + 1, 2),
                   "%s: rows that are null, not on a 16-byte boundary or with strides that are no multiples of 8", what);
@@ -172,7 +172,7 @@ int check_cache(const char *what, const lapis_hip_kv_cache *c) {
   LAPIS_REQUIRE(c, "%s: null cache", what);
   LAPIS_REQUIRE(c->heads > 0 && c->pages >= 0, "%s: a cache of %lld pages and %d heads", what, (long long)c->pages, c->heads);
   LAPIS_REQUIRE(c->page >= 1 && c->page <= 1024 && (c->page & (c->page - 1)) == 0, "%s: pages of %d slots (a power of two up to 1024)", what, c->page);
-  LAPIS_REQUIRE(c->pages * c->page <= INT32_MAX, "%s: %lld pages of %d slots: slots are numbered with 31 bits", what, (long long)c->pages, c->page);
+  LAPIS_REQUIRE(c->pages <= INT32_MAX / c->page, "%s: %lld pages of %d slots: slots are numbered with 31 bits", what, (long long)c->pages, c->page);
   LAPIS_REQUIRE(c->dim >= 8 && c->dim <= kMaxDim && c->dim % 8 == 0, "%s: rows of %d elements (a multiple of 8 up to %d)", what, c->dim, kMaxDim);
   const bool f8 = c->dtype == LAPIS_HIP_F8E4M3;
   LAPIS_REQUIRE(f8 || is_16bit(c->dtype), "%s: a cache of type %d", what, c->dtype);

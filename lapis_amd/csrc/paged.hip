@@ -403,6 +403,7 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
   LAPIS_REQUIRE(p->lists == p->seqs || p->lists == p->seqs * c->heads, "%s: %lld lists of pages for %lld sequences", what,
                 (long long)p->lists, (long long)p->seqs);
   LAPIS_REQUIRE(p->nnz >= 0 && p->nnz <= INT32_MAX && p->nnz * c->page <= INT32_MAX, "%s: %lld pages listed", what, (long long)p->nnz);
+  LAPIS_REQUIRE(p->lists <= INT32_MAX, "%s: %lld lists", what, (long long)p->lists);
   LAPIS_REQUIRE(is_16bit(p->dtype) && (c->dtype == p->dtype || c->dtype == LAPIS_HIP_F8E4M3), "%s: queries of type %d and a cache of type %d",
                 what, p->dtype, c->dtype);
   *a = {};
@@ -435,7 +436,9 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
   const int64_t copies = (int64_t)a->head_tiles * (a->each ? 1 : c->heads), wanted = std::max(2 * device_cu_count(), 1);
   const int64_t tokens = std::min<int64_t>(std::max<int64_t>(p->nnz * c->page * copies / wanted, 128), 1024);
   a->chunk = (int)std::max<int64_t>(tokens / c->page, 1);
-  a->units = (int)(p->nnz / a->chunk + p->lists);
+  const int64_t units = p->nnz / a->chunk + p->lists;
+  LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
+  a->units = (int)units;
   return LAPIS_HIP_OK;
 }
 

@@ -1,4 +1,5 @@
 """The paged cache: storing with and without 8-bit codes, loading, and attention of one token over its pages."""
+import ctypes
 import math
 
 import pytest
@@ -407,22 +408,58 @@ def test_scales_that_differ_by_powers_of_two_and_are_not_numbers(gpu):
     assert bool(torch.isnan(out[1]).any())  # whatever a token holds that is no number, its sequence shows it
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3)]
+
+
+class Cache(ctypes.Structure):
+    """lapis_hip_kv_cache"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("stride", ctypes.c_int64 * 3), ("scale_stride", ctypes.c_int64 * 3)] +
+                [("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("heads", "page", "dim", "dtype")])
+
+
+class PagedArgs(ctypes.Structure):
+    """lapis_hip_paged_args"""
+    _fields_ = ([(n, ctypes.c_int64) for n in ("seqs", "lists", "heads", "nnz")] + [("q", Rows), ("out", Rows), ("dtype", ctypes.c_int)] +
+                [(n, ctypes.c_void_p) for n in ("pos", "crd", "tokens", "lse")] + [("scale", ctypes.c_float), ("work", ctypes.c_void_p)])
+
+
 def test_partial_results_of_more_tokens_times_heads_than_31_bits(gpu):
     """2^31 tokens of 1024 heads: units of 1024 tokens."""
-    import ctypes
-
-    class Rows(ctypes.Structure):
-        _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3)]
-
-    class Cache(ctypes.Structure):
-        _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("stride", ctypes.c_int64 * 3), ("scale_stride", ctypes.c_int64 * 3)] +
-                    [("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("heads", "page", "dim", "dtype")])
-
-    class Args(ctypes.Structure):
-        _fields_ = ([(n, ctypes.c_int64) for n in ("seqs", "lists", "heads", "nnz")] + [("q", Rows), ("out", Rows), ("dtype", ctypes.c_int)] +
-                    [(n, ctypes.c_void_p) for n in ("pos", "crd", "tokens", "lse")] + [("scale", ctypes.c_float), ("work", ctypes.c_void_p)])
     gpu.init()
     nnz, bytes_ = (1 << 31) - 1, ctypes.c_int64(-1)
-    cache, args = Cache(heads=1024, page=1, dim=8), Args(seqs=2, lists=2, heads=1024, nnz=nnz)
+    cache, args = Cache(heads=1024, page=1, dim=8), PagedArgs(seqs=2, lists=2, heads=1024, nnz=nnz)
     gpu.check(gpu.load().lapis_hip_paged_attention_work(ctypes.byref(cache), ctypes.byref(args), ctypes.byref(bytes_)))
     assert bytes_.value == (nnz // 1024 + 2) * 1024 * 16 * (64 + 2) * 4
+
+
+@pytest.mark.parametrize("cache,args,what", [
+    (dict(heads=65535, page=16, dim=8), dict(seqs=65535, lists=65535 * 65535, heads=65535, nnz=0), "4294836225 lists"),
+    (dict(heads=32768, page=1, dim=8), dict(seqs=65535, lists=65535 * 32768, heads=32768, nnz=2147483647), "2149548031 units of work"),
+    (dict(heads=4, page=16, dim=8, pages=1 << 60), dict(seqs=1, lists=1, heads=4, nnz=0), "slots are numbered with 31 bits")])
+def test_sizes_that_numbers_do_not_hold_are_refused(gpu, cache, args, what):
+    x, i = torch.full((8, 8), 7.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(16, dtype=torch.int32, device="cuda")
+    c = Cache(k=x.data_ptr(), v=x.data_ptr(), **cache)
+    a = PagedArgs(pos=i.data_ptr(), crd=i.data_ptr(), tokens=i.data_ptr(), q=Rows(x.data_ptr()), out=Rows(x.data_ptr()), work=x.data_ptr(), **args)
+    gpu.init()
+    with pytest.raises(gpu.LapisHipError, match=what):
+        gpu.check(gpu.load().lapis_hip_paged_attention(ctypes.byref(c), ctypes.byref(a), None))
+    if "pages" in cache:
+        rows = Rows(x.data_ptr())
+        with pytest.raises(gpu.LapisHipError, match=what):
+            gpu.check(gpu.load().lapis_hip_kv_store(ctypes.byref(c), 1, ctypes.byref(rows), ctypes.byref(rows), 0, i.data_ptr(), None))
+    torch.cuda.synchronize()
+    assert bool((x == 7.0).all())
+
+
+def test_more_tokens_than_numbers_hold_are_refused(gpu):
+    x, i = torch.full((8, 8), 7.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(16, dtype=torch.int32, device="cuda")
+    c, rows = Cache(k=x.data_ptr(), v=x.data_ptr(), heads=4, page=1, dim=8, pages=1), Rows(x.data_ptr())
+    gpu.init()
+    for tokens in (1 << 62, 1 << 29, (1 << 63) - 1):  # times four heads: 0, 2^31 and -4 in 64 and 32 bits
+        for call in (lambda n: gpu.load().lapis_hip_kv_store(ctypes.byref(c), n, ctypes.byref(rows), ctypes.byref(rows), 0, i.data_ptr(), None),
+                     lambda n: gpu.load().lapis_hip_kv_load(ctypes.byref(c), n, i.data_ptr(), ctypes.byref(rows), ctypes.byref(rows), 0, None)):
+            with pytest.raises(gpu.LapisHipError, match="tokens of 4 heads"):
+                gpu.check(call(tokens))
+    torch.cuda.synchronize()
+    assert bool((x == 7.0).all())
