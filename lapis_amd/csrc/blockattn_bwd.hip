@@ -11,6 +11,15 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kParts = 8;  // of the units of work beside dK and dV, one to each XCD
 
+// Row `row` (the same for all lanes) of a 32x32 product that has been rounded to an operand, in its column's lanes of both halves.
+template <typename T>
+__device__ __forceinline__ float of_row(const vec8<T> (&f)[2], int row, int lane) {
+  float w = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) w = (row & ~4) == 8 * (e >> 2) + (e & 3) ? (float)f[e >> 3][e & 7] : w;
+  return __shfl(w, (lane & 31) | (row & 4) << 3, 64);  // rows with this bit are in the other half's lanes
+}
+
 // ---- dQ --------------------------------------------------------------------------------------------------------
 
 // As the forward kernel: 32 rows a wavefront, a query per lane.  dS^T = P^T * (scale V dO^T - scale delta) feeds dQ^T = K^T dS^T
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
           }
           df[e >> 3][e & 7] = (elem)ds;
         }
-        // a row that sees a key with an infinity or NaN has NaN in its score; the others take the key as zeros
+        // a key's elements that are no numbers count for the rows that see it, by themselves; the product takes them as zeros
         int clean = !bad;  // either way, but not as two sides of one branch: the sums would be kept twice
         if (clean) {
 #pragma unroll
@@ -159,6 +168,20 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
 #pragma unroll
             for (int i = 0; i < DT; ++i)
               acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, place_lane)), df[y], acc[i]);
+#pragma unroll 1
+          for (int row = 0; row < 32; ++row) {
+            const bool sees = (row < 16 ? now[2 * x] : now[2 * x + 1]) + (row & 15) <= limit;
+            const float w = of_row<T>(df, row, lane);
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                const vec4<T> k = *(const vec4<T> *)(kt + place_of<DP>(32 * x + row, 4 * i + (e >> 2)) + 4 * half);
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                  if (sees && abs_bits((float)k[n]) >= kInfBits) acc[i][e + n] += w * (float)k[n];
+              }
+          }
         }
       }
     }
@@ -311,6 +334,23 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
       if (bad) k = finite_only<T>(k);
       acc[i] = mfma16(k, df, acc[i]);
     }
+    if (bad)  // a key's elements that are no numbers, for the rows that see it
+#pragma unroll 1
+      for (int x = 0; x < 32; ++x) {
+        const bool sees = (x < 16 ? now0 : now1) + (x & 15) <= limit;
+        float w = 0.f;  // key x is element 4 (x / 16) + x % 4 of quarter x / 4 % 4
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w = e == 4 * (x >> 4) + (x & 3) ? (float)df[e] : w;
+        w = __shfl(w, col | (x >> 2 & 3) << 4, 64);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const int d = 16 * i + 4 * quarter;
+          const vec4<T> k = *(const vec4<T> *)(mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (sees && abs_bits((float)k[e]) >= kInfBits) acc[i][e] += w * (float)k[e];
+        }
+      }
     wave_lds_sync();
   }
 #pragma unroll
@@ -882,10 +922,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
 #pragma unroll 1
           for (unsigned left = bad; left != 0; left &= left - 1) {
             const int row = __builtin_ctz(left);
-            float w = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w = (row & ~4) == 8 * (e >> 2) + (e & 3) ? (float)f[e >> 3][e & 7] : w;
-            w = __shfl(w, (lane & 31) | (row & 4) << 3, 64);  // rows with this bit are in the other half's lanes
+            const float w = of_row<T>(f, row, lane);
             const bool sees = key <= infos[qg][t % (2 * BATCH)].last[row];
 #pragma unroll
             for (int i = 0; i < DT; ++i)

@@ -686,3 +686,36 @@ def test_scratch_of_more_queries_times_entries_than_31_bits(gpu):
     gpu.check(gpu.load().lapis_hip_block_attention_backward_work(ctypes.byref(a), ctypes.byref(bytes_)))
     partial, rows, units = 2 * (1 << 26) * 2 * 16 * 64 * 4, 4 << 30, 4 * ((1 << 26) + 2)
     assert partial + rows + units <= bytes_.value <= partial + rows + units + (1 << 20)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("batch,kv_heads,block_m,block_n,dim", [(1, 1, 16, 16, 64), (1, 1, 32, 64, 128), (4, 8, 40, 32, 96), (4, 8, 64, 128, 64)])
+def test_keys_of_minus_infinity(gpu, batch, kv_heads, block_m, block_n, dim, dtype):
+    """A key whose score is -infinity has no weight; in the one element it has infinite, dS k is 0 times infinity for the queries that see
+    it, whether a mask cuts their tile or not, and everything else is as without the key."""
+    n, element = 200, 5
+    q, k, v, dout = make(batch, n, n, 2 * kv_heads, kv_heads, dim, TYPES[dtype], block_n + 1)
+    q[..., element] = q[..., element].abs() + 1.0
+    rows, columns = -(-n // block_m), -(-n // block_n)
+    lists = batch * kv_heads * rows
+    pos, crd = torch.arange(lists + 1, dtype=torch.int32).cuda() * columns, torch.arange(columns, dtype=torch.int32).repeat(lists).cuda()
+    sizes = dict(block_m=block_m, block_n=block_n, causal=True)
+    w = ref.pair_weights(pos, crd, batch, kv_heads, n, n, block_m, block_n, True)
+    for key in (1, 77, 130):
+        there, without, zeroed = k.clone(), w.clone(), k.clone()
+        there[:, key, :, element], zeroed[:, key, :, element] = -math.inf, 0.0
+        without[..., key] = 0
+        out, lse = run_forward(gpu, q, there, v, pos, crd, **sizes)
+        grads = run_backward(gpu, dout, q, there, v, out, lse, pos, crd, **sizes)
+        torch.cuda.synchronize()
+        want, want_lse, bound, lse_bound = ref.forward(q, zeroed, v, without, dim ** -0.5)
+        ref.assert_within(out, want, bound, "out, key %d" % key)
+        ref.assert_within(lse, want_lse, lse_bound, "lse, key %d" % key)
+        wants, bounds = ref.backward(dout, q, zeroed, v, out, lse, without, dim ** -0.5)
+        dq = grads[0].cpu()
+        hit = torch.zeros(dq.shape, dtype=torch.bool)
+        hit[:, key:, :, element] = True
+        assert bool(torch.isnan(dq[hit]).all()), "key %d" % key
+        ref.assert_within(torch.where(hit, 0.0, dq.float()).to(dq.dtype), torch.where(hit, 0.0, wants[0]), bounds[0], "dq, key %d" % key)
+        for name, g, x, y in zip(("dk", "dv"), grads[1:], wants[1:], bounds[1:]):
+            ref.assert_within(g, x, y, "%s, key %d" % (name, key))
