@@ -81,6 +81,12 @@ double number(PyObject *o) {
   return v;
 }
 
+bool truth(PyObject *o) {
+  const int r = PyObject_IsTrue(o);
+  if (r < 0) throw Raised();
+  return r != 0;
+}
+
 // Every call asks for its stream after its operands have passed their checks: malformed operands are refused
 // without a GPU too.
 lapis_hip_stream_t stream_of(PyObject *o) {
@@ -892,7 +898,7 @@ struct SelectCall {
     p.keys = integer(a[7]);
     p.block_m = integer(a[8]);
     p.block_n = integer(a[9]);
-    p.causal = PyObject_IsTrue(a[10]);
+    p.causal = truth(a[10]);
     p.sink = integer(a[11]);
     p.local = integer(a[12]);
     if (p.block_m < 1 || p.block_n < 1 || p.queries < 0 || p.keys < 0) raise(PyExc_ValueError, "%s: sizes of blocks and of queries and keys", what);
@@ -982,7 +988,7 @@ lapis_hip_block_args block_of(const char *what, PyObject *q_, PyObject *k_, PyOb
   of_shape(what, "out", out, {p.batch, p.queries, p.heads, p.dim});
   p.block_m = integer(sizes[0]);
   p.block_n = integer(sizes[1]);
-  p.causal = PyObject_IsTrue(sizes[2]);
+  p.causal = truth(sizes[2]);
   if (p.block_m < 1 || p.block_n < 1) raise(PyExc_ValueError, "%s: blocks of %lld queries and %lld keys", what, (long long)p.block_m, (long long)p.block_n);
   if (p.kv_heads < 1 || p.heads % p.kv_heads != 0) raise(PyExc_ValueError, "%s: %lld heads over %lld key-value heads", what, (long long)p.heads, (long long)p.kv_heads);
   for (const at::Tensor *t : {&pos, &crd}) {

@@ -167,3 +167,12 @@ def test_scratch_sizes_are_asked_for_after_init():
     buffer, bytes_ = ctypes.create_string_buffer(1024), ctypes.c_int64(-1)
     for rc in (lib.lapis_hip_block_attention_backward_work(buffer, ctypes.byref(bytes_)), lib.lapis_hip_paged_attention_work(buffer, buffer, ctypes.byref(bytes_))):
         assert lib.lapis_hip_status_name(rc) == b"LAPIS_HIP_ERR_NOT_INITIALIZED" and bytes_.value == -1
+
+
+@pytest.mark.parametrize("call", [attention, gradient, select])
+def test_a_flag_that_has_no_truth_value(call):
+    class Flag:
+        def __bool__(self):
+            raise KeyError("neither")
+    with pytest.raises(KeyError, match="neither"):
+        call(causal=Flag())
