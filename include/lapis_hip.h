@@ -466,7 +466,8 @@ typedef struct lapis_hip_kv_cache {
 } lapis_hip_kv_cache;
 
 /* Row t of k and v (stride[0] unused) goes to slot slots[t] (page * cache->page + place in the page) of every head;
- * a slot outside [0, pages * page) writes nothing.  Slots are distinct (of two tokens for one slot either may win).
+ * a slot outside [0, pages * page) writes nothing.  Slots are distinct: of two tokens for one slot codes of one and the scale of the
+ * other may stay.
  * With LAPIS_HIP_F8E4M3: scale = max|x| / 448 over the row, codes = x / scale rounded to nearest even; a row of zeros has
  * scale 0; a NaN stays NaN, a row with an infinity reads back as NaN.  `dtype` is the rows' own. */
 int lapis_hip_kv_store(const lapis_hip_kv_cache *cache, int64_t tokens, const lapis_hip_rows *k, const lapis_hip_rows *v,

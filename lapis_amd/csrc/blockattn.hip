@@ -16,7 +16,7 @@ __device__ __forceinline__ float units_of_ln2(float scale) {
 // next tile is loaded straight into one while the other is computed).
 // S^T = K Q^T has a query per lane, so maxima, sums and factors of the softmax are one register and need one exchange
 // between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
-// 32 768 queries and keys, 32 heads over 8, dim 128, 16 blocks of 128 a row, bf16: 1289 us, 800 TFLOP/s where a large library
+// 32 768 queries and keys, 32 heads over 8, dim 128, 16 blocks of 128 a row, bf16: 1290 to 1350 us, 800 to 765 TFLOP/s where a large library
 // product reaches 1203.  Bound by issue: 72 % of the cycles issue something, vector instructions 41 %, products 32 %.
 template <typename T, int DP, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {

@@ -24,8 +24,8 @@ __device__ __forceinline__ float of_row(const vec8<T> (&f)[2], int row, int lane
 
 // As the forward kernel: 32 rows a wavefront, a query per lane.  dS^T = P^T * (scale V dO^T - scale delta) feeds dQ^T = K^T dS^T
 // from its registers.  rowsum(dO * O), times `scale`, and the log-sums in units of ln 2 are left for the other kernel.
-// 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 319 us in a trace (356 with 24 registers spilled and the products
-// one chain after the other), 590 TFLOP/s; bound by what a wavefront waits for between its chains of products.
+// 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 309 us in a trace (356 with 24 registers spilled and the products
+// one chain after the other), 610 TFLOP/s; bound by what a wavefront waits for between its chains of products.
 template <typename T, int DP, int NW, int KT>
 __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
@@ -601,14 +601,14 @@ constexpr int kMostDescents = 16;  // of positions: 17 times the entries at most
 // turn, three chains of products that do not wait for each other; where the rows of four tiles lie is worked out by 128
 // threads at once, and what an iteration needs from LDS is asked for a stage before its use.  (A single workgroup, 64 keys,
 // dim 128: 1.35 us an iteration with one chain after the other, 1.10 so; 8192 queries, 32 heads over 8, 16 blocks of 64
-// a row: 630 us to 549, in a trace.)  It is bound by what an iteration of a wavefront waits for: the products alone are 128 us.
+// a row: 630 us to 549, in a trace; 511 now.)  It is bound by what an iteration of a wavefront waits for: the products alone are 128 us.
 // The rows of a column lie all over Q and dO, beyond L2 in large passes (16 columns read each block of rows: 2.1 GB, 290 us
 // by themselves): S tiles are on their way or being computed, and no load but those into LDS is in the loop.
 // Columns are anything but equal (the first block is listed by all rows, the last by few): workgroups take units from a
 // counter, those of their XCD's part first, whose rows of Q and dO its L2 holds.
 // The kernel's arguments are more than the scalar registers hold beside the loop (148 spilled, and a wait for a spilled register in
 // the loop waits for the tiles on their way too), so whatever the loop does not need all the time is read from the arguments
-// again where it is used (54 spilled, none in the loop).
+// again where it is used (at dim 128, 64 keys, about 50 spilled, and 13 vector registers, none in the loop over tiles).
 struct DkvArgs {
   BlockArgs a;
   Columns cols;

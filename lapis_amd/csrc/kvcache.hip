@@ -2,9 +2,9 @@
 //
 // A row of `dim` elements belongs to a group of lanes, eight elements each (one 16-byte load); the row's maximum is
 // a DPP reduction over the group, so a row is read once and nothing is kept but registers.  Bound by memory: 32 768 tokens
-// of 8 heads, dim 128, bf16 into e4m3 in 49.8 us (4.1 TB/s), 20 000 tokens, dim 96, back into f16 in 24.0 (3.9 TB/s), where a
+// of 8 heads, dim 128, bf16 into e4m3 in 51.5 us (4.0 TB/s), 20 000 tokens, dim 96, back into f16 in 24.1 (3.9 TB/s), where a
 // large copy reaches 4.75; four rows a thread on their way, loads first, where that leaves every compute unit its workgroups
-// (one row a thread: 54 and 30).  48 tokens take 4.7 us, the call and the launch.
+// (one row a thread: 54 and 30).  48 tokens take 4.5 us, the call and the launch.
 #include "attn.hpp"
 
 namespace lapis {

@@ -52,7 +52,7 @@ __device__ __forceinline__ int turn(int row) {
   return DP >= 128 ? (row & 3) << 2 | ((row >> 2) & 3) : ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
 }
 // A tile that is only read by columns takes the part of it that serves that: rows eight apart have the same order then, one
-// address register fewer for each 32 columns (in the forward kernel the difference between spilling and not).
+// address register fewer for each 32 columns (the forward kernel at dim 128 has none to spare: it keeps three in memory, outside its loop).
 template <int DP>
 __device__ __forceinline__ int column_turn(int row) {
   return DP >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;

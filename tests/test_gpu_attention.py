@@ -115,7 +115,6 @@ def test_the_example(attention):
 
 def test_a_step_that_is_refused_changes_nothing(attention):
     """Two caches take the same tokens; one is asked for steps in between that are refused, just before a page is full and after."""
-    from lapis_amd import hip
     g = torch.Generator().manual_seed(7)
     r = lambda *s: torch.randn(s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
     caches = [attention.PagedCache(2, 14, 96, 2, 64, page=16) for _ in range(2)]
