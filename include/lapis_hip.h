@@ -443,7 +443,7 @@ int lapis_hip_normalize_mom2_f64(int64_t n, const double *mom1, const double *mo
  * with all its entries (positions that nobody wrote may make that rows times nnz of them).
  * Rows without an entry give zeros, and -infinity as the logarithm of their sum.
  * No entry point below allocates or synchronises: where scratch memory is needed the caller passes `work` of at least
- * the bytes the matching _work call says. */
+ * the bytes the matching _work call says, on a 16-byte boundary. */
 
 enum lapis_hip_dtype { LAPIS_HIP_BF16 = 0, LAPIS_HIP_F16 = 1, LAPIS_HIP_F8E4M3 = 2 };
 

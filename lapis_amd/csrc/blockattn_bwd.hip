@@ -1200,7 +1200,7 @@ extern "C" int lapis_hip_block_attention_backward(const lapis_hip_block_args *ar
   const int rc = read_block("block_attention_backward", args, true, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   if (a.batch == 0 || (a.heads == 0 && a.kv_heads == 0)) return LAPIS_HIP_OK;
-  LAPIS_REQUIRE(args->work, "block_attention_backward: null work");
+  LAPIS_REQUIRE(args->work && aligned16(args->work), "block_attention_backward: work that is null or not on a 16-byte boundary");
   char *work = static_cast<char *>(args->work);
   const bool bf16 = args->dtype == LAPIS_HIP_BF16;
   if (a.dim <= 64) return bf16 ? launch_backward<Bf16, 64>(a, work, as_stream(stream)) : launch_backward<F16, 64>(a, work, as_stream(stream));

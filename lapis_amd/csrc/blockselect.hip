@@ -588,7 +588,8 @@ extern "C" int lapis_hip_block_select(const lapis_hip_select_args *args, lapis_h
       return LAPIS_HIP_OK;
     }
   } else {
-    LAPIS_REQUIRE(a.q && a.k && a.scales && a.crd && (args->work || short_rows(a)), "block_select: null operands");
+    LAPIS_REQUIRE(a.q && a.k && a.scales && a.crd, "block_select: null operands");
+    LAPIS_REQUIRE(short_rows(a) || (args->work && aligned16(args->work)), "block_select: work that is null or not on a 16-byte boundary");
     const uintptr_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k);
     LAPIS_REQUIRE((low & 7u) == 0 && strides_of_8(args->k_stride, 3), "block_select: codes that are not on 8-byte boundaries or strides that are no multiples of 8");
   }

@@ -719,3 +719,32 @@ def test_keys_of_minus_infinity(gpu, batch, kv_heads, block_m, block_n, dim, dty
         ref.assert_within(torch.where(hit, 0.0, dq.float()).to(dq.dtype), torch.where(hit, 0.0, wants[0]), bounds[0], "dq, key %d" % key)
         for name, g, x, y in zip(("dk", "dv"), grads[1:], wants[1:], bounds[1:]):
             ref.assert_within(g, x, y, "%s, key %d" % (name, key))
+
+
+@pytest.mark.parametrize("queries,block_m", [(96, 16), (1100, 2)])
+def test_positions_outside_the_entries(gpu, queries, block_m):
+    """Ascending ones in front of the first entry and behind the last: as if they were at the ends."""
+    rows = -(-queries // block_m)
+    t = make(1, queries, 200, 2, 1, 64, torch.float16, 3)
+    pos, crd = random_lists(1, rows, 7, 4, rows, empty=0.1)
+    pos = pos.cpu()
+    pos[:2] -= 7
+    pos[-2:] += 1000
+    pos[0] = -2 ** 31
+    pos[-1] = 2 ** 31 - 1
+    check(gpu, "%d rows" % rows, t, pos.cuda(), crd, block_m, 32, True)
+
+
+def test_scratch_that_is_not_on_a_boundary_is_refused(gpu):
+    import ctypes
+    x, lse = torch.full((1, 8, 1, 8), 7.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(8, device="cuda")
+    pos, work = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    a = block_args(batch=1, queries=8, keys=32, heads=1, kv_heads=1, dim=8, block_m=8, block_n=16, nnz=0, causal=0, dtype=0, scale=1.0, pos=pos, crd=pos,
+                   q=x, k=x, v=x, out=x, lse=lse, dout=x, dq=x, dk=x, dv=x)
+    gpu.init()
+    for at in (0, work.data_ptr() + 8):
+        a.work = at
+        with pytest.raises(gpu.LapisHipError, match="16-byte boundary"):
+            gpu.check(gpu.load().lapis_hip_block_attention_backward(ctypes.byref(a), None))
+    torch.cuda.synchronize()
+    assert bool((x == 7.0).all())
