@@ -434,9 +434,9 @@ int lapis_hip_normalize_mom2_f64(int64_t n, const double *mom1, const double *mo
  * reference multiplies with such a structure (the batched CSRV product of examples/bspmm.py:22-50, whose values
  * are finished attention weights); it has no counterpart of what follows.
  *
- * Types: 16-bit elements (bf16, f16); a cache may hold e4m3 codes with one fp32 scale per row of `dim`.  Sums,
- * softmax statistics and scales are fp32.  `dim` is a multiple of 8; 16-bit operands lie on 16-byte boundaries,
- * codes on 8-byte ones, strides (in elements) are multiples of 8.  Outputs must not overlap inputs.
+ * Types: 16-bit elements (bf16, f16); a cache may hold e4m3 codes with one fp32 scale per row of `dim`, or 4-bit codes
+ * (LAPIS_HIP_F4E2M1).  Sums, softmax statistics and scales are fp32.  `dim` is a multiple of 8; 16-bit operands lie on 16-byte
+ * boundaries, 8-bit codes on 8-byte ones, strides (in elements) are multiples of 8.  Outputs must not overlap inputs.
  * Structures: positions and coordinates int32.  A coordinate outside [0, columns) (of pages: outside [0, pages))
  * and positions outside [0, nnz] are never followed: such an entry counts as absent.  Coordinates need not ascend.
  * Positions do; where they descend nothing outside the operands is read or written, rows overlap and are taken as they stand, each
@@ -445,7 +445,7 @@ int lapis_hip_normalize_mom2_f64(int64_t n, const double *mom1, const double *mo
  * No entry point below allocates or synchronises: where scratch memory is needed the caller passes `work` of at least
  * the bytes the matching _work call says, on a 16-byte boundary. */
 
-enum lapis_hip_dtype { LAPIS_HIP_BF16 = 0, LAPIS_HIP_F16 = 1, LAPIS_HIP_F8E4M3 = 2 };
+enum lapis_hip_dtype { LAPIS_HIP_BF16 = 0, LAPIS_HIP_F16 = 1, LAPIS_HIP_F8E4M3 = 2, LAPIS_HIP_F4E2M1 = 3 };
 
 /* Rows of `dim` neighbouring elements: row (b, token, head) starts at data + b*stride[0] + token*stride[1] +
  * head*stride[2].  A stride may be 0 (a broadcast input). */
@@ -455,27 +455,63 @@ typedef struct lapis_hip_rows {
 } lapis_hip_rows;
 
 /* A cache of keys and values in pages: row (page, head, slot) of both starts at page*stride[0] + head*stride[1] +
- * slot*stride[2]; its scale (dtype LAPIS_HIP_F8E4M3 only) at page*scale_stride[0] + head*scale_stride[1] + slot*scale_stride[2]. */
+ * slot*stride[2]; its scale (8-bit and 4-bit codes only) at page*scale_stride[0] + head*scale_stride[1] + slot*scale_stride[2].
+ * LAPIS_HIP_F8E4M3: a scale is a float, of a whole row.
+ * LAPIS_HIP_F4E2M1: codes of 4 bits (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, the element of even
+ * number in the low half; dim and strides are counted in elements and are multiples of 32, buffers lie on 16-byte boundaries.  The scales of
+ * a row are dim / 32 neighbouring bytes, one for each 32 elements: byte b stands for 2^(b - 127), 255 for NaN. */
 typedef struct lapis_hip_kv_cache {
   void *k, *v;
-  float *k_scale, *v_scale;
+  void *k_scale, *v_scale; /* float or uint8_t */
   int64_t stride[3], scale_stride[3];
   int64_t pages;
   int32_t heads, page, dim; /* page = slots of a page, a power of two up to 1024; dim up to 256 */
-  int32_t dtype;            /* LAPIS_HIP_BF16, LAPIS_HIP_F16 or LAPIS_HIP_F8E4M3 */
+  int32_t dtype;            /* LAPIS_HIP_BF16, LAPIS_HIP_F16, LAPIS_HIP_F8E4M3 or LAPIS_HIP_F4E2M1 */
 } lapis_hip_kv_cache;
 
 /* Row t of k and v (stride[0] unused) goes to slot slots[t] (page * cache->page + place in the page) of every head;
  * a slot outside [0, pages * page) writes nothing.  Slots are distinct: of two tokens for one slot codes of one and the scale of the
  * other may stay.
  * With LAPIS_HIP_F8E4M3: scale = max|x| / 448 over the row, codes = x / scale rounded to nearest even; a row of zeros has
- * scale 0; a NaN stays NaN, a row with an infinity reads back as NaN.  `dtype` is the rows' own. */
+ * scale 0; a NaN stays NaN, a row with an infinity reads back as NaN.  `dtype` is the rows' own.
+ * With LAPIS_HIP_F4E2M1, for each 32 elements: scale = the smallest power of two from 2^-100 on with max|x| <= 6 * scale, codes = x / scale
+ * rounded to nearest even; 32 elements with an infinity or a NaN among them read back as NaN.  Magnitudes beyond the largest value that
+ * codes have in the rows' type (49152 in f16, 1.5 * 2^127 in bf16) are stored as that value. */
 int lapis_hip_kv_store(const lapis_hip_kv_cache *cache, int64_t tokens, const lapis_hip_rows *k, const lapis_hip_rows *v,
                        int dtype, const int32_t *slots, lapis_hip_stream_t stream);
 /* The way back: row t of k and v is what slot slots[t] holds (scale * code, rounded to `dtype`); zeros for a slot
  * outside [0, pages * page). */
 int lapis_hip_kv_load(const lapis_hip_kv_cache *cache, int64_t tokens, const int32_t *slots, const lapis_hip_rows *k,
                       const lapis_hip_rows *v, int dtype, lapis_hip_stream_t stream);
+
+/* How rows are turned by their positions.  Pair i of a row of token t is turned by the angle
+ *   sum over axes a of positions(a, b, t) * frequencies[a * pairs + i]   (radians, in 64 bits):
+ * (x, y) becomes (x cos - y sin, x sin + y cos), each product and sum rounded to 32 bits, the result to the row's type.  A pair is elements
+ * i and i + pairs, or with `neighbours` 2i and 2i + 1; elements from 2 * pairs on stay as they are.  Position (a, b, t) lies at
+ * a*position_stride[0] + b*position_stride[1] + t*position_stride[2] (a stride may be 0).  An axis that a pair does not follow has frequency 0 there. */
+typedef struct lapis_hip_rotation {
+  const int32_t *positions;
+  int64_t position_stride[3];
+  const double *frequencies; /* axes x pairs */
+  int32_t axes, pairs;       /* axes up to 8; 2 * pairs <= dim */
+  int32_t neighbours;
+} lapis_hip_rotation;
+
+/* Rows of x (batch x tokens x heads) turned into out; `inverse`: by the opposite angle, which is also the gradient of the call without.
+ * dim up to 256.  out may be x itself (the same address and strides). */
+int lapis_hip_rotate(int64_t batch, int64_t tokens, int64_t heads, int64_t dim, const lapis_hip_rotation *rotation, int inverse,
+                     const lapis_hip_rows *x, const lapis_hip_rows *out, int dtype, lapis_hip_stream_t stream);
+
+/* lapis_hip_rotate of q (tokens x q_heads, into q_out, which may be q) and of k, and lapis_hip_kv_store of the turned k and of v, in one
+ * launch: codes are made from the turned elements in 32 bits.  stride[0] of rows and position_stride[1] are unused; q_heads may be 0. */
+typedef struct lapis_hip_append_args {
+  int64_t tokens, q_heads;
+  lapis_hip_rotation rotation;
+  lapis_hip_rows k, v, q, q_out;
+  int dtype;
+  const int32_t *slots;
+} lapis_hip_append_args;
+int lapis_hip_kv_append(const lapis_hip_kv_cache *cache, const lapis_hip_append_args *args, lapis_hip_stream_t stream);
 
 /* One new token of each of `seqs` sequences: out(s, h) = sum_t softmax_t(scale * q(s, h) . k_t) v_t over the tokens of
  * the pages that a CSR row lists, in list order; of the last page only as many slots count as tokens[row] leaves.
@@ -495,6 +531,22 @@ typedef struct lapis_hip_paged_args {
 } lapis_hip_paged_args;
 int lapis_hip_paged_attention_work(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, int64_t *bytes);
 int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, lapis_hip_stream_t stream);
+
+/* One new token of each of `seqs` sequences, the last of lengths[s], over a window and the first tokens: token t counts where
+ * t < lengths[s] and (t >= lengths[s] - window or t < sink).  Token t lies in page table[s * table_width + t / cache->page], at place
+ * t % cache->page; tokens beyond the table do not exist, nor do those of an entry outside [0, pages), and entries of pages without a token
+ * that counts are not read.  window >= 1, sink >= 0; all else as in lapis_hip_paged_attention.  Fewer than 2^31 tokens in a table's row. */
+typedef struct lapis_hip_paged_window_args {
+  int64_t seqs, heads, table_width, window, sink;
+  lapis_hip_rows q, out;
+  int dtype;
+  const int32_t *table, *lengths;
+  float *lse;
+  float scale;
+  void *work;
+} lapis_hip_paged_window_args;
+int lapis_hip_paged_window_attention_work(const lapis_hip_kv_cache *cache, const lapis_hip_paged_window_args *args, int64_t *bytes);
+int lapis_hip_paged_window_attention(const lapis_hip_kv_cache *cache, const lapis_hip_paged_window_args *args, lapis_hip_stream_t stream);
 
 /* 8-bit means: codes(b, h, j, :) * scales(b, h, j) is the mean of x over the `block` tokens from j * block on (fewer at the
  * end) and the heads of group h (heads / groups consecutive ones).  scale = max|mean| / 127, codes = mean / scale rounded
@@ -555,6 +607,23 @@ int lapis_hip_block_attention(const lapis_hip_block_args *args, lapis_hip_stream
  * reach 8192; entries of fewer share it.  _work answers after lapis_hip_init: it goes by the number of compute units. */
 int lapis_hip_block_attention_backward_work(const lapis_hip_block_args *args, int64_t *bytes);
 int lapis_hip_block_attention_backward(const lapis_hip_block_args *args, lapis_hip_stream_t stream);
+
+/* out = softmax(scale * q k^T) v, and lse(b, head, query) = log sum exp of its scores, over a window and the first keys: query i stands
+ * at p = i + keys - queries and sees key j where j <= p and (j > p - window or j < sink).  window >= 1, sink >= 0; heads is a multiple of
+ * kv_heads, dim <= 128.  A query that sees nothing gives zeros, and -infinity as its lse.  lse may be NULL in the forward call. */
+typedef struct lapis_hip_window_args {
+  int64_t batch, queries, keys, heads, kv_heads, dim, window, sink;
+  int dtype;
+  float scale;
+  lapis_hip_rows q, k, v, out;
+  float *lse;
+  lapis_hip_rows dout, dq, dk, dv; /* backward only */
+  void *work;                      /* backward only */
+} lapis_hip_window_args;
+int lapis_hip_window_attention(const lapis_hip_window_args *args, lapis_hip_stream_t stream);
+/* Gradients of the forward call whose out and lse these are, as of lapis_hip_block_attention_backward; _work answers after lapis_hip_init. */
+int lapis_hip_window_attention_backward_work(const lapis_hip_window_args *args, int64_t *bytes);
+int lapis_hip_window_attention_backward(const lapis_hip_window_args *args, lapis_hip_stream_t stream);
 
 #ifdef __cplusplus
 }

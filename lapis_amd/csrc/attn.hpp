@@ -78,8 +78,6 @@ constexpr unsigned kInfBits = 0x7f800000u;
 constexpr int kMaxDim = 256;       // of the cache and its attention
 constexpr int kMaxBlockDim = 128;  // of block attention
 
-int check_cache(const char *what, const lapis_hip_kv_cache *cache);
-
 inline bool is_16bit(int dtype) { return dtype == LAPIS_HIP_BF16 || dtype == LAPIS_HIP_F16; }
 inline bool strides_of_8(const int64_t *s, int n) {
   for (int i = 0; i < n; ++i)

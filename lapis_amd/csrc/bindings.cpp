@@ -731,40 +731,48 @@ struct Scratch {
   void *data() const { return held.defined() ? held.data_ptr() : nullptr; }
 };
 
-// k_cache, v_cache (pages, heads, slots of a page, dim) and their scales (pages, heads, slots) or None
+// k_cache, v_cache (pages, heads, slots of a page, dim) and their scales (pages, heads, slots) or None; with 4 bits (uint8) two elements to a
+// byte, scales (pages, heads, slots, dim / 32)
 lapis_hip_kv_cache cache_of(const char *what, PyObject *k, PyObject *v, PyObject *ks, PyObject *vs, bool output) {
   const at::Tensor &kt = tensor(what, "k_cache", k, 4), &vt = tensor(what, "v_cache", v, 4);
   lapis_hip_kv_cache c = {};
-  c.dtype = type_code(what, "k_cache", kt, true);
+  const bool f4 = kt.scalar_type() == at::kByte;
+  c.dtype = f4 ? LAPIS_HIP_F4E2M1 : type_code(what, "k_cache", kt, true);
   of_type(what, "v_cache", vt, kt.scalar_type());
   of_shape(what, "v_cache", vt, {kt.size(0), kt.size(1), kt.size(2), kt.size(3)});
   for (const at::Tensor *t : {&kt, &vt}) {
     dense_rows(what, t == &kt ? "k_cache" : "v_cache", *t);
     if (output) no_overlap(what, t == &kt ? "k_cache" : "v_cache", *t);
   }
+  const int64_t each = f4 ? 2 : 1;  // elements of an element of the tensor
   for (int i = 0; i < 3; ++i) {
-    c.stride[i] = stride_of(kt, i);
-    if (stride_of(vt, i) != c.stride[i]) raise(PyExc_ValueError, "%s: k_cache and v_cache have different strides", what);
+    c.stride[i] = each * stride_of(kt, i);
+    if (each * stride_of(vt, i) != c.stride[i]) raise(PyExc_ValueError, "%s: k_cache and v_cache have different strides", what);
   }
-  if (kt.size(1) > INT32_MAX || kt.size(2) > INT32_MAX || kt.size(3) > INT32_MAX) raise(PyExc_ValueError, "%s: a cache too large", what);
+  if (kt.size(1) > INT32_MAX || kt.size(2) > INT32_MAX || kt.size(3) > INT32_MAX / 2) raise(PyExc_ValueError, "%s: a cache too large", what);
   c.k = kt.data_ptr();
   c.v = vt.data_ptr();
   c.pages = kt.size(0);
   c.heads = (int32_t)kt.size(1);
   c.page = (int32_t)kt.size(2);
-  c.dim = (int32_t)kt.size(3);
-  const bool f8 = c.dtype == LAPIS_HIP_F8E4M3;
-  if (!f8) {
+  c.dim = (int32_t)(each * kt.size(3));
+  if (!f4 && c.dtype != LAPIS_HIP_F8E4M3) {
     if (ks != Py_None || vs != Py_None) raise(PyExc_ValueError, "%s: scales with a cache of %s", what, type_name(kt.scalar_type()));
     return c;
   }
+  if (f4 && c.dim % 32 != 0) raise(PyExc_ValueError, "%s: rows of %d elements in 4 bits, a multiple of 32 expected", what, (int)c.dim);
   for (int i = 0; i < 2; ++i) {
     const char *name = i ? "v_scale" : "k_scale";
-    const at::Tensor &t = tensor(what, name, i ? vs : ks, 3);
-    of_type(what, name, t, at::kFloat);
-    of_shape(what, name, t, {kt.size(0), kt.size(1), kt.size(2)});
+    const at::Tensor &t = tensor(what, name, i ? vs : ks, f4 ? 4 : 3);
+    of_type(what, name, t, f4 ? at::kByte : at::kFloat);
+    if (f4) {
+      of_shape(what, name, t, {kt.size(0), kt.size(1), kt.size(2), c.dim / 32});
+      dense_rows(what, name, t);
+    } else {
+      of_shape(what, name, t, {kt.size(0), kt.size(1), kt.size(2)});
+    }
     if (output) no_overlap(what, name, t);
-    (i ? c.v_scale : c.k_scale) = static_cast<float *>(t.data_ptr());
+    (i ? c.v_scale : c.k_scale) = t.data_ptr();
     for (int j = 0; j < 3; ++j) {
       if (i && c.scale_stride[j] != stride_of(t, j)) raise(PyExc_ValueError, "%s: k_scale and v_scale have different strides", what);
       c.scale_stride[j] = stride_of(t, j);
@@ -772,6 +780,9 @@ lapis_hip_kv_cache cache_of(const char *what, PyObject *k, PyObject *v, PyObject
   }
   return c;
 }
+
+// Whether rows or queries of `dtype` go with this cache.
+bool goes_with(const lapis_hip_kv_cache &c, int dtype) { return c.dtype == dtype || c.dtype == LAPIS_HIP_F8E4M3 || c.dtype == LAPIS_HIP_F4E2M1; }
 
 // store (k, v, slots, k_cache, v_cache, k_scale, v_scale, stream), load (k_cache, v_cache, slots, k, v, k_scale, v_scale, stream)
 PyObject *kv_move(const char *what, bool store, PyObject *const *a, Py_ssize_t n) {
@@ -782,7 +793,7 @@ PyObject *kv_move(const char *what, bool store, PyObject *const *a, Py_ssize_t n
     const at::Tensor &k = tensor(what, "k", rows[0], 3), &v = tensor(what, "v", rows[1], 3), &slots = tensor(what, "slots", a[2], 1);
     const int dtype = type_code(what, "k", k);
     of_type(what, "v", v, k.scalar_type());
-    if (c.dtype != LAPIS_HIP_F8E4M3 && c.dtype != dtype) raise(PyExc_TypeError, "%s: rows of %s and a cache of another 16-bit type", what, type_name(k.scalar_type()));
+    if (!goes_with(c, dtype)) raise(PyExc_TypeError, "%s: rows of %s and a cache of another 16-bit type", what, type_name(k.scalar_type()));
     of_shape(what, "k", k, {k.size(0), c.heads, c.dim});
     of_shape(what, "v", v, {k.size(0), c.heads, c.dim});
     of_type(what, "slots", slots, at::kInt);
@@ -813,7 +824,7 @@ LAPIS_PY(py_paged_attention) {
                      &tokens = tensor(what, "tokens", a[5], 1), &out = tensor(what, "out", a[6], 3);
     lapis_hip_paged_args p = {};
     p.dtype = type_code(what, "q", q);
-    if (c.dtype != LAPIS_HIP_F8E4M3 && c.dtype != p.dtype) raise(PyExc_TypeError, "%s: queries of %s and a cache of another 16-bit type", what, type_name(q.scalar_type()));
+    if (!goes_with(c, p.dtype)) raise(PyExc_TypeError, "%s: queries of %s and a cache of another 16-bit type", what, type_name(q.scalar_type()));
     of_shape(what, "q", q, {q.size(0), q.size(1), c.dim});
     of_type(what, "out", out, q.scalar_type());
     of_shape(what, "out", out, {q.size(0), q.size(1), c.dim});
@@ -851,6 +862,159 @@ LAPIS_PY(py_paged_attention) {
     check(lapis_hip_paged_attention(&c, &p, st));
     written({a[6], a[7]});
     return give(a[6]);
+  });
+}
+
+// The kernels run on the current device, on its streams.
+void on_current_device(const char *what, PyObject *const *a, Py_ssize_t n) {
+  on_device(what, a, n);
+  const auto current = c10::hip::getCurrentHIPStream().device_index();
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).device().index() != current)
+      raise(PyExc_ValueError, "%s: operands on device %d, the current one is %d", what, (int)THPVariable_Unpack(a[i]).device().index(), (int)current);
+}
+
+// (q, k_cache, v_cache, table, lengths, out, window, sink, lse, scale, k_scale, v_scale, stream)
+LAPIS_PY(py_paged_window_attention) {
+  return guarded([&] {
+    const char *what = "paged_window_attention";
+    arguments(what, n, 13);
+    const lapis_hip_kv_cache c = cache_of(what, a[1], a[2], a[10], a[11], false);
+    const at::Tensor &q = tensor(what, "q", a[0], 3), &table = tensor(what, "table", a[3], 2), &lengths = tensor(what, "lengths", a[4], 1),
+                     &out = tensor(what, "out", a[5], 3);
+    lapis_hip_paged_window_args p = {};
+    p.dtype = type_code(what, "q", q);
+    if (!goes_with(c, p.dtype)) raise(PyExc_TypeError, "%s: queries of %s and a cache of another 16-bit type", what, type_name(q.scalar_type()));
+    of_shape(what, "q", q, {q.size(0), q.size(1), c.dim});
+    of_type(what, "out", out, q.scalar_type());
+    of_shape(what, "out", out, {q.size(0), q.size(1), c.dim});
+    p.seqs = q.size(0);
+    p.heads = q.size(1);
+    of_type(what, "table", table, at::kInt);
+    of_type(what, "lengths", lengths, at::kInt);
+    of_shape(what, "table", table, {p.seqs, table.size(1)});
+    of_shape(what, "lengths", lengths, {p.seqs});
+    contiguous(what, "table", table);
+    contiguous(what, "lengths", lengths);
+    p.table_width = table.size(1);
+    p.window = integer(a[6]);
+    p.sink = integer(a[7]);
+    if (p.window < 1 || p.sink < 0) raise(PyExc_ValueError, "%s: a window of %lld and the first %lld tokens", what, (long long)p.window, (long long)p.sink);
+    p.q = rows_of(what, "q", q, false);
+    p.out = rows_of(what, "out", out, true);
+    for (lapis_hip_rows *r : {&p.q, &p.out}) r->stride[0] = r->stride[1];  // (sequence, head)
+    p.table = static_cast<const int32_t *>(table.data_ptr());
+    p.lengths = static_cast<const int32_t *>(lengths.data_ptr());
+    if (a[8] != Py_None) {
+      const at::Tensor &lse = tensor(what, "lse", a[8], 2);
+      of_type(what, "lse", lse, at::kFloat);
+      of_shape(what, "lse", lse, {p.seqs, p.heads});
+      contiguous(what, "lse", lse);
+      p.lse = static_cast<float *>(lse.data_ptr());
+    }
+    p.scale = a[9] == Py_None ? 1.0f / std::sqrt((float)c.dim) : (float)number(a[9]);
+    on_current_device(what, a, n);
+    const lapis_hip_stream_t st = stream_of(a[12]);
+    int64_t bytes = 0;
+    check(lapis_hip_paged_window_attention_work(&c, &p, &bytes));
+    const Scratch work(bytes, st);
+    p.work = work.data();
+    check(lapis_hip_paged_window_attention(&c, &p, st));
+    written({a[5], a[8]});
+    return give(a[5]);
+  });
+}
+
+// positions (axes, tokens) or (axes, batch, tokens), frequencies (axes, pairs), neighbours
+lapis_hip_rotation rotation_of(const char *what, PyObject *positions, PyObject *frequencies, PyObject *neighbours, bool batched) {
+  const at::Tensor &p = tensor(what, "positions", positions, batched ? 3 : 2), &f = tensor(what, "frequencies", frequencies, 2);
+  of_type(what, "positions", p, at::kInt);
+  of_type(what, "frequencies", f, at::kDouble);
+  contiguous(what, "frequencies", f);
+  of_shape(what, "frequencies", f, {p.size(0), f.size(1)});
+  if (f.size(0) > INT32_MAX || f.size(1) > INT32_MAX) raise(PyExc_ValueError, "%s: too many frequencies", what);
+  lapis_hip_rotation r = {};
+  r.positions = static_cast<const int32_t *>(p.data_ptr());
+  r.position_stride[0] = stride_of(p, 0);
+  if (batched) r.position_stride[1] = stride_of(p, 1);
+  r.position_stride[2] = stride_of(p, batched ? 2 : 1);
+  r.frequencies = static_cast<const double *>(f.data_ptr());
+  r.axes = (int32_t)f.size(0);
+  r.pairs = (int32_t)f.size(1);
+  r.neighbours = truth(neighbours);
+  return r;
+}
+
+// An output may be its input: the same rows, or none of them.
+void same_or_apart(const char *what, const char *name, const at::Tensor &in, const at::Tensor &out) {
+  if (in.data_ptr() != out.data_ptr() || in.numel() == 0) return;
+  for (int64_t i = 0; i < in.dim(); ++i)
+    if (stride_of(in, i) != stride_of(out, i)) raise(PyExc_ValueError, "%s: %s lies over its input in another order", what, name);
+}
+
+// (x, positions, frequencies, out, neighbours, inverse, stream)
+LAPIS_PY(py_rotate) {
+  return guarded([&] {
+    const char *what = "rotate";
+    arguments(what, n, 7);
+    const at::Tensor &x = tensor(what, "x", a[0], 4), &out = tensor(what, "out", a[3], 4);
+    const int dtype = type_code(what, "x", x);
+    of_type(what, "out", out, x.scalar_type());
+    of_shape(what, "out", out, {x.size(0), x.size(1), x.size(2), x.size(3)});
+    const lapis_hip_rotation r = rotation_of(what, a[1], a[2], a[4], true);
+    const at::Tensor &positions = THPVariable_Unpack(a[1]);
+    of_shape(what, "positions", positions, {positions.size(0), x.size(0), x.size(1)});
+    const int inverse = truth(a[5]);
+    const lapis_hip_rows from = rows_of(what, "x", x, false), to = rows_of(what, "out", out, true);
+    same_or_apart(what, "out", x, out);
+    on_current_device(what, a, n);
+    check(lapis_hip_rotate(x.size(0), x.size(1), x.size(2), x.size(3), &r, inverse, &from, &to, dtype, stream_of(a[6])));
+    written({a[3]});
+    return give(a[3]);
+  });
+}
+
+// (k, v, positions, frequencies, slots, k_cache, v_cache, k_scale, v_scale, q, q_out, neighbours, stream)
+LAPIS_PY(py_kv_append) {
+  return guarded([&] {
+    const char *what = "kv_append";
+    arguments(what, n, 13);
+    const lapis_hip_kv_cache c = cache_of(what, a[5], a[6], a[7], a[8], true);
+    const at::Tensor &k = tensor(what, "k", a[0], 3), &v = tensor(what, "v", a[1], 3), &slots = tensor(what, "slots", a[4], 1);
+    lapis_hip_append_args p = {};
+    p.dtype = type_code(what, "k", k);
+    of_type(what, "v", v, k.scalar_type());
+    if (!goes_with(c, p.dtype)) raise(PyExc_TypeError, "%s: rows of %s and a cache of another 16-bit type", what, type_name(k.scalar_type()));
+    p.tokens = k.size(0);
+    of_shape(what, "k", k, {p.tokens, c.heads, c.dim});
+    of_shape(what, "v", v, {p.tokens, c.heads, c.dim});
+    of_type(what, "slots", slots, at::kInt);
+    of_shape(what, "slots", slots, {p.tokens});
+    contiguous(what, "slots", slots);
+    p.rotation = rotation_of(what, a[2], a[3], a[11], false);
+    const at::Tensor &positions = THPVariable_Unpack(a[2]);
+    of_shape(what, "positions", positions, {positions.size(0), p.tokens});
+    p.k = rows_of(what, "k", k, false);
+    p.v = rows_of(what, "v", v, false);
+    p.slots = static_cast<const int32_t *>(slots.data_ptr());
+    if ((a[9] == Py_None) != (a[10] == Py_None)) raise(PyExc_TypeError, "%s: q and q_out come together", what);
+    if (a[9] != Py_None) {
+      const at::Tensor &q = tensor(what, "q", a[9], 3), &out = tensor(what, "q_out", a[10], 3);
+      p.q_heads = q.size(1);
+      for (const at::Tensor *t : {&q, &out}) {
+        of_type(what, t == &q ? "q" : "q_out", *t, k.scalar_type());
+        of_shape(what, t == &q ? "q" : "q_out", *t, {p.tokens, p.q_heads, c.dim});
+      }
+      p.q = rows_of(what, "q", q, false);
+      p.q_out = rows_of(what, "q_out", out, true);
+      same_or_apart(what, "q_out", q, out);
+    }
+    on_current_device(what, a, n);
+    check(lapis_hip_kv_append(&c, &p, stream_of(a[12])));
+    written({a[5], a[6], a[7], a[8], a[10]});
+    PyObject *result = PyTuple_Pack(2, a[5], a[6]);
+    if (!result) throw Raised();
+    return result;
   });
 }
 
@@ -1062,6 +1226,92 @@ LAPIS_PY(py_block_attention_backward) {
   });
 }
 
+// q, k, v, out, lse (None allowed with `forward`), window, sink, scale
+lapis_hip_window_args window_of(const char *what, PyObject *q_, PyObject *k_, PyObject *v_, PyObject *out_, PyObject *lse_, bool forward, PyObject *window,
+                                PyObject *sink, PyObject *scale) {
+  const at::Tensor &q = tensor(what, "q", q_, 4), &k = tensor(what, "k", k_, 4), &v = tensor(what, "v", v_, 4), &out = tensor(what, "out", out_, 4);
+  lapis_hip_window_args p = {};
+  p.dtype = type_code(what, "q", q);
+  p.batch = q.size(0);
+  p.queries = q.size(1);
+  p.heads = q.size(2);
+  p.dim = q.size(3);
+  p.keys = k.size(1);
+  p.kv_heads = k.size(2);
+  of_type(what, "k", k, q.scalar_type());
+  of_type(what, "v", v, q.scalar_type());
+  of_type(what, "out", out, q.scalar_type());
+  of_shape(what, "k", k, {p.batch, p.keys, p.kv_heads, p.dim});
+  of_shape(what, "v", v, {p.batch, p.keys, p.kv_heads, p.dim});
+  of_shape(what, "out", out, {p.batch, p.queries, p.heads, p.dim});
+  p.window = integer(window);
+  p.sink = integer(sink);
+  if (p.window < 1 || p.sink < 0) raise(PyExc_ValueError, "%s: a window of %lld and the first %lld keys", what, (long long)p.window, (long long)p.sink);
+  if (p.kv_heads < 1 || p.heads % p.kv_heads != 0) raise(PyExc_ValueError, "%s: %lld heads over %lld key-value heads", what, (long long)p.heads, (long long)p.kv_heads);
+  if (lse_ != Py_None || !forward) {
+    const at::Tensor &lse = tensor(what, "lse", lse_, 3);
+    of_type(what, "lse", lse, at::kFloat);
+    of_shape(what, "lse", lse, {p.batch, p.heads, p.queries});
+    contiguous(what, "lse", lse);
+    p.lse = static_cast<float *>(lse.data_ptr());
+  }
+  p.q = rows_of(what, "q", q, false);
+  p.k = rows_of(what, "k", k, false);
+  p.v = rows_of(what, "v", v, false);
+  p.out = rows_of(what, "out", out, forward);
+  p.scale = scale == Py_None ? 1.0f / std::sqrt((float)p.dim) : (float)number(scale);
+  return p;
+}
+
+// (q, k, v, out, window, sink, lse, scale, stream)
+LAPIS_PY(py_window_attention) {
+  return guarded([&] {
+    const char *what = "window_attention";
+    arguments(what, n, 9);
+    const lapis_hip_window_args p = window_of(what, a[0], a[1], a[2], a[3], a[6], true, a[4], a[5], a[7]);
+    on_current_device(what, a, n);
+    check(lapis_hip_window_attention(&p, stream_of(a[8])));
+    written({a[3], a[6]});
+    PyObject *result = PyTuple_Pack(2, a[3], a[6]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+
+// (dout, q, k, v, out, lse, dq, dk, dv, window, sink, scale, stream)
+LAPIS_PY(py_window_attention_backward) {
+  return guarded([&] {
+    const char *what = "window_attention_backward";
+    arguments(what, n, 13);
+    lapis_hip_window_args p = window_of(what, a[1], a[2], a[3], a[4], a[5], false, a[9], a[10], a[11]);
+    const at::ScalarType type = THPVariable_Unpack(a[1]).scalar_type();
+    const struct {
+      const char *name;
+      PyObject *o;
+      lapis_hip_rows *to;
+      bool queries, output;
+    } more[] = {{"dout", a[0], &p.dout, true, false}, {"dq", a[6], &p.dq, true, true}, {"dk", a[7], &p.dk, false, true}, {"dv", a[8], &p.dv, false, true}};
+    for (const auto &m : more) {
+      const at::Tensor &t = tensor(what, m.name, m.o, 4);
+      of_type(what, m.name, t, type);
+      if (m.queries) of_shape(what, m.name, t, {p.batch, p.queries, p.heads, p.dim});
+      else of_shape(what, m.name, t, {p.batch, p.keys, p.kv_heads, p.dim});
+      *m.to = rows_of(what, m.name, t, m.output);
+    }
+    on_current_device(what, a, n);
+    const lapis_hip_stream_t st = stream_of(a[12]);
+    int64_t bytes = 0;
+    check(lapis_hip_window_attention_backward_work(&p, &bytes));
+    const Scratch work(bytes, st);
+    p.work = work.data();
+    check(lapis_hip_window_attention_backward(&p, st));
+    written({a[6], a[7], a[8]});
+    PyObject *result = PyTuple_Pack(3, a[6], a[7], a[8]);
+    if (!result) throw Raised();
+    return result;
+  });
+}
+
 // setup(check, init)
 PyObject *py_setup(PyObject *, PyObject *args) {
   PyObject *check_fn, *init_fn;
@@ -1081,6 +1331,8 @@ PyMethodDef g_methods[] = {LAPIS_METHOD(spmv), LAPIS_METHOD(spmm), LAPIS_METHOD(
                            LAPIS_METHOD(dot_finish), LAPIS_METHOD(stage), LAPIS_METHOD(staged_plan), LAPIS_METHOD(fetch),
                            LAPIS_METHOD(kv_store), LAPIS_METHOD(kv_load), LAPIS_METHOD(paged_attention), LAPIS_METHOD(block_pool),
                            LAPIS_METHOD(block_select), LAPIS_METHOD(block_attention), LAPIS_METHOD(block_attention_backward),
+                           LAPIS_METHOD(rotate), LAPIS_METHOD(kv_append), LAPIS_METHOD(paged_window_attention),
+                           LAPIS_METHOD(window_attention), LAPIS_METHOD(window_attention_backward),
                            {"setup", py_setup, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_lapis_calls", "Device-resident calls of the gfx950 kernel library.", -1,
                         g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,4 +1,4 @@
-// Attention over the blocks that a CSR structure lists, forward.
+// Attention over the blocks that a CSR structure lists, or over a window and the first keys, forward.
 #include "blockattn.hpp"
 
 namespace lapis {
@@ -18,7 +18,7 @@ __device__ __forceinline__ float units_of_ln2(float scale) {
 // between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
 // 32 768 queries and keys, 32 heads over 8, dim 128, 16 blocks of 128 a row, bf16: 1290 to 1350 us, 800 to 765 TFLOP/s where a large library
 // product reaches 1203.  Bound by issue: 72 % of the cycles issue something, vector instructions 41 %, products 32 %.
-template <typename T, int DP, int NW, int KT>
+template <typename T, int DP, int NW, int KT, bool WINDOW>
 __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
@@ -30,8 +30,8 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   const int bh = list / a.rows, r = list - bh * a.rows, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const int q0 = r * a.block_m, held = min(a.block_m, a.queries - q0), rows = held * a.group;
   if (part * 32 * NW >= rows) return;  // the last block of queries is cut
-  int first, count;
-  entries_of(a, list, &first, &count);
+  int first = 0, count = 0;
+  if (!WINDOW) entries_of(a, list, &first, &count);
 
   const int row0 = part * 32 * NW + wave * 32, row = row0 + (lane & 31);
   const bool live = row < rows;
@@ -41,6 +41,9 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   const int low = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row0 / a.group + a.shift, a.keys - 1) : a.keys - 1);
   const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
   const int low_of_all = a.causal ? min(q0 + part * 32 * NW / a.group + a.shift, a.keys - 1) : a.keys - 1;
+  const int row_last_of_all = min(part * 32 * NW + 32 * NW, rows) - 1;
+  const int gone = limit - a.window;  // last key before this row's window
+  const int gone_any = high - a.window, gone_any_of_all = q0 + row_last_of_all / a.group + a.shift - a.window;
 
   vec8<T> qf[DP / 16];
   const elem *qp = (const elem *)a.q.data + b * a.q.stride[0] + query * a.q.stride[1] + head * a.q.stride[2];
@@ -51,7 +54,8 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     if (live && d < a.dim) x = *(const v4i *)(qp + d);
     qf[s] = __builtin_bit_cast(vec8<T>, x ^ flip);
   }
-  const KeyTiles<T, DP, NW, KT, true> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  KeyTiles<T, DP, NW, KT, true, WINDOW> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  if (WINDOW) keys.span = span_of(a, q0, held);
   const int tiles = keys.tiles();
   v4i now, next;  // first keys of each sixteen of this tile and the next
 
@@ -85,7 +89,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
-    if (top + 15 > low_of_all) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
+    if (top + 15 > low_of_all || (WINDOW && lowest <= gone_any_of_all)) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
       bool bad = false;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(v_tile[buffer] + (p * NW * 64 + tid) * 8));
@@ -104,14 +108,14 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
           s[x] = mfma32(kf, qf[y], s[x]);
         }
       }
-      const bool cut = top + 15 > low;
+      const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
       if (cut) {
 #pragma unroll
         for (int x = 0; x < ST; ++x)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = now[2 * x + (e >> 3)] + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
-            if (key > limit) s[x][e] = -INFINITY;
+            if (key > limit || (WINDOW && key <= gone && key >= a.sink)) s[x][e] = -INFINITY;
           }
       }
       float best = s[0][0];
@@ -158,7 +162,8 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
           int key0 = now[0];
 #pragma unroll
           for (int i = 1; i < CH; ++i) key0 = x >> 4 == i ? now[i] : key0;
-          const bool sees = key0 + (x & 15) <= limit;
+          const int key = key0 + (x & 15);
+          const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
 #pragma unroll
           for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -209,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
 // row per lane), V through LDS, where it is read by columns, 32 keys at a time, the next ones loaded as soon as the
 // registers are free.  SPLIT wavefronts share the keys of one list, by tiles in turn, and join through LDS.
 // 4096 queries, 16 heads each over 16 blocks of 32 of their own, dim 64, f16: 82 us; 1.07 GB of keys and values out of L2 at 13 TB/s.
-template <typename T, int DP, int SPLIT>
+template <typename T, int DP, int SPLIT, bool WINDOW>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
   constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8, RP = 64 / PIECES, PASSES = 32 / RP;
@@ -228,7 +233,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
   const int bh = any ? list / a.rows : 0, r = any ? list - bh * a.rows : 0, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const int q0 = r * a.block_m, rows = min(a.block_m, a.queries - q0) * a.group;
   int first = 0, count = 0;
-  if (any && part * 16 < rows) entries_of(a, list, &first, &count);
+  Span span = {};
+  if (any && part * 16 < rows) {
+    if constexpr (WINDOW) span = span_of(a, q0, min(a.block_m, a.queries - q0));
+    else entries_of(a, list, &first, &count);
+  }
   const int row0 = part * 16, row = row0 + col, row_last = min(row0 + 15, rows - 1);
   const bool live = any && row < rows;
   const int query = q0 + row / a.group, head = kh * a.group + row % a.group;
@@ -247,7 +256,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
   }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  const int tiles = tiles_of<32>(a, count);
+  const int gone = limit - a.window, gone_any = high - a.window;  // last key before this row's window, and any row's
+  const int tiles = WINDOW ? (span.count + 1) / 2 : tiles_of<32>(a, count);
   const int piece = lane % PIECES, v_row = lane / PIECES, vd = piece * 8 < a.dim ? piece * 8 : 0;
   v4i kr[2][KS], vr[PASSES];
   const auto load = [&](const int (&key0)[2]) {
@@ -266,7 +276,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
         vr[p] = *(const v4i *)(vp + from * a.v.stride[1] + min((p * RP & 15) + v_row, room) * a.v.stride[1] + vd);
     }
   };
-  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, 32ll * t + 16 * (lane & 1)) : kAbsent; };
+  const auto look_up = [&](int t) {
+    if constexpr (WINDOW) return span.first_key(2 * t + (lane & 1));
+    return tiles > 0 ? first_key(a, first, count, 32ll * t + 16 * (lane & 1)) : kAbsent;
+  };
 
   v4f acc[DT];
 #pragma unroll
@@ -287,7 +300,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
 #pragma unroll
       for (int x = 0; x < KS; ++x) s[i] = mfma16(__builtin_bit_cast(vec8<T>, kr[i][x]), qf[x], s[i]);
     }
-    const bool cut = max(now[0], now[1]) + 15 > low, skip = min(now[0], now[1]) > high;
+    const bool cut = max(now[0], now[1]) + 15 > low || (WINDOW && min(now[0], now[1]) <= gone_any), skip = min(now[0], now[1]) > high;
     bool bad = false;
     if (cut) {  // 0 times an infinity or NaN must not count
 #pragma unroll
@@ -308,7 +321,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (cut && now[i] + 4 * quarter + e > limit) s[i][e] = -INFINITY;
+        const int key = now[i] + 4 * quarter + e;
+        if (cut && (key > limit || (WINDOW && key <= gone && key >= a.sink))) s[i][e] = -INFINITY;
         best = fmaxf(best, s[i][e]);
       }
     best = rows_max(best) * c;
@@ -341,7 +355,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
     if (bad)  // an infinity or NaN only to the rows that see its key
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {
-        const bool sees = (x < 16 ? now[0] : now[1]) + (x & 15) <= limit;
+        const int key = (x < 16 ? now[0] : now[1]) + (x & 15);
+        const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
           const int d = 16 * i + 4 * quarter;
@@ -394,22 +409,22 @@ int read_view(const char *what, const lapis_hip_rows &r, View *v) {
   return LAPIS_HIP_OK;
 }
 
-template <typename T, int DP, int NW, int KT>
+template <typename T, int DP, int NW, int KT, bool WINDOW>
 int launch_wide(const BlockArgs &a, hipStream_t st) {
   const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)std::min(a.block_m, a.queries) * a.group, 32 * NW);
   LAPIS_REQUIRE(lists * tiles * 64 * NW < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
-  hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT>), dim3((unsigned)(lists * tiles)), dim3(64 * NW), 0, st, a, (int)tiles,
+  hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT, WINDOW>), dim3((unsigned)(lists * tiles)), dim3(64 * NW), 0, st, a, (int)tiles,
                      a.scale < 0.f ? (int)0x80008000u : 0);
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
 }
 
-template <typename T, int DP, int SPLIT>
+template <typename T, int DP, int SPLIT, bool WINDOW>
 int launch_narrow(const BlockArgs &a, hipStream_t st) {
   const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)a.block_m * a.group, 16);
   const long long blocks = ceil_div(lists * tiles * SPLIT, 4);
   LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
-  hipLaunchKernelGGL((block_narrow_kernel<T, DP, SPLIT>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, a.scale < 0.f ? (int)0x80008000u : 0);
+  hipLaunchKernelGGL((block_narrow_kernel<T, DP, SPLIT, WINDOW>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, a.scale < 0.f ? (int)0x80008000u : 0);
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
 }
@@ -422,10 +437,21 @@ int launch_forward(const BlockArgs &a, hipStream_t st) {
   const int64_t rows = (int64_t)a.block_m * a.group, lists = (int64_t)a.batch * a.kv_heads * a.rows, waves = ceil_div(rows, 16) * lists;
   if (rows <= 32 || ceil_div(rows, 128) * lists < device_cu_count() / 2) {
     const bool many = waves >= 8 * device_cu_count();  // two wavefronts a SIMD without sharing lists
-    if (a.dim <= 64) return many ? launch_narrow<T, 64, 1>(a, st) : launch_narrow<T, 64, 4>(a, st);
-    return many ? launch_narrow<T, 128, 1>(a, st) : launch_narrow<T, 128, 4>(a, st);
+    if (a.dim <= 64) return many ? launch_narrow<T, 64, 1, false>(a, st) : launch_narrow<T, 64, 4, false>(a, st);
+    return many ? launch_narrow<T, 128, 1, false>(a, st) : launch_narrow<T, 128, 4, false>(a, st);
   }
-  return a.dim <= 64 ? launch_wide<T, 64, 4, 64>(a, st) : launch_wide<T, 128, 4, 64>(a, st);
+  return a.dim <= 64 ? launch_wide<T, 64, 4, 64, false>(a, st) : launch_wide<T, 128, 4, 64, false>(a, st);
+}
+
+template <typename T>
+int launch_window(BlockArgs a, hipStream_t st) {
+  cut_queries(&a, 128);
+  // the same rule
+  if ((int64_t)a.batch * a.kv_heads * a.rows * ceil_div(a.block_m * a.group, 128) < device_cu_count() / 2) {
+    cut_queries(&a, 16);
+    return a.dim <= 64 ? launch_narrow<T, 64, 4, true>(a, st) : launch_narrow<T, 128, 4, true>(a, st);
+  }
+  return a.dim <= 64 ? launch_wide<T, 64, 4, 64, true>(a, st) : launch_wide<T, 128, 4, 64, true>(a, st);
 }
 
 }  // namespace
@@ -486,6 +512,26 @@ int read_block(const char *what, const lapis_hip_block_args *p, bool backward, B
   return rc;
 }
 
+int read_window(const char *what, const lapis_hip_window_args *p, bool backward, BlockArgs *a) {
+  LAPIS_REQUIRE(p, "%s: null arguments", what);
+  LAPIS_REQUIRE(p->window >= 1 && p->sink >= 0, "%s: a window of %lld and the first %lld keys", what, (long long)p->window, (long long)p->sink);
+  static const int32_t none = 0;  // of lists, which are not looked at
+  lapis_hip_block_args b = {};
+  b.batch = p->batch, b.queries = p->queries, b.keys = p->keys, b.heads = p->heads, b.kv_heads = p->kv_heads, b.dim = p->dim;
+  b.block_m = 1, b.block_n = 64;
+  b.causal = 1, b.dtype = p->dtype, b.scale = p->scale;
+  b.pos = b.crd = &none;
+  b.q = p->q, b.k = p->k, b.v = p->v, b.out = p->out, b.lse = p->lse;
+  b.dout = p->dout, b.dq = p->dq, b.dk = p->dk, b.dv = p->dv;
+  const int rc = read_block(what, &b, backward, a);
+  a->pos = a->crd = nullptr;
+  if (p->heads == 0) a->queries = 0;  // queries without a head are no rows: nothing of q is there to be read
+  // positions, and what is taken from them, stay within 32 bits
+  a->window = (int)std::min<int64_t>(p->window, 1 << 30);
+  a->sink = (int)std::min<int64_t>(p->sink, 1 << 30);
+  return rc;
+}
+
 }  // namespace lapis
 
 using namespace lapis;
@@ -497,4 +543,13 @@ extern "C" int lapis_hip_block_attention(const lapis_hip_block_args *args, lapis
   if (rc != LAPIS_HIP_OK) return rc;
   if (a.batch == 0 || a.queries == 0 || a.heads == 0) return LAPIS_HIP_OK;
   return args->dtype == LAPIS_HIP_BF16 ? launch_forward<Bf16>(a, as_stream(stream)) : launch_forward<F16>(a, as_stream(stream));
+}
+
+extern "C" int lapis_hip_window_attention(const lapis_hip_window_args *args, lapis_hip_stream_t stream) {
+  LAPIS_CHECK_INIT();
+  BlockArgs a;
+  const int rc = read_window("window_attention", args, false, &a);
+  if (rc != LAPIS_HIP_OK) return rc;
+  if (a.batch == 0 || a.queries == 0 || a.heads == 0) return LAPIS_HIP_OK;
+  return args->dtype == LAPIS_HIP_BF16 ? launch_window<Bf16>(a, as_stream(stream)) : launch_window<F16>(a, as_stream(stream));
 }

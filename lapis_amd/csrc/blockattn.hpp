@@ -1,4 +1,4 @@
-// What the forward and backward kernels of block-sparse attention are given.
+// What the forward and backward kernels of attention over lists of blocks and over windows are given.
 #pragma once
 #include "mfma.hpp"
 
@@ -18,6 +18,7 @@ struct BlockArgs {
   int block_m, block_n_log2, rows, columns;  // rows and columns of a list
   int causal, shift;                         // query i stands at i + shift
   float scale;
+  int window, sink;                          // instead of lists: keys behind position - window, and the first ones
 };
 
 // Entries of a row of the structure, whatever pos holds.
@@ -39,6 +40,25 @@ __device__ __forceinline__ int first_key(const BlockArgs &a, int first, int coun
   return e < count && (unsigned)block < (unsigned)a.columns ? key : kAbsent;
 }
 
+// The keys that queries q0 .. see, `held` of them, over a window: the first ones that lie before it, and from where it starts for the first
+// of them to the last one's own.  Sixteen at a time, as those of lists, so that the window starts at a multiple of sixteen and no key
+// comes twice.
+struct Span {
+  int sinks, start, count;  // sixteens of the first keys, first key of the window's, sixteens in all
+  __device__ __forceinline__ int first_key(int place16) const {
+    return place16 >= count ? kAbsent : place16 < sinks ? 16 * place16 : start + 16 * (place16 - sinks);
+  }
+};
+__device__ __forceinline__ Span span_of(const BlockArgs &a, int q0, int held) {
+  const int last = q0 + held - 1 + a.shift;
+  Span s = {0, 0, 0};
+  if (last < 0) return s;
+  s.start = max(0, q0 + a.shift - a.window + 1) & ~15;
+  s.sinks = (min(a.sink, s.start) + 15) / 16;
+  s.count = s.sinks + (last - s.start) / 16 + 1;
+  return s;
+}
+
 // Tiles of KT keys that a list has.  They are numbered with 31 bits: more would be 2^36 keys of one list, of the 2^30 there are.
 template <int KT>
 __device__ __forceinline__ int tiles_of(const BlockArgs &a, int count) {
@@ -48,7 +68,8 @@ __device__ __forceinline__ int tiles_of(const BlockArgs &a, int count) {
 // Tiles of KT keys and values of a list on their way into two LDS buffers each, a workgroup of NW wavefronts sharing the
 // work: sixteen rows at a time lie in one place.  A key that is not there is read from the last one: whoever uses the tile
 // gives it no weight, and looks for values that are no numbers wherever a mask cuts.
-template <typename T, int DP, int NW, int KT, bool V_BY_COLUMNS>
+// WINDOW: the tiles of a span.
+template <typename T, int DP, int NW, int KT, bool V_BY_COLUMNS, bool WINDOW = false>
 struct KeyTiles {
   typedef typename T::elem elem;
   static constexpr int PIECES = DP / 8, RP = NW * 64 / PIECES, PASSES = KT / RP, CH = KT / 16;
@@ -58,6 +79,7 @@ struct KeyTiles {
   const elem *kp, *vp;
   long long k_off, v_off;
   unsigned k_to, v_to;
+  Span span = {};
 
   __device__ __forceinline__ KeyTiles(const BlockArgs &a_, int b, int kh, int first_, int count_, int tid, const elem *k_tile, const elem *v_tile)
       : a(a_), first(first_), count(count_), wave(__builtin_amdgcn_readfirstlane(tid >> 6)), my_row(tid / PIECES), in16(my_row & 15),
@@ -69,9 +91,12 @@ struct KeyTiles {
     k_to = lds_address(k_tile) + wave * 1024;
     v_to = lds_address(v_tile) + wave * 1024;
   }
-  __device__ __forceinline__ int tiles() const { return tiles_of<KT>(a, count); }
+  __device__ __forceinline__ int tiles() const { return WINDOW ? (span.count + CH - 1) / CH : tiles_of<KT>(a, count); }
   // The first key of each sixteen of tile t, one to a lane: asked for a tile before they are needed.
-  __device__ __forceinline__ int look_up(int t) const { return first_key(a, first, count, (long long)t * KT + 16 * (threadIdx.x % CH)); }
+  __device__ __forceinline__ int look_up(int t) const {
+    if constexpr (WINDOW) return span.first_key(t * CH + (int)(threadIdx.x % CH));
+    return first_key(a, first, count, (long long)t * KT + 16 * (threadIdx.x % CH));
+  }
   static __device__ __forceinline__ v4i spread(int of_lane) {
     static_assert(CH == 4, "tiles of 64 keys");
     return v4i{__builtin_amdgcn_readlane(of_lane, 0), __builtin_amdgcn_readlane(of_lane, 1), __builtin_amdgcn_readlane(of_lane, 2),
@@ -95,5 +120,12 @@ struct KeyTiles {
 };
 
 int read_block(const char *what, const lapis_hip_block_args *p, bool backward, BlockArgs *a);
+// Sizes of lists are left to the caller: block_m and rows.
+int read_window(const char *what, const lapis_hip_window_args *p, bool backward, BlockArgs *a);
+// Queries a list gets where a workgroup has `rows` rows, a row for each head of the group.
+inline void cut_queries(BlockArgs *a, int rows) {
+  a->block_m = std::max(1, rows / std::max(a->group, 1));
+  a->rows = a->heads ? (int)ceil_div(a->queries, a->block_m) : 0;
+}
 
 }  // namespace lapis

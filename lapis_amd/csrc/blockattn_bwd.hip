@@ -1,4 +1,4 @@
-// Attention over the blocks that a CSR structure lists, backward.
+// Attention over the blocks that a CSR structure lists, or over a window and the first keys, backward.
 //
 // P and dS are computed twice, once beside dQ (rows of the structure, as in the forward pass) and once beside dK and dV
 // (its columns): nothing is added by atomics, so the same inputs give the same bits.  The columns' lists of rows are made
@@ -26,7 +26,7 @@ __device__ __forceinline__ float of_row(const vec8<T> (&f)[2], int row, int lane
 // from its registers.  rowsum(dO * O), times `scale`, and the log-sums in units of ln 2 are left for the other kernel.
 // 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 309 us in a trace (356 with 24 registers spilled and the products
 // one chain after the other), 610 TFLOP/s; bound by what a wavefront waits for between its chains of products.
-template <typename T, int DP, int NW, int KT>
+template <typename T, int DP, int NW, int KT, bool WINDOW>
 __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
@@ -39,8 +39,8 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
   const int bh = list / a.rows, r = list - bh * a.rows, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const int q0 = r * a.block_m, held = min(a.block_m, a.queries - q0), rows = held * a.group;
   if (part * 32 * NW >= rows) return;
-  int first, count;
-  entries_of(a, list, &first, &count);
+  int first = 0, count = 0;
+  if (!WINDOW) entries_of(a, list, &first, &count);
 
   const int row0 = part * 32 * NW + wave * 32, row = row0 + (lane & 31);
   const bool live = row < rows;
@@ -50,6 +50,9 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
   const int low = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row0 / a.group + a.shift, a.keys - 1) : a.keys - 1);
   const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
   const int low_of_all = a.causal ? min(q0 + part * 32 * NW / a.group + a.shift, a.keys - 1) : a.keys - 1;
+  const int row_last_of_all = min(part * 32 * NW + 32 * NW, rows) - 1;
+  const int gone = limit - a.window;  // last key before this row's window
+  const int gone_any = high - a.window, gone_any_of_all = q0 + row_last_of_all / a.group + a.shift - a.window;
 
   vec8<T> qf[DP / 16], gf[DP / 16];
   float off = INFINITY, del = 0.f;  // of a row without entries: weights 0
@@ -76,7 +79,8 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     off = lse == -INFINITY ? INFINITY : lse * kLog2e;
     if (half == 0) delta[at] = del, logs[at] = off;
   }
-  const KeyTiles<T, DP, NW, KT, false> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  KeyTiles<T, DP, NW, KT, false, WINDOW> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  if (WINDOW) keys.span = span_of(a, q0, held);
   const int tiles = keys.tiles();
   v4i now, next;  // first keys of each sixteen of this tile and the next
   v16f acc[DT];
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
-    if (top + 15 > low_of_all) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
+    if (top + 15 > low_of_all || (WINDOW && lowest <= gone_any_of_all)) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
       bool bad = false;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(k_tile[buffer] + (p * NW * 64 + tid) * 8));
@@ -117,7 +121,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     }
     if (lowest <= high) {
       const elem *kt = k_tile[buffer], *vt = v_tile[buffer];
-      const bool cut = top + 15 > low;
+      const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
       const bool bad = cut && bad_tile[buffer] == t + 1;
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
           float ds = p * __builtin_fmaf(g[e], a.scale, -del);
           if (cut) {
             const int key = now[2 * x + (e >> 3)] + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
-            ds = key > limit ? 0.f : ds;
+            ds = key > limit || (WINDOW && key <= gone && key >= a.sink) ? 0.f : ds;
           }
           df[e >> 3][e & 7] = (elem)ds;
         }
@@ -170,7 +174,8 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
               acc[i] = mfma32(finite_only<T>(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, place_lane)), df[y], acc[i]);
 #pragma unroll 1
           for (int row = 0; row < 32; ++row) {
-            const bool sees = (row < 16 ? now[2 * x] : now[2 * x + 1]) + (row & 15) <= limit;
+            const int key = (row < 16 ? now[2 * x] : now[2 * x + 1]) + (row & 15);
+            const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
             const float w = of_row<T>(df, row, lane);
 #pragma unroll
             for (int i = 0; i < DT; ++i)
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
 
 // Lists of few rows, as in the forward pass: 16 rows a wavefront, K and V from memory into the operands' registers, K through LDS
 // for the product by columns.  SPLIT wavefronts share the keys of one list and add up, in their order, through LDS.
-template <typename T, int DP, int SPLIT>
+template <typename T, int DP, int SPLIT, bool WINDOW>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta,
                                                                                float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
@@ -227,7 +232,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
   const int bh = any ? list / a.rows : 0, r = any ? list - bh * a.rows : 0, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const int q0 = r * a.block_m, rows = min(a.block_m, a.queries - q0) * a.group;
   int first = 0, count = 0;
-  if (any && part * 16 < rows) entries_of(a, list, &first, &count);
+  Span span = {};
+  if (any && part * 16 < rows) {
+    if constexpr (WINDOW) span = span_of(a, q0, min(a.block_m, a.queries - q0));
+    else entries_of(a, list, &first, &count);
+  }
   const int row0 = part * 16, row = row0 + col, row_last = min(row0 + 15, rows - 1);
   const bool live = any && row < rows;
   const int query = q0 + row / a.group, head = kh * a.group + row % a.group;
@@ -262,7 +271,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
   }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  const int tiles = tiles_of<32>(a, count);
+  const int gone = limit - a.window, gone_any = high - a.window;  // last key before this row's window, and any row's
+  const int tiles = WINDOW ? (span.count + 1) / 2 : tiles_of<32>(a, count);
   v4i kr[2][KS], vr[2][KS];
   const auto load = [&](int key0, int key1) {
 #pragma unroll
@@ -278,7 +288,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
       }
     }
   };
-  const auto look_up = [&](int t) { return tiles > 0 ? first_key(a, first, count, 32ll * t + 16 * (lane & 1)) : kAbsent; };
+  const auto look_up = [&](int t) {
+    if constexpr (WINDOW) return span.first_key(2 * t + (lane & 1));
+    return tiles > 0 ? first_key(a, first, count, 32ll * t + 16 * (lane & 1)) : kAbsent;
+  };
 
   v4f acc[DT];
 #pragma unroll
@@ -300,7 +313,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
         g[i] = mfma16(__builtin_bit_cast(vec8<T>, vr[i][x]), gf[x], g[i]);
       }
     }
-    const bool cut = max(now0, now1) + 15 > low, skip = min(now0, now1) > high;
+    const bool cut = max(now0, now1) + 15 > low || (WINDOW && min(now0, now1) <= gone_any), skip = min(now0, now1) > high;
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -322,7 +335,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
       for (int e = 0; e < 4; ++e) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], c, -off));
         float ds = p * __builtin_fmaf(g[i][e], a.scale, -del);
-        if (cut && (i ? now1 : now0) + 4 * quarter + e > limit) ds = 0.f;
+        const int key = (i ? now1 : now0) + 4 * quarter + e;
+        if (cut && (key > limit || (WINDOW && key <= gone && key >= a.sink))) ds = 0.f;
         df[4 * i + e] = (elem)ds;
       }
     wave_lds_sync();
@@ -337,7 +351,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
     if (bad)  // a key's elements that are no numbers, for the rows that see it
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {
-        const bool sees = (x < 16 ? now0 : now1) + (x & 15) <= limit;
+        const int key = (x < 16 ? now0 : now1) + (x & 15);
+        const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
         float w = 0.f;  // key x is element 4 (x / 16) + x % 4 of quarter x / 4 % 4
 #pragma unroll
         for (int e = 0; e < 8; ++e) w = e == 4 * (x >> 4) + (x & 3) ? (float)df[e] : w;
@@ -387,7 +402,40 @@ struct Columns {
   int *rows;          // nnz
   float *partial;     // of columns of several units: dk and dv of each
   int chunks, chunk_rows, per_unit, units, lists, sub;
+  // Of a window: columns with first keys, which all later queries see, in units of `per_unit` queries and these many of them; the others.
+  int sink_columns, sink_units, per_unit_other, other_units;
 };
+
+// A unit of work of a window: its column (counted through all lists), its number among the column's, and how many queries those have.
+struct WindowUnit {
+  int column, part, per_unit, of_column;
+};
+__device__ __forceinline__ WindowUnit window_unit(const Columns &t, int columns, int u) {
+  WindowUnit x;
+  const int of_sinks = t.sink_columns * t.sink_units * t.lists;
+  if (u < of_sinks) {
+    const int c = u / t.sink_units, list = c / t.sink_columns;
+    x.part = u - c * t.sink_units;
+    x.column = list * columns + (c - list * t.sink_columns);
+    x.per_unit = t.per_unit;
+    x.of_column = t.sink_units;
+  } else {
+    u -= of_sinks;
+    const int c = u / t.other_units, others = columns - t.sink_columns, list = c / others;
+    x.part = u - c * t.other_units;
+    x.column = list * columns + t.sink_columns + (c - list * others);
+    x.per_unit = t.per_unit_other;
+    x.of_column = t.other_units;
+  }
+  return x;
+}
+// The queries that see some key of a column: from `first` on, these many.
+__device__ __forceinline__ void queries_of(const BlockArgs &a, int column, int *first, int *count) {
+  const int key0 = column << a.block_n_log2, key1 = min(key0 + (1 << a.block_n_log2), a.keys) - 1;
+  *first = max(0, key0 - a.shift);
+  const int last = key0 < a.sink ? a.queries - 1 : (int)min(a.queries - 1ll, (long long)key1 - a.shift + a.window - 1);
+  *count = max(0, last - *first + 1);
+}
 
 __global__ void clear_kernel(int *p) { p[threadIdx.x] = 0; }
 
@@ -686,7 +734,8 @@ struct DkvShared {
 
 // ODD: positions descend.  A body of its own, as the kernel's own look for rows among its units costs the loop registers (8192 queries, 16
 // blocks of 64: 547 us against 510).
-template <typename T, int DP, int KG, int S, bool ODD>
+// WINDOW: the rows of a column are neighbouring queries.
+template <typename T, int DP, int KG, int S, bool ODD, bool WINDOW>
 __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, KG, S> &mem) {
   typedef typename T::elem elem;
   typedef typename DkvShared<T, DP, KG, S>::Info Info;
@@ -743,7 +792,18 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
     const int u = unit_l / cols.sub, sub = unit_l - u * cols.sub;
     int cc, from = 0, n = 0, start = 0;
     bool several = false;
-    if (ODD) {
+    if constexpr (WINDOW) {
+      const WindowUnit x = window_unit(*(const Columns *)&at_start->cols, a.columns, u);
+      cc = x.column;
+      int all;
+      queries_of(*(const BlockArgs *)&at_start->a, cc % a.columns, &start, &all);
+      from = x.part * x.per_unit;
+      if (from >= all && x.part > 0) continue;
+      several = x.of_column > 1 && all > x.per_unit;
+      n = min(all - from, x.per_unit);
+      start += from;  // first query
+      from = u;       // where its sums go, if there are several
+    } else if (ODD) {
       cc = u;
       n = rows_that_name(*(const BlockArgs *)&at_start->a, cc, *cols.odd, rows_of_unit, mem.found);
       if (tid == 0) cols.end[cc] = n;
@@ -762,6 +822,8 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
     const int in_block = sub * 32 * KG + kg * 32;
     const int key_low = (column << a.block_n_log2) + in_block, key = key_low + (lane & 31);
     const bool live = in_block + (lane & 31) < (1 << a.block_n_log2) && key < a.keys;
+    const int window = WINDOW ? args.a.window : 0;
+    const bool first_key = WINDOW && key < args.a.sink;
 
     // Where rows lie is worked out for four tiles of a group at a time, a row to each of 128 threads: one wavefront doing it in
     // every iteration is what all others wait for.  A thread's row: entry, query of the block and head of the group.
@@ -779,7 +841,9 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
         const int lane = looks_up & 31;
         int query = 0;
         bool there = entry < n;
-        if (there) {
+        if constexpr (WINDOW) {
+          query = start + entry;
+        } else if (there) {
           query = rows_of_unit[entry] * a.block_m + in;
           there = query < a.queries;
         }
@@ -882,7 +946,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
         unsigned bad = 0;
         if (now) {
           const Info &info = infos[qg][t % (2 * BATCH)];
-          const bool cut = same(__any(last < key_low + 31));
+          const bool cut = same(__any(last < key_low + 31 || (WINDOW && last - window >= key_low)));
           const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -913,7 +977,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
             for (int j = 0; j < 4; ++j) {
               const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * j + e] = key <= lim[e] ? s[4 * j + e] : 0.f;
+              for (int e = 0; e < 4; ++e) s[4 * j + e] = key <= lim[e] && (!WINDOW || first_key || key > lim[e] - window) ? s[4 * j + e] : 0.f;
             }
           }
 #pragma unroll
@@ -923,7 +987,8 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
           for (unsigned left = bad; left != 0; left &= left - 1) {
             const int row = __builtin_ctz(left);
             const float w = of_row<T>(f, row, lane);
-            const bool sees = key <= infos[qg][t % (2 * BATCH)].last[row];
+            const int lim = infos[qg][t % (2 * BATCH)].last[row];
+            const bool sees = key <= lim && (!WINDOW || first_key || key > lim - window);
 #pragma unroll
             for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -1011,7 +1076,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
     const DkvArgsAgain at_end = again();
     if (several) {
       const auto &cols = at_end->cols;
-      const long long slot = 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << at_end->a.block_n_log2;
+      const long long slot = WINDOW ? from : 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << at_end->a.block_n_log2;
       float *to = cols.partial + (slot * 2 + 1 - role) * each + (long long)(in_block + (lane & 31)) * DP;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -1037,8 +1102,14 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
 template <typename T, int DP, int KG, int S>
 __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
   __shared__ DkvShared<T, DP, KG, S> mem;
-  if (same(*args.cols.odd != 0)) dkv_units<T, DP, KG, S, true>(args, mem);
-  else dkv_units<T, DP, KG, S, false>(args, mem);
+  if (same(*args.cols.odd != 0)) dkv_units<T, DP, KG, S, true, false>(args, mem);
+  else dkv_units<T, DP, KG, S, false, false>(args, mem);
+}
+
+template <typename T, int DP, int KG, int S>
+__global__ __launch_bounds__(256, 2) void window_dkv_kernel(DkvArgs args) {
+  __shared__ DkvShared<T, DP, KG, S> mem;
+  dkv_units<T, DP, KG, S, false, true>(args, mem);
 }
 
 // Columns of several units: their sums, in the order of the units.  NaN where the rows of a column were not found.
@@ -1059,6 +1130,37 @@ __global__ __launch_bounds__(256) void join_units_kernel(BlockArgs a, Columns co
     if (key >= a.keys || d >= a.dim) continue;
     const float none = lost ? __builtin_nanf("") : 0.f;
     v4f sum = {none, none, none, none};
+    for (int j = 0; j < units; ++j) {
+      const v4f y = *(const v4f *)(from + j * 2 * each + x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += y[e];
+    }
+    const View &v = is_v ? a.dv : a.dk;
+    vec4<T> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (elem)sum[e];
+    *(vec4<T> *)((elem *)v.data + b * v.stride[0] + key * v.stride[1] + kh * v.stride[2] + d) = o;
+  }
+}
+
+// The same of a window: columns with first keys, then the others.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void join_window_kernel(BlockArgs a, Columns cols, bool sinks) {
+  typedef typename T::elem elem;
+  const int unit = sinks ? blockIdx.x * cols.sink_units : cols.lists * cols.sink_columns * cols.sink_units + blockIdx.x * cols.other_units;
+  const WindowUnit u = window_unit(cols, a.columns, unit);
+  const int bh = u.column / a.columns, column = u.column - bh * a.columns, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
+  int first, all;
+  queries_of(a, column, &first, &all);
+  if (all <= u.per_unit) return;
+  const int units = (all + u.per_unit - 1) / u.per_unit;
+  const long long each = (long long)DP << a.block_n_log2;
+  const float *from = cols.partial + 2ll * unit * each;
+  for (long long x = (blockIdx.y * 256 + threadIdx.x) * 4; x < 2 * each; x += gridDim.y * 1024) {
+    const bool is_v = x >= each;
+    const int at = (int)(is_v ? x - each : x), d = at % DP, key = (column << a.block_n_log2) + at / DP;
+    if (key >= a.keys || d >= a.dim) continue;
+    v4f sum = {0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < units; ++j) {
       const v4f y = *(const v4f *)(from + j * 2 * each + x);
 #pragma unroll
@@ -1156,7 +1258,7 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   c.partial = reinterpret_cast<float *>(work + l.partial);
   if (a.rows) {
     const DqGrid g = dq_grid(a);
-    const auto kernel = !g.few ? block_dq_kernel<T, DP, 4, 64> : g.many ? block_dq_narrow_kernel<T, DP, 1> : block_dq_narrow_kernel<T, DP, 4>;
+    const auto kernel = !g.few ? block_dq_kernel<T, DP, 4, 64, false> : g.many ? block_dq_narrow_kernel<T, DP, 1, false> : block_dq_narrow_kernel<T, DP, 4, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)g.blocks), dim3(256), 0, st, a, (int)g.tiles, delta, logs, c.odd);
   }
   if (c.lists && a.columns) {
@@ -1172,6 +1274,90 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
     if (a.block_n_log2 <= 5) launch_dkv<T, DP, 1, DP == 64 ? 4 : 3>(a, c, delta, logs, st);
     else launch_dkv<T, DP, 2, 4>(a, c, delta, logs, st);
     hipLaunchKernelGGL((join_units_kernel<T, DP>), dim3((unsigned)(c.lists * a.columns), 4), dim3(256), 0, st, a, c);
+  }
+  LAPIS_LAUNCH_CHECK();
+  return LAPIS_HIP_OK;
+}
+
+// ---- windows: host ---------------------------------------------------------------------------------------------
+
+struct WindowLayout {
+  int64_t delta, logs, next, partial, bytes;
+  bool few;  // rows: dQ by 16 of them
+  Columns columns;
+};
+
+int layout_of_window(BlockArgs *a, WindowLayout *layout) {
+  const char *what = "window_attention_backward";
+  WindowLayout &l = *layout = {};
+  a->block_n_log2 = 6;
+  a->columns = (int)ceil_div(a->keys, 64);
+  cut_queries(a, 128);
+  l.few = (int64_t)a->batch * a->kv_heads * a->rows * ceil_div(a->block_m * a->group, 128) < device_cu_count() / 2;  // the forward pass's rule
+  if (l.few) cut_queries(a, 16);
+  const int64_t lists = (int64_t)a->batch * a->kv_heads, columns = lists * a->columns;
+  const int64_t tiles = ceil_div((int64_t)a->block_m * a->group, l.few ? 16 : 128);
+  LAPIS_REQUIRE(lists <= 65535 && columns * 256 < (INT64_C(1) << 32), "%s: %lld lists of %d columns", what, (long long)lists, a->columns);
+  LAPIS_REQUIRE(lists * a->rows * tiles * 256 < (INT64_C(1) << 32), "%s: %lld rows", what, (long long)(lists * a->rows));
+  // Queries of a column.  Columns with first keys have all of them behind: they are cut into units as long as the others' columns, and all into
+  // shorter ones while there are not two for each compute unit.
+  Columns &c = l.columns;
+  c.lists = (int)lists;
+  c.sink_columns = (int)std::min<int64_t>(ceil_div(a->sink, 64), a->columns);
+  const int64_t others = a->columns - c.sink_columns, seen = std::max<int64_t>(1, std::min<int64_t>(a->queries, (int64_t)a->window + 63));
+  const int64_t group = std::max(a->group, 1), least = std::max<int64_t>(1, 256 / group);  // of a unit: fewer are not worth a join
+  const int64_t work = lists * (others * seen + (int64_t)c.sink_columns * a->queries);
+  const int64_t share = std::max<int64_t>(least, ceil_div(work, 2 * std::max(device_cu_count(), 1)));
+  const int64_t units_other = std::max<int64_t>(1, columns < 2 * device_cu_count() ? ceil_div(seen, share) : 1);
+  c.other_units = (int)units_other;
+  c.per_unit_other = (int)ceil_div(seen, units_other);
+  c.per_unit = (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(c.per_unit_other, least), std::max(a->queries, 1)));
+  c.sink_units = (int)std::max<int64_t>(1, ceil_div(a->queries, c.per_unit));
+  const int64_t units = lists * (c.sink_columns * (int64_t)c.sink_units + others * c.other_units);
+  LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
+  c.units = (int)units;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.delta = take(4ll * a->batch * a->heads * a->queries);
+  l.logs = take(4ll * a->batch * a->heads * a->queries);
+  l.next = take(4 * (1 + kParts));
+  const int64_t each = 2ll * (a->dim <= 64 ? 64 : 128) * 64 * 4;
+  const int64_t of_sinks = lists * c.sink_columns * (int64_t)c.sink_units;
+  l.partial = take((c.other_units > 1 ? units : c.sink_units > 1 ? of_sinks : 0) * each);
+  l.bytes = at;
+  return LAPIS_HIP_OK;
+}
+
+template <typename T, int DP>
+int launch_window_backward(BlockArgs a, char *work, hipStream_t st) {
+  WindowLayout l;
+  const int rc = layout_of_window(&a, &l);
+  if (rc != LAPIS_HIP_OK) return rc;
+  Columns &c = l.columns;
+  float *delta = reinterpret_cast<float *>(work + l.delta), *logs = reinterpret_cast<float *>(work + l.logs);
+  c.odd = reinterpret_cast<int *>(work + l.next);
+  c.next = c.odd + 1;
+  c.partial = reinterpret_cast<float *>(work + l.partial);
+  c.sub = 1;
+  const long long lists = c.lists;
+  if (a.rows && lists) {
+    const long long tiles = ceil_div((long long)a.block_m * a.group, l.few ? 16 : 128);
+    const auto kernel = l.few ? block_dq_narrow_kernel<T, DP, 4, true> : block_dq_kernel<T, DP, 4, 64, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(lists * a.rows * tiles)), dim3(256), 0, st, a, (int)tiles, delta, logs, c.odd);
+  }
+  if (lists && a.columns) {
+    if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
+    a.block_m = 1;
+    const int64_t grid = std::min<int64_t>(2 * device_cu_count(), c.units);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, 2, 4>), dim3((unsigned)grid), dim3(256), 0, st, DkvArgs{a, c, delta, logs});
+    if (c.sink_units > 1 && c.sink_columns)
+      hipLaunchKernelGGL((join_window_kernel<T, DP>), dim3((unsigned)(lists * c.sink_columns), 8), dim3(256), 0, st, a, c, true);
+    if (c.other_units > 1 && a.columns > c.sink_columns)
+      hipLaunchKernelGGL((join_window_kernel<T, DP>), dim3((unsigned)(lists * (a.columns - c.sink_columns)), 8), dim3(256), 0, st, a, c, false);
   }
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
@@ -1205,4 +1391,30 @@ extern "C" int lapis_hip_block_attention_backward(const lapis_hip_block_args *ar
   const bool bf16 = args->dtype == LAPIS_HIP_BF16;
   if (a.dim <= 64) return bf16 ? launch_backward<Bf16, 64>(a, work, as_stream(stream)) : launch_backward<F16, 64>(a, work, as_stream(stream));
   return bf16 ? launch_backward<Bf16, 128>(a, work, as_stream(stream)) : launch_backward<F16, 128>(a, work, as_stream(stream));
+}
+
+extern "C" int lapis_hip_window_attention_backward_work(const lapis_hip_window_args *args, int64_t *bytes) {
+  LAPIS_CHECK_INIT();  // the size goes by the number of compute units
+  BlockArgs a;
+  int rc = read_window("window_attention_backward", args, true, &a);
+  if (rc != LAPIS_HIP_OK) return rc;
+  LAPIS_REQUIRE(bytes, "window_attention_backward: null result");
+  WindowLayout l;
+  rc = layout_of_window(&a, &l);
+  *bytes = l.bytes;
+  return rc;
+}
+
+extern "C" int lapis_hip_window_attention_backward(const lapis_hip_window_args *args, lapis_hip_stream_t stream) {
+  LAPIS_CHECK_INIT();
+  BlockArgs a;
+  const int rc = read_window("window_attention_backward", args, true, &a);
+  if (rc != LAPIS_HIP_OK) return rc;
+  if (a.batch == 0 || (a.heads == 0 && a.kv_heads == 0)) return LAPIS_HIP_OK;
+  LAPIS_REQUIRE(args->work && aligned16(args->work), "window_attention_backward: work that is null or not on a 16-byte boundary");
+  char *work = static_cast<char *>(args->work);
+  const hipStream_t st = as_stream(stream);
+  const bool bf16 = args->dtype == LAPIS_HIP_BF16;
+  if (a.dim <= 64) return bf16 ? launch_window_backward<Bf16, 64>(a, work, st) : launch_window_backward<F16, 64>(a, work, st);
+  return bf16 ? launch_window_backward<Bf16, 128>(a, work, st) : launch_window_backward<F16, 128>(a, work, st);
 }

@@ -5,42 +5,13 @@
 // of 8 heads, dim 128, bf16 into e4m3 in 51.5 us (4.0 TB/s), 20 000 tokens, dim 96, back into f16 in 24.1 (3.9 TB/s), where a
 // large copy reaches 4.75; four rows a thread on their way, loads first, where that leaves every compute unit its workgroups
 // (one row a thread: 54 and 30).  48 tokens take 4.5 us, the call and the launch.
-#include "attn.hpp"
+#include "kvcache.hpp"
 
 namespace lapis {
 namespace {
 
-struct CacheView {
-  char *data[2];
-  float *scale[2];
-  long long stride[3], scale_stride[3];
-  long long slots;  // pages * page
-  int heads, page_log2, dim;
-};
-struct RowsView {
-  char *data[2];
-  long long stride[2][2];  // token, head
-};
-
-CacheView view_of(const lapis_hip_kv_cache *c) {
-  CacheView v = {};
-  v.data[0] = static_cast<char *>(c->k);
-  v.data[1] = static_cast<char *>(c->v);
-  v.scale[0] = c->k_scale;
-  v.scale[1] = c->v_scale;
-  for (int i = 0; i < 3; ++i) {
-    v.stride[i] = c->stride[i];
-    v.scale_stride[i] = c->scale_stride[i];
-  }
-  v.slots = c->pages * c->page;
-  v.heads = c->heads;
-  v.page_log2 = __builtin_ctz((unsigned)c->page);
-  v.dim = c->dim;
-  return v;
-}
-
 // Group of L lanes per (token, head) and of N of them, 256 / L rows apart; blockIdx.z: keys or values.
-template <typename T, bool F8, int L, int N>
+template <typename T, int CODES, int L, int N>
 __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, long long rows, const int *__restrict__ slots) {
   typedef typename T::elem elem;
   const long long row0 = (long long)linear_block() * (256 / L * N) + threadIdx.x / L;
@@ -61,33 +32,21 @@ __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, 
     const int h = (int)((unsigned)row % (unsigned)c.heads);
     const long long slot = slot_of[i];
     if (slot < 0 || slot >= c.slots) continue;
-    const long long page = slot >> c.page_log2, in = slot & ((1 << c.page_log2) - 1);
-    const long long to = page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d;
-    const vec8<T> e = read[i];
-    if (!F8) {
-      if (d < c.dim) *(vec8<T> *)((elem *)c.data[which] + to) = e;
-      continue;
+    if constexpr (CODES == kNoCodes) {
+      const long long page = slot >> c.page_log2, in = slot & ((1 << c.page_log2) - 1);
+      if (d < c.dim) *(vec8<T> *)((elem *)c.data[which] + page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d) = read[i];
+    } else {
+      float f[8];
+      widen<T>(read[i], f);
+      put_elements<T, CODES, L>(c, which, slot, h, d, f);
     }
-    float f[8];
-    widen<T>(e, f);
-    unsigned top = 0;  // of the finite and infinite elements: a NaN keeps its place and leaves its neighbours alone
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]) > kInfBits ? 0u : abs_bits(f[i]));
-    const float amax = __builtin_bit_cast(float, group_max<L>(top));
-    const float scale = amax / 448.0f;
-    if (scale > 0.0f) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] / scale;
-    }
-    if (d < c.dim) *(v2i *)(c.data[which] + to) = narrow_f8(f);
-    if (d == 0) c.scale[which][page * c.scale_stride[0] + h * c.scale_stride[1] + in * c.scale_stride[2]] = scale;
   }
 }
 
-template <typename T, bool F8, int L, int N>
+template <typename T, int CODES, int L, int N>
 __global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, long long rows, const int *__restrict__ slots) {
   typedef typename T::elem elem;
-  typedef typename std::conditional<F8, v2i, v4i>::type raw;  // eight elements
+  typedef typename std::conditional<CODES == kF8, v2i, typename std::conditional<CODES == kF4, unsigned, v4i>::type>::type raw;  // eight elements
   const long long row0 = (long long)linear_block() * (256 / L * N) + threadIdx.x / L;
   const int d = (threadIdx.x % L) * 8, which = blockIdx.z;
   if (d >= c.dim) return;
@@ -101,8 +60,11 @@ __global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, l
     scale[i] = 0.f;
     if (slot >= 0 && slot < c.slots) {
       const long long page = slot >> c.page_log2, in = slot & ((1 << c.page_log2) - 1);
-      read[i] = load_stream((const raw *)(c.data[which] + (page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d) * (F8 ? 1 : 2)));
-      if (F8) scale[i] = c.scale[which][page * c.scale_stride[0] + h * c.scale_stride[1] + in * c.scale_stride[2]];
+      const long long at = page * c.stride[0] + h * c.stride[1] + in * c.stride[2] + d;
+      read[i] = load_stream((const raw *)(c.data[which] + (CODES == kF4 ? at / 2 : CODES == kF8 ? at : at * 2)));
+      const long long scale_at = page * c.scale_stride[0] + h * c.scale_stride[1] + in * c.scale_stride[2];
+      if (CODES == kF8) scale[i] = ((const float *)c.scale[which])[scale_at];
+      if (CODES == kF4) scale[i] = scale_of_byte(((const unsigned char *)c.scale[which])[scale_at + d / 32]);
     }
   }
 #pragma unroll
@@ -111,11 +73,15 @@ __global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, l
     if (row >= rows) return;
     const unsigned t = (unsigned)row / (unsigned)c.heads, h = (unsigned)row - t * c.heads;
     vec8<T> e;
-    if constexpr (F8) {
+    if constexpr (CODES != kNoCodes) {
       float f[8];
-      widen_f8(read[i], f);
+      if constexpr (CODES == kF4) {
+        widen_f4(read[i], scale[i], f);
+      } else {
+        widen_f8(read[i], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = f[j] * scale[i];
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * scale[i];
+      }
       e = narrow<T>(f);
     } else {
       e = __builtin_bit_cast(vec8<T>, read[i]);
@@ -130,7 +96,7 @@ int kv_move(const char *what, const lapis_hip_kv_cache *cache, int64_t tokens, c
   const int rc = check_cache(what, cache);
   if (rc != LAPIS_HIP_OK) return rc;
   LAPIS_REQUIRE(k && v && tokens >= 0, "%s: null rows or a negative number of tokens", what);
-  LAPIS_REQUIRE(is_16bit(dtype) && (cache->dtype == dtype || cache->dtype == LAPIS_HIP_F8E4M3),
+  LAPIS_REQUIRE(is_16bit(dtype) && (cache->dtype == dtype || codes_of(cache->dtype) != kNoCodes),
                 "%s: rows of type %d and a cache of type %d", what, dtype, cache->dtype);
   if (tokens == 0) return LAPIS_HIP_OK;
   LAPIS_REQUIRE(slots, "%s: null slots", what);
@@ -141,13 +107,14 @@ int kv_move(const char *what, const lapis_hip_kv_cache *cache, int64_t tokens, c
                   "%s: rows that are null, not on a 16-byte boundary or with strides that are no multiples of 8", what);
   const CacheView c = view_of(cache);
   RowsView x = {{static_cast<char *>(k->data), static_cast<char *>(v->data)}, {{k->stride[1], k->stride[2]}, {v->stride[1], v->stride[2]}}};
-  const bool f8 = cache->dtype == LAPIS_HIP_F8E4M3, bf16 = dtype == LAPIS_HIP_BF16;
+  const Codes codes = codes_of(cache->dtype);
+  const bool bf16 = dtype == LAPIS_HIP_BF16;
   const auto go = [&](auto lanes, auto times) {
     constexpr int L = decltype(lanes)::value, N = decltype(times)::value;
     const auto pick = [&](auto type) {
       typedef decltype(type) T;
-      if (STORE) return f8 ? kv_store_kernel<T, true, L, N> : kv_store_kernel<T, false, L, N>;
-      return f8 ? kv_load_kernel<T, true, L, N> : kv_load_kernel<T, false, L, N>;
+      if (STORE) return codes == kF4 ? kv_store_kernel<T, kF4, L, N> : codes == kF8 ? kv_store_kernel<T, kF8, L, N> : kv_store_kernel<T, kNoCodes, L, N>;
+      return codes == kF4 ? kv_load_kernel<T, kF4, L, N> : codes == kF8 ? kv_load_kernel<T, kF8, L, N> : kv_load_kernel<T, kNoCodes, L, N>;
     };
     dim3 grid = grid_of(ceil_div(rows * L, 256 * N));
     grid.z = 2;
@@ -174,13 +141,16 @@ int check_cache(const char *what, const lapis_hip_kv_cache *c) {
   LAPIS_REQUIRE(c->page >= 1 && c->page <= 1024 && (c->page & (c->page - 1)) == 0, "%s: pages of %d slots (a power of two up to 1024)", what, c->page);
   LAPIS_REQUIRE(c->pages <= INT32_MAX / c->page, "%s: %lld pages of %d slots: slots are numbered with 31 bits", what, (long long)c->pages, c->page);
   LAPIS_REQUIRE(c->dim >= 8 && c->dim <= kMaxDim && c->dim % 8 == 0, "%s: rows of %d elements (a multiple of 8 up to %d)", what, c->dim, kMaxDim);
-  const bool f8 = c->dtype == LAPIS_HIP_F8E4M3;
-  LAPIS_REQUIRE(f8 || is_16bit(c->dtype), "%s: a cache of type %d", what, c->dtype);
+  const Codes codes = codes_of(c->dtype);
+  LAPIS_REQUIRE(codes != kNoCodes || is_16bit(c->dtype), "%s: a cache of type %d", what, c->dtype);
+  LAPIS_REQUIRE(codes != kF4 || c->dim % 32 == 0, "%s: rows of %d elements in 4 bits (a multiple of 32)", what, c->dim);
   if (c->pages == 0) return LAPIS_HIP_OK;
-  LAPIS_REQUIRE(c->k && c->v && (!f8 || (c->k_scale && c->v_scale)), "%s: null cache buffers", what);
+  LAPIS_REQUIRE(c->k && c->v && (codes == kNoCodes || (c->k_scale && c->v_scale)), "%s: null cache buffers", what);
   const uintptr_t low = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v);
-  LAPIS_REQUIRE((low & (f8 ? 7u : 15u)) == 0 && strides_of_8(c->stride, 3),
-                "%s: cache buffers that are not on %d-byte boundaries or strides that are no multiples of 8", what, f8 ? 8 : 16);
+  const int boundary = codes == kF8 ? 8 : 16, strides = codes == kF4 ? 32 : 8;
+  for (int i = 0; i < 3; ++i)
+    LAPIS_REQUIRE((low & (boundary - 1u)) == 0 && c->stride[i] % strides == 0,
+                  "%s: cache buffers that are not on %d-byte boundaries or strides that are no multiples of %d", what, boundary, strides);
   return LAPIS_HIP_OK;
 }
 

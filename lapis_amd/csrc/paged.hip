@@ -1,4 +1,6 @@
-// Attention of one new token of each sequence over the pages of a cache that a CSR row lists.
+// Attention of one new token of each sequence over the pages of a cache that a CSR row lists, or over the window and the first tokens
+// of a table of pages.
+#include "kvcache.hpp"
 #include "mfma.hpp"
 
 namespace lapis {
@@ -9,7 +11,7 @@ struct PagedArgs {
   char *out;
   long long q_stride[2], out_stride[2];
   const char *k, *v;
-  const float *k_scale, *v_scale;
+  const void *k_scale, *v_scale;
   long long stride[3], scale_stride[3];
   long long pages, nnz;
   int seqs, lists, heads, kv_heads, group, dim, page_log2;
@@ -18,6 +20,11 @@ struct PagedArgs {
   float *lse;
   float scale;
   int chunk, units, head_tiles;  // pages a unit, units of all lists, tiles of 16 heads
+  int chunk_tokens;
+  const int *table, *lengths;    // of a window instead of lists
+  long long table_width;
+  int window, sink, units_each;  // units of a sequence
+  bool windowed;
   float *partial, *sums;         // of each unit: 16 x DP, and 16 maxima and sums
 };
 
@@ -26,6 +33,20 @@ __device__ __forceinline__ void list_of(const PagedArgs &a, long long row, int *
   const long long lo = min(max((long long)a.pos[row], 0ll), a.nnz), hi = min(max((long long)a.pos[row + 1], lo), a.nnz);
   *first = (int)lo;
   *tokens = a.pages > 0 ? (int)max(0ll, min((long long)a.tokens[row], (hi - lo) << a.page_log2)) : 0;
+}
+
+// Of a window: how many first tokens count that lie before it, where it starts, and tokens that count in all.  They are numbered in order.
+struct Window {
+  int sinks, first, count;
+  __device__ __forceinline__ int token(int x) const { return x < sinks ? x : (int)((unsigned)first + (unsigned)(x - sinks)); }
+};
+__device__ __forceinline__ Window window_of(const PagedArgs &a, int seq) {
+  const int length = a.pages > 0 ? (int)min((long long)max(a.lengths[seq], 0), a.table_width << a.page_log2) : 0;
+  Window w;
+  w.first = max(0, length - a.window);
+  w.sinks = min(a.sink, w.first);
+  w.count = w.sinks + (length - w.first);
+  return w;
 }
 
 // Lists are cut into units of `chunk` pages.  Unit numbers start at pos[row] / chunk + row for each list, which leaves it at
@@ -66,6 +87,25 @@ __device__ __forceinline__ vec8<T> codes_to(v2i x, float by = 1.0f) {
   return __builtin_bit_cast(vec8<T>, r);
 }
 
+// Eight 4-bit codes times their scale, as numbers of a 16-bit type (codes and scales have values of their own there but for
+// float16's subnormal numbers, where they are rounded once).
+template <typename T>
+__device__ __forceinline__ vec8<T> codes_to(unsigned x, float by) {
+  v4u r;
+  if constexpr (std::is_same<T, Bf16>::value) {
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, by, 0));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, by, 1));
+    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, by, 2));
+    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, by, 3));
+  } else {
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, by, 0));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, by, 1));
+    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, by, 2));
+    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, by, 3));
+  }
+  return __builtin_bit_cast(vec8<T>, r);
+}
+
 __device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0x7f800000u); }
 
 // A unit: up to 16 heads of a group against a stretch of a list.  Its four wavefronts take tiles of 32 tokens in turn, each by
@@ -80,15 +120,19 @@ __device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_ca
 // largest so far: exact for scales down to 2^-22 of that one, rounded to multiples of 2^-24 units below.
 // Bound by memory: 64 sequences of up to 8192 tokens, 32 heads over 8, dim 128, 8-bit cache: 153 us at 4.5 TB/s (a large copy
 // reaches 4.75), 160 with float16 queries; one sequence of 16 384 tokens, bf16: 22.4 us, 16.9 of them here (4.0 TB/s) and 5.4 for the join.
-template <typename T, bool F8, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(PagedArgs a) {
+template <typename T, int CODES, int DP, bool WINDOW>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8 ? 3 : 2) void paged_kernel(PagedArgs a) {
   typedef typename T::elem elem;
-  typedef typename std::conditional<F8, v2i, v4i>::type raw;  // eight elements
-  constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8, RP = 64 / PIECES, PASSES = 32 / RP, WIDTH = F8 ? 1 : 2;
+  constexpr bool F8 = CODES == kF8, F4 = CODES == kF4;
+  typedef typename std::conditional<F8, v2i, typename std::conditional<F4, unsigned, v4i>::type>::type raw;  // eight elements
+  typedef typename std::conditional<F4, v4u, raw>::type raw_v;                                                // what a lane loads of V at once
+  constexpr int KS = DP / 32, DT = DP / 16, PIECES = DP / 8, WIDTH = F8 ? 1 : 2;
+  constexpr int V_PIECES = F4 ? DP / 32 : PIECES, RP = 64 / V_PIECES, PASSES = 32 / RP;
   constexpr bool SCALED = F8 && std::is_same<T, F16>::value;
   struct Tokens {
     long long at[32];     // element offsets of the tile's rows
-    float ks[32], vs[32]; // SCALED: vs holds mantissas, and vp powers of two, those of a lane's rows side by side
+    long long scale_at[F4 ? 32 : 1];
+    float ks[F4 ? 4 : 32], vs[F4 ? 4 : 32]; // SCALED: vs holds mantissas, and vp powers of two, those of a lane's rows side by side
     float vp[SCALED ? 32 : 4];
   };
   union Own {  // of a wavefront
@@ -103,27 +147,38 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
   const int ht = block % a.head_tiles;
   block /= a.head_tiles;
   int kh = 0;
-  if (!a.each) {
+  if (WINDOW || !a.each) {
     kh = block % a.kv_heads;
     block /= a.kv_heads;
   }
-  const int u = block, row = list_of_unit(a, u, lane);
-  const int seq = a.each ? row / a.kv_heads : row;
-  if (a.each) kh = row - seq * a.kv_heads;
-  int first, count;
-  list_of(a, row, &first, &count);
-  const int part = (int)(u - unit_start(a, row));
-  const int chunk = a.chunk << a.page_log2;  // tokens
+  const int u = block;
+  int seq, part, first = 0, count;
+  Window w = {};
+  if constexpr (WINDOW) {
+    seq = u / a.units_each;
+    part = u - seq * a.units_each;
+    w = window_of(a, seq);
+    count = w.count;
+  } else {
+    const int row = list_of_unit(a, u, lane);
+    seq = a.each ? row / a.kv_heads : row;
+    if (a.each) kh = row - seq * a.kv_heads;
+    list_of(a, row, &first, &count);
+    part = (int)(u - unit_start(a, row));
+  }
+  const int chunk = a.chunk_tokens;
   const long long from_l = (long long)part * chunk;
   if (part < 0 || (from_l >= count && part != 0)) return;  // a unit number left over (a list without tokens still writes its zeros)
   const int from = (int)from_l, n = min(chunk, count - from), tiles = (n + 31) / 32;
   const int head0 = kh * a.group + ht * 16, heads = min(16, a.group - ht * 16);
 
-  // element j of step s of this lane's operands stands for dimension 32 s + 8 quarter + j
+  // Element j of step s of this lane's operands stands for dimension 32 s + 8 quarter + j; with 4-bit codes for DP / 4 quarter + 8 s + j, so
+  // that a lane's part of a row is what one load brings (dim 128: 32 elements and their scale).
+  const auto dim_of = [&](int s) { return F4 ? DP / 4 * quarter + 8 * s : 32 * s + 8 * quarter; };
   vec8<T> qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const int d = 32 * s + 8 * quarter;
+    const int d = dim_of(s);
     qf[s] = vec8<T>{};
     if (col < heads && d < a.dim) qf[s] = *(const vec8<T> *)((const elem *)a.q + seq * a.q_stride[0] + (head0 + col) * a.q_stride[1] + d);
   }
@@ -133,43 +188,88 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
   int page = -1;  // of token `lane & 31` of the tile after the one being loaded
   const auto page_of = [&](int t) {
     const int x = t * 32 + (lane & 31);
-    page = t < tiles && x < n ? a.crd[first + ((from + x) >> a.page_log2)] : -1;
+    page = -1;
+    if (t < tiles && x < n) {
+      if constexpr (WINDOW) page = a.table[seq * a.table_width + (w.token(from + x) >> a.page_log2)];
+      else page = a.crd[first + ((from + x) >> a.page_log2)];
+    }
   };
   unsigned there_next = 0;
   const auto put_tokens = [&](int t) {  // pages into places of rows, for lanes 0 .. 31
     Tokens &x = tokens_of[wave][(t / 4) & 1];
     const bool there = (unsigned)page < (unsigned long long)a.pages;
     there_next = (unsigned)__ballot(there);
-    const int in = (from + t * 32 + (lane & 31)) & ((1 << a.page_log2) - 1);
+    const int number = from + t * 32 + (lane & 31), in = (WINDOW ? w.token(number) : number) & ((1 << a.page_log2) - 1);
     if (lane < 32) {
       x.at[lane] = there ? page * a.stride[0] + kh * a.stride[1] + in * a.stride[2] : 0;
-      if (F8) {
+      if (CODES != kNoCodes) {
         const long long s = there ? page * a.scale_stride[0] + kh * a.scale_stride[1] + in * a.scale_stride[2] : 0;
-        x.ks[lane] = there ? a.k_scale[s] : 0.f;
-        const float vs = there ? a.v_scale[s] : 0.f;
-        x.vs[lane] = SCALED ? 2.f * __builtin_amdgcn_frexp_mantf(vs) : vs;  // (of an infinity or NaN: itself, and its power is infinite)
-        if (SCALED) x.vp[lane % RP * PASSES + lane / RP] = power_of_two(vs);
+        if constexpr (F4) {
+          x.scale_at[lane] = s;
+        } else {
+          x.ks[lane] = there ? ((const float *)a.k_scale)[s] : 0.f;
+          const float vs = there ? ((const float *)a.v_scale)[s] : 0.f;
+          x.vs[lane] = SCALED ? 2.f * __builtin_amdgcn_frexp_mantf(vs) : vs;  // (of an infinity or NaN: itself, and its power is infinite)
+          if (SCALED) x.vp[lane % RP * PASSES + lane / RP] = power_of_two(vs);
+        }
       }
     }
     wave_lds_sync();
   };
-  raw kr[2][KS], vr[PASSES];
+  raw kr[2][KS];
+  raw_v vr[PASSES];
+  constexpr int K_SCALES = DP > 128 ? 2 : 1;  // of a lane's part of a row in 4 bits
+  unsigned kb[F4 ? 2 : 1][K_SCALES], vb[F4 ? PASSES : 1];
   const auto load = [&](int t) {
     const Tokens &x = tokens_of[wave][(t / 4) & 1];
+    if constexpr (F4) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const char *k = a.k + x.at[16 * i + col] * WIDTH;
+      for (int i = 0; i < 2; ++i) {
+        const char *k = a.k + x.at[16 * i + col] / 2;
+        const unsigned char *scales = (const unsigned char *)a.k_scale + x.scale_at[16 * i + col];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d = 32 * s + 8 * quarter;
-        kr[i][s] = *(const raw *)(k + (d < a.dim ? d : 0) * WIDTH);
-        if (a.dim < 32 * s + 32 && d >= a.dim) kr[i][s] = raw{};
+        for (int g = 0; g < K_SCALES; ++g) {  // 32 elements at a time (dim 64: 16)
+          const int d = DP / 4 * quarter + 32 * g;
+          const bool inside = d < a.dim;
+          const char *from = k + (inside ? d / 2 : 0);
+          kb[i][g] = scales[inside ? d / 32 : 0];
+          if constexpr (DP == 64) {
+            const v2u two = *(const v2u *)from;
+            kr[i][0] = two[0], kr[i][1] = two[1];
+          } else {
+            const v4u four = *(const v4u *)from;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) kr[i][4 * g + s] = four[s];
+          }
+          if (!inside) kb[i][g] = 127;
+#pragma unroll
+          for (int s = 0; s < KS / K_SCALES; ++s)
+            if (!inside) kr[i][KS / K_SCALES * g + s] = 0;
+        }
       }
-    }
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int d = (lane % PIECES) * 8;
-      vr[p] = *(const raw *)(a.v + (x.at[p * RP + lane / PIECES] + (d < a.dim ? d : 0)) * WIDTH);
+      for (int p = 0; p < PASSES; ++p) {
+        const int d = (lane % V_PIECES) * 32, row = p * RP + lane / V_PIECES;
+        const bool inside = d < a.dim;
+        vr[p] = *(const raw_v *)(a.v + (x.at[row] + (inside ? d : 0)) / 2);
+        vb[p] = ((const unsigned char *)a.v_scale)[x.scale_at[row] + (inside ? d / 32 : 0)];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const char *k = a.k + x.at[16 * i + col] * WIDTH;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int d = 32 * s + 8 * quarter;
+          kr[i][s] = *(const raw *)(k + (d < a.dim ? d : 0) * WIDTH);
+          if (a.dim < 32 * s + 32 && d >= a.dim) kr[i][s] = raw{};
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int d = (lane % PIECES) * 8;
+        vr[p] = *(const raw_v *)(a.v + (x.at[p * RP + lane / PIECES] + (d < a.dim ? d : 0)) * WIDTH);
+      }
     }
   };
 
@@ -193,6 +293,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
       for (int x = 0; x < KS; ++x) {
         vec8<T> k;
         if constexpr (F8) k = codes_to<T>(kr[i][x]);
+        else if constexpr (F4) k = codes_to<T>(kr[i][x], scale_of_byte(kb[i][x / (KS / K_SCALES)]));
         else k = __builtin_bit_cast(vec8<T>, kr[i][x]);
         s[i] = mfma16(k, qf[x], s[i]);
       }
@@ -205,13 +306,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
     }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int r = p * RP + lane / PIECES, piece = lane % PIECES;
-      vec8<T> v;
-      if constexpr (SCALED) v = codes_to<T>(vr[p], tok.vp[lane / PIECES * PASSES + p] * per_unit);
-      else if constexpr (F8) v = codes_to<T>(vr[p]);
-      else v = __builtin_bit_cast(vec8<T>, vr[p]);
-      if (there != 0xffffffffu && !(there >> r & 1)) v = vec8<T>{};  // whatever an unused slot holds: 0 times it must be 0
-      *(vec8<T> *)(mine.v + r * DP + ((piece ^ turn16<DP>(r)) * 8)) = v;
+      const int r = p * RP + lane / V_PIECES, piece = lane % V_PIECES;
+      const bool used = there == 0xffffffffu || (there >> r & 1);  // whatever an unused slot holds: 0 times it must be 0
+      const auto put = [&](int at, vec8<T> v) { *(vec8<T> *)(mine.v + r * DP + ((at ^ turn16<DP>(r)) * 8)) = used ? v : vec8<T>{}; };
+      if constexpr (F4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put(4 * piece + i, codes_to<T>(vr[p][i], scale_of_byte(vb[p])));
+      } else if constexpr (SCALED) {
+        put(piece, codes_to<T>(vr[p], tok.vp[lane / PIECES * PASSES + p] * per_unit));
+      } else if constexpr (F8) {
+        put(piece, codes_to<T>(vr[p]));
+      } else {
+        put(piece, __builtin_bit_cast(vec8<T>, vr[p]));
+      }
     }
     const unsigned now = there;
     put_tokens(t + 4);
@@ -220,7 +327,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
     page_of(t + 8);
 
     float ks[8], vs[8];
-    if (F8) {
+    if constexpr (F8) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const v4f k4 = *(const v4f *)(tok.ks + 16 * i + 4 * quarter), v4 = *(const v4f *)(tok.vs + 16 * i + 4 * quarter);
@@ -283,7 +390,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
   __syncthreads();
 
   const bool whole = count <= chunk;
-  const long long unit_id = (long long)(a.each ? u : u * a.kv_heads + kh) * a.head_tiles + ht;
+  const long long unit_id = (long long)(!WINDOW && a.each ? u : u * a.kv_heads + kh) * a.head_tiles + ht;
   for (int x = tid; x < 16 * PIECES; x += 256) {
     const int h = x / PIECES, d = (x % PIECES) * 8;
     if (h >= heads || d >= a.dim) continue;
@@ -315,7 +422,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : F8 ? 3 : 2) void paged_kernel(P
 
 // Lists of several units: one workgroup per (sequence, head), 64 units at a time, a quarter of them to each wavefront and
 // four of those on their way (one after the other they took 45 us for 64 units); always in the same order.
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   typedef typename T::elem elem;
   constexpr int E = DP / 64;
@@ -323,14 +430,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   __shared__ float factor[64];
   __shared__ __attribute__((aligned(16))) float part[3][DP];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.y, head = blockIdx.x, kh = head / a.group, in = head - kh * a.group;
-  const long long row = a.each ? (long long)seq * a.kv_heads + kh : seq;
+  const long long row = !WINDOW && a.each ? (long long)seq * a.kv_heads + kh : seq;
   int first, count;
-  list_of(a, row, &first, &count);
-  const int chunk = a.chunk << a.page_log2, needed = (int)(((long long)count + chunk - 1) / chunk);
+  if constexpr (WINDOW) count = window_of(a, seq).count;
+  else list_of(a, row, &first, &count);
+  const int chunk = a.chunk_tokens, needed = (int)(((long long)count + chunk - 1) / chunk);
   if (needed <= 1) return;
-  const long long u0 = unit_start(a, row);
+  const long long u0 = WINDOW ? row * a.units_each : unit_start(a, row);
   const int units = (int)min((long long)needed, a.units - u0);  // fewer only where positions descend
-  const auto id = [&](int x) { return ((a.each ? u0 + x : (u0 + x) * a.kv_heads + kh) * a.head_tiles + in / 16) * 16 + in % 16; };
+  const auto id = [&](int x) { return ((!WINDOW && a.each ? u0 + x : (u0 + x) * a.kv_heads + kh) * a.head_tiles + in / 16) * 16 + in % 16; };
   float most = -INFINITY;
   for (int x = lane; x < units; x += 64) most = fmaxf(most, a.sums[id(x) * 2]);
   for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
@@ -376,67 +484,116 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   if (a.lse && lane == 0) a.lse[(long long)seq * a.heads + head] = sum == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
-template <typename T, bool F8, int DP>
+// Whether some sequence may have several units, whose results are joined.
+bool several_units(const PagedArgs &a) { return a.windowed ? a.units_each > 1 : a.nnz > a.chunk; }
+
+template <typename T, int CODES, int DP, bool WINDOW>
 int launch_paged(const PagedArgs &a, hipStream_t st) {
-  const long long blocks = (long long)a.units * (a.each ? 1 : a.kv_heads) * a.head_tiles;
+  const long long blocks = (long long)a.units * (!WINDOW && a.each ? 1 : a.kv_heads) * a.head_tiles;
   LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "paged_attention: %lld units of work", blocks);
-  hipLaunchKernelGGL((paged_kernel<T, F8, DP>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((paged_kernel<T, CODES, DP, WINDOW>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   LAPIS_LAUNCH_CHECK();
-  if (a.nnz > a.chunk) {  // some list may have several units
-    hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(256), 0, st, a);
+  if (several_units(a)) {
+    hipLaunchKernelGGL((paged_join_kernel<T, DP, WINDOW>), dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(256), 0, st, a);
     LAPIS_LAUNCH_CHECK();
   }
   return LAPIS_HIP_OK;
 }
 
-template <typename T, bool F8>
-int launch_paged(const PagedArgs &a, hipStream_t st) {
-  return a.dim <= 64 ? launch_paged<T, F8, 64>(a, st) : a.dim <= 128 ? launch_paged<T, F8, 128>(a, st) : launch_paged<T, F8, 256>(a, st);
+template <bool WINDOW>
+int launch_paged(const PagedArgs &a, int dtype, int cache_dtype, hipStream_t st) {
+  const auto with = [&](auto type, auto codes) {
+    typedef decltype(type) T;
+    constexpr int CODES = decltype(codes)::value;
+    return a.dim <= 64 ? launch_paged<T, CODES, 64, WINDOW>(a, st) : a.dim <= 128 ? launch_paged<T, CODES, 128, WINDOW>(a, st) : launch_paged<T, CODES, 256, WINDOW>(a, st);
+  };
+  const auto of = [&](auto type) {
+    switch (codes_of(cache_dtype)) {
+      case kF4: return with(type, std::integral_constant<int, kF4>());
+      case kF8: return with(type, std::integral_constant<int, kF8>());
+      default: return with(type, std::integral_constant<int, kNoCodes>());
+    }
+  };
+  return dtype == LAPIS_HIP_BF16 ? of(Bf16()) : of(F16());
 }
 
-int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_paged_args *p, PagedArgs *a) {
-  const int rc = check_cache(what, c);
-  if (rc != LAPIS_HIP_OK) return rc;
-  LAPIS_REQUIRE(p, "%s: null arguments", what);
-  LAPIS_REQUIRE(p->seqs >= 0 && p->seqs <= 65535 && p->heads >= 0 && p->heads <= 65535 && p->heads % c->heads == 0,
-                "%s: %lld sequences and %lld heads over a cache of %d", what, (long long)p->seqs, (long long)p->heads, c->heads);
-  LAPIS_REQUIRE(p->lists == p->seqs || p->lists == p->seqs * c->heads, "%s: %lld lists of pages for %lld sequences", what,
-                (long long)p->lists, (long long)p->seqs);
-  LAPIS_REQUIRE(p->nnz >= 0 && p->nnz <= INT32_MAX && p->nnz * c->page <= INT32_MAX, "%s: %lld pages listed", what, (long long)p->nnz);
-  LAPIS_REQUIRE(p->lists <= INT32_MAX, "%s: %lld lists", what, (long long)p->lists);
-  LAPIS_REQUIRE(is_16bit(p->dtype) && (c->dtype == p->dtype || c->dtype == LAPIS_HIP_F8E4M3), "%s: queries of type %d and a cache of type %d",
-                what, p->dtype, c->dtype);
+// What calls over lists and over windows have alike.
+int read_paged(const char *what, const lapis_hip_kv_cache *c, int64_t seqs, int64_t heads, int dtype, const lapis_hip_rows &q, const lapis_hip_rows &out,
+               float *lse, float scale, PagedArgs *a) {
+  LAPIS_REQUIRE(seqs >= 0 && seqs <= 65535 && heads >= 0 && heads <= 65535 && heads % c->heads == 0,
+                "%s: %lld sequences and %lld heads over a cache of %d", what, (long long)seqs, (long long)heads, c->heads);
+  LAPIS_REQUIRE(is_16bit(dtype) && (c->dtype == dtype || codes_of(c->dtype) != kNoCodes), "%s: queries of type %d and a cache of type %d", what, dtype, c->dtype);
   *a = {};
-  a->q = static_cast<const char *>(p->q.data);
-  a->out = static_cast<char *>(p->out.data);
-  for (int i = 0; i < 2; ++i) a->q_stride[i] = p->q.stride[2 * i], a->out_stride[i] = p->out.stride[2 * i];
+  a->q = static_cast<const char *>(q.data);
+  a->out = static_cast<char *>(out.data);
+  for (int i = 0; i < 2; ++i) a->q_stride[i] = q.stride[2 * i], a->out_stride[i] = out.stride[2 * i];
   a->k = static_cast<const char *>(c->k);
   a->v = static_cast<const char *>(c->v);
   a->k_scale = c->k_scale;
   a->v_scale = c->v_scale;
   for (int i = 0; i < 3; ++i) a->stride[i] = c->stride[i], a->scale_stride[i] = c->scale_stride[i];
   a->pages = c->pages;
-  a->nnz = p->nnz;
-  a->seqs = (int)p->seqs;
-  a->heads = (int)p->heads;
+  a->seqs = (int)seqs;
+  a->heads = (int)heads;
   a->kv_heads = c->heads;
   a->dim = c->dim;
   a->page_log2 = __builtin_ctz((unsigned)c->page);
+  a->lse = lse;
+  a->scale = scale;
+  a->group = a->heads / c->heads;
+  a->head_tiles = (int)ceil_div(std::max(a->group, 1), 16);
+  return LAPIS_HIP_OK;
+}
+
+int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_paged_args *p, PagedArgs *a) {
+  int rc = check_cache(what, c);
+  if (rc != LAPIS_HIP_OK) return rc;
+  LAPIS_REQUIRE(p, "%s: null arguments", what);
+  rc = read_paged(what, c, p->seqs, p->heads, p->dtype, p->q, p->out, p->lse, p->scale, a);
+  if (rc != LAPIS_HIP_OK) return rc;
+  LAPIS_REQUIRE(p->lists == p->seqs || p->lists == p->seqs * c->heads, "%s: %lld lists of pages for %lld sequences", what,
+                (long long)p->lists, (long long)p->seqs);
+  LAPIS_REQUIRE(p->nnz >= 0 && p->nnz <= INT32_MAX && p->nnz * c->page <= INT32_MAX, "%s: %lld pages listed", what, (long long)p->nnz);
+  LAPIS_REQUIRE(p->lists <= INT32_MAX, "%s: %lld lists", what, (long long)p->lists);
+  a->nnz = p->nnz;
   a->each = p->lists != p->seqs;
   a->pos = p->pos;
   a->crd = p->crd;
   a->tokens = p->tokens;
-  a->lse = p->lse;
-  a->scale = p->scale;
   a->lists = (int)p->lists;
-  a->group = a->heads / c->heads;
-  a->head_tiles = (int)ceil_div(std::max(a->group, 1), 16);
   // Units for two workgroups a compute unit, of 128 to 1024 tokens: shorter ones cost more than they spread (a partial result
   // and its join), longer ones leave compute units waiting for the last.
   const int64_t copies = (int64_t)a->head_tiles * (a->each ? 1 : c->heads), wanted = std::max(2 * device_cu_count(), 1);
   const int64_t tokens = std::min<int64_t>(std::max<int64_t>(p->nnz * c->page * copies / wanted, 128), 1024);
   a->chunk = (int)std::max<int64_t>(tokens / c->page, 1);
+  a->chunk_tokens = a->chunk * c->page;
   const int64_t units = p->nnz / a->chunk + p->lists;
+  LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
+  a->units = (int)units;
+  return LAPIS_HIP_OK;
+}
+
+int read_window(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_paged_window_args *p, PagedArgs *a) {
+  int rc = check_cache(what, c);
+  if (rc != LAPIS_HIP_OK) return rc;
+  LAPIS_REQUIRE(p, "%s: null arguments", what);
+  rc = read_paged(what, c, p->seqs, p->heads, p->dtype, p->q, p->out, p->lse, p->scale, a);
+  if (rc != LAPIS_HIP_OK) return rc;
+  LAPIS_REQUIRE(p->window >= 1 && p->sink >= 0, "%s: a window of %lld and the first %lld tokens", what, (long long)p->window, (long long)p->sink);
+  LAPIS_REQUIRE(p->table_width >= 0 && p->table_width <= INT32_MAX / c->page, "%s: a table of %lld pages", what, (long long)p->table_width);
+  a->windowed = true;
+  a->table = p->table;
+  a->lengths = p->lengths;
+  a->table_width = p->table_width;
+  const int64_t longest = p->table_width * c->page;
+  a->window = (int)std::min<int64_t>(p->window, INT32_MAX);
+  a->sink = (int)std::min<int64_t>(p->sink, INT32_MAX);
+  // tokens that count in a sequence, at most; units as above
+  const int64_t most = std::min(longest, std::min(p->window, longest) + std::min(p->sink, longest));
+  const int64_t copies = (int64_t)a->head_tiles * c->heads, wanted = std::max(2 * device_cu_count(), 1);
+  a->chunk_tokens = (int)(std::min<int64_t>(std::max<int64_t>(p->seqs * most * copies / wanted, 128), 1024) / 32 * 32);
+  a->units_each = (int)std::max<int64_t>(1, ceil_div(most, a->chunk_tokens));
+  const int64_t units = p->seqs * a->units_each;
   LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
   a->units = (int)units;
   return LAPIS_HIP_OK;
@@ -445,9 +602,9 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
 // bytes of the partial results, and where the sums lie behind them
 int64_t partial_bytes(const PagedArgs &a, int64_t *sums_at) {
   const int dp = a.dim <= 64 ? 64 : a.dim <= 128 ? 128 : 256;
-  const int64_t ids = (int64_t)a.units * (a.each ? 1 : a.kv_heads) * a.head_tiles * 16;
+  const int64_t ids = (int64_t)a.units * (!a.windowed && a.each ? 1 : a.kv_heads) * a.head_tiles * 16;
   *sums_at = ids * dp * 4;
-  return a.nnz > a.chunk ? ids * (dp + 2) * 4 : 0;
+  return several_units(a) ? ids * (dp + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -455,32 +612,62 @@ int64_t partial_bytes(const PagedArgs &a, int64_t *sums_at) {
 
 using namespace lapis;
 
-extern "C" int lapis_hip_paged_attention_work(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, int64_t *bytes) {
-  PagedArgs a;
-  const int rc = read_paged("paged_attention", cache, args, &a);
-  if (rc != LAPIS_HIP_OK) return rc;
-  LAPIS_REQUIRE(bytes, "paged_attention: null result");
+namespace {
+
+int paged_work(const PagedArgs &a, const char *what, int64_t *bytes) {
+  LAPIS_REQUIRE(bytes, "%s: null result", what);
   int64_t sums_at;
   *bytes = partial_bytes(a, &sums_at);
   return LAPIS_HIP_OK;
 }
 
-extern "C" int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, lapis_hip_stream_t stream) {
+int check_rows(const PagedArgs &a, const char *what, const lapis_hip_rows &q, const lapis_hip_rows &out) {
+  LAPIS_REQUIRE(aligned16(a.q) && aligned16(a.out) && strides_of_8(q.stride, 3) && strides_of_8(out.stride, 3),
+                "%s: queries or results that are not on 16-byte boundaries or strides that are no multiples of 8", what);
+  return LAPIS_HIP_OK;
+}
+
+int give_work(PagedArgs &a, const char *what, void *work) {
+  int64_t sums_at;
+  if (partial_bytes(a, &sums_at) == 0) return LAPIS_HIP_OK;
+  LAPIS_REQUIRE(work && aligned16(work), "%s: work that is null or not on a 16-byte boundary", what);
+  a.partial = static_cast<float *>(work);
+  a.sums = reinterpret_cast<float *>(static_cast<char *>(work) + sums_at);
+  return LAPIS_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" int lapis_hip_paged_attention_work(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, int64_t *bytes) {
   PagedArgs a;
   const int rc = read_paged("paged_attention", cache, args, &a);
+  return rc != LAPIS_HIP_OK ? rc : paged_work(a, "paged_attention", bytes);
+}
+
+extern "C" int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const lapis_hip_paged_args *args, lapis_hip_stream_t stream) {
+  PagedArgs a;
+  int rc = read_paged("paged_attention", cache, args, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   if (a.seqs == 0 || a.heads == 0) return LAPIS_HIP_OK;
   LAPIS_REQUIRE(a.q && a.out && a.pos && a.tokens && (a.crd || a.nnz == 0), "paged_attention: null operands");
-  LAPIS_REQUIRE(aligned16(a.q) && aligned16(a.out) && strides_of_8(args->q.stride, 3) && strides_of_8(args->out.stride, 3),
-                "paged_attention: queries or results that are not on 16-byte boundaries or strides that are no multiples of 8");
-  int64_t sums_at;
-  if (partial_bytes(a, &sums_at) > 0) {
-    LAPIS_REQUIRE(args->work && aligned16(args->work), "paged_attention: work that is null or not on a 16-byte boundary");
-    a.partial = static_cast<float *>(args->work);
-    a.sums = reinterpret_cast<float *>(static_cast<char *>(args->work) + sums_at);
-  }
-  const bool f8 = cache->dtype == LAPIS_HIP_F8E4M3, bf16 = args->dtype == LAPIS_HIP_BF16;
-  const hipStream_t st = as_stream(stream);
-  if (bf16) return f8 ? launch_paged<Bf16, true>(a, st) : launch_paged<Bf16, false>(a, st);
-  return f8 ? launch_paged<F16, true>(a, st) : launch_paged<F16, false>(a, st);
+  rc = check_rows(a, "paged_attention", args->q, args->out);
+  if (rc == LAPIS_HIP_OK) rc = give_work(a, "paged_attention", args->work);
+  return rc != LAPIS_HIP_OK ? rc : launch_paged<false>(a, args->dtype, cache->dtype, as_stream(stream));
+}
+
+extern "C" int lapis_hip_paged_window_attention_work(const lapis_hip_kv_cache *cache, const lapis_hip_paged_window_args *args, int64_t *bytes) {
+  PagedArgs a;
+  const int rc = read_window("paged_window_attention", cache, args, &a);
+  return rc != LAPIS_HIP_OK ? rc : paged_work(a, "paged_window_attention", bytes);
+}
+
+extern "C" int lapis_hip_paged_window_attention(const lapis_hip_kv_cache *cache, const lapis_hip_paged_window_args *args, lapis_hip_stream_t stream) {
+  PagedArgs a;
+  int rc = read_window("paged_window_attention", cache, args, &a);
+  if (rc != LAPIS_HIP_OK) return rc;
+  if (a.seqs == 0 || a.heads == 0) return LAPIS_HIP_OK;
+  LAPIS_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0), "paged_window_attention: null operands");
+  rc = check_rows(a, "paged_window_attention", args->q, args->out);
+  if (rc == LAPIS_HIP_OK) rc = give_work(a, "paged_window_attention", args->work);
+  return rc != LAPIS_HIP_OK ? rc : launch_paged<true>(a, args->dtype, cache->dtype, as_stream(stream));
 }

@@ -109,6 +109,13 @@ _SIGNATURES = {
     "lapis_hip_kv_load": [_vp, _i64, _vp, _vp, _vp, _int, _vp],
     "lapis_hip_paged_attention_work": [_vp, _vp, ctypes.POINTER(_i64)],
     "lapis_hip_paged_attention": [_vp, _vp, _vp],
+    "lapis_hip_rotate": [_i64, _i64, _i64, _i64, _vp, _int, _vp, _vp, _int, _vp],
+    "lapis_hip_kv_append": [_vp, _vp, _vp],
+    "lapis_hip_paged_window_attention_work": [_vp, _vp, ctypes.POINTER(_i64)],
+    "lapis_hip_paged_window_attention": [_vp, _vp, _vp],
+    "lapis_hip_window_attention": [_vp, _vp],
+    "lapis_hip_window_attention_backward_work": [_vp, ctypes.POINTER(_i64)],
+    "lapis_hip_window_attention_backward": [_vp, _vp],
     "lapis_hip_block_pool": [_i64, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp, _vp, _vp],
     "lapis_hip_block_select_entries": [_vp, ctypes.POINTER(_i64)],
     "lapis_hip_block_select_work": [_vp, ctypes.POINTER(_i64)],
@@ -533,7 +540,10 @@ def bspmm_csrv(n1, n2, pos, crd, val, V, out, stream=None):
 def kv_store(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None, stream=None):
     """New tokens' keys and values (tokens x heads x dim) into slots (page * page size + place) of a cache in pages
     (pages x heads x page size x dim).  A float8_e4m3fn cache comes with scales (pages x heads x page size, float32):
-    each row is divided by its largest element / 448 and rounded.  Tokens whose slot is outside the cache are left out."""
+    each row is divided by its largest element / 448 and rounded.  A uint8 cache holds 4 bits an element (pages x heads x page
+    size x dim / 2, dim a multiple of 32, the even element in the low half) as 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign, times a power of
+    two for each 32 elements, 2 ** (byte - 127) of the scales (pages x heads x page size x dim / 32, uint8).  Tokens whose slot is
+    outside the cache are left out."""
     return _calls.kv_store(k, v, slots, k_cache, v_cache, k_scale, v_scale, stream)
 
 
@@ -542,11 +552,34 @@ def kv_load(k_cache, v_cache, slots, k, v, k_scale=None, v_scale=None, stream=No
     return _calls.kv_load(k_cache, v_cache, slots, k, v, k_scale, v_scale, stream)
 
 
+def rotate(x, positions, frequencies, out, neighbours=False, inverse=False, stream=None):
+    """Rows of x (batch x tokens x heads x dim) turned by their positions into ``out``, which may be x.  Pair i of a row of token t
+    is turned by the sum over axes of ``positions`` (axes x batch x tokens, int32) * ``frequencies`` (axes x pairs, float64, radians):
+    elements i and i + pairs, or with ``neighbours`` 2i and 2i + 1; elements from 2 * pairs on stay.  ``inverse`` turns back, which
+    is also the gradient."""
+    return _calls.rotate(x, positions, frequencies, out, neighbours, inverse, stream)
+
+
+def kv_append(k, v, positions, frequencies, slots, k_cache, v_cache, k_scale=None, v_scale=None, q=None, q_out=None, neighbours=False,
+              stream=None):
+    """``kv_store`` of keys that are turned by their positions (axes x tokens, as in ``rotate``) on the way, and of values; ``q`` (tokens
+    x query heads x dim) is turned into ``q_out``, which may be q.  One launch."""
+    return _calls.kv_append(k, v, positions, frequencies, slots, k_cache, v_cache, k_scale, v_scale, q, q_out, neighbours, stream)
+
+
 def paged_attention(q, k_cache, v_cache, pos, crd, tokens, out, lse=None, scale=None, k_scale=None, v_scale=None, stream=None):
     """One new token of each sequence (q: sequences x heads x dim) against the pages its CSR row (pos, crd) lists:
     ``tokens`` of them count.  One row per sequence, or one per sequence and key-value head.  ``scale`` defaults to
     dim ** -0.5; ``lse`` (sequences x heads, float32) gets the logarithms of the softmax sums."""
     return _calls.paged_attention(q, k_cache, v_cache, pos, crd, tokens, out, lse, scale, k_scale, v_scale, stream)
+
+
+def paged_window_attention(q, k_cache, v_cache, table, lengths, out, window, sink=0, lse=None, scale=None, k_scale=None, v_scale=None,
+                           stream=None):
+    """One new token of each sequence (q: sequences x heads x dim), the last of its ``lengths`` tokens (int32), against the last
+    ``window`` of them and the first ``sink``.  Token t of a sequence lies in page table[sequence, t // page size] (``table``: sequences x
+    pages, int32); entries of pages that hold no token of those are not read."""
+    return _calls.paged_window_attention(q, k_cache, v_cache, table, lengths, out, window, sink, lse, scale, k_scale, v_scale, stream)
 
 
 def block_pool(x, block, codes, scales, stream=None):
@@ -578,3 +611,15 @@ def block_attention_backward(dout, q, k, v, out, lse, pos, crd, dq, dk, dv, bloc
                              stream=None):
     """Gradients of ``block_attention`` from its inputs, its results and the gradient of ``out``."""
     return _calls.block_attention_backward(dout, q, k, v, out, lse, pos, crd, dq, dk, dv, block_m, block_n, causal, scale, stream)
+
+
+def window_attention(q, k, v, out, window, sink=0, lse=None, scale=None, stream=None):
+    """softmax(scale q k^T) v into ``out``, where query i, at p = i + keys - queries, sees the last ``window`` keys up to p and the
+    first ``sink``; ``lse`` (batch x heads x queries, float32) gets what the backward pass needs.  q: batch x queries x heads x dim; k, v:
+    batch x keys x kv_heads x dim."""
+    return _calls.window_attention(q, k, v, out, window, sink, lse, scale, stream)
+
+
+def window_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, window, sink=0, scale=None, stream=None):
+    """Gradients of ``window_attention`` from its inputs, its results and the gradient of ``out``."""
+    return _calls.window_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, window, sink, scale, stream)
