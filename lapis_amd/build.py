@@ -26,7 +26,7 @@ INCLUDE = os.path.join(ROOT, "include")
 
 KERNEL_SOURCES = ["runtime.hip", "spmv.hip", "rowchunk.hip", "colblock.hip", "colgroup.hip", "spmm.hip", "blas1.hip",
                   "cg.hip", "staging.hip", "calibrate.hip", "kvcache.hip", "rotate.hip", "paged.hip", "blockselect.hip", "blockattn.hip",
-                  "blockattn_bwd.hip"]
+                  "blockattn_bwd.hip", "windowattn_bwd.hip"]
 SHIM_SOURCES = ["module_shim.hip"]
 
 KERNEL_LIB = os.path.join(LIBDIR, "liblapis_hip.so")

@@ -122,6 +122,8 @@ struct KeyTiles {
 int read_block(const char *what, const lapis_hip_block_args *p, bool backward, BlockArgs *a);
 // Sizes of lists are left to the caller: block_m and rows.
 int read_window(const char *what, const lapis_hip_window_args *p, bool backward, BlockArgs *a);
+// dQ over windows, by lists of block_m queries; rowsum(dO * O) times `scale` and the log-sums in units of ln 2 are left in delta and logs.
+void launch_window_dq(const BlockArgs &a, bool bf16, bool few, float *delta, float *logs, hipStream_t st);
 // Queries a list gets where a workgroup has `rows` rows, a row for each head of the group.
 inline void cut_queries(BlockArgs *a, int rows) {
   a->block_m = std::max(1, rows / std::max(a->group, 1));

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
   __shared__ int bad_tile[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
-  if (block == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
+  if (!WINDOW && block == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
   const int list = block / tiles_of_list, part = block - list * tiles_of_list;
   const int bh = list / a.rows, r = list - bh * a.rows, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
   const int q0 = r * a.block_m, held = min(a.block_m, a.queries - q0), rows = held * a.group;
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
   };
   __shared__ __attribute__((aligned(16))) Own own[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
-  if (blockIdx.x == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
+  if (!WINDOW && blockIdx.x == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
   const int block = (int)(xcd_contiguous_block(blockIdx.x, gridDim.x) * (4 / SPLIT)) + wave / SPLIT, share = wave % SPLIT;
   const int list = block / tiles_of_list, part = block - list * tiles_of_list;
   const bool any = list < a.batch * a.kv_heads * a.rows;
@@ -402,40 +402,7 @@ struct Columns {
   int *rows;          // nnz
   float *partial;     // of columns of several units: dk and dv of each
   int chunks, chunk_rows, per_unit, units, lists, sub;
-  // Of a window: columns with first keys, which all later queries see, in units of `per_unit` queries and these many of them; the others.
-  int sink_columns, sink_units, per_unit_other, other_units;
 };
-
-// A unit of work of a window: its column (counted through all lists), its number among the column's, and how many queries those have.
-struct WindowUnit {
-  int column, part, per_unit, of_column;
-};
-__device__ __forceinline__ WindowUnit window_unit(const Columns &t, int columns, int u) {
-  WindowUnit x;
-  const int of_sinks = t.sink_columns * t.sink_units * t.lists;
-  if (u < of_sinks) {
-    const int c = u / t.sink_units, list = c / t.sink_columns;
-    x.part = u - c * t.sink_units;
-    x.column = list * columns + (c - list * t.sink_columns);
-    x.per_unit = t.per_unit;
-    x.of_column = t.sink_units;
-  } else {
-    u -= of_sinks;
-    const int c = u / t.other_units, others = columns - t.sink_columns, list = c / others;
-    x.part = u - c * t.other_units;
-    x.column = list * columns + t.sink_columns + (c - list * others);
-    x.per_unit = t.per_unit_other;
-    x.of_column = t.other_units;
-  }
-  return x;
-}
-// The queries that see some key of a column: from `first` on, these many.
-__device__ __forceinline__ void queries_of(const BlockArgs &a, int column, int *first, int *count) {
-  const int key0 = column << a.block_n_log2, key1 = min(key0 + (1 << a.block_n_log2), a.keys) - 1;
-  *first = max(0, key0 - a.shift);
-  const int last = key0 < a.sink ? a.queries - 1 : (int)min(a.queries - 1ll, (long long)key1 - a.shift + a.window - 1);
-  *count = max(0, last - *first + 1);
-}
 
 __global__ void clear_kernel(int *p) { p[threadIdx.x] = 0; }
 
@@ -734,8 +701,7 @@ struct DkvShared {
 
 // ODD: positions descend.  A body of its own, as the kernel's own look for rows among its units costs the loop registers (8192 queries, 16
 // blocks of 64: 547 us against 510).
-// WINDOW: the rows of a column are neighbouring queries.
-template <typename T, int DP, int KG, int S, bool ODD, bool WINDOW>
+template <typename T, int DP, int KG, int S, bool ODD>
 __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, KG, S> &mem) {
   typedef typename T::elem elem;
   typedef typename DkvShared<T, DP, KG, S>::Info Info;
@@ -792,18 +758,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
     const int u = unit_l / cols.sub, sub = unit_l - u * cols.sub;
     int cc, from = 0, n = 0, start = 0;
     bool several = false;
-    if constexpr (WINDOW) {
-      const WindowUnit x = window_unit(*(const Columns *)&at_start->cols, a.columns, u);
-      cc = x.column;
-      int all;
-      queries_of(*(const BlockArgs *)&at_start->a, cc % a.columns, &start, &all);
-      from = x.part * x.per_unit;
-      if (from >= all && x.part > 0) continue;
-      several = x.of_column > 1 && all > x.per_unit;
-      n = min(all - from, x.per_unit);
-      start += from;  // first query
-      from = u;       // where its sums go, if there are several
-    } else if (ODD) {
+    if (ODD) {
       cc = u;
       n = rows_that_name(*(const BlockArgs *)&at_start->a, cc, *cols.odd, rows_of_unit, mem.found);
       if (tid == 0) cols.end[cc] = n;
@@ -822,8 +777,6 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
     const int in_block = sub * 32 * KG + kg * 32;
     const int key_low = (column << a.block_n_log2) + in_block, key = key_low + (lane & 31);
     const bool live = in_block + (lane & 31) < (1 << a.block_n_log2) && key < a.keys;
-    const int window = WINDOW ? args.a.window : 0;
-    const bool first_key = WINDOW && key < args.a.sink;
 
     // Where rows lie is worked out for four tiles of a group at a time, a row to each of 128 threads: one wavefront doing it in
     // every iteration is what all others wait for.  A thread's row: entry, query of the block and head of the group.
@@ -841,9 +794,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
         const int lane = looks_up & 31;
         int query = 0;
         bool there = entry < n;
-        if constexpr (WINDOW) {
-          query = start + entry;
-        } else if (there) {
+        if (there) {
           query = rows_of_unit[entry] * a.block_m + in;
           there = query < a.queries;
         }
@@ -946,7 +897,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
         unsigned bad = 0;
         if (now) {
           const Info &info = infos[qg][t % (2 * BATCH)];
-          const bool cut = same(__any(last < key_low + 31 || (WINDOW && last - window >= key_low)));
+          const bool cut = same(__any(last < key_low + 31));
           const float *lse = sums[qg][t % S][0], *dl = sums[qg][t % S][1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -977,7 +928,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
             for (int j = 0; j < 4; ++j) {
               const v4i lim = *(const v4i *)(info.last + 8 * j + 4 * half);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * j + e] = key <= lim[e] && (!WINDOW || first_key || key > lim[e] - window) ? s[4 * j + e] : 0.f;
+              for (int e = 0; e < 4; ++e) s[4 * j + e] = key <= lim[e] ? s[4 * j + e] : 0.f;
             }
           }
 #pragma unroll
@@ -987,8 +938,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
           for (unsigned left = bad; left != 0; left &= left - 1) {
             const int row = __builtin_ctz(left);
             const float w = of_row<T>(f, row, lane);
-            const int lim = infos[qg][t % (2 * BATCH)].last[row];
-            const bool sees = key <= lim && (!WINDOW || first_key || key > lim - window);
+            const bool sees = key <= infos[qg][t % (2 * BATCH)].last[row];
 #pragma unroll
             for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -1076,7 +1026,7 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
     const DkvArgsAgain at_end = again();
     if (several) {
       const auto &cols = at_end->cols;
-      const long long slot = WINDOW ? from : 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << at_end->a.block_n_log2;
+      const long long slot = 2ll * (start / cols.per_unit) + from / cols.per_unit, each = (long long)DP << at_end->a.block_n_log2;
       float *to = cols.partial + (slot * 2 + 1 - role) * each + (long long)(in_block + (lane & 31)) * DP;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -1102,14 +1052,8 @@ __device__ __forceinline__ void dkv_units(const DkvArgs &args, DkvShared<T, DP, 
 template <typename T, int DP, int KG, int S>
 __global__ __launch_bounds__(256, 2) void block_dkv_kernel(DkvArgs args) {
   __shared__ DkvShared<T, DP, KG, S> mem;
-  if (same(*args.cols.odd != 0)) dkv_units<T, DP, KG, S, true, false>(args, mem);
-  else dkv_units<T, DP, KG, S, false, false>(args, mem);
-}
-
-template <typename T, int DP, int KG, int S>
-__global__ __launch_bounds__(256, 2) void window_dkv_kernel(DkvArgs args) {
-  __shared__ DkvShared<T, DP, KG, S> mem;
-  dkv_units<T, DP, KG, S, false, true>(args, mem);
+  if (same(*args.cols.odd != 0)) dkv_units<T, DP, KG, S, true>(args, mem);
+  else dkv_units<T, DP, KG, S, false>(args, mem);
 }
 
 // Columns of several units: their sums, in the order of the units.  NaN where the rows of a column were not found.
@@ -1130,37 +1074,6 @@ __global__ __launch_bounds__(256) void join_units_kernel(BlockArgs a, Columns co
     if (key >= a.keys || d >= a.dim) continue;
     const float none = lost ? __builtin_nanf("") : 0.f;
     v4f sum = {none, none, none, none};
-    for (int j = 0; j < units; ++j) {
-      const v4f y = *(const v4f *)(from + j * 2 * each + x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += y[e];
-    }
-    const View &v = is_v ? a.dv : a.dk;
-    vec4<T> o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (elem)sum[e];
-    *(vec4<T> *)((elem *)v.data + b * v.stride[0] + key * v.stride[1] + kh * v.stride[2] + d) = o;
-  }
-}
-
-// The same of a window: columns with first keys, then the others.
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void join_window_kernel(BlockArgs a, Columns cols, bool sinks) {
-  typedef typename T::elem elem;
-  const int unit = sinks ? blockIdx.x * cols.sink_units : cols.lists * cols.sink_columns * cols.sink_units + blockIdx.x * cols.other_units;
-  const WindowUnit u = window_unit(cols, a.columns, unit);
-  const int bh = u.column / a.columns, column = u.column - bh * a.columns, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
-  int first, all;
-  queries_of(a, column, &first, &all);
-  if (all <= u.per_unit) return;
-  const int units = (all + u.per_unit - 1) / u.per_unit;
-  const long long each = (long long)DP << a.block_n_log2;
-  const float *from = cols.partial + 2ll * unit * each;
-  for (long long x = (blockIdx.y * 256 + threadIdx.x) * 4; x < 2 * each; x += gridDim.y * 1024) {
-    const bool is_v = x >= each;
-    const int at = (int)(is_v ? x - each : x), d = at % DP, key = (column << a.block_n_log2) + at / DP;
-    if (key >= a.keys || d >= a.dim) continue;
-    v4f sum = {0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < units; ++j) {
       const v4f y = *(const v4f *)(from + j * 2 * each + x);
 #pragma unroll
@@ -1279,91 +1192,24 @@ int launch_backward(const BlockArgs &a, char *work, hipStream_t st) {
   return LAPIS_HIP_OK;
 }
 
-// ---- windows: host ---------------------------------------------------------------------------------------------
-
-struct WindowLayout {
-  int64_t delta, logs, next, partial, bytes;
-  bool few;  // rows: dQ by 16 of them
-  Columns columns;
-};
-
-int layout_of_window(BlockArgs *a, WindowLayout *layout) {
-  const char *what = "window_attention_backward";
-  WindowLayout &l = *layout = {};
-  a->block_n_log2 = 6;
-  a->columns = (int)ceil_div(a->keys, 64);
-  cut_queries(a, 128);
-  l.few = (int64_t)a->batch * a->kv_heads * a->rows * ceil_div(a->block_m * a->group, 128) < device_cu_count() / 2;  // the forward pass's rule
-  if (l.few) cut_queries(a, 16);
-  const int64_t lists = (int64_t)a->batch * a->kv_heads, columns = lists * a->columns;
-  const int64_t tiles = ceil_div((int64_t)a->block_m * a->group, l.few ? 16 : 128);
-  LAPIS_REQUIRE(lists <= 65535 && columns * 256 < (INT64_C(1) << 32), "%s: %lld lists of %d columns", what, (long long)lists, a->columns);
-  LAPIS_REQUIRE(lists * a->rows * tiles * 256 < (INT64_C(1) << 32), "%s: %lld rows", what, (long long)(lists * a->rows));
-  // Queries of a column.  Columns with first keys have all of them behind: they are cut into units as long as the others' columns, and all into
-  // shorter ones while there are not two for each compute unit.
-  Columns &c = l.columns;
-  c.lists = (int)lists;
-  c.sink_columns = (int)std::min<int64_t>(ceil_div(a->sink, 64), a->columns);
-  const int64_t others = a->columns - c.sink_columns, seen = std::max<int64_t>(1, std::min<int64_t>(a->queries, (int64_t)a->window + 63));
-  const int64_t group = std::max(a->group, 1), least = std::max<int64_t>(1, 256 / group);  // of a unit: fewer are not worth a join
-  const int64_t work = lists * (others * seen + (int64_t)c.sink_columns * a->queries);
-  const int64_t share = std::max<int64_t>(least, ceil_div(work, 2 * std::max(device_cu_count(), 1)));
-  const int64_t units_other = std::max<int64_t>(1, columns < 2 * device_cu_count() ? ceil_div(seen, share) : 1);
-  c.other_units = (int)units_other;
-  c.per_unit_other = (int)ceil_div(seen, units_other);
-  c.per_unit = (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(c.per_unit_other, least), std::max(a->queries, 1)));
-  c.sink_units = (int)std::max<int64_t>(1, ceil_div(a->queries, c.per_unit));
-  const int64_t units = lists * (c.sink_columns * (int64_t)c.sink_units + others * c.other_units);
-  LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
-  c.units = (int)units;
-  int64_t at = 0;
-  const auto take = [&](int64_t bytes) {
-    const int64_t here = at;
-    at += (bytes + 255) / 256 * 256;
-    return here;
-  };
-  l.delta = take(4ll * a->batch * a->heads * a->queries);
-  l.logs = take(4ll * a->batch * a->heads * a->queries);
-  l.next = take(4 * (1 + kParts));
-  const int64_t each = 2ll * (a->dim <= 64 ? 64 : 128) * 64 * 4;
-  const int64_t of_sinks = lists * c.sink_columns * (int64_t)c.sink_units;
-  l.partial = take((c.other_units > 1 ? units : c.sink_units > 1 ? of_sinks : 0) * each);
-  l.bytes = at;
-  return LAPIS_HIP_OK;
-}
-
-template <typename T, int DP>
-int launch_window_backward(BlockArgs a, char *work, hipStream_t st) {
-  WindowLayout l;
-  const int rc = layout_of_window(&a, &l);
-  if (rc != LAPIS_HIP_OK) return rc;
-  Columns &c = l.columns;
-  float *delta = reinterpret_cast<float *>(work + l.delta), *logs = reinterpret_cast<float *>(work + l.logs);
-  c.odd = reinterpret_cast<int *>(work + l.next);
-  c.next = c.odd + 1;
-  c.partial = reinterpret_cast<float *>(work + l.partial);
-  c.sub = 1;
-  const long long lists = c.lists;
-  if (a.rows && lists) {
-    const long long tiles = ceil_div((long long)a.block_m * a.group, l.few ? 16 : 128);
-    const auto kernel = l.few ? block_dq_narrow_kernel<T, DP, 4, true> : block_dq_kernel<T, DP, 4, 64, true>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(lists * a.rows * tiles)), dim3(256), 0, st, a, (int)tiles, delta, logs, c.odd);
-  }
-  if (lists && a.columns) {
-    if (a.rows == 0) hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1 + kParts), 0, st, c.odd);  // no dQ kernel has done it
-    a.block_m = 1;
-    const int64_t grid = std::min<int64_t>(2 * device_cu_count(), c.units);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, 2, 4>), dim3((unsigned)grid), dim3(256), 0, st, DkvArgs{a, c, delta, logs});
-    if (c.sink_units > 1 && c.sink_columns)
-      hipLaunchKernelGGL((join_window_kernel<T, DP>), dim3((unsigned)(lists * c.sink_columns), 8), dim3(256), 0, st, a, c, true);
-    if (c.other_units > 1 && a.columns > c.sink_columns)
-      hipLaunchKernelGGL((join_window_kernel<T, DP>), dim3((unsigned)(lists * (a.columns - c.sink_columns)), 8), dim3(256), 0, st, a, c, false);
-  }
-  LAPIS_LAUNCH_CHECK();
-  return LAPIS_HIP_OK;
-}
-
 }  // namespace
+
+void launch_window_dq(const BlockArgs &a, bool bf16, bool few, float *delta, float *logs, hipStream_t st) {
+  const long long tiles = ceil_div((long long)a.block_m * a.group, few ? 16 : 128);
+  const auto go = [&](auto type, auto dim) {
+    typedef decltype(type) T;
+    constexpr int DP = decltype(dim)::value;
+    const auto kernel = few ? block_dq_narrow_kernel<T, DP, 4, true> : block_dq_kernel<T, DP, 4, 64, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)a.batch * a.kv_heads * a.rows * tiles)), dim3(256), 0, st, a, (int)tiles, delta, logs, nullptr);
+  };
+  const auto with = [&](auto type) {
+    if (a.dim <= 64) go(type, std::integral_constant<int, 64>());
+    else go(type, std::integral_constant<int, 128>());
+  };
+  if (bf16) with(Bf16());
+  else with(F16());
+}
+
 }  // namespace lapis
 
 using namespace lapis;
@@ -1391,30 +1237,4 @@ extern "C" int lapis_hip_block_attention_backward(const lapis_hip_block_args *ar
   const bool bf16 = args->dtype == LAPIS_HIP_BF16;
   if (a.dim <= 64) return bf16 ? launch_backward<Bf16, 64>(a, work, as_stream(stream)) : launch_backward<F16, 64>(a, work, as_stream(stream));
   return bf16 ? launch_backward<Bf16, 128>(a, work, as_stream(stream)) : launch_backward<F16, 128>(a, work, as_stream(stream));
-}
-
-extern "C" int lapis_hip_window_attention_backward_work(const lapis_hip_window_args *args, int64_t *bytes) {
-  LAPIS_CHECK_INIT();  // the size goes by the number of compute units
-  BlockArgs a;
-  int rc = read_window("window_attention_backward", args, true, &a);
-  if (rc != LAPIS_HIP_OK) return rc;
-  LAPIS_REQUIRE(bytes, "window_attention_backward: null result");
-  WindowLayout l;
-  rc = layout_of_window(&a, &l);
-  *bytes = l.bytes;
-  return rc;
-}
-
-extern "C" int lapis_hip_window_attention_backward(const lapis_hip_window_args *args, lapis_hip_stream_t stream) {
-  LAPIS_CHECK_INIT();
-  BlockArgs a;
-  const int rc = read_window("window_attention_backward", args, true, &a);
-  if (rc != LAPIS_HIP_OK) return rc;
-  if (a.batch == 0 || (a.heads == 0 && a.kv_heads == 0)) return LAPIS_HIP_OK;
-  LAPIS_REQUIRE(args->work && aligned16(args->work), "window_attention_backward: work that is null or not on a 16-byte boundary");
-  char *work = static_cast<char *>(args->work);
-  const hipStream_t st = as_stream(stream);
-  const bool bf16 = args->dtype == LAPIS_HIP_BF16;
-  if (a.dim <= 64) return bf16 ? launch_window_backward<Bf16, 64>(a, work, st) : launch_window_backward<F16, 64>(a, work, st);
-  return bf16 ? launch_window_backward<Bf16, 128>(a, work, st) : launch_window_backward<F16, 128>(a, work, st);
 }

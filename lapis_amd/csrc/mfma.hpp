@@ -99,6 +99,13 @@ __device__ __forceinline__ void load_to_lds(const void *from, unsigned to) {
 __device__ __forceinline__ void load_word_to_lds(const void *from, unsigned to) {  // 4 bytes a lane
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
 }
+// the same from `offset` bytes behind an address that all lanes share
+__device__ __forceinline__ void load_to_lds(const void *from, unsigned offset, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+}
+__device__ __forceinline__ void load_word_to_lds(const void *from, unsigned offset, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+}
 // all but the last N loads of this wavefront
 template <int N = 0>
 __device__ __forceinline__ void lds_loads_done() {
