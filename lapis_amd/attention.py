@@ -1,13 +1,18 @@
-"""Block-sparse attention over CSR structures, put together: training or prefill over chosen blocks of keys, and decoding
-over the pages of a cache.
+"""Block-sparse attention over CSR structures, put together: training or prefill over chosen blocks of keys or over windows, and
+decoding over the pages of a cache.
 
 ``choose_blocks``   8-bit means of the blocks of queries and keys, and the best blocks of keys to each as a CSR structure
 ``attend``          attention over such a structure, differentiable in q, k and v
-``PagedCache``      keys and values in pages: ``prefill`` a sequence, ``step`` all of them by one token
+``rotate``          queries or keys turned by the positions of their tokens, differentiable
+``attend_window``   attention over the last keys of each query and the first ones, differentiable in q, k and v
+``PagedCache``      keys and values in pages: ``prefill`` a sequence, ``step`` or ``step_window`` all of them by one token
 
 ``python -m lapis_amd.attention`` trains one layer to look values up in a long sequence, then answers from a cache token by
 token.  Tensors are torch CUDA tensors of bfloat16 or float16: q is batch x queries x heads x dim, k and v are batch x keys x
 key-value heads x dim.
+
+A backward pass may be captured into a graph with the forward pass it belongs to.  As for all of torch's: no graph of autograd that was
+made outside of the capture may still live on the same leaves, or the process ends; drop its tensors first.
 """
 from dataclasses import dataclass
 
@@ -74,15 +79,70 @@ def attend(q, k, v, blocks, scale=None):
     return _Attend.apply(q, k, v, blocks, scale)
 
 
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, neighbours):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.neighbours = neighbours
+        return hip.rotate(x, positions, frequencies, torch.empty(x.shape, dtype=x.dtype, device=x.device), neighbours)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        dout = dout.contiguous()  # a broadcast one has strides that the kernel would take, but not every dout has
+        return hip.rotate(dout, *ctx.saved_tensors, torch.empty_like(dout), ctx.neighbours, True), None, None, None
+
+
+def rotate(x, positions, frequencies, neighbours=False):
+    """Queries or keys (x: batch x tokens x heads x dim) turned by their ``positions`` (axes x batch x tokens, int32) times
+    ``frequencies`` (axes x pairs, float64): elements i and i + pairs, or with ``neighbours`` 2i and 2i + 1.  Differentiable in x."""
+    return _Rotate.apply(x, positions, frequencies, neighbours)
+
+
+class _AttendWindow(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sink, scale):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device)
+        hip.window_attention(q, k, v, out, window, sink, lse, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.sizes = window, sink, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+        hip.window_attention_backward(dout.contiguous(), q, k, v, out, lse, dq, dk, dv, *ctx.sizes)
+        return dq, dk, dv, None, None, None
+
+
+def attend_window(q, k, v, window, sink=0, scale=None):
+    """softmax(scale q k^T) v where a query, the last of which stands at the last key, sees the last ``window`` keys up to its own and
+    the first ``sink``; ``scale`` defaults to dim ** -0.5."""
+    return _AttendWindow.apply(q, k, v, window, sink, scale)
+
+
 class PagedCache:
     """Keys and values of ``sequences`` sequences in pages, with the 8-bit mean of each full page.  ``dtype`` is that of the
-    rows that come in; with ``f8`` the cache holds them as e4m3 codes with a scale each."""
+    rows that come in; with ``f8`` the cache holds them as e4m3 codes with a scale each, with ``f4`` as codes of 4 bits with a power of
+    two for each 32 elements.  With ``frequencies`` (and ``neighbours``, as of ``rotate``) the queries and keys that come in are turned by the
+    positions of their tokens: by ``positions`` (axes x tokens, int32) where a call is given them, else by the numbers of the tokens in their
+    sequences on every axis."""
 
-    def __init__(self, sequences, pages, longest, heads, dim, page=64, dtype=torch.bfloat16, f8=False, device="cuda"):
-        kept = torch.float8_e4m3fn if f8 else dtype
-        self.page, self.dtype = page, dtype
-        self.k, self.v = (torch.zeros((pages, heads, page, dim), dtype=dtype, device=device).to(kept) for _ in range(2))
-        self.k_scale, self.v_scale = (torch.zeros((pages, heads, page), device=device) if f8 else None for _ in range(2))
+    def __init__(self, sequences, pages, longest, heads, dim, page=64, dtype=torch.bfloat16, f8=False, device="cuda", f4=False,
+                 frequencies=None, neighbours=False):
+        if f8 and f4:
+            raise ValueError("PagedCache: codes of 8 bits and of 4 bits")
+        if f4 and dim % 32:
+            raise ValueError("PagedCache: rows of %d elements, of which each 32 have a scale" % dim)
+        kept, row, scales = (torch.uint8, dim // 2, (dim // 32,)) if f4 else (torch.float8_e4m3fn if f8 else dtype, dim, ())
+        self.page, self.dtype, self.frequencies, self.neighbours = page, dtype, frequencies, neighbours
+        self.k, self.v = (torch.zeros((pages, heads, page, row), dtype=dtype, device=device).to(kept) for _ in range(2))
+        self.k_scale, self.v_scale = (
+            torch.zeros((pages, heads, page) + scales, dtype=torch.uint8 if f4 else torch.float32, device=device) if f8 or f4 else None
+            for _ in range(2))
         self.codes = torch.zeros((pages, heads, dim), dtype=torch.int8, device=device)
         self.scales = torch.zeros((pages, heads), device=device)
         self.table = torch.zeros((sequences, -(-longest // page)), dtype=torch.int32, device=device)
@@ -108,27 +168,49 @@ class PagedCache:
                 self.table[s, first:first + n] = torch.tensor(new, dtype=torch.int32).to(self.table.device)
             self.held[s] += new
 
-    def _store(self, k, v, slots):
-        hip.kv_store(k, v, slots, self.k, self.v, self.k_scale, self.v_scale)
+    def _store(self, q, k, v, slots, numbers, positions):
+        """Into ``slots``; tokens of these numbers in their sequences.  Returns q as it is used (None if there is none)."""
+        if self.frequencies is None:
+            hip.kv_store(k, v, slots, self.k, self.v, self.k_scale, self.v_scale)
+            return q
+        if positions is None:
+            positions = numbers.to(torch.int32).expand(self.frequencies.shape[0], -1)
+        turned = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        hip.kv_append(k, v, positions, self.frequencies, slots, self.k, self.v, self.k_scale, self.v_scale, q, turned, self.neighbours)
+        return turned
 
-    def _keep_means(self, pages, k):
-        """k: pages x page x heads x dim."""
+    def _keep_means(self, pages, k=None):
+        """k: pages x page x heads x dim; without it the keys are read back."""
+        if k is None:
+            slots = (pages[:, None] * self.page + torch.arange(self.page, device=pages.device)).to(torch.int32).reshape(-1)
+            rows, unused = (torch.empty((slots.numel(), self.k.shape[1], self.codes.shape[2]), dtype=self.dtype, device=pages.device)
+                            for _ in range(2))
+            hip.kv_load(self.k, self.v, slots, rows, unused, self.k_scale, self.v_scale)
+            k = rows.reshape(-1, self.page, *rows.shape[1:])
         codes, scales = _means(k, self.page, k.shape[2])
         self.codes[pages], self.scales[pages] = codes[:, :, 0], scales[:, :, 0]
 
-    def prefill(self, sequence, k, v):
-        """The tokens (k, v: tokens x heads x dim) of an empty sequence."""
+    def _check_positions(self, what, positions):
+        if positions is not None and self.frequencies is None:
+            raise ValueError("PagedCache.%s: positions, and no frequencies" % what)
+
+    def prefill(self, sequence, k, v, q=None, positions=None):
+        """The tokens (k, v: tokens x heads x dim) of an empty sequence.  Returns their queries (q: tokens x query heads x dim), turned
+        if the cache turns its keys."""
         if self.lengths[sequence]:
             raise ValueError("PagedCache.prefill: sequence %d holds %d tokens" % (sequence, self.lengths[sequence]))
+        self._check_positions("prefill", positions)
         tokens, page = k.shape[0], self.page
         self._open([sequence], tokens)
         t = torch.arange(tokens, device=k.device)
         slots = self.table[sequence][t // page] * page + t % page
-        self._store(k, v, slots.to(torch.int32))
+        q = self._store(q, k, v, slots.to(torch.int32), t, positions)
         full = tokens // page
         if full:
-            self._keep_means(self.table[sequence, :full].long(), k[:full * page].reshape(full, page, *k.shape[1:]))
+            self._keep_means(self.table[sequence, :full].long(),
+                             k[:full * page].reshape(full, page, *k.shape[1:]) if self.frequencies is None else None)
         self.length[sequence] = self.lengths[sequence] = tokens
+        return q
 
     def release(self, sequence):
         """Gives the pages of a sequence back."""
@@ -136,7 +218,19 @@ class PagedCache:
         self.held[sequence] = []
         self.length[sequence] = self.lengths[sequence] = 0
 
-    def step(self, q, k, v, count, sink=1, local=2, scale=None):
+    def _append(self, q, k, v, positions):
+        """A token more of every sequence.  Returns q as it is used and the lengths that the caller makes the cache's own when all is
+        done: what was written counts from then on."""
+        page, sequences = self.page, len(self.lengths)
+        self._open(range(sequences), 1)
+        at = self.table.gather(1, (self.length // page).long()[:, None])[:, 0]
+        q = self._store(q, k, v, at * page + self.length % page, self.length, positions)
+        length, lengths = self.length + 1, [n + 1 for n in self.lengths]
+        if any(n % page == 0 for n in lengths):  # pages that are full now
+            self._keep_means(torch.tensor([self.held[s][n // page - 1] for s, n in enumerate(lengths) if n % page == 0], device=k.device))
+        return q, length, lengths
+
+    def step(self, q, k, v, count, sink=1, local=2, scale=None, positions=None):
         """One token more of every sequence (k, v: sequences x heads x dim), and what it reads (q: sequences x query heads x
         dim) from the ``count`` best pages of each sequence and key-value head; the last ``local`` (at least 1) and first
         ``sink`` pages are always among them.  A sequence that was released begins anew with its token.  Where the call raises, the
@@ -145,19 +239,13 @@ class PagedCache:
             raise ValueError("PagedCache.step: the page of the token itself is always attended to: local = %d" % local)
         if sink < 0 or count < sink + local:
             raise ValueError("PagedCache.step: %d pages, the first %d and the last %d always among them" % (count, sink, local))
+        self._check_positions("step", positions)
         page, sequences, groups = self.page, len(self.lengths), self.k.shape[1]
-        q_codes, _ = _means(q[:, None], 1, groups)
-        self._open(range(sequences), 1)
-        at = self.table.gather(1, (self.length // page).long()[:, None])[:, 0]
-        self._store(k, v, at * page + self.length % page)
-        # the numbers of the cache itself change when all is done: what was written counts from then on
-        length, lengths = self.length + 1, [n + 1 for n in self.lengths]
-        if any(n % page == 0 for n in lengths):  # pages that are full now
-            pages = torch.tensor([self.held[s][n // page - 1] for s, n in enumerate(lengths) if n % page == 0], device=q.device)
-            slots = (pages[:, None] * page + torch.arange(page, device=q.device)).to(torch.int32).reshape(-1)
-            rows, unused = (torch.empty((slots.numel(), groups, q.shape[2]), dtype=self.dtype, device=q.device) for _ in range(2))
-            hip.kv_load(self.k, self.v, slots, rows, unused, self.k_scale, self.v_scale)
-            self._keep_means(pages, rows.reshape(-1, page, *rows.shape[1:]))
+        if self.frequencies is None:
+            q_codes, _ = _means(q[:, None], 1, groups)
+        q, length, lengths = self._append(q, k, v, positions)
+        if self.frequencies is not None:
+            q_codes, _ = _means(q[:, None], 1, groups)
 
         blocks = (length + (page - 1)) // page
         pos = torch.empty(sequences * groups + 1, dtype=torch.int32, device=q.device)
@@ -168,6 +256,16 @@ class PagedCache:
         tokens = (blocks.clamp(max=count) * page - (blocks * page - length)).repeat_interleave(groups)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         hip.paged_attention(q, self.k, self.v, pos, crd, tokens, out, None, scale, self.k_scale, self.v_scale)
+        self.length.copy_(length)
+        self.lengths = lengths
+        return out
+
+    def step_window(self, q, k, v, window, sink=0, scale=None, positions=None):
+        """As ``step``, but a token reads the last ``window`` tokens of its sequence, itself among them, and the first ``sink``."""
+        self._check_positions("step_window", positions)
+        q, length, lengths = self._append(q, k, v, positions)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        hip.paged_window_attention(q, self.k, self.v, self.table, length, out, window, sink, None, scale, self.k_scale, self.v_scale)
         self.length.copy_(length)
         self.lengths = lengths
         return out
