@@ -1,4 +1,10 @@
 // Rows turned by their positions, and on their way into a paged cache.
+//
+// Pair (x, y) of a row becomes (x cos - y sin, x sin + y cos) of an angle that is one for all heads of a token.  Bound by memory: 16384 tokens of 32 heads,
+// dim 128, bf16, three axes, in 55 us (4.9 TB/s read and written, what a large copy reaches); a prompt of 32768 tokens, 32 heads of queries and 8 of keys and
+// values, into 4-bit codes in 158 us (4.5 TB/s).  There it waits: its vector instructions take 70 % of the time, so everything that a row needs
+// (which row it is, its slot) is asked for before the angles are made and rows are numbered without divisions (193 us before).  48
+// tokens into 8-bit codes take 4 us, the launch.
 #include "kvcache.hpp"
 
 namespace lapis {
@@ -6,12 +12,25 @@ namespace {
 
 enum { kQuery = 0, kKey = 1, kValue = 2 };
 
+// Division of numbers below 2^31 by one that the host knows: q = r * m / 2^p, where p = 31 + ceil(log2 d) and m = ceil(2^p / d).  With
+// m d = 2^p + e, 0 <= e < d, q is too large by r e / (d 2^p) < 1 / d: not enough to reach the next integer.
+struct Divisor {
+  unsigned m, shift;
+  __host__ static Divisor of(int64_t d) {
+    unsigned p = 31;
+    while ((INT64_C(1) << (p - 31)) < d) ++p;
+    return {(unsigned)(((INT64_C(1) << p) + d - 1) / d), p};
+  }
+  __device__ __forceinline__ unsigned divide(unsigned r) const { return (unsigned)((unsigned long long)r * m >> shift); }
+};
+
 struct TurnArgs {
   const char *x[3];  // queries, keys, values
   char *out;         // of queries
   long long x_stride[3][3], out_stride[3];
   int heads, all_heads;  // of queries; with keys and values
   int tokens, dim, axes, pairs;
+  Divisor by_heads, by_tokens;  // all_heads, tokens
   long long rows;  // tokens of all batch entries times all heads
   bool neighbours;
   double sign;
@@ -22,15 +41,22 @@ struct TurnArgs {
   CacheView cache;
 };
 
-// Where a row lies: its token (of all batch entries), what it is, and which head.
+// Where a row lies: its token (of all batch entries), batch entry, what it is, and which head.
 struct Row {
-  unsigned token, head;
+  unsigned token, b, t, head;
   int kind;
+  __device__ __forceinline__ const char *data(const TurnArgs &a) const {  // (selects of values: an index would be a load before the load)
+    const auto one_of = [&](auto q, auto k, auto v) { return kind == kQuery ? q : kind == kKey ? k : v; };
+    const auto stride = [&](int i) { return one_of(a.x_stride[kQuery][i], a.x_stride[kKey][i], a.x_stride[kValue][i]); };
+    return one_of(a.x[kQuery], a.x[kKey], a.x[kValue]) + 2 * (b * stride(0) + t * stride(1) + head * stride(2));
+  }
 };
 __device__ __forceinline__ Row row_of(const TurnArgs &a, unsigned r) {
   Row x;
-  x.token = r / (unsigned)a.all_heads;
+  x.token = a.by_heads.divide(r);
   x.head = r - x.token * a.all_heads;
+  x.b = a.by_tokens.divide(x.token);
+  x.t = x.token - x.b * a.tokens;
   x.kind = kQuery;
   if (x.head >= (unsigned)a.heads) {
     x.head -= a.heads;
@@ -55,22 +81,23 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
   const bool inside = d < a.dim, whole = !a.neighbours && pairs % 8 == 0;  // whole: the other elements are eight neighbours too
   const int other = d < pairs ? d + pairs : d - pairs;
   vec8<T> x[N], y[N];
+  int slots[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const Row r = row_of(a, min(row0 + i * (256 / L), last_row));
-    const unsigned b = r.token / (unsigned)a.tokens, t = r.token - b * a.tokens;
-    const elem *p = (const elem *)a.x[r.kind] + b * a.x_stride[r.kind][0] + t * a.x_stride[r.kind][1] + r.head * a.x_stride[r.kind][2];
+    const elem *p = (const elem *)r.data(a);
     x[i] = y[i] = vec8<T>{};
+    slots[i] = r.kind == kQuery ? -1 : a.slots[r.token];
     if (inside) {
       x[i] = *(const vec8<T> *)(p + d);
       if (whole && d < 2 * pairs && r.kind != kValue) y[i] = *(const vec8<T> *)(p + other);
     }
   }
-  const unsigned t0 = (unsigned)block_row / a.all_heads, t1 = min((unsigned)block_row + (256 / L * N - 1), last_row) / a.all_heads;
+  const unsigned t0 = a.by_heads.divide((unsigned)block_row), t1 = a.by_heads.divide(min((unsigned)block_row + (256 / L * N - 1), last_row));
   const int angles = (int)(t1 - t0 + 1) * pairs;
   float *cosines = lds, *sines = lds + angles;
   for (int i = threadIdx.x; i < angles; i += 256) {
-    const unsigned tt = i / pairs, pair = i - tt * pairs, token = t0 + tt, b = token / (unsigned)a.tokens, t = token - b * a.tokens;
+    const unsigned tt = i / pairs, pair = i - tt * pairs, token = t0 + tt, b = a.by_tokens.divide(token), t = token - b * a.tokens;
     double angle = 0.0;
     for (int x = 0; x < a.axes; ++x)
       angle += (double)a.positions[x * a.position_stride[0] + b * a.position_stride[1] + t * a.position_stride[2]] * a.frequencies[x * pairs + pair];
@@ -85,7 +112,6 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
     const unsigned row = row0 + i * (256 / L);
     if (row > last_row) return;
     const Row r = row_of(a, row);
-    const unsigned b = r.token / (unsigned)a.tokens, t = r.token - b * a.tokens;
     float f[8];
     widen<T>(x[i], f);
     const int at = (int)(r.token - t0) * pairs;
@@ -93,9 +119,9 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
       if (whole) {
         float g[8];
         widen<T>(y[i], g);
-        const float *c = cosines + at + (d < pairs ? d : d - pairs), *s = sines + at + (d < pairs ? d : d - pairs);
+        const v4f *c = (const v4f *)(cosines + at + (d < pairs ? d : d - pairs)), *s = (const v4f *)(sines + at + (d < pairs ? d : d - pairs));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = f[j] * c[j] + g[j] * (d < pairs ? -s[j] : s[j]);
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * c[j / 4][j % 4] + g[j] * (d < pairs ? -s[j / 4][j % 4] : s[j / 4][j % 4]);
       } else if (a.neighbours) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -107,7 +133,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
           }
         }
       } else {
-        const elem *p = (const elem *)a.x[r.kind] + b * a.x_stride[r.kind][0] + t * a.x_stride[r.kind][1] + r.head * a.x_stride[r.kind][2];
+        const elem *p = (const elem *)r.data(a);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int e = d + j;
@@ -120,10 +146,10 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
       }
     }
     if (r.kind == kQuery) {
-      if (inside) *(vec8<T> *)((elem *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + r.head * a.out_stride[2] + d) = narrow<T>(f);
+      if (inside) *(vec8<T> *)((elem *)a.out + r.b * a.out_stride[0] + r.t * a.out_stride[1] + r.head * a.out_stride[2] + d) = narrow<T>(f);
       continue;
     }
-    const long long slot = a.slots[r.token];
+    const long long slot = slots[i];
     if (slot >= 0 && slot < a.cache.slots) put_elements<T, CODES, L>(a.cache, r.kind - kKey, slot, r.head, d, f);
   }
 }
@@ -150,14 +176,17 @@ int read_rows(const char *what, const lapis_hip_rows &r, const char **data, long
 }
 
 template <typename T, int CODES>
-int launch_turn(const TurnArgs &a, hipStream_t st) {
+int launch_turn(TurnArgs a, hipStream_t st) {
+  a.by_heads = Divisor::of(a.all_heads);
+  a.by_tokens = Divisor::of(a.tokens);
   const auto go = [&](auto lanes, auto times) {
     constexpr int L = decltype(lanes)::value, N = decltype(times)::value, ROWS = 256 / L * N;
     const int64_t tokens = std::min<int64_t>(ROWS, (ROWS - 2) / a.all_heads + 2);  // that a workgroup has rows of, at most
     hipLaunchKernelGGL((turn_kernel<T, CODES, L, N>), grid_of(ceil_div(a.rows, ROWS)), dim3(256), (size_t)(tokens * a.pairs * 8), st, a);
   };
   const auto with = [&](auto lanes) {
-    // four rows a thread only where that leaves every compute unit its workgroups
+    // four rows a thread only where that leaves every compute unit its workgroups (the prompt above with its reading back: 205 us, with two rows 210, with
+    // eight 225; the 16384 tokens 55, 59 and 60)
     if (a.rows * decltype(lanes)::value >= 256 * 16 * device_cu_count()) go(lanes, std::integral_constant<int, 4>());
     else go(lanes, std::integral_constant<int, 1>());
   };
