@@ -19,6 +19,7 @@ struct WindowColumns {
   int queries, shift, window;
   long long of_list, all, chunk;
   int workgroups;
+  bool whole;  // a cut in a column of all keys moves to its nearer end: such columns are one workgroup's each
   // Of each workgroup dk and dv of the column that it begins in the middle of, and of the one that it leaves unfinished; behind them, of each
   // list, those of whole columns that first keys are in: sink_columns of first keys, as many of all keys.
   float *partial;
@@ -78,6 +79,14 @@ __device__ __forceinline__ Column find_column(const WindowColumns &t, long long 
     lo += pick * step;
     n = min(step, n - pick * step);
   }
+}
+
+// Where the work of workgroup w begins, and that of the one before ends.
+__device__ __forceinline__ long long cut_of(const WindowColumns &t, long long w, int lane) {
+  const long long at = w * t.chunk;
+  if (!t.whole || at >= t.all) return min(at, t.all);
+  const Column c = find_column(t, at, lane);
+  return c.k < t.sink_columns ? at : at - c.start < c.end - at ? c.start : c.end;
 }
 
 // Row `row` (the same for all lanes) of a 32x32 product that has been rounded to an operand, in its column's lanes of both halves.
@@ -149,7 +158,7 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(DkvArgs) {
     return join<T>(read(at + rows + more), read((at ^ 32u) + rows + 8 * ROW + more));  // (row + 8: the other bit of its turn)
   };
 
-  const long long work_start = w * again().cols.chunk, work_end = min(work_start + again().cols.chunk, again().cols.all);
+  const long long work_start = cut_of(again().cols, w, lane), work_end = cut_of(again().cols, w + 1ll, lane);
   for (long long work = work_start; work < work_end;) {
     const DkvArgs &args = again();
     const BlockArgs &a = args.a;
@@ -455,10 +464,11 @@ __global__ __launch_bounds__(256) void window_join_kernel(BlockArgs a, WindowCol
         const int k = i ? cols.sink_columns + column : column;
         const long long edge = list * cols.of_list + cols.before(k + (lane & 1)), start = same_lane(edge, 0), end = same_lane(edge, 1);
         const long long w = start / cols.chunk, last = (end - 1) / cols.chunk;
+        const bool whole = w == last || (i && cols.whole);
         if (lane == 0) {
-          found_whole[i] = w == last;
-          found_from[i] = w == last ? 2ll * cols.workgroups + 2 * list * cols.sink_columns + k : w;
-          found_to[i] = w == last ? found_from[i] + 1 : last + 1;
+          found_whole[i] = whole;
+          found_from[i] = whole ? 2ll * cols.workgroups + 2 * list * cols.sink_columns + k : w;
+          found_to[i] = whole ? found_from[i] + 1 : last + 1;
         }
       }
     }
@@ -528,6 +538,7 @@ int layout_of(BlockArgs *a, WindowLayout *layout) {
   c.all = lists * c.of_list;
   c.chunk = std::max<int64_t>({1, ceil_div(c.all, cus), ceil_div(kLeastTiles * 32, group)});
   c.workgroups = (int)ceil_div(c.all, c.chunk);
+  c.whole = lists * c.columns <= cus && 2 * (a->window + kKeys + c.overhead) <= 3 * c.chunk;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -553,7 +564,7 @@ int launch_backward(BlockArgs a, char *work, hipStream_t st) {
   if (a.rows && c.lists) launch_window_dq(a, std::is_same<T, Bf16>::value, l.few, delta, logs, st);
   if (c.all) {
     hipLaunchKernelGGL((window_dkv_kernel<T, DP>), dim3((unsigned)c.workgroups), dim3(512), 0, st, DkvArgs{a, c, delta, logs});
-    const int joined = c.lists * c.sink_columns + c.workgroups - 1;
+    const int joined = c.lists * c.sink_columns + (c.whole ? 0 : c.workgroups - 1);
     if (joined) hipLaunchKernelGGL((window_join_kernel<T, DP>), dim3((unsigned)joined, 16), dim3(256), 0, st, a, c);
   }
   LAPIS_LAUNCH_CHECK();
