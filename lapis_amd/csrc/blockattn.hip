@@ -18,13 +18,13 @@ __device__ __forceinline__ float units_of_ln2(float scale) {
 // between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
 // 32 768 queries and keys, 32 heads over 8, dim 128, 16 blocks of 128 a row, bf16: 1290 to 1350 us, 800 to 765 TFLOP/s where a large library
 // product reaches 1203.  Bound by issue: 72 % of the cycles issue something, vector instructions 41 %, products 32 %.
-template <typename T, int DP, int NW, int KT, bool WINDOW>
-__global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
+template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
+__global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
-  __shared__ __attribute__((aligned(16))) elem k_tile[2][KT * DP], v_tile[2][KT * DP];
-  __shared__ int bad_tile[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  __shared__ __attribute__((aligned(16))) elem k_tile[SIDES][2][KT * DP], v_tile[SIDES][2][KT * DP];
+  __shared__ int bad_tile[SIDES][2];
+  const int tid = threadIdx.x % (64 * NW), side = SIDES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW)), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
   const int list = block / tiles_of_list, part = block - list * tiles_of_list;
   const int bh = list / a.rows, r = list - bh * a.rows, b = bh / a.kv_heads, kh = bh - b * a.kv_heads;
@@ -54,9 +54,9 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     if (live && d < a.dim) x = *(const v4i *)(qp + d);
     qf[s] = __builtin_bit_cast(vec8<T>, x ^ flip);
   }
-  KeyTiles<T, DP, NW, KT, true, WINDOW> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  KeyTiles<T, DP, NW, KT, true, WINDOW> keys(a, b, kh, first, count, tid, k_tile[side][0], v_tile[side][0]);
   if (WINDOW) keys.span = span_of(a, q0, held);
-  const int tiles = keys.tiles();
+  const int tiles = keys.tiles(), steps = SIDES == 1 ? tiles : (tiles + SIDES - 1) / SIDES;
   v4i now, next;  // first keys of each sixteen of this tile and the next
 
   v16f acc[DT];
@@ -65,15 +65,15 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   const float c = units_of_ln2(a.scale);
   float m = -INFINITY, l = 0.f;  // of this row; l of this half's keys
 
-  if (tid < 2) bad_tile[tid] = 0;
+  if (tid < 2) bad_tile[side][tid] = 0;
   if (a.dim < DP) {  // what no row fills stays zero
-    for (int i = tid; i < 2 * KT * PIECES; i += 64 * NW) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < SIDES * 2 * KT * PIECES; i += 64 * NW * SIDES) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
     __syncthreads();
   }
   int ahead = 0;
   if (tiles > 0) {
-    ahead = keys.look_up(1);
-    next = keys.spread(keys.look_up(0));
+    ahead = keys.look_up(SIDES + side);
+    next = keys.spread(keys.look_up(side));
     keys.template load<0>(next);
   }
   lds_loads_done();
@@ -81,23 +81,25 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
   const auto step = [&](int t, auto which) {
     constexpr int buffer = decltype(which)::value;  // t & 1, known where addresses are made
     now = next;
-    if (t + 1 < tiles) {
+    if (t + 1 < steps) {
       next = keys.spread(ahead);
-      ahead = keys.look_up(t + 2);
+      ahead = keys.look_up(SIDES * (t + 2) + side);
       keys.template load<1 - buffer>(next);
     }
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
-    if (top + 15 > low_of_all || (WINDOW && lowest <= gone_any_of_all)) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
+    const bool cuts = top + 15 > low_of_all || (WINDOW && lowest <= gone_any_of_all);
+    if (cuts) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
       bool bad = false;
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(v_tile[buffer] + (p * NW * 64 + tid) * 8));
-      if (__any(bad) && lane == 0) bad_tile[buffer] = t + 1;
-      __syncthreads();
+      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(v_tile[side][buffer] + (p * NW * 64 + tid) * 8));
+      if (__any(bad) && lane == 0) bad_tile[side][buffer] = t + 1;
+      if (SIDES == 1) __syncthreads();
     }
+    if (SIDES > 1) __syncthreads();  // of all, as one side's tile may be cut and not the other's
     if (lowest <= high) {
-      const elem *kt = k_tile[buffer], *vt = v_tile[buffer];
+      const elem *kt = k_tile[side][buffer], *vt = v_tile[side][buffer];
       v16f s[ST];
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
           l += s[x][e];
           pf[2 * x + (e >> 3)][e & 7] = (elem)s[x][e];
         }
-      if (cut && bad_tile[buffer] == t + 1) {
+      if (cut && bad_tile[side][buffer] == t + 1) {
         // the finite values as always; an infinity or NaN only to the rows that see its key
 #pragma unroll
         for (int y = 0; y < 2 * ST; ++y)
@@ -186,12 +188,34 @@ __global__ __launch_bounds__(64 * NW, 2) void block_forward_kernel(BlockArgs a, 
     lds_loads_done();
     __syncthreads();
   };
-  for (int t = 0; t < tiles; t += 2) {
+  for (int t = 0; t < steps; t += 2) {
     step(t, std::integral_constant<int, 0>());
-    if (t + 1 < tiles) step(t + 1, std::integral_constant<int, 1>());
+    if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>());
   }
 
   l = halves_sum(l);
+  if constexpr (SIDES > 1) {  // (the last step has ended with a barrier)
+    float *sums = (float *)k_tile + wave * (DT * 1024) + lane * 4;
+    float *rows_of_wave = (float *)v_tile + wave * 128 + lane;
+    if (side) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *(v4f *)(sums + (4 * i + e / 4) * 256) = v4f{acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]};
+      rows_of_wave[0] = m;
+      rows_of_wave[64] = l;
+    }
+    __syncthreads();
+    if (side) return;
+    const float other = rows_of_wave[0], most = fmaxf(m, other), off = most == -INFINITY ? 0.f : most;
+    const float mine = __builtin_amdgcn_exp2f(m - off), theirs = __builtin_amdgcn_exp2f(other - off);
+    l = l * mine + rows_of_wave[64] * theirs;
+    m = most;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][e] = acc[i][e] * mine + sums[(4 * i + e / 4) * 256 + e % 4] * theirs;
+  }
   const float factor = l == 0.f ? 0.f : 1.f / l;
   if (!live) return;
   elem *op = (elem *)a.out.data + b * a.out.stride[0] + query * a.out.stride[1] + head * a.out.stride[2];
@@ -409,11 +433,11 @@ int read_view(const char *what, const lapis_hip_rows &r, View *v) {
   return LAPIS_HIP_OK;
 }
 
-template <typename T, int DP, int NW, int KT, bool WINDOW>
+template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
 int launch_wide(const BlockArgs &a, hipStream_t st) {
   const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)std::min(a.block_m, a.queries) * a.group, 32 * NW);
-  LAPIS_REQUIRE(lists * tiles * 64 * NW < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
-  hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT, WINDOW>), dim3((unsigned)(lists * tiles)), dim3(64 * NW), 0, st, a, (int)tiles,
+  LAPIS_REQUIRE(lists * tiles * 64 * NW * SIDES < (INT64_C(1) << 32), "%s: %lld rows", WINDOW ? "window_attention" : "block_attention", lists);
+  hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT, WINDOW, SIDES>), dim3((unsigned)(lists * tiles)), dim3(64 * NW * SIDES), 0, st, a, (int)tiles,
                      a.scale < 0.f ? (int)0x80008000u : 0);
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
@@ -423,7 +447,7 @@ template <typename T, int DP, int SPLIT, bool WINDOW>
 int launch_narrow(const BlockArgs &a, hipStream_t st) {
   const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)a.block_m * a.group, 16);
   const long long blocks = ceil_div(lists * tiles * SPLIT, 4);
-  LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "block_attention: %lld rows of the structure", lists);
+  LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "%s: %lld rows", WINDOW ? "window_attention" : "block_attention", lists);
   hipLaunchKernelGGL((block_narrow_kernel<T, DP, SPLIT, WINDOW>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, a.scale < 0.f ? (int)0x80008000u : 0);
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;
@@ -451,6 +475,7 @@ int launch_window(BlockArgs a, hipStream_t st) {
     cut_queries(&a, 16);
     return a.dim <= 64 ? launch_narrow<T, 64, 4, true>(a, st) : launch_narrow<T, 128, 4, true>(a, st);
   }
+  if (few_workgroups(a)) return a.dim <= 64 ? launch_wide<T, 64, 4, 64, true, 2>(a, st) : launch_wide<T, 128, 4, 64, true, 2>(a, st);
   return a.dim <= 64 ? launch_wide<T, 64, 4, 64, true>(a, st) : launch_wide<T, 128, 4, 64, true>(a, st);
 }
 

@@ -130,4 +130,11 @@ inline void cut_queries(BlockArgs *a, int rows) {
   a->rows = a->heads ? (int)ceil_div(a->queries, a->block_m) : 0;
 }
 
+// Windows: no more workgroups of 128 rows than compute units, so that a SIMD would have one wavefront.  Then two sides of a workgroup share its
+// keys, by tiles in turn, and join through LDS.  One side and two, forward and dQ: 2048 queries, 16 heads, window 2048, dim 128: 66.7 and 48.2 us, 98.6 and
+// 78.9; 1024 queries, 32 heads over 8, window 512: 27.1 and 24.0, 40.3 and 37.1; window 100 of 1024 queries, 16 heads: 19.3 and 16.6, 23.6 and 22.4.
+inline bool few_workgroups(const BlockArgs &a) {
+  return (int64_t)a.batch * a.kv_heads * a.rows * ceil_div((int64_t)a.block_m * a.group, 128) <= device_cu_count();
+}
+
 }  // namespace lapis

@@ -26,13 +26,13 @@ __device__ __forceinline__ float of_row(const vec8<T> (&f)[2], int row, int lane
 // from its registers.  rowsum(dO * O), times `scale`, and the log-sums in units of ln 2 are left for the other kernel.
 // 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 309 us in a trace (356 with 24 registers spilled and the products
 // one chain after the other), 610 TFLOP/s; bound by what a wavefront waits for between its chains of products.
-template <typename T, int DP, int NW, int KT, bool WINDOW>
-__global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
+template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
+__global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
-  __shared__ __attribute__((aligned(16))) elem k_tile[2][KT * DP], v_tile[2][KT * DP];
-  __shared__ int bad_tile[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  __shared__ __attribute__((aligned(16))) elem k_tile[SIDES][2][KT * DP], v_tile[SIDES][2][KT * DP];
+  __shared__ int bad_tile[SIDES][2];
+  const int tid = threadIdx.x % (64 * NW), side = SIDES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW)), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const unsigned block = xcd_contiguous_block(blockIdx.x, gridDim.x);
   if (!WINDOW && block == 0 && tid <= kParts) odd[tid] = 0;  // for the kernels after this one: the flag and the counters behind it
   const int list = block / tiles_of_list, part = block - list * tiles_of_list;
@@ -77,26 +77,26 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     const long long at = ((long long)b * a.heads + head) * a.queries + query;
     const float lse = a.lse[at];
     off = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    if (half == 0) delta[at] = del, logs[at] = off;
+    if (half == 0 && side == 0) delta[at] = del, logs[at] = off;
   }
-  KeyTiles<T, DP, NW, KT, false, WINDOW> keys(a, b, kh, first, count, tid, k_tile[0], v_tile[0]);
+  KeyTiles<T, DP, NW, KT, false, WINDOW> keys(a, b, kh, first, count, tid, k_tile[side][0], v_tile[side][0]);
   if (WINDOW) keys.span = span_of(a, q0, held);
-  const int tiles = keys.tiles();
+  const int tiles = keys.tiles(), steps = SIDES == 1 ? tiles : (tiles + SIDES - 1) / SIDES;
   v4i now, next;  // first keys of each sixteen of this tile and the next
   v16f acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = v16f{};
   const float c = a.scale * kLog2e;
 
-  if (tid < 2) bad_tile[tid] = 0;
+  if (tid < 2) bad_tile[side][tid] = 0;
   if (a.dim < DP) {  // what no row fills stays zero
-    for (int i = tid; i < 2 * KT * PIECES; i += 64 * NW) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < SIDES * 2 * KT * PIECES; i += 64 * NW * SIDES) ((v4i *)k_tile)[i] = ((v4i *)v_tile)[i] = v4i{0, 0, 0, 0};
     __syncthreads();
   }
   int ahead = 0;
   if (tiles > 0) {
-    ahead = keys.look_up(1);
-    next = keys.spread(keys.look_up(0));
+    ahead = keys.look_up(SIDES + side);
+    next = keys.spread(keys.look_up(side));
     keys.template load<0>(next);
   }
   lds_loads_done();
@@ -104,25 +104,27 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
   const auto step = [&](int t, auto which) {
     constexpr int buffer = decltype(which)::value;  // t & 1, known where addresses are made
     now = next;
-    if (t + 1 < tiles) {
+    if (t + 1 < steps) {
       next = keys.spread(ahead);
-      ahead = keys.look_up(t + 2);
+      ahead = keys.look_up(SIDES * (t + 2) + side);
       keys.template load<1 - buffer>(next);
     }
     int lowest = now[0], top = now[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) lowest = min(lowest, now[i]), top = max(top, now[i]);
-    if (top + 15 > low_of_all || (WINDOW && lowest <= gone_any_of_all)) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
+    const bool cuts = top + 15 > low_of_all || (WINDOW && lowest <= gone_any_of_all);
+    if (cuts) {  // somebody's mask cuts this tile: 0 times an infinity or NaN must not count
       bool bad = false;
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(k_tile[buffer] + (p * NW * 64 + tid) * 8));
-      if (__any(bad) && lane == 0) bad_tile[buffer] = t + 1;
-      __syncthreads();
+      for (int p = 0; p < PASSES; ++p) bad |= not_finite<T>(*(const vec8<T> *)(k_tile[side][buffer] + (p * NW * 64 + tid) * 8));
+      if (__any(bad) && lane == 0) bad_tile[side][buffer] = t + 1;
+      if (SIDES == 1) __syncthreads();
     }
+    if (SIDES > 1) __syncthreads();  // of all, as one side's tile may be cut and not the other's
     if (lowest <= high) {
-      const elem *kt = k_tile[buffer], *vt = v_tile[buffer];
+      const elem *kt = k_tile[side][buffer], *vt = v_tile[side][buffer];
       const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
-      const bool bad = cut && bad_tile[buffer] == t + 1;
+      const bool bad = cut && bad_tile[side][buffer] == t + 1;
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
         int place_lane = lane;  // made anew each time, or the compiler keeps the places of all operands in registers
@@ -193,9 +195,24 @@ __global__ __launch_bounds__(64 * NW, 2) void block_dq_kernel(BlockArgs a, int t
     lds_loads_done();
     __syncthreads();
   };
-  for (int t = 0; t < tiles; t += 2) {
+  for (int t = 0; t < steps; t += 2) {
     step(t, std::integral_constant<int, 0>());
-    if (t + 1 < tiles) step(t + 1, std::integral_constant<int, 1>());
+    if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>());
+  }
+  if constexpr (SIDES > 1) {  // (the last step has ended with a barrier)
+    float *sums = (float *)k_tile + wave * (DT * 1024) + lane * 4;
+    if (side) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *(v4f *)(sums + (4 * i + e / 4) * 256) = v4f{acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]};
+    }
+    __syncthreads();
+    if (side) return;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][e] += sums[(4 * i + e / 4) * 256 + e % 4];
   }
   if (!live) return;
   elem *dp = (elem *)a.dq.data + b * a.dq.stride[0] + query * a.dq.stride[1] + head * a.dq.stride[2];
@@ -1199,8 +1216,9 @@ void launch_window_dq(const BlockArgs &a, bool bf16, bool few, float *delta, flo
   const auto go = [&](auto type, auto dim) {
     typedef decltype(type) T;
     constexpr int DP = decltype(dim)::value;
-    const auto kernel = few ? block_dq_narrow_kernel<T, DP, 4, true> : block_dq_kernel<T, DP, 4, 64, true>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)a.batch * a.kv_heads * a.rows * tiles)), dim3(256), 0, st, a, (int)tiles, delta, logs, nullptr);
+    const bool sides = !few && few_workgroups(a);
+    const auto kernel = few ? block_dq_narrow_kernel<T, DP, 4, true> : sides ? block_dq_kernel<T, DP, 4, 64, true, 2> : block_dq_kernel<T, DP, 4, 64, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)a.batch * a.kv_heads * a.rows * tiles)), dim3(sides ? 512 : 256), 0, st, a, (int)tiles, delta, logs, nullptr);
   };
   const auto with = [&](auto type) {
     if (a.dim <= 64) go(type, std::integral_constant<int, 64>());
