@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
   const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
   const int low_of_all = a.causal ? min(q0 + part * 32 * NW / a.group + a.shift, a.keys - 1) : a.keys - 1;
   const int row_last_of_all = min(part * 32 * NW + 32 * NW, rows) - 1;
-  const int gone = limit - a.window;  // last key before this row's window
+  const Sight<WINDOW> row_sees(a, limit);
   const int gone_any = high - a.window, gone_any_of_all = q0 + row_last_of_all / a.group + a.shift - a.window;
 
   vec8<T> qf[DP / 16];
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = now[2 * x + (e >> 3)] + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
-            if (key > limit || (WINDOW && key <= gone && key >= a.sink)) s[x][e] = -INFINITY;
+            s[x][e] = row_sees.sees(key) ? s[x][e] : -INFINITY;
           }
       }
       float best = s[0][0];
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
 #pragma unroll
           for (int i = 1; i < CH; ++i) key0 = x >> 4 == i ? now[i] : key0;
           const int key = key0 + (x & 15);
-          const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
+          const bool sees = row_sees.sees(key);
 #pragma unroll
           for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -280,7 +280,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
   }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  const int gone = limit - a.window, gone_any = high - a.window;  // last key before this row's window, and any row's
+  const Sight<WINDOW> row_sees(a, limit);
+  const int gone_any = high - a.window;  // last key before any row's window
   const int tiles = WINDOW ? (span.count + 1) / 2 : tiles_of<32>(a, count);
   const int piece = lane % PIECES, v_row = lane / PIECES, vd = piece * 8 < a.dim ? piece * 8 : 0;
   v4i kr[2][KS], vr[PASSES];
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = now[i] + 4 * quarter + e;
-        if (cut && (key > limit || (WINDOW && key <= gone && key >= a.sink))) s[i][e] = -INFINITY;
+        if (cut) s[i][e] = row_sees.sees(key) ? s[i][e] : -INFINITY;
         best = fmaxf(best, s[i][e]);
       }
     best = rows_max(best) * c;
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {
         const int key = (x < 16 ? now[0] : now[1]) + (x & 15);
-        const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
+        const bool sees = row_sees.sees(key);
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
           const int d = 16 * i + 4 * quarter;
@@ -436,7 +437,7 @@ int read_view(const char *what, const lapis_hip_rows &r, View *v) {
 template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
 int launch_wide(const BlockArgs &a, hipStream_t st) {
   const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)std::min(a.block_m, a.queries) * a.group, 32 * NW);
-  LAPIS_REQUIRE(lists * tiles * 64 * NW * SIDES < (INT64_C(1) << 32), "%s: %lld rows", WINDOW ? "window_attention" : "block_attention", lists);
+  LAPIS_REQUIRE(lists * tiles * 64 * NW * SIDES < (INT64_C(1) << 32), WINDOW ? "window_attention: %lld rows" : "block_attention: %lld rows of the structure", lists);
   hipLaunchKernelGGL((block_forward_kernel<T, DP, NW, KT, WINDOW, SIDES>), dim3((unsigned)(lists * tiles)), dim3(64 * NW * SIDES), 0, st, a, (int)tiles,
                      a.scale < 0.f ? (int)0x80008000u : 0);
   LAPIS_LAUNCH_CHECK();
@@ -447,7 +448,7 @@ template <typename T, int DP, int SPLIT, bool WINDOW>
 int launch_narrow(const BlockArgs &a, hipStream_t st) {
   const long long lists = (long long)a.batch * a.kv_heads * a.rows, tiles = ceil_div((long long)a.block_m * a.group, 16);
   const long long blocks = ceil_div(lists * tiles * SPLIT, 4);
-  LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "%s: %lld rows", WINDOW ? "window_attention" : "block_attention", lists);
+  LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), WINDOW ? "window_attention: %lld rows" : "block_attention: %lld rows of the structure", lists);
   hipLaunchKernelGGL((block_narrow_kernel<T, DP, SPLIT, WINDOW>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)tiles, a.scale < 0.f ? (int)0x80008000u : 0);
   LAPIS_LAUNCH_CHECK();
   return LAPIS_HIP_OK;

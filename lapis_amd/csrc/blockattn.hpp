@@ -59,6 +59,19 @@ __device__ __forceinline__ Span span_of(const BlockArgs &a, int q0, int held) {
   return s;
 }
 
+// Which keys a row sees: up to `limit`, and over a window the last ones of them and the first ones.  (Differences of whole numbers and no || or &&:
+// those become branches, a dozen instructions for each key of a tile that wait for one another.  1001 queries behind 2437 keys, window 300: 21.2 us and FIXME.)
+template <bool WINDOW>
+struct Sight {
+  int limit, sinks;
+  unsigned window;
+  __device__ __forceinline__ Sight(const BlockArgs &a, int limit_) : limit(WINDOW ? max(limit_, -1) : limit_), sinks(min(a.sink, limit + 1)), window((unsigned)a.window) {}
+  __device__ __forceinline__ bool sees(int key) const {
+    if constexpr (WINDOW) return (int)((unsigned)(limit - key) < window) | (int)(key < sinks);  // (0 <= limit - key < window)
+    else return key <= limit;
+  }
+};
+
 // Tiles of KT keys that a list has.  They are numbered with 31 bits: more would be 2^36 keys of one list, of the 2^30 there are.
 template <int KT>
 __device__ __forceinline__ int tiles_of(const BlockArgs &a, int count) {

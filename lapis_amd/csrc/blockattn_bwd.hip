@@ -51,7 +51,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
   const int high = __builtin_amdgcn_readfirstlane(a.causal ? min(q0 + row_last / a.group + a.shift, a.keys - 1) : a.keys - 1);
   const int low_of_all = a.causal ? min(q0 + part * 32 * NW / a.group + a.shift, a.keys - 1) : a.keys - 1;
   const int row_last_of_all = min(part * 32 * NW + 32 * NW, rows) - 1;
-  const int gone = limit - a.window;  // last key before this row's window
+  const Sight<WINDOW> row_sees(a, limit);
   const int gone_any = high - a.window, gone_any_of_all = q0 + row_last_of_all / a.group + a.shift - a.window;
 
   vec8<T> qf[DP / 16], gf[DP / 16];
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
           float ds = p * __builtin_fmaf(g[e], a.scale, -del);
           if (cut) {
             const int key = now[2 * x + (e >> 3)] + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
-            ds = key > limit || (WINDOW && key <= gone && key >= a.sink) ? 0.f : ds;
+            ds = row_sees.sees(key) ? ds : 0.f;
           }
           df[e >> 3][e & 7] = (elem)ds;
         }
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
 #pragma unroll 1
           for (int row = 0; row < 32; ++row) {
             const int key = (row < 16 ? now[2 * x] : now[2 * x + 1]) + (row & 15);
-            const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
+            const bool sees = row_sees.sees(key);
             const float w = of_row<T>(df, row, lane);
 #pragma unroll
             for (int i = 0; i < DT; ++i)
@@ -288,7 +288,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
   }
   const elem *kp = (const elem *)a.k.data + b * a.k.stride[0] + kh * a.k.stride[2];
   const elem *vp = (const elem *)a.v.data + b * a.v.stride[0] + kh * a.v.stride[2];
-  const int gone = limit - a.window, gone_any = high - a.window;  // last key before this row's window, and any row's
+  const Sight<WINDOW> row_sees(a, limit);
+  const int gone_any = high - a.window;  // last key before any row's window
   const int tiles = WINDOW ? (span.count + 1) / 2 : tiles_of<32>(a, count);
   v4i kr[2][KS], vr[2][KS];
   const auto load = [&](int key0, int key1) {
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], c, -off));
         float ds = p * __builtin_fmaf(g[i][e], a.scale, -del);
         const int key = (i ? now1 : now0) + 4 * quarter + e;
-        if (cut && (key > limit || (WINDOW && key <= gone && key >= a.sink))) ds = 0.f;
+        if (cut) ds = row_sees.sees(key) ? ds : 0.f;
         df[4 * i + e] = (elem)ds;
       }
     wave_lds_sync();
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {
         const int key = (x < 16 ? now0 : now1) + (x & 15);
-        const bool sees = key <= limit && (!WINDOW || key > gone || key < a.sink);
+        const bool sees = row_sees.sees(key);
         float w = 0.f;  // key x is element 4 (x / 16) + x % 4 of quarter x / 4 % 4
 #pragma unroll
         for (int e = 0; e < 8; ++e) w = e == 4 * (x >> 4) + (x & 3) ? (float)df[e] : w;
