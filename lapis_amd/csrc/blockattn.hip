@@ -111,7 +111,9 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
         }
       }
       const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
+      int clean = 1;
       if (cut) {
+        clean = bad_tile[side][buffer] != t + 1;
 #pragma unroll
         for (int x = 0; x < ST; ++x)
 #pragma unroll
@@ -135,7 +137,12 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
         for (int i = 0; i < DT; ++i) acc[i] *= keep;
       }
       const float off = m == -INFINITY ? 0.f : m;
-      vec8<T> pf[2 * ST];
+      // values by columns, read some products ahead, the first of them before the exponentials
+      constexpr int N = 2 * ST * DT, AHEAD = 4;
+      vec8<T> pf[2 * ST], va[N];
+      const auto read = [&](int n) { va[n] = columns_in_order<T, DP, true>(vt, 16 * (n / DT), 32 * (n % DT), lane); };
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) read(n);
 #pragma unroll
       for (int x = 0; x < ST; ++x)
 #pragma unroll
@@ -152,7 +159,16 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
           l += s[x][e];
           pf[2 * x + (e >> 3)][e & 7] = (elem)s[x][e];
         }
-      if (cut && bad_tile[side][buffer] == t + 1) {
+      if (clean) {  // either way, but not as two sides of one branch: the sums would be kept twice
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (n + AHEAD < N) read(n + AHEAD);
+          acc[n % DT] = mfma32(va[n], pf[n / DT], acc[n % DT]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      asm volatile("" : "+v"(clean));
+      if (__builtin_amdgcn_readfirstlane(clean) == 0) {
         // the finite values as always; an infinity or NaN only to the rows that see its key
 #pragma unroll
         for (int y = 0; y < 2 * ST; ++y)
@@ -178,11 +194,6 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
               }
             }
         }
-      } else {
-#pragma unroll
-        for (int y = 0; y < 2 * ST; ++y)
-#pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP, true>(vt, 16 * y, 32 * i, lane), pf[y], acc[i]);
       }
     }
     lds_loads_done();
