@@ -352,15 +352,26 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
     if (t + SPLIT < tiles) load(next);
     ahead = look_up(t + 2 * SPLIT);
     if (skip) continue;
+    if (cut) {
+      asm volatile("");  // (one branch, not one for each element)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = row_sees.sees(now[i] + 4 * quarter + e) ? s[i][e] : -INFINITY;
+    }
+    wave_lds_sync();
+    vec8<T> pf, va[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {  // asked for before the exponentials
+      const int x = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
+      const elem *p = mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7);  // row + 16 has the same order of pieces
+      va[i] = join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP));
+    }
     float best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = now[i] + 4 * quarter + e;
-        if (cut) s[i][e] = row_sees.sees(key) ? s[i][e] : -INFINITY;
-        best = fmaxf(best, s[i][e]);
-      }
+      for (int e = 0; e < 4; ++e) best = fmaxf(best, s[i][e]);
     best = rows_max(best) * c;
     if (__any(best > m + 8.f)) {  // as in the kernel above
       const float to = fmaxf(m, best), keep = to == m ? 1.f : __builtin_amdgcn_exp2f(m - to);
@@ -370,7 +381,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
       for (int i = 0; i < DT; ++i) acc[i] *= keep;
     }
     const float off = m == -INFINITY ? 0.f : m;
-    vec8<T> pf;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -379,15 +389,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_narrow_kernel(Blo
         l += p;
         pf[4 * i + e] = (elem)p;
       }
-    wave_lds_sync();
+    if (bad) {
+      asm volatile("");
 #pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      const int x = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
-      const elem *p = mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7);  // row + 16 has the same order of pieces
-      vec8<T> v = join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP));
-      if (bad) v = finite_only<T>(v);
-      acc[i] = mfma16(v, pf, acc[i]);
+      for (int i = 0; i < DT; ++i) va[i] = finite_only<T>(va[i]);
     }
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i] = mfma16(va[i], pf, acc[i]);
     if (bad)  // an infinity or NaN only to the rows that see its key
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {

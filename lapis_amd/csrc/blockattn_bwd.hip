@@ -147,25 +147,33 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
           g = mfma32(va[y], gf[y], g);
           __builtin_amdgcn_sched_barrier(0);
         }
-        vec8<T> df[2];
+        // keys by columns for dQ, read some products ahead, the first of them before the exponentials
+        vec8<T> kc[2 * DT], df[2];
+        const auto read_columns = [&](int n) { kc[n] = columns_in_order<T, DP>(kt, 32 * x + 16 * (n / DT), 32 * (n % DT), place_lane); };
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) read_columns(n);
         // dS is rounded to the operands' type for the product, with `scale` in it: smaller by its factor in float16's range
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -off));
-          float ds = p * __builtin_fmaf(g[e], a.scale, -del);
-          if (cut) {
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -off)) * __builtin_fmaf(g[e], a.scale, -del);
+        if (cut) {
+          asm volatile("");  // (one branch, not one for each element)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
             const int key = now[2 * x + (e >> 3)] + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
-            ds = row_sees.sees(key) ? ds : 0.f;
+            s[e] = row_sees.sees(key) ? s[e] : 0.f;
           }
-          df[e >> 3][e & 7] = (elem)ds;
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) df[e >> 3][e & 7] = (elem)s[e];
         // a key's elements that are no numbers count for the rows that see it, by themselves; the product takes them as zeros
         int clean = !bad;  // either way, but not as two sides of one branch: the sums would be kept twice
         if (clean) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] = mfma32(columns_in_order<T, DP>(kt, 32 * x + 16 * y, 32 * i, place_lane), df[y], acc[i]);
+          for (int n = 0; n < 2 * DT; ++n) {
+            if (n + AHEAD < 2 * DT) read_columns(n + AHEAD);
+            acc[n % DT] = mfma32(kc[n], df[n / DT], acc[n % DT]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
         asm volatile("" : "+v"(clean));
         if (__builtin_amdgcn_readfirstlane(clean) == 0) {
@@ -346,26 +354,36 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void block_dq_narrow_kernel(
     if (t + SPLIT < tiles) load(next0, next1);
     ahead = look_up(t + 2 * SPLIT);
     if (skip) continue;
-    vec8<T> df;
+    vec8<T> df, kc[DT];
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {  // asked for before the exponentials
+      const int x = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
+      const elem *p = mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7);  // row + 16 has the same order of pieces
+      kc[i] = join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP));
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], c, -off));
-        float ds = p * __builtin_fmaf(g[i][e], a.scale, -del);
-        const int key = (i ? now1 : now0) + 4 * quarter + e;
-        if (cut) ds = row_sees.sees(key) ? ds : 0.f;
-        df[4 * i + e] = (elem)ds;
-      }
-    wave_lds_sync();
+      for (int e = 0; e < 4; ++e) s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], c, -off)) * __builtin_fmaf(g[i][e], a.scale, -del);
+    if (cut) {
+      asm volatile("");  // (one branch, not one for each element)
 #pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      const int x = 4 * quarter + (col >> 2), d = 16 * i + 4 * (col & 3);
-      const elem *p = mine + x * DP + ((d >> 3) ^ turn16<DP>(x)) * 8 + (d & 7);  // row + 16 has the same order of pieces
-      vec8<T> k = join<T>(read_columns<T>(p), read_columns<T>(p + 16 * DP));
-      if (bad) k = finite_only<T>(k);
-      acc[i] = mfma16(k, df, acc[i]);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = row_sees.sees((i ? now1 : now0) + 4 * quarter + e) ? s[i][e] : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) df[4 * i + e] = (elem)s[i][e];
+    if (bad) {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < DT; ++i) kc[i] = finite_only<T>(kc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i] = mfma16(kc[i], df, acc[i]);
     if (bad)  // a key's elements that are no numbers, for the rows that see it
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {
