@@ -16,8 +16,11 @@ __device__ __forceinline__ float units_of_ln2(float scale) {
 // next tile is loaded straight into one while the other is computed).
 // S^T = K Q^T has a query per lane, so maxima, sums and factors of the softmax are one register and need one exchange
 // between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
-// 32 768 queries and keys, 32 heads over 8, dim 128, 16 blocks of 128 a row, bf16: 1290 to 1350 us, 800 to 765 TFLOP/s where a large library
-// product reaches 1203.  Bound by issue: 72 % of the cycles issue something, vector instructions 41 %, products 32 %.
+// Operands from LDS are asked for some products ahead (a fence after each product keeps it so: left alone the compiler reads each pair of them and
+// waits), and the two ways of taking values, with infinities and NaN apart and without, are no two sides of one branch (64 registers less).
+// 32 768 queries and keys, 32 heads over 8, dim 128, bf16: 16 blocks of 128 a row 1140 to 1160 us, a window of 2048 and the first 16 keys 1125 to 1170
+// (930 to 980 TFLOP/s where a large library product reaches 1203 to 1400).  Near the card's power: with operands that are zeros it
+// is 20 % faster and that product 30 %; exponentials of half a tile under the products of the other half change nothing.
 template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
 __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {
   typedef typename T::elem elem;
@@ -100,15 +103,18 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
     if (SIDES > 1) __syncthreads();  // of all, as one side's tile may be cut and not the other's
     if (lowest <= high) {
       const elem *kt = k_tile[side][buffer], *vt = v_tile[side][buffer];
-      v16f s[ST];
+      // keys by rows, read some products ahead; the chains of products of the tile's halves in turn
+      constexpr int KN = ST * DP / 16, K_AHEAD = 4;
+      v16f s[ST] = {};
+      vec8<T> ka[KN];
+      const auto read_keys = [&](int n) { ka[n] = *(const vec8<T> *)(kt + place_of<DP>(32 * (n % ST) + (lane & 31), 2 * (n / ST) + half)); };
 #pragma unroll
-      for (int x = 0; x < ST; ++x) {
-        s[x] = v16f{};
+      for (int n = 0; n < K_AHEAD; ++n) read_keys(n);
 #pragma unroll
-        for (int y = 0; y < DP / 16; ++y) {
-          const vec8<T> kf = *(const vec8<T> *)(kt + place_of<DP>(32 * x + (lane & 31), 2 * y + half));
-          s[x] = mfma32(kf, qf[y], s[x]);
-        }
+      for (int n = 0; n < KN; ++n) {
+        if (n + K_AHEAD < KN) read_keys(n + K_AHEAD);
+        s[n % ST] = mfma32(ka[n], qf[n / ST], s[n % ST]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
       int clean = 1;

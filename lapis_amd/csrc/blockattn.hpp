@@ -92,6 +92,8 @@ struct KeyTiles {
   const elem *kp, *vp;
   long long k_off, v_off;
   unsigned k_to, v_to;
+  unsigned k_together, v_together;  // bytes from a tile's first row to this thread's part, where its rows lie one behind the other
+  bool near;                        // they reach that far
   Span span = {};
 
   __device__ __forceinline__ KeyTiles(const BlockArgs &a_, int b, int kh, int first_, int count_, int tid, const elem *k_tile, const elem *v_tile)
@@ -103,6 +105,9 @@ struct KeyTiles {
     v_off = in16 * a.v.stride[1] + vd;
     k_to = lds_address(k_tile) + wave * 1024;
     v_to = lds_address(v_tile) + wave * 1024;
+    near = (unsigned long long)a.k.stride[1] < (1u << 26) && (unsigned long long)a.v.stride[1] < (1u << 26);
+    k_together = (my_row * (unsigned)a.k.stride[1] + kd) * 2;
+    v_together = (my_row * (unsigned)a.v.stride[1] + vd) * 2;
   }
   __device__ __forceinline__ int tiles() const { return WINDOW ? (span.count + CH - 1) / CH : tiles_of<KT>(a, count); }
   // The first key of each sixteen of tile t, one to a lane: asked for a tile before they are needed.
@@ -119,6 +124,30 @@ struct KeyTiles {
   template <int BUFFER>
   __device__ __forceinline__ void load(v4i key0) const {
     constexpr unsigned buffer = BUFFER * KT * DP * 2;
+    static_assert(KT == 64 && RP <= 32, "my_row * stride has 32 bits");
+    if (near && key0[3] == key0[0] + 48 && key0[0] <= a.keys - KT) {  // most tiles: one behind the other, so that the addresses are a few additions
+      const elem *k = kp + key0[0] * a.k.stride[1], *v = vp + key0[0] * a.v.stride[1];
+      const auto all = [&](auto which) {
+        constexpr int p = decltype(which)::value;
+        load_to_lds_behind<buffer + p * NW * 1024>(k + p * RP * a.k.stride[1], k_together, k_to);
+      };
+      const auto all_v = [&](auto which) {
+        constexpr int p = decltype(which)::value;
+        load_to_lds_behind<buffer + p * NW * 1024>(v + p * RP * a.v.stride[1], v_together, v_to);
+      };
+      static_assert(PASSES == 2 || PASSES == 4, "passes of a tile");
+      if (kd < a.dim) {
+        all(std::integral_constant<int, 0>());
+        all(std::integral_constant<int, 1>());
+        if constexpr (PASSES == 4) all(std::integral_constant<int, 2>()), all(std::integral_constant<int, 3>());
+      }
+      if (vd < a.dim) {
+        all_v(std::integral_constant<int, 0>());
+        all_v(std::integral_constant<int, 1>());
+        if constexpr (PASSES == 4) all_v(std::integral_constant<int, 2>()), all_v(std::integral_constant<int, 3>());
+      }
+      return;
+    }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int at = RP == 16 ? key0[p] : __builtin_amdgcn_readfirstlane(my_row < 16 ? key0[p * RP / 16] : key0[p * RP / 16 + (RP > 16)]);

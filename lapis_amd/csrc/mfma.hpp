@@ -106,6 +106,11 @@ __device__ __forceinline__ void load_to_lds(const void *from, unsigned offset, u
 __device__ __forceinline__ void load_word_to_lds(const void *from, unsigned offset, unsigned to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
 }
+// the same to a place MORE bytes behind `to`
+template <unsigned MORE>
+__device__ __forceinline__ void load_to_lds_behind(const void *from, unsigned offset, unsigned to) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from), "n"(MORE) : "memory", "scc");
+}
 // all but the last N loads of this wavefront
 template <int N = 0>
 __device__ __forceinline__ void lds_loads_done() {
