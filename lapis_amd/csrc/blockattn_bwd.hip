@@ -125,10 +125,11 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
       const elem *kt = k_tile[side][buffer], *vt = v_tile[side][buffer];
       const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
       const bool bad = cut && bad_tile[side][buffer] == t + 1;
+      int place_lane = lane;  // made anew for each tile, or the compiler keeps the places of all operands in registers
+      asm volatile("" : "+v"(place_lane));
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
-        int place_lane = lane;  // made anew each time, or the compiler keeps the places of all operands in registers
-        asm volatile("" : "+v"(place_lane));
+        if (DP <= 64) asm volatile("" : "+v"(place_lane));  // or for each half of it: 159 registers, three wavefronts a SIMD
         // two chains of products that do not wait for each other, their operands read two products ahead
         constexpr int N = DP / 16, AHEAD = 2;
         v16f s = {}, g = {};
