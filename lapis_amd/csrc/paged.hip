@@ -131,9 +131,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8
   constexpr bool SCALED = F8 && std::is_same<T, F16>::value;
   struct Tokens {
     long long at[32];     // element offsets of the tile's rows
-    long long scale_at[F4 ? 32 : 1];
     float ks[F4 ? 4 : 32], vs[F4 ? 4 : 32]; // SCALED: vs holds mantissas, and vp powers of two, those of a lane's rows side by side
     float vp[SCALED ? 32 : 4];
+    long long scale_at[F4 ? 32 : 2];
   };
   union Own {  // of a wavefront
     elem v[32 * DP];
@@ -307,8 +307,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int r = p * RP + lane / V_PIECES, piece = lane % V_PIECES;
-      const bool used = there == 0xffffffffu || (there >> r & 1);  // whatever an unused slot holds: 0 times it must be 0
-      const auto put = [&](int at, vec8<T> v) { *(vec8<T> *)(mine.v + r * DP + ((at ^ turn16<DP>(r)) * 8)) = used ? v : vec8<T>{}; };
+      const auto put = [&](int at, vec8<T> v) {
+        if (there != 0xffffffffu && !(there >> r & 1)) v = vec8<T>{};  // whatever an unused slot holds: 0 times it must be 0
+        *(vec8<T> *)(mine.v + r * DP + ((at ^ turn16<DP>(r)) * 8)) = v;
+      };
       if constexpr (F4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) put(4 * piece + i, codes_to<T>(vr[p][i], scale_of_byte(vb[p])));

@@ -538,7 +538,7 @@ int layout_of(BlockArgs *a, WindowLayout *layout) {
   c.all = lists * c.of_list;
   c.chunk = std::max<int64_t>({1, ceil_div(c.all, cus), ceil_div(kLeastTiles * 32, group)});
   c.workgroups = (int)ceil_div(c.all, c.chunk);
-  c.whole = lists * c.columns <= cus && 2 * (a->window + kKeys + c.overhead) <= 3 * c.chunk;
+  c.whole = lists * c.columns <= cus && 2ll * (a->window + kKeys + c.overhead) <= 3 * c.chunk;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
