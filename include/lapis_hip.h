@@ -621,7 +621,10 @@ typedef struct lapis_hip_window_args {
   void *work;                      /* backward only */
 } lapis_hip_window_args;
 int lapis_hip_window_attention(const lapis_hip_window_args *args, lapis_hip_stream_t stream);
-/* Gradients of the forward call whose out and lse these are, as of lapis_hip_block_attention_backward; _work answers after lapis_hip_init. */
+/* Gradients of the forward call whose out and lse these are, as of lapis_hip_block_attention_backward; _work answers after lapis_hip_init.  Refused:
+ * strides of q and dout between tokens or heads that are negative or 2^25 elements and more, heads of a group that with 63 tokens spread over
+ * 2^31 elements, and 2^29 or more queries times heads of a group.  Scratch: 8 bytes for each row, 256 KB for each compute unit and 256 KB for each 128
+ * keys among the first ones of each batch entry and key-value head; `work` may be NULL where _work says 0. */
 int lapis_hip_window_attention_backward_work(const lapis_hip_window_args *args, int64_t *bytes);
 int lapis_hip_window_attention_backward(const lapis_hip_window_args *args, lapis_hip_stream_t stream);
 

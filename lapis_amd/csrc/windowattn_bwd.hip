@@ -526,10 +526,14 @@ int layout_of(BlockArgs *a, WindowLayout *layout) {
   c.columns = (int)ceil_div(a->keys, kKeys);
   LAPIS_REQUIRE(lists * c.columns * 256 < (INT64_C(1) << 32), "%s: %lld lists of %lld keys", what, (long long)lists, (long long)a->keys);
   LAPIS_REQUIRE((int64_t)a->queries * a->group < (1 << 29), "%s: %d queries of %d heads", what, a->queries, a->group);
-  for (const View *v : {&a->q, &a->dout})  // rows of a tile lie within 32-bit offsets
+  const int group = std::max(a->group, 1);
+  for (const View *v : {&a->q, &a->dout}) {  // the rows of a stage lie within 32-bit offsets: 64 of them from any head of a group on
     for (int i = 1; i < 3; ++i)
       LAPIS_REQUIRE(v->stride[i] >= 0 && v->stride[i] < (1 << 25), "%s: queries or their gradients with a stride of %lld elements", what, v->stride[i]);
-  const int group = std::max(a->group, 1);
+    const int64_t last = group + 62, query = last / group;
+    const int64_t farthest = std::max(query * v->stride[1] + (last - query * group) * v->stride[2], (query - 1) * v->stride[1] + (group - 1) * v->stride[2]);
+    LAPIS_REQUIRE(2 * (farthest + kMaxBlockDim) < (INT64_C(1) << 32), "%s: %d heads of a group with a stride of %lld elements", what, group, v->stride[2]);
+  }
   c.queries = a->queries, c.shift = a->shift, c.window = a->window;
   // first keys that some query's window has left behind
   c.sink_columns = (int)ceil_div(std::min(std::max((int64_t)a->keys - a->window, INT64_C(0)), std::min<int64_t>(a->sink, a->keys)), kKeys);
