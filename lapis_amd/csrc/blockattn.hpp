@@ -60,7 +60,7 @@ __device__ __forceinline__ Span span_of(const BlockArgs &a, int q0, int held) {
 }
 
 // Which keys a row sees: up to `limit`, and over a window the last ones of them and the first ones.  (Differences of whole numbers and no || or &&:
-// those become branches, a dozen instructions for each key of a tile that wait for one another.  1001 queries behind 2437 keys, window 300: 21.2 us and FIXME.)
+// those become branches, a dozen instructions for each key of a tile that wait for one another.  1001 queries behind 2437 keys, window 300, 12 heads: 22.2 us so and 19.9 without.)
 template <bool WINDOW>
 struct Sight {
   int limit, sinks;

@@ -1,9 +1,10 @@
-// Keys and values into a cache of pages and back out of it, quantised to e4m3 with one scale per row on the way.
+// Keys and values into a cache of pages and back out of it, quantised on the way: to e4m3 with one scale per row, or to e2m1 with a power of two
+// for each 32 elements.
 //
 // A row of `dim` elements belongs to a group of lanes, eight elements each (one 16-byte load); the row's maximum is
 // a DPP reduction over the group, so a row is read once and nothing is kept but registers.  Bound by memory: 32 768 tokens
-// of 8 heads, dim 128, bf16 into e4m3 in 51.5 us (4.0 TB/s), 20 000 tokens, dim 96, back into f16 in 24.1 (3.9 TB/s), where a
-// large copy reaches 4.75; four rows a thread on their way, loads first, where that leaves every compute unit its workgroups
+// of 8 heads, dim 128, bf16 into e4m3 in 50 us (4.1 TB/s), 20 000 tokens, dim 96, back into f16 in 22.1 (4.2 TB/s), where a
+// large copy reaches 4.75; 32 768 tokens of 8 heads, dim 128, out of 4-bit codes in 41 us (4.1 TB/s, most of it written); four rows a thread on their way, loads first, where that leaves every compute unit its workgroups
 // (one row a thread: 54 and 30).  48 tokens take 4.5 us, the call and the launch.
 #include "kvcache.hpp"
 
@@ -12,7 +13,7 @@ namespace {
 
 // Group of L lanes per (token, head) and of N of them, 256 / L rows apart; blockIdx.z: keys or values.
 template <typename T, int CODES, int L, int N>
-__global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, long long rows, const int *__restrict__ slots) {
+__global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, long long rows, Divisor by_heads, const int *__restrict__ slots) {
   typedef typename T::elem elem;
   const long long row0 = (long long)linear_block() * (256 / L * N) + threadIdx.x / L;
   const int d = (threadIdx.x % L) * 8, which = blockIdx.z;
@@ -20,7 +21,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, 
   int slot_of[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const unsigned row = (unsigned)min(row0 + i * (256 / L), rows - 1), t = row / (unsigned)c.heads, h = row - t * c.heads;
+    const unsigned row = (unsigned)min(row0 + i * (256 / L), rows - 1), t = by_heads.divide(row), h = row - t * c.heads;
     slot_of[i] = slots[t];
     read[i] = vec8<T>{};
     if (d < c.dim) read[i] = load_stream((const vec8<T> *)((const elem *)x.data[which] + t * x.stride[which][0] + h * x.stride[which][1] + d));
@@ -29,7 +30,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, 
   for (int i = 0; i < N; ++i) {
     const long long row = row0 + i * (256 / L);
     if (row >= rows) return;
-    const int h = (int)((unsigned)row % (unsigned)c.heads);
+    const int h = (int)((unsigned)row - by_heads.divide((unsigned)row) * c.heads);
     const long long slot = slot_of[i];
     if (slot < 0 || slot >= c.slots) continue;
     if constexpr (CODES == kNoCodes) {
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(CacheView c, RowsView x, 
 }
 
 template <typename T, int CODES, int L, int N>
-__global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, long long rows, const int *__restrict__ slots) {
+__global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, long long rows, Divisor by_heads, const int *__restrict__ slots) {
   typedef typename T::elem elem;
   typedef typename std::conditional<CODES == kF8, v2i, typename std::conditional<CODES == kF4, unsigned, v4i>::type>::type raw;  // eight elements
   const long long row0 = (long long)linear_block() * (256 / L * N) + threadIdx.x / L;
@@ -54,7 +55,7 @@ __global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, l
   float scale[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const unsigned row = (unsigned)min(row0 + i * (256 / L), rows - 1), t = row / (unsigned)c.heads, h = row - t * c.heads;
+    const unsigned row = (unsigned)min(row0 + i * (256 / L), rows - 1), t = by_heads.divide(row), h = row - t * c.heads;
     const long long slot = slots[t];
     read[i] = raw{};
     scale[i] = 0.f;
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(256) void kv_load_kernel(CacheView c, RowsView x, l
   for (int i = 0; i < N; ++i) {
     const long long row = row0 + i * (256 / L);
     if (row >= rows) return;
-    const unsigned t = (unsigned)row / (unsigned)c.heads, h = (unsigned)row - t * c.heads;
+    const unsigned t = by_heads.divide((unsigned)row), h = (unsigned)row - t * c.heads;
     vec8<T> e;
     if constexpr (CODES != kNoCodes) {
       float f[8];
@@ -118,7 +119,7 @@ int kv_move(const char *what, const lapis_hip_kv_cache *cache, int64_t tokens, c
     };
     dim3 grid = grid_of(ceil_div(rows * L, 256 * N));
     grid.z = 2;
-    hipLaunchKernelGGL((bf16 ? pick(Bf16()) : pick(F16())), grid, dim3(256), 0, as_stream(stream), c, x, rows, slots);
+    hipLaunchKernelGGL((bf16 ? pick(Bf16()) : pick(F16())), grid, dim3(256), 0, as_stream(stream), c, x, rows, Divisor::of(c.heads), slots);
   };
   const auto with = [&](auto lanes) {
     // four rows a thread only where that leaves every compute unit its workgroups

@@ -36,6 +36,18 @@ inline CacheView view_of(const lapis_hip_kv_cache *c) {
   return v;
 }
 
+// Division of numbers below 2^31 by one that the host knows: q = r * m / 2^p, where p = 31 + ceil(log2 d) and m = ceil(2^p / d).  With
+// m d = 2^p + e, 0 <= e < d, q is too large by r e / (d 2^p) < 1 / d: not enough to reach the next integer.
+struct Divisor {
+  unsigned m, shift;
+  __host__ static Divisor of(int64_t d) {
+    unsigned p = 31;
+    while ((INT64_C(1) << (p - 31)) < d) ++p;
+    return {(unsigned)(((INT64_C(1) << p) + d - 1) / d), p};
+  }
+  __device__ __forceinline__ unsigned divide(unsigned r) const { return (unsigned)((unsigned long long)r * m >> shift); }
+};
+
 // The scale of 4-bit codes that a byte stands for; 255 makes an infinity, which the conversions take for NaN.
 __device__ __forceinline__ float scale_of_byte(unsigned b) { return __builtin_bit_cast(float, b << 23); }
 

@@ -120,6 +120,11 @@ __device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_ca
 // largest so far: exact for scales down to 2^-22 of that one, rounded to multiples of 2^-24 units below.
 // Bound by memory: 64 sequences of up to 8192 tokens, 32 heads over 8, dim 128, 8-bit cache: 153 us at 4.5 TB/s (a large copy
 // reaches 4.75), 160 with float16 queries; one sequence of 16 384 tokens, bf16: 22.4 us, 16.9 of them here (4.0 TB/s) and 5.4 for the join.
+// 4-bit codes become 16-bit operands by one conversion with their scale (exact: two bits of mantissa times a power of two), K in registers and V on
+// its way into LDS; 128 registers, four workgroups a compute unit, as a row is 64 bytes and its 32 elements a lane one load.  64 sequences of up to 8192
+// tokens: 86 us with the join, 78 of them here (4.5 TB/s); one of 16 384: 14.5, 9.3 here (launch, look-ups and two tiles one after the other) and 4.9.
+// Windows number their tokens first ones first, so that a unit may hold the end of those and the start of the others; table entries are asked for as
+// those of lists are.  128 sequences, window 4096 and 64 first tokens, 4 bits: 133 us, 119 of them here (4.8 TB/s); 4 sequences, bf16: 21.2, 16.0 here (4.2 TB/s).
 template <typename T, int CODES, int DP, bool WINDOW>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8 ? 3 : 2) void paged_kernel(PagedArgs a) {
   typedef typename T::elem elem;

@@ -1,28 +1,15 @@
 // Rows turned by their positions, and on their way into a paged cache.
 //
 // Pair (x, y) of a row becomes (x cos - y sin, x sin + y cos) of an angle that is one for all heads of a token.  Bound by memory: 16384 tokens of 32 heads,
-// dim 128, bf16, three axes, in 55 us (4.9 TB/s read and written, what a large copy reaches); a prompt of 32768 tokens, 32 heads of queries and 8 of keys and
-// values, into 4-bit codes in 158 us (4.5 TB/s).  There it waits: its vector instructions take 70 % of the time, so everything that a row needs
-// (which row it is, its slot) is asked for before the angles are made and rows are numbered without divisions (193 us before).  48
-// tokens into 8-bit codes take 4 us, the launch.
+// dim 128, bf16, three axes, in 53 us (5.1 TB/s read and written, more than a large copy out of memory reaches); a prompt of 32768 tokens, 32 heads of queries and 8 of keys and
+// values, into 4-bit codes in 141 us (5.0 TB/s; 193 with divisions and with slots asked for after the angles, 158 with every lane working out its
+// own row: vector instructions in 93 % of the cycles).  48 tokens into 8-bit codes take 4 us, the launch.
 #include "kvcache.hpp"
 
 namespace lapis {
 namespace {
 
 enum { kQuery = 0, kKey = 1, kValue = 2 };
-
-// Division of numbers below 2^31 by one that the host knows: q = r * m / 2^p, where p = 31 + ceil(log2 d) and m = ceil(2^p / d).  With
-// m d = 2^p + e, 0 <= e < d, q is too large by r e / (d 2^p) < 1 / d: not enough to reach the next integer.
-struct Divisor {
-  unsigned m, shift;
-  __host__ static Divisor of(int64_t d) {
-    unsigned p = 31;
-    while ((INT64_C(1) << (p - 31)) < d) ++p;
-    return {(unsigned)(((INT64_C(1) << p) + d - 1) / d), p};
-  }
-  __device__ __forceinline__ unsigned divide(unsigned r) const { return (unsigned)((unsigned long long)r * m >> shift); }
-};
 
 struct TurnArgs {
   const char *x[3];  // queries, keys, values
@@ -45,10 +32,11 @@ struct TurnArgs {
 struct Row {
   unsigned token, b, t, head;
   int kind;
-  __device__ __forceinline__ const char *data(const TurnArgs &a) const {  // (selects of values: an index would be a load before the load)
+  // Of the row `more` heads further.  (Selects of values: an index would be a load before the load.)
+  __device__ __forceinline__ const char *data(const TurnArgs &a, unsigned more) const {
     const auto one_of = [&](auto q, auto k, auto v) { return kind == kQuery ? q : kind == kKey ? k : v; };
     const auto stride = [&](int i) { return one_of(a.x_stride[kQuery][i], a.x_stride[kKey][i], a.x_stride[kValue][i]); };
-    return one_of(a.x[kQuery], a.x[kKey], a.x[kValue]) + 2 * (b * stride(0) + t * stride(1) + head * stride(2));
+    return one_of(a.x[kQuery], a.x[kKey], a.x[kValue]) + 2 * (b * stride(0) + t * stride(1) + head * stride(2)) + 2 * (more * stride(2));
   }
 };
 __device__ __forceinline__ Row row_of(const TurnArgs &a, unsigned r) {
@@ -70,7 +58,9 @@ __device__ __forceinline__ Row row_of(const TurnArgs &a, unsigned r) {
 // of a token side by side.  Cosines and sines are one for all heads of a token: they are computed once a workgroup, in 64 bits
 // (positions of a million leave 32 bits no fraction), while the first rows are on their way, and read from LDS.  A lane reads the other
 // elements of its pairs from memory a second time (out of L1): the row may be written over, but by this wavefront and after it.
-template <typename T, int CODES, int L, int N>
+// TOGETHER: the 64 / L rows that a wavefront has at a time are neighbouring heads of one token and of one kind, so that which rows they are and where
+// they lie is worked out once for the wavefront, in scalar registers.
+template <typename T, int CODES, int L, int N, bool TOGETHER>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
   typedef typename T::elem elem;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -80,12 +70,17 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
   const unsigned last_row = (unsigned)(a.rows - 1), row0 = (unsigned)block_row + threadIdx.x / L;
   const bool inside = d < a.dim, whole = !a.neighbours && pairs % 8 == 0;  // whole: the other elements are eight neighbours too
   const int other = d < pairs ? d + pairs : d - pairs;
+  const unsigned more = TOGETHER ? threadIdx.x % 64 / L : 0, wave_row = __builtin_amdgcn_readfirstlane(row0);
+  const auto my_row = [&](int i) {
+    if constexpr (TOGETHER) return row_of(a, min(wave_row + i * (256 / L), last_row + 1 - 64 / L));
+    else return row_of(a, min(row0 + i * (256 / L), last_row));
+  };
   vec8<T> x[N], y[N];
   int slots[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const Row r = row_of(a, min(row0 + i * (256 / L), last_row));
-    const elem *p = (const elem *)r.data(a);
+    const Row r = my_row(i);
+    const elem *p = (const elem *)r.data(a, more);
     x[i] = y[i] = vec8<T>{};
     slots[i] = r.kind == kQuery ? -1 : a.slots[r.token];
     if (inside) {
@@ -109,9 +104,8 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const unsigned row = row0 + i * (256 / L);
-    if (row > last_row) return;
-    const Row r = row_of(a, row);
+    if ((TOGETHER ? wave_row : row0) + i * (256 / L) > last_row) return;
+    const Row r = my_row(i);
     float f[8];
     widen<T>(x[i], f);
     const int at = (int)(r.token - t0) * pairs;
@@ -133,7 +127,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
           }
         }
       } else {
-        const elem *p = (const elem *)r.data(a);
+        const elem *p = (const elem *)r.data(a, more);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int e = d + j;
@@ -146,11 +140,11 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
       }
     }
     if (r.kind == kQuery) {
-      if (inside) *(vec8<T> *)((elem *)a.out + r.b * a.out_stride[0] + r.t * a.out_stride[1] + r.head * a.out_stride[2] + d) = narrow<T>(f);
+      if (inside) *(vec8<T> *)((elem *)a.out + r.b * a.out_stride[0] + r.t * a.out_stride[1] + r.head * a.out_stride[2] + more * a.out_stride[2] + d) = narrow<T>(f);
       continue;
     }
     const long long slot = slots[i];
-    if (slot >= 0 && slot < a.cache.slots) put_elements<T, CODES, L>(a.cache, r.kind - kKey, slot, r.head, d, f);
+    if (slot >= 0 && slot < a.cache.slots) put_elements<T, CODES, L>(a.cache, r.kind - kKey, slot, r.head + more, d, f);
   }
 }
 
@@ -179,16 +173,19 @@ template <typename T, int CODES>
 int launch_turn(TurnArgs a, hipStream_t st) {
   a.by_heads = Divisor::of(a.all_heads);
   a.by_tokens = Divisor::of(a.tokens);
-  const auto go = [&](auto lanes, auto times) {
+  const auto go = [&](auto lanes, auto times, auto together) {
     constexpr int L = decltype(lanes)::value, N = decltype(times)::value, ROWS = 256 / L * N;
+    constexpr bool TOGETHER = decltype(together)::value;
     const int64_t tokens = std::min<int64_t>(ROWS, (ROWS - 2) / a.all_heads + 2);  // that a workgroup has rows of, at most
-    hipLaunchKernelGGL((turn_kernel<T, CODES, L, N>), grid_of(ceil_div(a.rows, ROWS)), dim3(256), (size_t)(tokens * a.pairs * 8), st, a);
+    hipLaunchKernelGGL((turn_kernel<T, CODES, L, N, TOGETHER>), grid_of(ceil_div(a.rows, ROWS)), dim3(256), (size_t)(tokens * a.pairs * 8), st, a);
   };
   const auto with = [&](auto lanes) {
-    // four rows a thread only where that leaves every compute unit its workgroups (the prompt above with its reading back: 205 us, with two rows 210, with
-    // eight 225; the 16384 tokens 55, 59 and 60)
-    if (a.rows * decltype(lanes)::value >= 256 * 16 * device_cu_count()) go(lanes, std::integral_constant<int, 4>());
-    else go(lanes, std::integral_constant<int, 1>());
+    constexpr int L = decltype(lanes)::value;
+    // four rows a thread only where that leaves every compute unit its workgroups (the prompt above with its reading back: 182 us, with two rows 183, with
+    // eight 186, and 204 where rows are each lane's own; the 16384 tokens 53, 53, 55 and 55)
+    if (a.rows * L < 256 * 16 * device_cu_count()) go(lanes, std::integral_constant<int, 1>(), std::false_type());
+    else if (a.heads % (64 / L) || a.cache.heads % (64 / L)) go(lanes, std::integral_constant<int, 4>(), std::false_type());
+    else go(lanes, std::integral_constant<int, 4>(), std::true_type());
   };
   if (a.dim <= 64) with(std::integral_constant<int, 8>());
   else if (a.dim <= 128) with(std::integral_constant<int, 16>());
