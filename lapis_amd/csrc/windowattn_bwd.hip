@@ -122,8 +122,8 @@ __device__ __forceinline__ const DkvArgs &again() {
 }
 
 // 8192 queries and keys, 32 heads over 8, dim 128, window 1024 and the first 16 keys, bf16: 406 us in a trace (372 at best), 645 to 700 TFLOP/s of its four
-// products, and 20 for the join.  Bound by LDS and by the card's power: 1.5 KB of operands a product, three quarters of what LDS gives, products in 40 % of
-// the cycles; the whole backward pass takes a quarter less time with operands that are zeros.  3 x 701 queries, 937 keys, 6 heads, dim 72, window 200: 31 us, of
+// products, and 20 for the join.  Bound by the card's power: products run in 40 % of the cycles, LDS in 37 %, other orders of the work take the same time
+// (weights of half a tile under the products of the other half too), and the whole pass a quarter less with operands that are zeros.  3 x 701 queries, 937 keys, 6 heads, dim 72, window 200: 31 us, of
 // which a first stage takes 8 (launch, instructions and operands from memory) and each stage of 64 rows 2.5.
 //
 // 128 keys of a list and a stretch of the queries that see them, rows (a query times a head of the group) packed into tiles of 32.
