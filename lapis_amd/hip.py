@@ -621,5 +621,6 @@ def window_attention(q, k, v, out, window, sink=0, lse=None, scale=None, stream=
 
 
 def window_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, window, sink=0, scale=None, stream=None):
-    """Gradients of ``window_attention`` from its inputs, its results and the gradient of ``out``."""
+    """Gradients of ``window_attention`` from its inputs, its results and the gradient of ``out``.  Tokens and heads of q and ``dout`` lie
+    less than 2 ** 25 elements apart."""
     return _calls.window_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, window, sink, scale, stream)
