@@ -490,11 +490,17 @@ __global__ __launch_bounds__(256) void window_join_kernel(BlockArgs a, WindowCol
     if (key >= a.keys || d >= a.dim) continue;
     v4f sum = {0.f, 0.f, 0.f, 0.f};
     for (int i = column < cols.sink_columns && key < a.sink ? 0 : 1; i < 2; ++i) {
-      for (long long w = found_from[i]; w < found_to[i]; ++w) {
-        const long long slot = found_whole[i] ? w : 2 * w + (w == found_from[i]);
-        const v4f y = *(const v4f *)(cols.partial + slot * 2 * EACH + x);
+      for (long long w = found_from[i]; w < found_to[i]; w += 4) {  // four on their way, added in order
+        v4f y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += y[e];
+        for (int n = 0; n < 4; ++n) {
+          const long long of = min(w + n, found_to[i] - 1), slot = found_whole[i] ? of : 2 * of + (of == found_from[i]);
+          y[n] = *(const v4f *)(cols.partial + slot * 2 * EACH + x);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] += w + n < found_to[i] ? y[n][e] : 0.f;
       }
     }
     const View &v = is_v ? a.dv : a.dk;
