@@ -110,11 +110,16 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
       const auto read_keys = [&](int n) { ka[n] = *(const vec8<T> *)(kt + place_of<DP>(32 * (n % ST) + (lane & 31), 2 * (n / ST) + half)); };
 #pragma unroll
       for (int n = 0; n < K_AHEAD; ++n) read_keys(n);
-#pragma unroll
-      for (int n = 0; n < KN; ++n) {
+      const auto score = [&](int n) {
         if (n + K_AHEAD < KN) read_keys(n + K_AHEAD);
         s[n % ST] = mfma32(ka[n], qf[n / ST], s[n % ST]);
         __builtin_amdgcn_sched_barrier(0);
+      };
+#pragma unroll
+      for (int n = 0; n < KN * 3 / 4; ++n) score(n);
+      if (DP <= 64 || a.dim > 96) {  // the last quarter of a row, if it is there (dim 96, 8192 queries, window 1024: 188 us with it, 178 without; dim 128 the same)
+#pragma unroll
+        for (int n = KN * 3 / 4; n < KN; ++n) score(n);
       }
       const bool cut = top + 15 > low || (WINDOW && lowest <= gone_any);
       int clean = 1;
@@ -146,7 +151,10 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
       // values by columns, read some products ahead, the first of them before the exponentials
       constexpr int N = 2 * ST * DT, AHEAD = 4;
       vec8<T> pf[2 * ST], va[N];
-      const auto read = [&](int n) { va[n] = columns_in_order<T, DP, true>(vt, 16 * (n / DT), 32 * (n % DT), lane); };
+      constexpr int LAST = DP <= 64 ? 0 : N / DT, FIRST = N - LAST;  // products of the last 32 columns come last
+      const auto key_of = [](int n) { return n < FIRST ? n / (FIRST * DT / N) : n - FIRST; };
+      const auto column_of = [](int n) { return n < FIRST ? n % (FIRST * DT / N) : DT - 1; };
+      const auto read = [&](int n) { va[n] = columns_in_order<T, DP, true>(vt, 16 * key_of(n), 32 * column_of(n), lane); };
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) read(n);
 #pragma unroll
@@ -166,11 +174,16 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(Block
           pf[2 * x + (e >> 3)][e & 7] = (elem)s[x][e];
         }
       if (clean) {  // either way, but not as two sides of one branch: the sums would be kept twice
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
+        const auto product = [&](int n) {
           if (n + AHEAD < N) read(n + AHEAD);
-          acc[n % DT] = mfma32(va[n], pf[n / DT], acc[n % DT]);
+          acc[column_of(n)] = mfma32(va[n], pf[key_of(n)], acc[column_of(n)]);
           __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int n = 0; n < FIRST; ++n) product(n);
+        if (LAST && a.dim > 96) {
+#pragma unroll
+          for (int n = FIRST; n < N; ++n) product(n);
         }
       }
       asm volatile("" : "+v"(clean));

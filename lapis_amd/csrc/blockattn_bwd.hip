@@ -142,16 +142,24 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
         };
 #pragma unroll
         for (int y = 0; y < AHEAD; ++y) read(y);
-#pragma unroll
-        for (int y = 0; y < N; ++y) {
+        const auto score = [&](int y) {
           if (y + AHEAD < N) read(y + AHEAD);
           s = mfma32(ka[y], qf[y], s);
           g = mfma32(va[y], gf[y], g);
           __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int y = 0; y < N * 3 / 4; ++y) score(y);
+        if (DP <= 64 || a.dim > 96) {  // the last quarter of a row, if it is there
+#pragma unroll
+          for (int y = N * 3 / 4; y < N; ++y) score(y);
         }
         // keys by columns for dQ, read some products ahead, the first of them before the exponentials
         vec8<T> kc[2 * DT], df[2];
-        const auto read_columns = [&](int n) { kc[n] = columns_in_order<T, DP>(kt, 32 * x + 16 * (n / DT), 32 * (n % DT), place_lane); };
+        constexpr int LAST = DP <= 64 ? 0 : 2, FIRST = 2 * DT - LAST;  // products of the last 32 columns come last
+        const auto key_of = [](int n) { return n < FIRST ? n / (FIRST / 2) : n - FIRST; };
+        const auto column_of = [](int n) { return n < FIRST ? n % (FIRST / 2) : DT - 1; };
+        const auto read_columns = [&](int n) { kc[n] = columns_in_order<T, DP>(kt, 32 * x + 16 * key_of(n), 32 * column_of(n), place_lane); };
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) read_columns(n);
         // dS is rounded to the operands' type for the product, with `scale` in it: smaller by its factor in float16's range
@@ -170,11 +178,16 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
         // a key's elements that are no numbers count for the rows that see it, by themselves; the product takes them as zeros
         int clean = !bad;  // either way, but not as two sides of one branch: the sums would be kept twice
         if (clean) {
-#pragma unroll
-          for (int n = 0; n < 2 * DT; ++n) {
+          const auto product = [&](int n) {
             if (n + AHEAD < 2 * DT) read_columns(n + AHEAD);
-            acc[n % DT] = mfma32(kc[n], df[n / DT], acc[n % DT]);
+            acc[column_of(n)] = mfma32(kc[n], df[key_of(n)], acc[column_of(n)]);
             __builtin_amdgcn_sched_barrier(0);
+          };
+#pragma unroll
+          for (int n = 0; n < FIRST; ++n) product(n);
+          if (LAST && a.dim > 96) {
+#pragma unroll
+            for (int n = FIRST; n < 2 * DT; ++n) product(n);
           }
         }
         asm volatile("" : "+v"(clean));

@@ -120,7 +120,7 @@ __device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_ca
 // largest so far: exact for scales down to 2^-22 of that one, rounded to multiples of 2^-24 units below.
 // Bound by memory: 64 sequences of up to 8192 tokens, 32 heads over 8, dim 128, 8-bit cache: 153 us at 4.5 TB/s (a large copy
 // reaches 4.75), 160 with float16 queries; one sequence of 16 384 tokens, bf16: 22.4 us, 16.9 of them here (4.0 TB/s) and 5.4 for the join.
-// 4-bit codes become 16-bit operands by one conversion with their scale (exact: two bits of mantissa times a power of two), K in registers and V on
+// 4-bit codes become 16-bit operands by one conversion with their scale (exact, in float16 down to its subnormal numbers: two bits of mantissa times a power of two), K in registers and V on
 // its way into LDS; 128 registers, four workgroups a compute unit, as a row is 64 bytes and its 32 elements a lane one load.  64 sequences of up to 8192
 // tokens: 86 us with the join, 78 of them here (4.5 TB/s); one of 16 384: 14.5, 9.3 here (launch, look-ups and two tiles one after the other) and 4.9.
 // Windows number their tokens first ones first, so that a unit may hold the end of those and the start of the others; table entries are asked for as

@@ -342,12 +342,17 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(DkvArgs) {
         };
 #pragma unroll
         for (int y = 0; y < AHEAD; ++y) read(y);
-#pragma unroll
-        for (int y = 0; y < N; ++y) {
+        const auto score = [&](int y) {
           if (y + AHEAD < N) read(y + AHEAD);
           s = mfma32(qa[y], ka[y], s);
           g = mfma32(ga[y], va[y], g);
           __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int y = 0; y < N * 3 / 4; ++y) score(y);
+        if (DP <= 64 || dim > 96) {  // the last quarter of a row, if it is there (dim 96, 8192 queries, window 1024: 635 us with dQ's, 595 without)
+#pragma unroll
+          for (int y = N * 3 / 4; y < N; ++y) score(y);
         }
       }
       vec8<T> p[2], ds[2];
@@ -382,19 +387,27 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(DkvArgs) {
       }
       if (looks && mem.bad == t) mend(slot, p, ds);
       {
+        constexpr int LAST = DP <= 64 ? 0 : N / DT, FIRST = N - LAST;  // products of the last 32 columns come last
+        const auto row_of = [](int y) { return y < FIRST ? y / (FIRST * DT / N) : y - FIRST; };
+        const auto column_of = [](int y) { return y < FIRST ? y % (FIRST * DT / N) : DT - 1; };
         vec8<T> xg[N], xq[N];
         const auto read = [&](int y) {
-          xg[y] = columns_of(y, at + ONE);
-          xq[y] = columns_of(y, at);
+          xg[y] = columns_of(row_of(y) * DT + column_of(y), at + ONE);
+          xq[y] = columns_of(row_of(y) * DT + column_of(y), at);
+        };
+        const auto products = [&](int y) {
+          if (y + AHEAD < N) read(y + AHEAD);
+          accv[column_of(y)] = mfma32(xg[y], p[row_of(y)], accv[column_of(y)]);
+          acck[column_of(y)] = mfma32(xq[y], ds[row_of(y)], acck[column_of(y)]);
+          __builtin_amdgcn_sched_barrier(0);
         };
 #pragma unroll
         for (int y = 0; y < AHEAD; ++y) read(y);
 #pragma unroll
-        for (int y = 0; y < N; ++y) {
-          if (y + AHEAD < N) read(y + AHEAD);
-          accv[y % DT] = mfma32(xg[y], p[y / DT], accv[y % DT]);
-          acck[y % DT] = mfma32(xq[y], ds[y / DT], acck[y % DT]);
-          __builtin_amdgcn_sched_barrier(0);
+        for (int y = 0; y < FIRST; ++y) products(y);
+        if (LAST && dim > 96) {
+#pragma unroll
+          for (int y = FIRST; y < N; ++y) products(y);
         }
       }
       lds_loads_done();
