@@ -125,7 +125,10 @@ struct KeyTiles {
   __device__ __forceinline__ void load(v4i key0) const {
     constexpr unsigned buffer = BUFFER * KT * DP * 2;
     static_assert(KT == 64 && RP <= 32, "my_row * stride has 32 bits");
-    if (near && key0[3] == key0[0] + 48 && key0[0] <= a.keys - KT) {  // most tiles: one behind the other, so that the addresses are a few additions
+    // Most tiles: one behind the other, so that the addresses are a few additions.  The sixteens of a window ascend without a repetition, so that its
+    // last one says it; those of lists of blocks of 16 come in any order.
+    const bool follow = (key0[3] == key0[0] + 48) & (WINDOW || ((key0[1] == key0[0] + 16) & (key0[2] == key0[0] + 32)));
+    if (near && follow && key0[0] <= a.keys - KT) {
       const elem *k = kp + key0[0] * a.k.stride[1], *v = vp + key0[0] * a.v.stride[1];
       const auto all = [&](auto which) {
         constexpr int p = decltype(which)::value;
