@@ -41,11 +41,12 @@ struct Window {
   __device__ __forceinline__ int token(int x) const { return x < sinks ? x : (int)((unsigned)first + (unsigned)(x - sinks)); }
 };
 __device__ __forceinline__ Window window_of(const PagedArgs &a, int seq) {
-  const int length = a.pages > 0 ? (int)min((long long)max(a.lengths[seq], 0), a.table_width << a.page_log2) : 0;
+  // The window goes back from the sequence's own last token, whether the table holds it or not.
+  const int length = max(a.lengths[seq], 0), held = a.pages > 0 ? (int)min((long long)length, a.table_width << a.page_log2) : 0;
   Window w;
-  w.first = max(0, length - a.window);
+  w.first = min(max(0, length - a.window), held);
   w.sinks = min(a.sink, w.first);
-  w.count = w.sinks + (length - w.first);
+  w.count = w.sinks + (held - w.first);
   return w;
 }
 
