@@ -99,6 +99,15 @@ def rotate(x, positions, frequencies, neighbours=False):
     return _Rotate.apply(x, positions, frequencies, neighbours)
 
 
+def _near(q, kv_heads):
+    """q as the gradient of windows takes it: its tokens and heads less than 2 ** 25 elements apart, and 63 tokens and a group's heads
+    within 2 ** 31.  The forward pass takes any."""
+    token, head = (q.stride(i) if q.shape[i] > 1 else 0 for i in (1, 2))
+    group = max(q.shape[2] // kv_heads, 1)
+    near = max(token, head) < 2 ** 25 and (62 // group + 1) * token + (group - 1) * head + 128 < 2 ** 31
+    return q if near else q.contiguous()
+
+
 class _AttendWindow(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sink, scale):
@@ -114,7 +123,7 @@ class _AttendWindow(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        hip.window_attention_backward(dout.contiguous(), q, k, v, out, lse, dq, dk, dv, *ctx.sizes)
+        hip.window_attention_backward(dout.contiguous(), _near(q, k.shape[2]), k, v, out, lse, dq, dk, dv, *ctx.sizes)
         return dq, dk, dv, None, None, None
 
 
