@@ -14,10 +14,10 @@ def test_gradient_of_queries_far_apart(gpu, heads, token, head):
     g = torch.Generator().manual_seed(heads)
     r = lambda *s: torch.randn(s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
     q, k, v, dout = r(1, 4, heads, 64), r(1, 9, 1, 64), r(1, 9, 1, 64), r(1, 4, heads, 64)
-    far = strided(q, token, head)
+    far = strided(q, token, head)  # (where both strides are the same, a token's heads are the next one's too: what far holds is not what q does)
     assert (far.stride(1), far.stride(2)) == (token, head)
     results = []
-    for x in (q, far):
+    for x in (far.contiguous(), far):
         leaves = [t.detach().requires_grad_() for t in (x, k, v)]
         out = attention.attend_window(*leaves, 3, 1)
         results.append((out, *torch.autograd.grad(out, leaves, dout)))
