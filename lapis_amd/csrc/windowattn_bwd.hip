@@ -142,6 +142,7 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(DkvArgs) {
   constexpr int PIECES = DP / 8, RP = 512 / PIECES, PASSES = Lds::ROWS / RP, DT = DP / 32, N = DP / 16;
   constexpr unsigned ROW = 2 * DP, ONE = Lds::ROWS * ROW, STAGE = 2 * ONE, VALUES = kKeys * ROW;  // bytes: a row, a stage's queries, a stage, from K to V
   __shared__ Lds mem;
+  static_assert(offsetof(Lds, kv) == 0 && offsetof(Lds, tiles) == 2 * VALUES && sizeof(mem.tiles) == 2 * STAGE, "keys, values and stages are cleared together");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int kg = wave & 3, rg = wave >> 2;  // which keys, which tiles
   const int w = (int)xcd_contiguous_block(blockIdx.x, gridDim.x), group = again().a.group, dim = again().a.dim;
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(DkvArgs) {
 
     __syncthreads();  // the column before
     if (dim < DP)     // what no row fills stays zero
-      for (int i = tid; i < (int)(2 * STAGE + 2 * VALUES) / 16; i += 512) ((v4i *)mem.kv)[i] = v4i{0, 0, 0, 0};
+      for (int i = tid; i < (int)(2 * STAGE + 2 * VALUES) / 16; i += 512) ((v4i *)&mem)[i] = v4i{0, 0, 0, 0};
     if (tid == 0) mem.bad = -1;
     __syncthreads();
     if (stages > 0) {
