@@ -535,7 +535,10 @@ int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const lapis_hip_p
 /* One new token of each of `seqs` sequences, the last of lengths[s], over a window and the first tokens: token t counts where
  * t < lengths[s] and (t >= lengths[s] - window or t < sink).  Token t lies in page table[s * table_width + t / cache->page], at place
  * t % cache->page; tokens beyond the table do not exist, nor do those of an entry outside [0, pages), and entries of pages without a token
- * that counts are not read.  window >= 1, sink >= 0; all else as in lapis_hip_paged_attention.  Fewer than 2^31 tokens in a table's row. */
+ * that counts are not read.  window >= 1, sink >= 0; all else as in lapis_hip_paged_attention.  Fewer than 2^31 tokens in a table's row.
+ * Scratch goes by the table and the window, not by the lengths: of every sequence the min(table_width * cache->page, window + sink) tokens that may
+ * count are cut into units, and each has 64 * (dim rounded up to 64, 128 or 256, and 2) bytes for each 16 heads of each group.  A unit has 128 tokens
+ * or more, 1024 or more where there are many, so many more that a sequence has about four for each compute unit at most (256 of them and dim 128: 8.5 MB). */
 typedef struct lapis_hip_paged_window_args {
   int64_t seqs, heads, table_width, window, sink;
   lapis_hip_rows q, out;

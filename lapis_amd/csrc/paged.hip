@@ -596,10 +596,14 @@ int read_window(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_p
   const int64_t longest = p->table_width * c->page;
   a->window = (int)std::min<int64_t>(p->window, INT32_MAX);
   a->sink = (int)std::min<int64_t>(p->sink, INT32_MAX);
-  // tokens that count in a sequence, at most; units as above
+  // Tokens that count in a sequence, at most; units as above, but no more than four a compute unit for any one sequence: every sequence has as many, whatever
+  // its length, and a partial result for each.  A table of 2^20 tokens, 8 key-value heads, dim 128, 16 and 4 bits, units of 1024 tokens always and so: 64
+  // sequences of 8192, 752 us, 404 and 4.4 GB of scratch memory, and 425, 188 and 0.5 GB; one of them of 2^20, 3935 and 1607 us, and 3545 and 1216; a
+  // single one of 2^20, 770 and 284, and 719 and 228.
   const int64_t most = std::min(longest, std::min(p->window, longest) + std::min(p->sink, longest));
-  const int64_t copies = (int64_t)a->head_tiles * c->heads, wanted = std::max(2 * device_cu_count(), 1);
-  a->chunk_tokens = (int)(std::min<int64_t>(std::max<int64_t>(p->seqs * most * copies / wanted, 128), 1024) / 32 * 32);
+  const int64_t copies = std::min<int64_t>((int64_t)a->head_tiles * c->heads, 65535), wanted = std::max(2 * device_cu_count(), 1);  // (a cache may have more heads than that, a call with queries not)
+  const int64_t longest_unit = std::min<int64_t>(std::max<int64_t>(1024, most * copies / (2 * wanted)), 1 << 30);
+  a->chunk_tokens = (int)(std::min<int64_t>(std::max<int64_t>(p->seqs * most * copies / wanted, 128), longest_unit) / 32 * 32);
   a->units_each = (int)std::max<int64_t>(1, ceil_div(most, a->chunk_tokens));
   const int64_t units = p->seqs * a->units_each;
   LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);

@@ -24,3 +24,30 @@ def test_window_of_a_sequence_longer_than_its_table(gpu, heads, kv_heads, dim, p
         t = torch.tensor([t for t in range(min(n, held)) if t >= n - window or t < sink], dtype=torch.long)
         k, v = (x[table[s, t // page].long(), :, t % page] for x in values)
         check_row(out[s], lse[s], q[s], k, v, dim ** -0.5, "%d tokens, %d in the table" % (n, held))
+
+
+@pytest.mark.parametrize("kind", ["same", "f4"])
+def test_a_table_far_wider_than_its_sequences(gpu, kind):
+    """Scratch memory stays with what a sequence may spread over, not with what its table could name; and the longer units of such a table."""
+    page, width, kv_heads, dim, lengths = 64, 2 ** 14, 8, 64, [3, 20000, 0, 700, 8192, 64, 9000, 1]
+    g = torch.Generator().manual_seed(5)
+    held = [-(-n // page) for n in lengths]
+    (kc, vc), (ks, vs), values = rows_of_cache(kind, torch.bfloat16, sum(held), kv_heads, page, dim, g)
+    table, order, at = torch.full((len(lengths), width), -1, dtype=torch.int32), torch.randperm(sum(held), generator=g).to(torch.int32), 0
+    for s, n in enumerate(held):
+        table[s, :n] = order[at:at + n]
+        at += n
+    q = torch.randn((len(lengths), 16, dim), generator=g).to(torch.bfloat16)
+    out, lse = torch.full_like(q, 9.0).cuda(), torch.full((len(lengths), 16), 9.0, device="cuda")
+    operands = q.cuda(), kc, vc, table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), out, 2 ** 30
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    gpu.paged_window_attention(*operands, lse=lse, k_scale=ks, v_scale=vs)
+    scratch = torch.cuda.max_memory_allocated() - before
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    # a unit more for each head where the tokens do not divide, units cut to multiples of 32 tokens, and the allocator's own rounding up
+    assert scratch <= len(lengths) * (4 * cus * 1.04 + kv_heads) * 64 * (dim + 2) + 2 ** 21
+    for s, n in enumerate(lengths):
+        t = torch.arange(n)
+        k, v = (x[table[s, t // page].long(), :, t % page] for x in values)
+        check_row(out[s], lse[s], q[s], k, v, dim ** -0.5, "%d tokens" % n)
