@@ -6,6 +6,8 @@
 namespace lapis {
 namespace {
 
+// What lists and windows need each for themselves lies in one place: arguments of four lines of 64 bytes, the grid's size behind them among it.  With a fifth
+// line, which every workgroup waits for before it knows its unit, a call takes 0.1 to 0.5 us more (5 sequences of 628 tokens 10.1 us and 9.7, one of 34 4.5 and 4.3).
 struct PagedArgs {
   const char *q;
   char *out;
@@ -13,26 +15,34 @@ struct PagedArgs {
   const char *k, *v;
   const void *k_scale, *v_scale;
   long long stride[3], scale_stride[3];
-  long long pages, nnz;
-  int seqs, lists, heads, kv_heads, group, dim, page_log2;
-  bool each;  // a list per key-value head
-  const int *pos, *crd, *tokens;
-  float *lse;
-  float scale;
-  int chunk, units, head_tiles;  // pages a unit, units of all lists, tiles of 16 heads
-  int chunk_tokens;
-  const int *table, *lengths;    // of a window instead of lists
-  long long table_width;
-  int window, sink, units_each;  // units of a sequence
+  long long pages;
+  int seqs, heads, kv_heads, group, dim, page_log2;
+  union {
+    struct {
+      const int *pos, *crd, *tokens;
+      long long nnz;
+      int rows;
+      bool each;  // a list per key-value head
+    } lists;
+    struct {
+      const int *table, *lengths;
+      long long table_width;
+      int window, sink, units_each;  // units of a sequence
+    } windows;
+  };
   bool windowed;
+  float scale;
+  float *lse;
+  int chunk, units, head_tiles;  // pages (of windows: tokens) a unit, units of all lists, tiles of 16 heads
   float *partial, *sums;         // of each unit: 16 x DP, and 16 maxima and sums
 };
+static_assert(sizeof(PagedArgs) + sizeof(int) <= 256, "arguments and the number of workgroups in four lines");
 
 // Pages that a row lists and tokens that count in them, whatever pos and tokens hold.
 __device__ __forceinline__ void list_of(const PagedArgs &a, long long row, int *first, int *tokens) {
-  const long long lo = min(max((long long)a.pos[row], 0ll), a.nnz), hi = min(max((long long)a.pos[row + 1], lo), a.nnz);
+  const long long lo = min(max((long long)a.lists.pos[row], 0ll), a.lists.nnz), hi = min(max((long long)a.lists.pos[row + 1], lo), a.lists.nnz);
   *first = (int)lo;
-  *tokens = a.pages > 0 ? (int)max(0ll, min((long long)a.tokens[row], (hi - lo) << a.page_log2)) : 0;
+  *tokens = a.pages > 0 ? (int)max(0ll, min((long long)a.lists.tokens[row], (hi - lo) << a.page_log2)) : 0;
 }
 
 // Of a window: how many first tokens count that lie before it, where it starts, and tokens that count in all.  They are numbered in order.
@@ -42,10 +52,10 @@ struct Window {
 };
 __device__ __forceinline__ Window window_of(const PagedArgs &a, int seq) {
   // The window goes back from the sequence's own last token, whether the table holds it or not.
-  const int length = max(a.lengths[seq], 0), held = a.pages > 0 ? (int)min((long long)length, a.table_width << a.page_log2) : 0;
+  const int length = max(a.windows.lengths[seq], 0), held = a.pages > 0 ? (int)min((long long)length, a.windows.table_width << a.page_log2) : 0;
   Window w;
-  w.first = min(max(0, length - a.window), held);
-  w.sinks = min(a.sink, w.first);
+  w.first = min(max(0, length - a.windows.window), held);
+  w.sinks = min(a.windows.sink, w.first);
   w.count = w.sinks + (held - w.first);
   return w;
 }
@@ -53,12 +63,12 @@ __device__ __forceinline__ Window window_of(const PagedArgs &a, int seq) {
 // Lists are cut into units of `chunk` pages.  Unit numbers start at pos[row] / chunk + row for each list, which leaves it at
 // least the units it needs, so they are known without a sum over the lists before; those left over do nothing.
 __device__ __forceinline__ long long unit_start(const PagedArgs &a, long long row) {
-  return min(max((long long)a.pos[row], 0ll), a.nnz) / a.chunk + row;
+  return min(max((long long)a.lists.pos[row], 0ll), a.lists.nnz) / a.chunk + row;
 }
 
 // The list that unit u belongs to (the last one that starts at or before it): 64 candidates a step.
 __device__ __forceinline__ int list_of_unit(const PagedArgs &a, int u, int lane) {
-  int lo = 0, n = a.lists;
+  int lo = 0, n = a.lists.rows;
   while (n > 1) {
     const int step = (n + 63) / 64, at = lo + lane * step;
     const unsigned long long before = __ballot(lane * step < n && unit_start(a, at) <= u);
@@ -153,7 +163,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8
   const int ht = block % a.head_tiles;
   block /= a.head_tiles;
   int kh = 0;
-  if (WINDOW || !a.each) {
+  if (WINDOW || !a.lists.each) {
     kh = block % a.kv_heads;
     block /= a.kv_heads;
   }
@@ -161,18 +171,18 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8
   int seq, part, first = 0, count;
   Window w = {};
   if constexpr (WINDOW) {
-    seq = u / a.units_each;
-    part = u - seq * a.units_each;
+    seq = u / a.windows.units_each;
+    part = u - seq * a.windows.units_each;
     w = window_of(a, seq);
     count = w.count;
   } else {
     const int row = list_of_unit(a, u, lane);
-    seq = a.each ? row / a.kv_heads : row;
-    if (a.each) kh = row - seq * a.kv_heads;
+    seq = a.lists.each ? row / a.kv_heads : row;
+    if (a.lists.each) kh = row - seq * a.kv_heads;
     list_of(a, row, &first, &count);
     part = (int)(u - unit_start(a, row));
   }
-  const int chunk = a.chunk_tokens;
+  const int chunk = WINDOW ? a.chunk : a.chunk << a.page_log2;
   const long long from_l = (long long)part * chunk;
   if (part < 0 || (from_l >= count && part != 0)) return;  // a unit number left over (a list without tokens still writes its zeros)
   const int from = (int)from_l, n = min(chunk, count - from), tiles = (n + 31) / 32;
@@ -196,8 +206,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8
     const int x = t * 32 + (lane & 31);
     page = -1;
     if (t < tiles && x < n) {
-      if constexpr (WINDOW) page = a.table[seq * a.table_width + (w.token(from + x) >> a.page_log2)];
-      else page = a.crd[first + ((from + x) >> a.page_log2)];
+      if constexpr (WINDOW) page = a.windows.table[seq * a.windows.table_width + (w.token(from + x) >> a.page_log2)];
+      else page = a.lists.crd[first + ((from + x) >> a.page_log2)];
     }
   };
   unsigned there_next = 0;
@@ -398,7 +408,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8
   __syncthreads();
 
   const bool whole = count <= chunk;
-  const long long unit_id = (long long)(!WINDOW && a.each ? u : u * a.kv_heads + kh) * a.head_tiles + ht;
+  const long long unit_id = (long long)(!WINDOW && a.lists.each ? u : u * a.kv_heads + kh) * a.head_tiles + ht;
   for (int x = tid; x < 16 * PIECES; x += 256) {
     const int h = x / PIECES, d = (x % PIECES) * 8;
     if (h >= heads || d >= a.dim) continue;
@@ -438,15 +448,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   __shared__ float factor[64];
   __shared__ __attribute__((aligned(16))) float part[3][DP];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.y, head = blockIdx.x, kh = head / a.group, in = head - kh * a.group;
-  const long long row = !WINDOW && a.each ? (long long)seq * a.kv_heads + kh : seq;
+  const long long row = !WINDOW && a.lists.each ? (long long)seq * a.kv_heads + kh : seq;
   int first, count;
   if constexpr (WINDOW) count = window_of(a, seq).count;
   else list_of(a, row, &first, &count);
-  const int chunk = a.chunk_tokens, needed = (int)(((long long)count + chunk - 1) / chunk);
+  const int chunk = WINDOW ? a.chunk : a.chunk << a.page_log2, needed = (int)(((long long)count + chunk - 1) / chunk);
   if (needed <= 1) return;
-  const long long u0 = WINDOW ? row * a.units_each : unit_start(a, row);
+  const long long u0 = WINDOW ? row * a.windows.units_each : unit_start(a, row);
   const int units = (int)min((long long)needed, a.units - u0);  // fewer only where positions descend
-  const auto id = [&](int x) { return ((!WINDOW && a.each ? u0 + x : (u0 + x) * a.kv_heads + kh) * a.head_tiles + in / 16) * 16 + in % 16; };
+  const auto id = [&](int x) { return ((!WINDOW && a.lists.each ? u0 + x : (u0 + x) * a.kv_heads + kh) * a.head_tiles + in / 16) * 16 + in % 16; };
   float most = -INFINITY;
   for (int x = lane; x < units; x += 64) most = fmaxf(most, a.sums[id(x) * 2]);
   for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
@@ -493,11 +503,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 }
 
 // Whether some sequence may have several units, whose results are joined.
-bool several_units(const PagedArgs &a) { return a.windowed ? a.units_each > 1 : a.nnz > a.chunk; }
+bool several_units(const PagedArgs &a) { return a.windowed ? a.windows.units_each > 1 : a.lists.nnz > a.chunk; }
 
 template <typename T, int CODES, int DP, bool WINDOW>
 int launch_paged(const PagedArgs &a, hipStream_t st) {
-  const long long blocks = (long long)a.units * (!WINDOW && a.each ? 1 : a.kv_heads) * a.head_tiles;
+  const long long blocks = (long long)a.units * (!WINDOW && a.lists.each ? 1 : a.kv_heads) * a.head_tiles;
   LAPIS_REQUIRE(blocks * 256 < (INT64_C(1) << 32), "paged_attention: %lld units of work", blocks);
   hipLaunchKernelGGL((paged_kernel<T, CODES, DP, WINDOW>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   LAPIS_LAUNCH_CHECK();
@@ -563,18 +573,17 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
                 (long long)p->lists, (long long)p->seqs);
   LAPIS_REQUIRE(p->nnz >= 0 && p->nnz <= INT32_MAX && p->nnz * c->page <= INT32_MAX, "%s: %lld pages listed", what, (long long)p->nnz);
   LAPIS_REQUIRE(p->lists <= INT32_MAX, "%s: %lld lists", what, (long long)p->lists);
-  a->nnz = p->nnz;
-  a->each = p->lists != p->seqs;
-  a->pos = p->pos;
-  a->crd = p->crd;
-  a->tokens = p->tokens;
-  a->lists = (int)p->lists;
+  a->lists.nnz = p->nnz;
+  a->lists.each = p->lists != p->seqs;
+  a->lists.pos = p->pos;
+  a->lists.crd = p->crd;
+  a->lists.tokens = p->tokens;
+  a->lists.rows = (int)p->lists;
   // Units for two workgroups a compute unit, of 128 to 1024 tokens: shorter ones cost more than they spread (a partial result
   // and its join), longer ones leave compute units waiting for the last.
-  const int64_t copies = (int64_t)a->head_tiles * (a->each ? 1 : c->heads), wanted = std::max(2 * device_cu_count(), 1);
+  const int64_t copies = (int64_t)a->head_tiles * (a->lists.each ? 1 : c->heads), wanted = std::max(2 * device_cu_count(), 1);
   const int64_t tokens = std::min<int64_t>(std::max<int64_t>(p->nnz * c->page * copies / wanted, 128), 1024);
   a->chunk = (int)std::max<int64_t>(tokens / c->page, 1);
-  a->chunk_tokens = a->chunk * c->page;
   const int64_t units = p->nnz / a->chunk + p->lists;
   LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
   a->units = (int)units;
@@ -590,12 +599,12 @@ int read_window(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_p
   LAPIS_REQUIRE(p->window >= 1 && p->sink >= 0, "%s: a window of %lld and the first %lld tokens", what, (long long)p->window, (long long)p->sink);
   LAPIS_REQUIRE(p->table_width >= 0 && p->table_width <= INT32_MAX / c->page, "%s: a table of %lld pages", what, (long long)p->table_width);
   a->windowed = true;
-  a->table = p->table;
-  a->lengths = p->lengths;
-  a->table_width = p->table_width;
+  a->windows.table = p->table;
+  a->windows.lengths = p->lengths;
+  a->windows.table_width = p->table_width;
   const int64_t longest = p->table_width * c->page;
-  a->window = (int)std::min<int64_t>(p->window, INT32_MAX);
-  a->sink = (int)std::min<int64_t>(p->sink, INT32_MAX);
+  a->windows.window = (int)std::min<int64_t>(p->window, INT32_MAX);
+  a->windows.sink = (int)std::min<int64_t>(p->sink, INT32_MAX);
   // Tokens that count in a sequence, at most; units as above, but no more than four a compute unit for any one sequence: every sequence has as many, whatever
   // its length, and a partial result for each.  A table of 2^20 tokens, 8 key-value heads, dim 128, 16 and 4 bits, units of 1024 tokens always and so: 64
   // sequences of 8192, 752 us, 404 and 4.4 GB of scratch memory, and 425, 188 and 0.5 GB; one of them of 2^20, 3935 and 1607 us, and 3545 and 1216; a
@@ -603,9 +612,9 @@ int read_window(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_p
   const int64_t most = std::min(longest, std::min(p->window, longest) + std::min(p->sink, longest));
   const int64_t copies = std::min<int64_t>((int64_t)a->head_tiles * c->heads, 65535), wanted = std::max(2 * device_cu_count(), 1);  // (a cache may have more heads than that, a call with queries not)
   const int64_t longest_unit = std::min<int64_t>(std::max<int64_t>(1024, most * copies / (2 * wanted)), 1 << 30);
-  a->chunk_tokens = (int)(std::min<int64_t>(std::max<int64_t>(p->seqs * most * copies / wanted, 128), longest_unit) / 32 * 32);
-  a->units_each = (int)std::max<int64_t>(1, ceil_div(most, a->chunk_tokens));
-  const int64_t units = p->seqs * a->units_each;
+  a->chunk = (int)(std::min<int64_t>(std::max<int64_t>(p->seqs * most * copies / wanted, 128), longest_unit) / 32 * 32);
+  a->windows.units_each = (int)std::max<int64_t>(1, ceil_div(most, a->chunk));
+  const int64_t units = p->seqs * a->windows.units_each;
   LAPIS_REQUIRE(units <= INT32_MAX, "%s: %lld units of work", what, (long long)units);
   a->units = (int)units;
   return LAPIS_HIP_OK;
@@ -614,7 +623,7 @@ int read_window(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_p
 // bytes of the partial results, and where the sums lie behind them
 int64_t partial_bytes(const PagedArgs &a, int64_t *sums_at) {
   const int dp = a.dim <= 64 ? 64 : a.dim <= 128 ? 128 : 256;
-  const int64_t ids = (int64_t)a.units * (!a.windowed && a.each ? 1 : a.kv_heads) * a.head_tiles * 16;
+  const int64_t ids = (int64_t)a.units * (!a.windowed && a.lists.each ? 1 : a.kv_heads) * a.head_tiles * 16;
   *sums_at = ids * dp * 4;
   return several_units(a) ? ids * (dp + 2) * 4 : 0;
 }
@@ -661,7 +670,7 @@ extern "C" int lapis_hip_paged_attention(const lapis_hip_kv_cache *cache, const 
   int rc = read_paged("paged_attention", cache, args, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   if (a.seqs == 0 || a.heads == 0) return LAPIS_HIP_OK;
-  LAPIS_REQUIRE(a.q && a.out && a.pos && a.tokens && (a.crd || a.nnz == 0), "paged_attention: null operands");
+  LAPIS_REQUIRE(a.q && a.out && a.lists.pos && a.lists.tokens && (a.lists.crd || a.lists.nnz == 0), "paged_attention: null operands");
   rc = check_rows(a, "paged_attention", args->q, args->out);
   if (rc == LAPIS_HIP_OK) rc = give_work(a, "paged_attention", args->work);
   return rc != LAPIS_HIP_OK ? rc : launch_paged<false>(a, args->dtype, cache->dtype, as_stream(stream));
@@ -678,7 +687,7 @@ extern "C" int lapis_hip_paged_window_attention(const lapis_hip_kv_cache *cache,
   int rc = read_window("paged_window_attention", cache, args, &a);
   if (rc != LAPIS_HIP_OK) return rc;
   if (a.seqs == 0 || a.heads == 0) return LAPIS_HIP_OK;
-  LAPIS_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0), "paged_window_attention: null operands");
+  LAPIS_REQUIRE(a.q && a.out && a.windows.lengths && (a.windows.table || a.windows.table_width == 0), "paged_window_attention: null operands");
   rc = check_rows(a, "paged_window_attention", args->q, args->out);
   if (rc == LAPIS_HIP_OK) rc = give_work(a, "paged_window_attention", args->work);
   return rc != LAPIS_HIP_OK ? rc : launch_paged<true>(a, args->dtype, cache->dtype, as_stream(stream));
