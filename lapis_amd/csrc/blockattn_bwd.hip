@@ -27,8 +27,10 @@ __device__ __forceinline__ float of_row(const vec8<T> (&f)[2], int row, int lane
 // 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 275 us in a trace (309 with a branch for each masked element and operands read where
 // they are used, 356 with 24 registers spilled and the products one chain after the other), 690 TFLOP/s; a window of 1024 and the first 16 keys
 // 293.  Bound by what a wavefront waits for between its chains of products: they run in a third of the cycles.
+// Head dims up to 64: three wavefronts a SIMD, 168 registers, one of them read back from memory once a tile (left to itself the compiler takes 169 and two wavefronts; 1981
+// queries, 40 heads over 8, dim 32, 9 blocks of 32: 26.5 us with two, 21.7 with three; 8192 queries, 32 heads, dim 64, 16 blocks of 64: 159 and 143).
 template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
-__global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
+__global__ __launch_bounds__(64 * NW * SIDES, DP <= 64 && SIDES == 1 ? 3 : 2) void block_dq_kernel(BlockArgs a, int tiles_of_list, float *__restrict__ delta, float *__restrict__ logs, int *odd) {
   typedef typename T::elem elem;
   constexpr int PIECES = DP / 8, PASSES = KT * PIECES / (NW * 64), ST = KT / 32, DT = DP / 32, CH = KT / 16;
   __shared__ __attribute__((aligned(16))) elem k_tile[SIDES][2][KT * DP], v_tile[SIDES][2][KT * DP];
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_dq_kernel(BlockArgs 
       asm volatile("" : "+v"(place_lane));
 #pragma unroll
       for (int x = 0; x < ST; ++x) {
-        if (DP <= 64) asm volatile("" : "+v"(place_lane));  // or for each half of it: 159 registers, three wavefronts a SIMD
+        if (DP <= 64) asm volatile("" : "+v"(place_lane));  // or for each half of it: three wavefronts a SIMD
         // two chains of products that do not wait for each other, their operands read two products ahead
         constexpr int N = DP / 16, AHEAD = 2;
         v16f s = {}, g = {};
