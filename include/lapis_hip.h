@@ -435,8 +435,11 @@ int lapis_hip_normalize_mom2_f64(int64_t n, const double *mom1, const double *mo
  * are finished attention weights); it has no counterpart of what follows.
  *
  * Types: 16-bit elements (bf16, f16); a cache may hold e4m3 codes with one fp32 scale per row of `dim`, or 4-bit codes
- * (LAPIS_HIP_F4E2M1).  Sums, softmax statistics and scales are fp32.  `dim` is a multiple of 8; 16-bit operands lie on 16-byte
- * boundaries, 8-bit codes on 8-byte ones, strides (in elements) are multiples of 8.  Outputs must not overlap inputs.
+ * (LAPIS_HIP_F4E2M1).  Sums, softmax statistics and scales are fp32.  What goes into a matrix product has the operands' type (over
+ * a cache the queries'): softmax weights (with 8-bit codes times the value's scale) and, in the backward passes, score gradients are rounded
+ * to it once, and so are 4-bit codes times their scale, which is exact but beyond float16's range and below its normal numbers.
+ * `dim` is a multiple of 8; 16-bit operands lie on 16-byte boundaries, 8-bit codes on 8-byte ones, strides (in elements) are multiples
+ * of 8.  Outputs must not overlap inputs.
  * Structures: positions and coordinates int32.  A coordinate outside [0, columns) (of pages: outside [0, pages))
  * and positions outside [0, nnz] are never followed: such an entry counts as absent.  Coordinates need not ascend.
  * Positions do; where they descend nothing outside the operands is read or written, rows overlap and are taken as they stand, each

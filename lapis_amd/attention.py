@@ -270,7 +270,8 @@ class PagedCache:
         return out
 
     def step_window(self, q, k, v, window, sink=0, scale=None, positions=None):
-        """As ``step``, but a token reads the last ``window`` tokens of its sequence, itself among them, and the first ``sink``."""
+        """As ``step``, but a token reads the last ``window`` tokens of its sequence, itself among them, and the first ``sink``.  Pages that
+        the window has left behind stay the sequence's until ``release``: another call may ask for more of them."""
         self._check_positions("step_window", positions)
         q, length, lengths = self._append(q, k, v, positions)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

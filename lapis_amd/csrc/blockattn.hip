@@ -18,8 +18,8 @@ __device__ __forceinline__ float units_of_ln2(float scale) {
 // between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
 // Operands from LDS are asked for some products ahead (a fence after each product keeps it so: left alone the compiler reads each pair of them and
 // waits), and the two ways of taking values, with infinities and NaN apart and without, are no two sides of one branch (64 registers less).
-// 32 768 queries and keys, 32 heads over 8, dim 128, bf16: 16 blocks of 128 a row 1140 to 1160 us, a window of 2048 and the first 16 keys 1125 to 1170
-// (930 to 980 TFLOP/s where a large library product reaches 1203 to 1400).  Near the card's power: with operands that are zeros it
+// 32 768 queries and keys, 32 heads over 8, dim 128, bf16: 16 blocks of 128 a row 1120 to 1165 us, a window of 2048 and the first 16 keys 1116 to 1170
+// (885 to 965 TFLOP/s where a large library product reaches 1203 to 1400).  Near the card's power: with operands that are zeros it
 // is 20 % faster and that product 30 %; exponentials of half a tile under the products of the other half change nothing.
 template <typename T, int DP, int NW, int KT, bool WINDOW, int SIDES = 1>
 __global__ __launch_bounds__(64 * NW * SIDES, 2) void block_forward_kernel(BlockArgs a, int tiles_of_list, int flip) {

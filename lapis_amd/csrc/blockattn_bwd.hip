@@ -24,7 +24,7 @@ __device__ __forceinline__ float of_row(const vec8<T> (&f)[2], int row, int lane
 
 // As the forward kernel: 32 rows a wavefront, a query per lane.  dS^T = P^T * (scale V dO^T - scale delta) feeds dQ^T = K^T dS^T
 // from its registers.  rowsum(dO * O), times `scale`, and the log-sums in units of ln 2 are left for the other kernel.
-// 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 275 us in a trace (309 with a branch for each masked element and operands read where
+// 8192 queries, 32 heads over 8, dim 128, 16 blocks of 64 a row: 273 us in a trace (309 with a branch for each masked element and operands read where
 // they are used, 356 with 24 registers spilled and the products one chain after the other), 690 TFLOP/s; a window of 1024 and the first 16 keys
 // 293.  Bound by what a wavefront waits for between its chains of products: they run in a third of the cycles.
 // Head dims up to 64: three wavefronts a SIMD, 168 registers, one of them read back from memory once a tile (left to itself the compiler takes 169 and two wavefronts; 1981

@@ -4,7 +4,7 @@
 // A row of `dim` elements belongs to a group of lanes, eight elements each (one 16-byte load); the row's maximum is
 // a DPP reduction over the group, so a row is read once and nothing is kept but registers.  Bound by memory: 32 768 tokens
 // of 8 heads, dim 128, bf16 into e4m3 in 50 us (4.1 TB/s), 20 000 tokens, dim 96, back into f16 in 22.1 (4.2 TB/s), where a
-// large copy reaches 4.75; 32 768 tokens of 8 heads, dim 128, out of 4-bit codes in 41 us (4.1 TB/s, most of it written); four rows a thread on their way, loads first, where that leaves every compute unit its workgroups
+// large copy reaches 4.75; 32 768 tokens of 8 heads, dim 128, into 4-bit codes in 36 to 39 us and out of them in 41 (4.1 TB/s, most of it written); four rows a thread on their way, loads first, where that leaves every compute unit its workgroups
 // (one row a thread: 54 and 30).  48 tokens take 4.5 us, the call and the launch.
 #include "kvcache.hpp"
 

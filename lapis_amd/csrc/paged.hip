@@ -133,9 +133,9 @@ __device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_ca
 // reaches 4.75), 160 with float16 queries; one sequence of 16 384 tokens, bf16: 22.4 us, 16.9 of them here (4.0 TB/s) and 5.4 for the join.
 // 4-bit codes become 16-bit operands by one conversion with their scale (exact, in float16 down to its subnormal numbers: two bits of mantissa times a power of two), K in registers and V on
 // its way into LDS; 128 registers, four workgroups a compute unit, as a row is 64 bytes and its 32 elements a lane one load.  64 sequences of up to 8192
-// tokens: 86 us with the join, 78 of them here (4.5 TB/s); one of 16 384: 14.5, 9.3 here (launch, look-ups and two tiles one after the other) and 4.9.
+// tokens: 86 us with the join, 78 of them here (4.5 TB/s); one of 16 384: 14.4, 9.6 here (launch, look-ups and two tiles one after the other) and 4.6.
 // Windows number their tokens first ones first, so that a unit may hold the end of those and the start of the others; table entries are asked for as
-// those of lists are.  128 sequences, window 4096 and 64 first tokens, 4 bits: 133 us, 119 of them here (4.8 TB/s); 4 sequences, bf16: 21.2, 16.0 here (4.2 TB/s).
+// those of lists are.  128 sequences, window 4096 and 64 first tokens, 4 bits: 133 us, 119 of them here (4.8 TB/s); 4 sequences, bf16: 21.0, 17.0 here (4.0 TB/s).
 template <typename T, int CODES, int DP, bool WINDOW>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : CODES == kF4 ? 4 : CODES == kF8 ? 3 : 2) void paged_kernel(PagedArgs a) {
   typedef typename T::elem elem;
@@ -580,7 +580,8 @@ int read_paged(const char *what, const lapis_hip_kv_cache *c, const lapis_hip_pa
   a->lists.tokens = p->tokens;
   a->lists.rows = (int)p->lists;
   // Units for two workgroups a compute unit, of 128 to 1024 tokens: shorter ones cost more than they spread (a partial result
-  // and its join), longer ones leave compute units waiting for the last.
+  // and its join), longer ones leave compute units waiting for the last.  Two of them too where three (8 bits) or four (4 bits) fit a compute unit: one sequence
+  // of 16 384 tokens, 32 heads over 8, dim 128, 4 bits 14.2 us, for four 17.4; 64 of 8192 123.9 and 123.7; 8 bits, for two and three: 18.2 and 21.3, 223 and 223.
   const int64_t copies = (int64_t)a->head_tiles * (a->lists.each ? 1 : c->heads), wanted = std::max(2 * device_cu_count(), 1);
   const int64_t tokens = std::min<int64_t>(std::max<int64_t>(p->nnz * c->page * copies / wanted, 128), 1024);
   a->chunk = (int)std::max<int64_t>(tokens / c->page, 1);

@@ -1,8 +1,8 @@
 // Rows turned by their positions, and on their way into a paged cache.
 //
 // Pair (x, y) of a row becomes (x cos - y sin, x sin + y cos) of an angle that is one for all heads of a token.  Bound by memory: 16384 tokens of 32 heads,
-// dim 128, bf16, three axes, in 53 us (5.1 TB/s read and written, more than a large copy out of memory reaches); a prompt of 32768 tokens, 32 heads of queries and 8 of keys and
-// values, into 4-bit codes in 141 us (5.0 TB/s; 193 with divisions and with slots asked for after the angles, 158 with every lane working out its
+// dim 128, bf16, three axes, in 58 us (4.6 TB/s read and written, where a large copy reaches 4.7); a prompt of 32768 tokens, 32 heads of queries and 8 of keys and
+// values, into 4-bit codes in 142 us (4.9 TB/s; 193 with divisions and with slots asked for after the angles, 158 with every lane working out its
 // own row: vector instructions in 93 % of the cycles).  48 tokens into 8-bit codes take 4 us, the launch.
 #include "kvcache.hpp"
 
@@ -181,8 +181,8 @@ int launch_turn(TurnArgs a, hipStream_t st) {
   };
   const auto with = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
-    // four rows a thread only where that leaves every compute unit its workgroups (the prompt above with its reading back: 182 us, with two rows 183, with
-    // eight 186, and 204 where rows are each lane's own; the 16384 tokens 53, 53, 55 and 55)
+    // four rows a thread only where that leaves every compute unit its workgroups (the prompt above with its reading back: 183 us, with two rows 178, with
+    // eight 184, and 193 where rows are each lane's own; the 16384 tokens 58, 63, 57 and 61)
     if (a.rows * L < 256 * 16 * device_cu_count()) go(lanes, std::integral_constant<int, 1>(), std::false_type());
     else if (a.heads % (64 / L) || a.cache.heads % (64 / L)) go(lanes, std::integral_constant<int, 4>(), std::false_type());
     else go(lanes, std::integral_constant<int, 4>(), std::true_type());

@@ -121,7 +121,7 @@ __device__ __forceinline__ const DkvArgs &again() {
   return *(const DkvArgs *)p;
 }
 
-// 8192 queries and keys, 32 heads over 8, dim 128, window 1024 and the first 16 keys, bf16: 406 us in a trace (372 at best), 645 to 700 TFLOP/s of its four
+// 8192 queries and keys, 32 heads over 8, dim 128, window 1024 and the first 16 keys, bf16: 406 us in a trace (364 at best), 645 to 700 TFLOP/s of its four
 // products, and 20 for the join.  Bound by the card's power: products run in 40 % of the cycles, LDS in 37 %, other orders of the work take the same time
 // (weights of half a tile under the products of the other half too), and the whole pass a quarter less with operands that are zeros.  3 x 701 queries, 937 keys, 6 heads, dim 72, window 200: 31 us, of
 // which a first stage takes 8 (launch, instructions and operands from memory) and each stage of 64 rows 2.5.
@@ -534,7 +534,9 @@ struct WindowLayout {
 };
 
 constexpr int kColumnTiles = 6;  // what a column costs beside its tiles (a stage of two takes 2.5 us, a column's loads, start and end 7)
-constexpr int kLeastTiles = 12;  // of a workgroup: fewer are not worth a join
+// Of a workgroup.  With 6, 12 and 24: 3 x 701 queries over 937 keys, 6 heads, dim 72, window 200 62, 53 and 67 us; 1024 queries, 16 heads, dim 64, window 100 46, 42
+// and 52; 512 queries, 8 heads over 2, dim 128, window 256 42, 47 and 59; 128 queries over 4096 keys, 8 heads, dim 128 82, 100 and 110.
+constexpr int kLeastTiles = 12;
 
 int layout_of(BlockArgs *a, WindowLayout *layout) {
   const char *what = "window_attention_backward";
