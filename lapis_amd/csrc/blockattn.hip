@@ -15,7 +15,8 @@ __device__ __forceinline__ float units_of_ln2(float scale) {
 // A workgroup takes 32 * NW rows of one list, a wavefront 32 of them.  Tiles of KT keys go through LDS (two buffers: the
 // next tile is loaded straight into one while the other is computed).
 // S^T = K Q^T has a query per lane, so maxima, sums and factors of the softmax are one register and need one exchange
-// between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.
+// between the halves of the wavefront; P^T feeds O^T = V^T P^T from the registers it was computed in.  For that it is rounded to the operands' type, the one
+// rounding before the result's own (the sums that divide it take it in 32 bits): products of 32-bit operands have a sixteenth of the rate.
 // Operands from LDS are asked for some products ahead (a fence after each product keeps it so: left alone the compiler reads each pair of them and
 // waits), and the two ways of taking values, with infinities and NaN apart and without, are no two sides of one branch (64 registers less).
 // 32 768 queries and keys, 32 heads over 8, dim 128, bf16: 16 blocks of 128 a row 1120 to 1165 us, a window of 2048 and the first 16 keys 1116 to 1170

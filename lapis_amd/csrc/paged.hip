@@ -122,7 +122,7 @@ __device__ __forceinline__ float power_of_two(float x) { return __builtin_bit_ca
 // A unit: up to 16 heads of a group against a stretch of a list.  Its four wavefronts take tiles of 32 tokens in turn, each by
 // itself; their maxima, sums and results are joined through LDS.
 //   S^T = K Q^T (16x16x32, a head per lane): K goes from memory into the operand's registers, each lane a piece of one token.
-//   O^T = V^T P^T: P^T stays in its registers, V goes through LDS, where it is read by columns.
+//   O^T = V^T P^T: P^T stays in its registers, rounded to the queries' type as a product's operands are, V goes through LDS, where it is read by columns.
 // The next tile is loaded into the same registers as soon as they have been used, so all but the first products of a tile
 // run under its successor's loads; eight wavefronts a compute unit have 64 KB (8-bit cache) to 128 KB on their way.
 // 8-bit codes are multiplied as they are (exact in 16 bits); a key's scale multiplies its score, a value's scale its weight.  With

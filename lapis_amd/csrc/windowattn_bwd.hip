@@ -129,7 +129,8 @@ __device__ __forceinline__ const DkvArgs &again() {
 // 128 keys of a list and a stretch of the queries that see them, rows (a query times a head of the group) packed into tiles of 32.
 // Four wavefronts have 32 keys each, a key per lane, and four more the same keys and every other tile: a wavefront computes all four
 // products of its tile, S = Q K^T and dP = dO V^T, which turn into P and dS and feed dV^T = dO^T P and dK^T = Q^T dS from their
-// registers, and the halves' sums are added up at the column's end.
+// registers, each rounded once to the operands' type (products of 32-bit operands have a sixteenth of the rate), and the halves' sums are added up at the
+// column's end.
 // Two wavefronts a SIMD, one in its products while the other is in its weights: with one alone (K and V in its registers, three tiles
 // in work at a time) each of its 440 instructions a tile took its turn, 3400 cycles where the products take 1100; the sums leave no
 // registers for K and V of 32 keys in two, so they are read from LDS, beside the queries.
