@@ -686,7 +686,7 @@ void written(std::initializer_list<PyObject *> outputs) {
     if (o != Py_None && !THPVariable_Unpack(o).is_inference()) THPVariable_Unpack(o).unsafeGetTensorImpl()->bump_version();
 }
 
-// The kernels read and write device memory only, of one device.
+// The kernels read and write device memory only, of one device: the current one, on whose streams they run.
 void on_device(const char *what, PyObject *const *a, Py_ssize_t n) {
   int device = -1;
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -696,6 +696,9 @@ void on_device(const char *what, PyObject *const *a, Py_ssize_t n) {
     if (device >= 0 && t.device().index() != device) raise(PyExc_ValueError, "%s: operands on different devices", what);
     device = t.device().index();
   }
+  if (device < 0) return;
+  const int current = c10::hip::getCurrentHIPStream().device_index();
+  if (device != current) raise(PyExc_ValueError, "%s: operands on device %d, the current one is %d", what, device, current);
 }
 
 // Rows of a tensor (batch, tokens, heads, dim); with three dimensions (tokens, heads, dim).
@@ -865,15 +868,6 @@ LAPIS_PY(py_paged_attention) {
   });
 }
 
-// The kernels run on the current device, on its streams.
-void on_current_device(const char *what, PyObject *const *a, Py_ssize_t n) {
-  on_device(what, a, n);
-  const auto current = c10::hip::getCurrentHIPStream().device_index();
-  for (Py_ssize_t i = 0; i < n; ++i)
-    if (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).device().index() != current)
-      raise(PyExc_ValueError, "%s: operands on device %d, the current one is %d", what, (int)THPVariable_Unpack(a[i]).device().index(), (int)current);
-}
-
 // (q, k_cache, v_cache, table, lengths, out, window, sink, lse, scale, k_scale, v_scale, stream)
 LAPIS_PY(py_paged_window_attention) {
   return guarded([&] {
@@ -913,7 +907,7 @@ LAPIS_PY(py_paged_window_attention) {
       p.lse = static_cast<float *>(lse.data_ptr());
     }
     p.scale = a[9] == Py_None ? 1.0f / std::sqrt((float)c.dim) : (float)number(a[9]);
-    on_current_device(what, a, n);
+    on_device(what, a, n);
     const lapis_hip_stream_t st = stream_of(a[12]);
     int64_t bytes = 0;
     check(lapis_hip_paged_window_attention_work(&c, &p, &bytes));
@@ -967,7 +961,7 @@ LAPIS_PY(py_rotate) {
     const int inverse = truth(a[5]);
     const lapis_hip_rows from = rows_of(what, "x", x, false), to = rows_of(what, "out", out, true);
     same_or_apart(what, "out", x, out);
-    on_current_device(what, a, n);
+    on_device(what, a, n);
     check(lapis_hip_rotate(x.size(0), x.size(1), x.size(2), x.size(3), &r, inverse, &from, &to, dtype, stream_of(a[6])));
     written({a[3]});
     return give(a[3]);
@@ -1009,7 +1003,7 @@ LAPIS_PY(py_kv_append) {
       p.q_out = rows_of(what, "q_out", out, true);
       same_or_apart(what, "q_out", q, out);
     }
-    on_current_device(what, a, n);
+    on_device(what, a, n);
     check(lapis_hip_kv_append(&c, &p, stream_of(a[12])));
     written({a[5], a[6], a[7], a[8], a[10]});
     PyObject *result = PyTuple_Pack(2, a[5], a[6]);
@@ -1269,7 +1263,7 @@ LAPIS_PY(py_window_attention) {
     const char *what = "window_attention";
     arguments(what, n, 9);
     const lapis_hip_window_args p = window_of(what, a[0], a[1], a[2], a[3], a[6], true, a[4], a[5], a[7]);
-    on_current_device(what, a, n);
+    on_device(what, a, n);
     check(lapis_hip_window_attention(&p, stream_of(a[8])));
     written({a[3], a[6]});
     PyObject *result = PyTuple_Pack(2, a[3], a[6]);
@@ -1298,7 +1292,7 @@ LAPIS_PY(py_window_attention_backward) {
       else of_shape(what, m.name, t, {p.batch, p.keys, p.kv_heads, p.dim});
       *m.to = rows_of(what, m.name, t, m.output);
     }
-    on_current_device(what, a, n);
+    on_device(what, a, n);
     const lapis_hip_stream_t st = stream_of(a[12]);
     int64_t bytes = 0;
     check(lapis_hip_window_attention_backward_work(&p, &bytes));
