@@ -111,6 +111,9 @@ def _near(q, kv_heads):
 class _AttendWindow(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sink, scale):
+        group = q.shape[2] // max(k.shape[2], 1)
+        if any(ctx.needs_input_grad) and q.shape[1] * group >= 2 ** 29:
+            raise ValueError("attend_window: a gradient of %d queries of %d heads of a group, fewer than 2 ** 29 together expected" % (q.shape[1], group))
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device)
         hip.window_attention(q, k, v, out, window, sink, lse, scale)
